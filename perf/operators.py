@@ -95,7 +95,7 @@ def draw(rng) -> dict:
         while work(c)["bytes"] > 1.0e9:
             c["N"] = max(1, c["N"] // 2)
         return c
-    s = rng.choice((8, 16, 32, 64, 128))
+    s = rng.choice((16, 32, 64, 128))
     b = _log(rng, 1, 64)
     u = rng.random()
     if u < 0.45:                                   # a decode step
