@@ -1,0 +1,147 @@
+// gr_paged.hip -- prebuilt instances of attention over a paged cache
+// (gr_paged.h) behind gr_paged_attn().
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "gr_host.h"
+#include "gr_paged.h"
+#include "gr_paged_host.h"
+#include "grammar_rt.h"
+
+namespace {
+
+template <class T, int D, int BN, int NW, int KG>
+__global__ __launch_bounds__(64 * NW * KG) __attribute__((amdgpu_waves_per_eu(NW* KG == 4 && KG > 1 && D == 128 ? 1 : 2)))
+void gr_paged_kernel(gr_paged_args a) {
+  extern __shared__ __attribute__((aligned(16))) char gr_lds[];
+  gr_paged_body<T, D, BN, NW, KG>(a, gr_lds);
+}
+
+template <class T, int D, int BM>
+__global__ __launch_bounds__(256) void gr_paged_merge_kernel(gr_paged_args a) {
+  gr_paged_merge_body<T, D, BM>(a);
+}
+
+// How a call is cut into workgroups.
+struct Plan {
+  int nw;                        // waves of 32 rows
+  long long tiles;               // row tiles of a key head
+  int parts, chunk, chunk_long;
+};
+
+Plan plan_of(const gr_paged_cache& c, const gr_paged_batch& b, int Hq) {
+  Plan p;
+  const int G = Hq / c.heads;
+  const long long most = b.starts && b.max_new > 0 && b.max_new < b.rows ? b.max_new : b.rows;
+  p.nw = most * G <= 32 ? 1 : most * G <= 64 ? 2 : 4;
+  const int BM = 32 * p.nw;
+  // packed rows: every sequence may have a part-filled tile
+  p.tiles = b.starts ? (long long)b.rows * G / BM + b.B : (long long)b.B * (((long long)b.rows * G + BM - 1) / BM);
+  const int cus = gr::cu_count() > 0 ? gr::cu_count() : 256;
+  const long long cap = (long long)b.width * c.page_size;
+  const long long len = b.max_len > 0 && b.max_len < cap ? b.max_len : cap;
+  const long long wgs = p.tiles * c.heads;
+  const long long want = 4LL * cus;
+  long long parts = wgs >= want ? 1 : (want + wgs - 1) / wgs;
+  if (parts > (len + 255) / 256) parts = (len + 255) / 256;
+  p.parts = (int)(parts < 1 ? 1 : parts > 256 ? 256 : parts);
+  p.chunk = p.parts == 1 ? 1 << 30 : (int)(((len + p.parts - 1) / p.parts + 63) / 64 * 64);
+  p.chunk_long = p.chunk;
+  return p;
+}
+
+size_t part_bytes(const Plan& p, int heads, int D, int parts) {
+  return parts <= 1 ? 0 : (size_t)p.tiles * heads * parts * 32 * p.nw * (D + 2) * sizeof(float);
+}
+
+template <class T, int D, int BN, int NW, int KG>
+int launch_tiles(const gr_paged_args& a, hipStream_t st) {
+  constexpr int BM = 32 * NW;
+  const long long wgs = (long long)a.tiles * a.Hkv;
+  hipLaunchKernelGGL((gr_paged_kernel<T, D, BN, NW, KG>), dim3((unsigned)(wgs * a.parts)), dim3(64 * NW * KG),
+                     (gr_paged_lds<D, BN, NW, KG>::BYTES), st, a);
+  int rc = gr::hip_check(hipGetLastError(), GR_E_LAUNCH, "gr_paged_attn launch");
+  if (rc || a.parts == 1) return rc;
+  hipLaunchKernelGGL((gr_paged_merge_kernel<T, D, BM>), dim3((unsigned)wgs, NW), dim3(256), 0, st, a);
+  return gr::hip_check(hipGetLastError(), GR_E_LAUNCH, "gr_paged_attn merge launch");
+}
+
+template <class T, int D>
+int launch(const gr_paged_args& a, int nw, hipStream_t st) {
+  if (nw == 1) return launch_tiles<T, D, 32, 1, 4>(a, st);
+  if (nw == 2) return launch_tiles<T, D, 32, 2, 4>(a, st);
+  return launch_tiles<T, D, 64, 4, 1>(a, st);
+}
+
+int check_heads(const gr_paged_cache* c, const gr_paged_batch* b, int Hq) {
+  if (Hq <= 0 || Hq % c->heads)
+    return gr::fail(GR_E_ARG, "gr_paged_attn: %d query heads are not a multiple of the cache's %d", Hq, c->heads);
+  const long long tokens = b->starts ? (long long)b->rows : (long long)b->B * b->rows;
+  if (tokens * Hq >= (1LL << 30)) return gr::fail(GR_E_ARG, "gr_paged_attn: %lld tokens of %d heads are too many for one call", tokens, Hq);
+  return GR_OK;
+}
+
+}  // namespace
+
+extern "C" size_t gr_paged_attn_workspace(const gr_paged_cache* cache, const gr_paged_batch* batch, int Hq) {
+  if (gr::check_paged(cache, batch, "gr_paged_attn_workspace") || check_heads(cache, batch, Hq) || batch->rows == 0) return 0;
+  const Plan p = plan_of(*cache, *batch, Hq);
+  return part_bytes(p, cache->heads, cache->head_dim, p.parts);
+}
+
+extern "C" int gr_paged_attn(const gr_paged_cache* cache, const gr_paged_batch* batch, const void* q, void* o, float* lse,
+                             int Hq, const long long* q_strides, const long long* o_strides, int causal, float scale,
+                             void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = gr::check_paged(cache, batch, "gr_paged_attn");
+  if (rc || (rc = check_heads(cache, batch, Hq))) return rc;
+  if (batch->rows == 0) return GR_OK;
+  if (!q || !o || !q_strides || !o_strides) return gr::fail(GR_E_ARG, "gr_paged_attn: null argument");
+  if (!gr::aligned16(q) || !gr::aligned16(o) || !gr::aligned16(workspace))
+    return gr::fail(GR_E_ARG, "gr_paged_attn: base pointers must be 16-byte aligned");
+  if ((uintptr_t)lse & 3) return gr::fail(GR_E_ARG, "gr_paged_attn: lse must be 4-byte aligned");
+  for (int i = 0; i < 3; ++i)
+    if (q_strides[i] < 0 || q_strides[i] % 8 || o_strides[i] < 0 || o_strides[i] % 8)
+      return gr::fail(GR_E_ARG, "gr_paged_attn: strides must be non-negative multiples of 8 elements");
+  if (!(scale > 0.f)) return gr::fail(GR_E_ARG, "gr_paged_attn: scale must be positive");
+  Plan p = plan_of(*cache, *batch, Hq);
+  // the most parts that the workspace holds
+  while (p.parts > 1 && part_bytes(p, cache->heads, cache->head_dim, p.parts) > (workspace ? workspace_bytes : 0)) --p.parts;
+  if (p.tiles * cache->heads * p.parts > 0x7fffffffLL / 256) return gr::fail(GR_E_ARG, "gr_paged_attn: grid out of range");
+  gr_paged_args a = {};
+  a.q = q;
+  a.o = o;
+  a.lse = lse;
+  a.q_sb = q_strides[0]; a.q_st = q_strides[1]; a.q_sh = q_strides[2];
+  a.o_sb = o_strides[0]; a.o_st = o_strides[1]; a.o_sh = o_strides[2];
+  a.k = cache->k;
+  a.v = cache->v;
+  a.k_sp = cache->k_strides[0]; a.k_sh = cache->k_strides[1]; a.k_ss = cache->k_strides[2];
+  a.v_sp = cache->v_strides[0]; a.v_sh = cache->v_strides[1]; a.v_ss = cache->v_strides[2];
+  a.table = batch->table;
+  a.table_stride = batch->table_stride;
+  a.lens = batch->lens;
+  a.starts = batch->starts;
+  a.B = batch->B;
+  a.rows = batch->rows;
+  a.width = batch->width;
+  a.pages = cache->pages;
+  a.page_shift = gr::page_shift(cache->page_size);
+  a.Hq = Hq;
+  a.Hkv = cache->heads;
+  a.G = Hq / cache->heads;
+  a.causal = causal;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.tiles = (int)p.tiles;
+  a.parts = p.parts;
+  a.chunk = p.chunk;
+  a.chunk_long = p.chunk_long;
+  if (p.parts > 1) {
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = a.part_o + (size_t)p.tiles * cache->heads * p.parts * 32 * p.nw * cache->head_dim;
+  }
+  hipStream_t st = (hipStream_t)stream;
+  if (cache->dtype == GR_F16)
+    return cache->head_dim == 64 ? launch<_Float16, 64>(a, p.nw, st) : launch<_Float16, 128>(a, p.nw, st);
+  return cache->head_dim == 64 ? launch<__bf16, 64>(a, p.nw, st) : launch<__bf16, 128>(a, p.nw, st);
+}

@@ -1,0 +1,138 @@
+// gr_rotary.hip -- prebuilt instances of the position rotation (gr_rotary.h)
+// behind gr_rotary() and gr_paged_append().
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "gr_host.h"
+#include "gr_paged_host.h"
+#include "gr_rotary.h"
+#include "grammar_rt.h"
+
+namespace {
+
+template <class T, bool APPEND, bool INTER, int ITER>
+__global__ __launch_bounds__(256) void gr_rope_kernel(gr_rope_args a, int inverse) {
+  gr_rope_body<T, APPEND, INTER, ITER>(a, inverse != 0);
+}
+
+template <class T, bool APPEND, bool INTER>
+int launch(const gr_rope_args& a, int inverse, const char* who, hipStream_t st) {
+  const int rows = a.q.heads + a.k.heads + a.v.heads;
+  const int rpp = 64 / (a.D / 16), passes = (rows + rpp - 1) / rpp;
+  // As many passes to a wave as leave every CU 8 waves, at most 4
+  const long long full = (long long)a.tokens * passes;
+  const int cus = gr::cu_count() > 0 ? gr::cu_count() : 256;
+  const int iter = passes >= 4 && full >= 32LL * cus ? 4 : passes >= 2 && full >= 16LL * cus ? 2 : 1;
+  const long long waves = (long long)a.tokens * ((passes + iter - 1) / iter);
+  if (waves > 0x7fffffffLL / 64) return gr::fail(GR_E_ARG, "%s: %d tokens of %d head rows are too many for one call", who, a.tokens, rows);
+  const dim3 grid((unsigned)((waves + 3) / 4));
+  if (iter == 4) hipLaunchKernelGGL((gr_rope_kernel<T, APPEND, INTER, 4>), grid, dim3(256), 0, st, a, inverse);
+  else if (iter == 2) hipLaunchKernelGGL((gr_rope_kernel<T, APPEND, INTER, 2>), grid, dim3(256), 0, st, a, inverse);
+  else hipLaunchKernelGGL((gr_rope_kernel<T, APPEND, INTER, 1>), grid, dim3(256), 0, st, a, inverse);
+  return gr::hip_check(hipGetLastError(), GR_E_LAUNCH, who);
+}
+
+template <class T, bool APPEND>
+int launch_inter(const gr_rope_args& a, bool inter, int inverse, const char* who, hipStream_t st) {
+  return inter ? launch<T, APPEND, true>(a, inverse, who, st) : launch<T, APPEND, false>(a, inverse, who, st);
+}
+
+// The rotation's own arguments: head_dim a multiple of 16 up to 256, at most 8 axes.
+int take_rotary(gr_rope_args& a, const gr_rotary_spec* r, const char* who) {
+  if (!r->turns || ((uintptr_t)r->turns & 7)) return gr::fail(GR_E_ARG, "%s: the rotation's turns must be an 8-byte aligned buffer", who);
+  if (r->head_dim < 16 || r->head_dim > 256 || r->head_dim % 16)
+    return gr::fail(GR_E_ARG, "%s: head dim %d unsupported (a multiple of 16 up to 256)", who, r->head_dim);
+  if (r->pairs < 8 || r->pairs % 8 || 2 * r->pairs > r->head_dim)
+    return gr::fail(GR_E_ARG, "%s: %d rotated pairs unsupported (a multiple of 8, at most half the head dim)", who, r->pairs);
+  if (r->naxes < 1 || r->naxes > 8) return gr::fail(GR_E_ARG, "%s: %d position axes unsupported (1 to 8)", who, r->naxes);
+  if (r->naxes > 1 && (!r->axes || ((uintptr_t)r->axes & 7)))
+    return gr::fail(GR_E_ARG, "%s: the pairs' axes must be an 8-byte aligned buffer", who);
+  a.D = r->head_dim;
+  a.pairs = r->pairs;
+  a.naxes = r->naxes;
+  a.turns = reinterpret_cast<const unsigned long long*>(r->turns);
+  a.axes = r->axes;
+  return GR_OK;
+}
+
+int take_rows(gr_rope_rows& k, const void* src, void* dst, int heads, const long long* ss, const long long* ds,
+              const char* name, const char* who) {
+  if (!src || !dst || !ss || !ds) return gr::fail(GR_E_ARG, "%s: null argument (%s)", who, name);
+  if (heads <= 0) return gr::fail(GR_E_ARG, "%s: %s needs at least one head", who, name);
+  if (!gr::aligned16(src) || !gr::aligned16(dst)) return gr::fail(GR_E_ARG, "%s: base pointers must be 16-byte aligned (%s)", who, name);
+  for (int i = 0; i < 3; ++i)
+    if (ss[i] < 0 || ss[i] % 8 || ds[i] < 0 || ds[i] % 8)
+      return gr::fail(GR_E_ARG, "%s: strides must be non-negative multiples of 8 elements (%s)", who, name);
+  k = {src, dst, ss[0], ss[1], ss[2], ds[0], ds[1], ds[2], heads};
+  return GR_OK;
+}
+
+}  // namespace
+
+extern "C" int gr_rotary(const gr_rotary_spec* rotary, const void* q, void* q_out, int Hq, const long long* q_strides,
+                         const long long* q_out_strides, const void* k, void* k_out, int Hk, const long long* k_strides,
+                         const long long* k_out_strides, int dtype, int B, int N, const int* positions,
+                         const long long* position_strides, int inverse, void* stream) {
+  const char* const who = "gr_rotary";
+  if (!rotary || !positions || !position_strides) return gr::fail(GR_E_ARG, "gr_rotary: null argument");
+  if (B <= 0 || N <= 0 || (long long)B * N > 0x7fffffffLL) return gr::fail(GR_E_ARG, "gr_rotary: B and N must be positive, B N below 2^31");
+  gr_rope_args a = {};
+  int rc = take_rotary(a, rotary, who);
+  if (rc) return rc;
+  if ((rc = take_rows(a.q, q, q_out, Hq, q_strides, q_out_strides, "q", who))) return rc;
+  if (k && (rc = take_rows(a.k, k, k_out, Hk, k_strides, k_out_strides, "k", who))) return rc;
+  a.tokens = B * N;
+  a.per_seq = N;
+  a.pos = positions;
+  for (int i = 0; i < 3; ++i) a.ps[i] = position_strides[i];
+  hipStream_t st = (hipStream_t)stream;
+  const bool inter = rotary->interleaved != 0;
+  if (dtype == GR_F16) return launch_inter<_Float16, false>(a, inter, inverse, who, st);
+  if (dtype == GR_BF16) return launch_inter<__bf16, false>(a, inter, inverse, who, st);
+  if (dtype == GR_F32) return launch_inter<float, false>(a, inter, inverse, who, st);
+  return gr::fail(GR_E_ARG, "gr_rotary: dtype %d unsupported (GR_F16, GR_BF16 or GR_F32)", dtype);
+}
+
+extern "C" int gr_paged_append(const gr_paged_cache* cache, const gr_paged_batch* batch, const gr_rotary_spec* rotary,
+                               const void* q, void* q_out, int Hq, const long long* q_strides,
+                               const long long* q_out_strides, const void* k, const void* v,
+                               const long long* k_strides, const long long* v_strides, const int* positions,
+                               const long long* position_strides, void* stream) {
+  const char* const who = "gr_paged_append";
+  gr_rope_args a = {};
+  int rc = gr::check_paged(cache, batch, who);
+  if (rc) return rc;
+  if (batch->rows == 0) return GR_OK;
+  if (!k || !v || (positions && !position_strides)) return gr::fail(GR_E_ARG, "gr_paged_append: null argument");
+  const gr_rotary_spec none = {nullptr, nullptr, 0, 1, cache->head_dim, 0};
+  const gr_rotary_spec* r = rotary ? rotary : &none;
+  if (rotary && (rc = take_rotary(a, rotary, who))) return rc;
+  if (r->head_dim != cache->head_dim)
+    return gr::fail(GR_E_ARG, "gr_paged_append: the rotation's head dim %d is not the cache's %d", r->head_dim, cache->head_dim);
+  a.D = cache->head_dim;
+  a.naxes = r->naxes;
+  if (q && (rc = take_rows(a.q, q, q_out, Hq, q_strides, q_out_strides, "q", who))) return rc;
+  // a cache's strides are {page, head, slot}
+  const long long kd[3] = {cache->k_strides[0], cache->k_strides[2], cache->k_strides[1]};
+  const long long vd[3] = {cache->v_strides[0], cache->v_strides[2], cache->v_strides[1]};
+  if ((rc = take_rows(a.k, k, cache->k, cache->heads, k_strides, kd, "k", who))) return rc;
+  if ((rc = take_rows(a.v, v, cache->v, cache->heads, v_strides, vd, "v", who))) return rc;
+  a.tokens = batch->starts ? batch->rows : batch->B * batch->rows;
+  a.per_seq = batch->starts ? 1 : batch->rows;
+  a.pos = positions;
+  if (positions)
+    for (int i = 0; i < 3; ++i) a.ps[i] = position_strides[i];
+  a.table = batch->table;
+  a.table_stride = batch->table_stride;
+  a.width = batch->width;
+  a.pages = cache->pages;
+  a.page_shift = gr::page_shift(cache->page_size);
+  a.B = batch->B;
+  a.lens = batch->lens;
+  a.starts = batch->starts;
+  hipStream_t st = (hipStream_t)stream;
+  const bool inter = r->interleaved != 0;
+  if (cache->dtype == GR_F16) return launch_inter<_Float16, true>(a, inter, 0, who, st);
+  return launch_inter<__bf16, true>(a, inter, 0, who, st);
+}

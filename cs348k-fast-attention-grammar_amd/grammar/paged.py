@@ -1,0 +1,210 @@
+"""Python face of the paged key/value cache: appending new tokens
+(gr_paged_append) and attention over what is cached (gr_paged_attn).
+
+A `PagedCache` is two tensors of pages, [pages, heads, page_size, D]. A batch of
+sequences is described by three int32 tensors on the GPU: `table` [B, width],
+each sequence's page ids in order; `lens` [B], its keys, the new tokens' among
+them; and for packed batches `starts` [B + 1], the first row of each sequence's
+new tokens. New token i of n stands at position len - n + i. Uniform batches
+are [B, heads, n, D] like the framework's other attention calls, packed ones
+[rows, heads, D]; rows of a packed batch that belong to no sequence are neither
+read nor written. A decode step is paged_append and paged_attention with n = 1,
+a prompt the same two calls with its tokens, whole or in chunks, and both may
+share a packed batch. The reference has no cache (its attention takes as many
+keys as queries, run_attention_search.py:34-114).
+
+Lengths, starts and page ids are read on the GPU, so one bound or captured call
+serves every step. What lies outside of the cache or the table is not touched:
+such keys do not exist. There is no CPU path: CPU tensors or a missing library
+raise.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+from . import runtime as rt
+from .rotary import Rotary, _pair, check_out, check_positions, head_strides
+
+
+class PagedCache:
+    """Key and value pages: tensors [pages, heads, page_size, D] of one shape,
+    fp16 or bf16, D 64 or 128, page_size a power of two from 16 on, unit stride
+    along D, other strides multiples of 8 (so [pages, page_size, heads, D]
+    storage serves, transposed)."""
+
+    def __init__(self, k, v):
+        for name, t in (("k", k), ("v", v)):
+            if not t.is_cuda:
+                raise ValueError(f"PagedCache: {name} must be a GPU tensor (no CPU path)")
+            if t.dim() != 4 or t.shape != k.shape or t.dtype != k.dtype or t.device != k.device or t.stride(3) != 1:
+                raise ValueError("PagedCache: k and v must be [pages, heads, page_size, D] of one shape, dtype and "
+                                 "device with unit stride on D")
+        pages, heads, size, D = k.shape
+        if rt.dtype_code(k.dtype) == rt.GR_F32:
+            raise ValueError("PagedCache: fp16 or bf16")
+        if D not in (64, 128) or size < 16 or size & (size - 1) or size > 1 << 20:
+            raise ValueError(f"PagedCache: D {D} must be 64 or 128 and page_size {size} a power of two from 16 to 2^20")
+        self.k, self.v = k, v
+        self.pages, self.heads, self.page_size, self.head_dim = pages, heads, size, D
+        self.desc = rt.PagedCacheDesc(k.data_ptr(), v.data_ptr(), rt._ll3(*k.stride()[:3]), rt._ll3(*v.stride()[:3]),
+                                      rt.dtype_code(k.dtype), pages, heads, size, D)
+        self.ref = ctypes.addressof(self.desc)
+
+    @classmethod
+    def empty(cls, pages: int, heads: int, page_size: int, head_dim: int, dtype, device="cuda"):
+        """A cache of unwritten pages (their contents are never read before
+        they are appended to)."""
+        import torch
+        shape = (pages, heads, page_size, head_dim)
+        return cls(torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device))
+
+
+def _batch(cache, table, lens, starts, x, name, max_new, max_len, who):
+    """(gr_paged_batch, leading sizes of the tokens) of a call on `x`: [B, heads,
+    n, D] or, with starts, [rows, heads, D]."""
+    import torch
+    dev = cache.k.device
+    for n, t, dim in (("table", table, 2), ("lens", lens, 1), ("starts", starts, 1)):
+        if t is None and n == "starts":
+            continue
+        if t.dtype != torch.int32 or t.dim() != dim or t.device != dev or (t.shape[dim - 1] > 1 and t.stride(dim - 1) != 1):
+            raise ValueError(f"{who}: {n} must be a {dim}-D int32 tensor on {dev} with unit stride")
+    B, width = table.shape
+    if lens.shape[0] != B or B == 0 or width == 0:
+        raise ValueError(f"{who}: table {tuple(table.shape)} and lens {tuple(lens.shape)} do not describe a batch")
+    if starts is None:
+        if x.dim() != 4 or x.shape[0] != B:
+            raise ValueError(f"{who}: {name} must be [{B}, heads, n, D] (packed rows need starts)")
+        lead = (B, x.shape[2])
+    else:
+        if x.dim() != 3 or starts.shape[0] != B + 1:
+            raise ValueError(f"{who}: with starts [{B + 1}], {name} must be packed [rows, heads, D]")
+        lead = (x.shape[0],)
+    return rt.PagedBatch(table.data_ptr(), table.stride(0), lens.data_ptr(), starts.data_ptr() if starts is not None else None,
+                         B, lead[-1], width, int(max_new), int(max_len)), lead
+
+
+def _heads_ok(t, name, lead, heads, cache, who):
+    if not t.is_cuda:
+        raise ValueError(f"{who}: {name} must be a GPU tensor (no CPU path)")
+    want = (lead[0], heads, lead[1], cache.head_dim) if len(lead) == 2 else (lead[0], heads, cache.head_dim)
+    if tuple(t.shape) != want or t.dtype != cache.k.dtype or t.device != cache.k.device:
+        raise ValueError(f"{who}: {name} must be {want} of the cache's dtype and device, not {tuple(t.shape)} {t.dtype}")
+
+
+def _append_args(k, v, cache, table, lens, starts, q, rotary, positions, max_new, out):
+    who = "paged_append"
+    desc, lead = _batch(cache, table, lens, starts, k, "k", max_new, 0, who)
+    _heads_ok(k, "k", lead, cache.heads, cache, who)
+    _heads_ok(v, "v", lead, cache.heads, cache, who)
+    head = (cache.ref, ctypes.addressof(desc), rotary.ref if rotary is not None else None)
+    if rotary is not None and (rotary.head_dim != cache.head_dim or rotary.device != cache.k.device):
+        raise ValueError(f"{who}: the rotation is for heads of {rotary.head_dim} on {rotary.device}")
+    if q is None:
+        if out is not None:
+            raise ValueError(f"{who}: `out` is the queries' and needs q")
+        head += (None, None, 0, None, None)
+    else:
+        if rotary is None:
+            raise ValueError(f"{who}: q is only rotated here, which needs `rotary`")
+        Hq = q.shape[1] if q.dim() >= 3 else 0
+        _heads_ok(q, "q", lead, Hq, cache, who)
+        out = check_out(out, q, "out", who)
+        head += (q.data_ptr(), out.data_ptr(), Hq, head_strides(q, "q", who), head_strides(out, "out", who))
+    if positions is None:
+        place = (None, None)
+    else:
+        if rotary is None:
+            raise ValueError(f"{who}: positions need `rotary`")
+        place = (positions.data_ptr(), check_positions(positions, rotary, lead, who))
+    args = head + (k.data_ptr(), v.data_ptr(), head_strides(k, "k", who), head_strides(v, "v", who)) + place
+    return args, out, (desc, k, v, cache, table, lens, starts, q, rotary, positions, out)
+
+
+def paged_append(k, v, cache: PagedCache, table, lens, *, starts=None, q=None, rotary: Rotary | None = None,
+                 positions=None, max_new: int = 0, out=None, stream=None):
+    """Puts the new tokens' keys and values into their pages, in one launch.
+
+    k, v: [B, heads, n, D], or [rows, heads, D] with `starts`; any strides that
+    are multiples of 8, unit on D (slices of a projection's output serve).
+    rotary: a `Rotary` that turns the keys on the way, and q ([.., Hq, .., D]) if
+    given, into a new tensor laid out as q or into `out` (which may be q).
+    positions: int32, [B, n], [n] or (packed) [rows], with several axes led by
+    them; default: each token's place len - n + i, on every axis.
+    Returns the rotated queries, or None without q. A token whose place is
+    outside of the table or on a page id outside of the cache is not stored.
+    max_new: the most new tokens of a sequence, where known."""
+    args, out, keep = _append_args(k, v, cache, table, lens, starts, q, rotary, positions, max_new, out)
+    with rt.on_device(k):
+        rt.check(rt.lib().gr_paged_append(*args, rt._stream_ptr(stream)), "gr_paged_append")
+    return out
+
+
+def bind_paged_append(k, v, cache: PagedCache, table, lens, *, starts=None, q=None, rotary: Rotary | None = None,
+                      positions=None, max_new: int = 0, out=None, stream=None):
+    """Validate once and return (launch, out): launch() enqueues gr_paged_append
+    on these tensors with pre-packed arguments; arguments as paged_append."""
+    args, out, keep = _append_args(k, v, cache, table, lens, starts, q, rotary, positions, max_new, out)
+    return rt.launcher(rt.lib().gr_paged_append, args, k, stream, "gr_paged_append", out, keep), out
+
+
+def _attn_args(q, cache, table, lens, starts, causal, scale, max_new, max_len, out, lse, workspace, stream):
+    import torch
+    who = "paged_attention"
+    desc, lead = _batch(cache, table, lens, starts, q, "q", max_new, max_len, who)
+    Hq = q.shape[1]
+    _heads_ok(q, "q", lead, Hq, cache, who)
+    if Hq == 0 or Hq % cache.heads:
+        raise ValueError(f"{who}: {Hq} query heads are not a multiple of the cache's {cache.heads}")
+    out = check_out(out, q, "out", who)
+    if lse is not None:
+        want = (lead[0], lead[1], Hq) if len(lead) == 2 else (lead[0], Hq)
+        if tuple(lse.shape) != want or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != q.device:
+            raise ValueError(f"{who}: lse must be a contiguous {want} float32 tensor")
+    if scale is None:
+        scale = 1.0 / math.sqrt(cache.head_dim)
+    ref = ctypes.addressof(desc)
+    need = int(rt.lib().gr_paged_attn_workspace(cache.ref, ref, Hq))
+    if need and workspace is None:
+        workspace = rt.workspace(need, q.device, stream)
+    size = workspace.numel() * workspace.element_size() if workspace is not None else 0
+    args = (cache.ref, ref, q.data_ptr(), out.data_ptr(), lse.data_ptr() if lse is not None else None, Hq,
+            head_strides(q, "q", who), head_strides(out, "out", who), int(bool(causal)), float(scale),
+            workspace.data_ptr() if workspace is not None else None, size)
+    return args, out, (desc, q, cache, table, lens, starts, out, lse, workspace)
+
+
+def paged_attention(q, cache: PagedCache, table, lens, *, starts=None, causal: bool = True, scale: float | None = None,
+                    max_new: int = 0, max_len: int = 0, out=None, lse=None, workspace=None, stream=None):
+    """O = softmax(scale * Q K^T) V of the new tokens over the cached keys.
+
+    q: [B, Hq, n, D], or [rows, Hq, D] with `starts`; Hq a multiple of the
+    cache's heads, query head h reading key head h // (Hq / heads). Token i
+    of n sees the keys up to its own place len - n + i (causal=True) or all len
+    keys. A row that sees none gets 0.
+    max_new, max_len: the most new tokens and keys of a sequence, where known;
+    they only choose how the work is shared out.
+    lse: float32 [B, n, Hq] or [rows, Hq] to receive the log-sum-exp of the scaled
+    scores (natural log). workspace: device memory for calls whose keys are
+    shared out (allocated here unless given; rt.lib().gr_paged_attn_workspace
+    names the size; with less the keys are shared out less).
+    Returns the result, laid out as q, or `out`."""
+    args, out, keep = _attn_args(q, cache, table, lens, starts, causal, scale, max_new, max_len, out, lse, workspace,
+                                 stream)
+    with rt.on_device(q):
+        rt.check(rt.lib().gr_paged_attn(*args, rt._stream_ptr(stream)), "gr_paged_attn")
+    return out
+
+
+def bind_paged_attention(q, cache: PagedCache, table, lens, *, starts=None, causal: bool = True,
+                         scale: float | None = None, max_new: int = 0, max_len: int = 0, out=None, lse=None,
+                         workspace=None, stream=None):
+    """Validate once and return (launch, out): launch() enqueues gr_paged_attn on
+    these tensors with pre-packed arguments and the workspace allocated here, for
+    loops on fixed buffers; arguments as paged_attention. Launches of one binding
+    share its workspace: those that may overlap in time (two streams, two
+    captured graphs) need bindings of their own."""
+    args, out, keep = _attn_args(q, cache, table, lens, starts, causal, scale, max_new, max_len, out, lse, workspace,
+                                 stream)
+    return rt.launcher(rt.lib().gr_paged_attn, args, q, stream, "gr_paged_attn", out, keep), out

@@ -1,0 +1,193 @@
+"""Python face of the position rotation of queries and keys (gr_rotary).
+
+`rotary(q, k, positions, rot)` turns the pairs of every head by position times
+frequency, differentiably; `rotary_fwd` is the launch alone, for callers that
+give the output tensors. `Rotary` holds what a model fixes once: which elements
+of a head form pairs, their frequencies and, for images and video, which
+position axis (time, height, width) each pair turns with. The reference has no
+positions; its attention (run_attention_search.py:34-114) is what the rotated
+heads go to.
+
+There is no CPU path: CPU tensors or a missing library raise.
+"""
+from __future__ import annotations
+
+import ctypes
+import functools
+import math
+
+from . import runtime as rt
+
+_pair = functools.lru_cache(maxsize=1024)(lambda *s: (ctypes.c_longlong * len(s))(*s))
+
+
+class Rotary:
+    """The rotation of heads of `head_dim` elements.
+
+    rotary_dim: the first elements of a head that are rotated (a multiple of
+    16; default: all). Pair j is elements j and j + rotary_dim / 2, or 2j and
+    2j + 1 with interleaved=True.
+    sections: how many pairs turn with each position axis, in order (default:
+    all with one axis; at most 8 axes).
+    Frequencies, radians a position: base ** (-j / pairs) for pair j of all
+    pairs, or with per_axis=True base ** (-j / n) for pair j of the n of an axis;
+    inv_freq (one number a pair) replaces them.
+    device: where the tables of this object live (one object a GPU)."""
+
+    def __init__(self, head_dim: int, *, rotary_dim: int | None = None, base: float = 10000.0, sections=None,
+                 per_axis: bool = False, interleaved: bool = False, inv_freq=None, device="cuda"):
+        import torch
+        rd = head_dim if rotary_dim is None else int(rotary_dim)
+        if head_dim % 16 or not 16 <= head_dim <= 256:
+            raise ValueError(f"Rotary: head_dim {head_dim} must be a multiple of 16 up to 256")
+        if rd % 16 or not 16 <= rd <= head_dim:
+            raise ValueError(f"Rotary: rotary_dim {rd} must be a multiple of 16 up to head_dim {head_dim}")
+        pairs = rd // 2
+        sections = [pairs] if sections is None else [int(s) for s in sections]
+        if not 1 <= len(sections) <= 8 or min(sections) < 0 or sum(sections) != pairs:
+            raise ValueError(f"Rotary: sections {sections} must be 1 to 8 counts that sum to the {pairs} pairs")
+        axes = [a for a, n in enumerate(sections) for _ in range(n)]
+        if inv_freq is None:
+            if not base > 0:
+                raise ValueError(f"Rotary: base {base} must be positive")
+            place = [j / n for n in sections for j in range(n)] if per_axis else [j / pairs for j in range(pairs)]
+            freqs = [float(base) ** -x for x in place]
+        else:
+            freqs = [float(f) for f in (inv_freq.tolist() if hasattr(inv_freq, "tolist") else inv_freq)]
+            if len(freqs) != pairs or not all(math.isfinite(f) for f in freqs):
+                raise ValueError(f"Rotary: inv_freq must be {pairs} finite numbers")
+        self.head_dim, self.rotary_dim, self.interleaved = int(head_dim), rd, bool(interleaved)
+        self.sections, self.naxes = tuple(sections), len(sections)
+        self.inv_freq = tuple(freqs)
+        # turns a position, modulo one, as whole numbers of 2^-64 (two's complement)
+        whole = [round(math.ldexp((f / (2 * math.pi)) % 1.0, 64)) % (1 << 64) for f in freqs]
+        self.turns = torch.tensor([w - (1 << 64) if w >> 63 else w for w in whole], dtype=torch.int64, device=device)
+        self.axes = torch.tensor(axes, dtype=torch.uint8, device=device)
+        self.device = self.turns.device
+        self.desc = rt.RotarySpec(self.turns.data_ptr(), self.axes.data_ptr(), pairs, self.naxes, self.head_dim,
+                                  int(self.interleaved))
+        self.ref = ctypes.addressof(self.desc)
+
+
+def check_positions(positions, rot, lead: tuple, who: str):
+    """The strides {axis, batch, token} of int32 `positions`: [*lead] or, with
+    several axes, [axes, *lead]; a batch of positions may be left out."""
+    import torch
+    if positions.dtype != torch.int32 or positions.device != rot.device:
+        raise ValueError(f"{who}: positions must be an int32 tensor on {rot.device}")
+    shape, st = tuple(positions.shape), positions.stride()
+    if rot.naxes > 1:
+        if shape[:1] != (rot.naxes,):
+            raise ValueError(f"{who}: positions {shape} must lead with the {rot.naxes} axes")
+        axis, shape, st = st[0], shape[1:], st[1:]
+    else:
+        axis = 0
+    if shape == lead:
+        return _pair(axis, *((0,) * (2 - len(st))), *st)
+    if len(lead) == 2 and shape == lead[1:]:
+        return _pair(axis, 0, st[0])
+    raise ValueError(f"{who}: positions {tuple(positions.shape)} do not match the tokens {lead}")
+
+
+def head_strides(t, name: str, who: str):
+    """{batch, token, head} strides of [B, H, N, D] or packed [T, H, D] heads."""
+    if t.stride(-1) != 1:
+        raise ValueError(f"{who}: {name} must have unit stride on its last dimension")
+    st = [s if n > 1 else 0 for s, n in zip(t.stride(), t.shape)]      # a single row's stride says nothing
+    return _pair(st[0], st[2], st[1]) if len(st) == 4 else _pair(0, st[0], st[1])
+
+
+def check_out(out, like, name: str, who: str):
+    """`out`, checked, or a new tensor laid out as `like`."""
+    import torch
+    if out is None:
+        return torch.empty_like(like)
+    if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device:
+        raise ValueError(f"{who}: bad `{name}` tensor")
+    return out
+
+
+def rotary_fwd(q, k, positions, rot: Rotary, *, inverse: bool = False, out=None, k_out=None, stream=None):
+    """q [B, Hq, N, D] and k [B, Hk, N, D] (or None) rotated to `positions`: int32,
+    [N] or [B, N], with several axes [axes, N] or [axes, B, N]. fp16, bf16 or
+    fp32 on the GPU, any strides that are multiples of 8 with a unit one on D.
+    Returns (q', k'), new tensors laid out as the given ones, or `out` and
+    `k_out`, which may be q and k themselves. inverse=True rotates back."""
+    who = "rotary"
+    for name, t in (("q", q), ("k", k)):
+        if t is None:
+            if name == "k":
+                continue
+            raise ValueError(f"{who}: q must be given")
+        if not t.is_cuda:
+            raise ValueError(f"{who}: {name} must be a GPU tensor (no CPU path)")
+        if t.dim() != 4 or t.shape[3] != rot.head_dim or t.dtype != q.dtype or t.device != rot.device:
+            raise ValueError(f"{who}: {name} must be [B, H, N, {rot.head_dim}] of q's dtype on {rot.device}")
+    B, Hq, N, _ = q.shape
+    if k is not None and (k.shape[0] != B or k.shape[2] != N):
+        raise ValueError(f"{who}: k {tuple(k.shape)} does not match q {tuple(q.shape)}")
+    ps = check_positions(positions, rot, (B, N), who)
+    out = check_out(out, q, "out", who)
+    if k is not None:
+        k_out = check_out(k_out, k, "k_out", who)
+    if B == 0 or N == 0:
+        return out, k_out
+    args = (rot.ref, q.data_ptr(), out.data_ptr(), Hq, head_strides(q, "q", who), head_strides(out, "out", who))
+    if k is None:
+        args += (None, None, 0, None, None)
+    else:
+        args += (k.data_ptr(), k_out.data_ptr(), k.shape[1], head_strides(k, "k", who), head_strides(k_out, "k_out", who))
+    with rt.on_device(q):
+        rt.check(rt.lib().gr_rotary(*args, rt.dtype_code(q.dtype), B, N, positions.data_ptr(), ps, int(bool(inverse)),
+                                    rt._stream_ptr(stream)), "gr_rotary")
+    return out, k_out
+
+
+def _dense(t):
+    """t with strides the kernels take: itself, or a contiguous copy (the
+    gradient of a sum is a broadcast one, of a slice a strided one)."""
+    import torch
+    st = t.stride()
+    ok = st[3] == 1 and t.data_ptr() % 16 == 0 and all(n == 1 or (s > 0 and s % 8 == 0) for s, n in zip(st, t.shape[:3]))
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def _autograd_function():
+    import torch
+
+    class RotaryFunction(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, q, k, positions, rot, inverse):
+            ctx.set_materialize_grads(False)
+            ctx.save_for_backward(positions)
+            ctx.rot, ctx.inverse = rot, inverse
+            return rotary_fwd(_dense(q), None if k is None else _dense(k), positions, rot, inverse=inverse)
+
+        @staticmethod
+        def backward(ctx, dq, dk):
+            # a rotation's gradient is the rotation back, of the queries' and
+            # the keys' gradients in one launch where both came
+            positions, = ctx.saved_tensors
+            dq = dq if ctx.needs_input_grad[0] else None
+            dk = dk if ctx.needs_input_grad[1] else None
+            if dq is None and dk is None:
+                return None, None, None, None, None
+            apply = RotaryFunction.apply
+            if dq is None:
+                return None, apply(dk, None, positions, ctx.rot, not ctx.inverse)[0], None, None, None
+            dq, dk = apply(dq, dk, positions, ctx.rot, not ctx.inverse)
+            return dq, dk, None, None, None
+    return RotaryFunction
+
+
+_ROTARY_FN = None
+
+
+def rotary(q, k, positions, rot: Rotary):
+    """rotary_fwd, differentiable in q and k (either may need no gradient; k
+    may be None): both rotations are one launch of gr_rotary, and so are their
+    gradients."""
+    global _ROTARY_FN
+    if _ROTARY_FN is None:
+        _ROTARY_FN = _autograd_function()
+    return _ROTARY_FN.apply(q, k, positions, rot, False)

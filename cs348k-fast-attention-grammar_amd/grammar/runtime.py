@@ -10,6 +10,7 @@ loading fails loudly otherwise -- there is no CPU fallback on this path.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import os
@@ -125,8 +126,34 @@ def lib() -> ctypes.CDLL:
                                      ctypes.c_float, i32, vp, ctypes.c_size_t, vp]
         L.gr_attn_decode_noalloc.argtypes = [vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, _ll3, _ll3, _ll3, _ll3,
                                              ctypes.c_float, i32, vp]
+        pll = ctypes.POINTER(ctypes.c_longlong)
+        L.gr_rotary.argtypes = [vp, vp, vp, i32, pll, pll, vp, vp, i32, pll, pll, i32, i32, i32, vp, pll, i32, vp]
+        L.gr_paged_append.argtypes = [vp, vp, vp, vp, vp, i32, pll, pll, vp, vp, pll, pll, vp, pll, vp]
+        L.gr_paged_attn_workspace.argtypes = [vp, vp, i32]
+        L.gr_paged_attn_workspace.restype = sz
+        L.gr_paged_attn.argtypes = [vp, vp, vp, vp, vp, i32, pll, pll, i32, ctypes.c_float, vp, sz, vp]
         _lib = L
         return L
+
+
+class RotarySpec(ctypes.Structure):
+    """gr_rotary_spec."""
+    _fields_ = [("turns", ctypes.c_void_p), ("axes", ctypes.c_void_p), ("pairs", ctypes.c_int),
+                ("naxes", ctypes.c_int), ("head_dim", ctypes.c_int), ("interleaved", ctypes.c_int)]
+
+
+class PagedCacheDesc(ctypes.Structure):
+    """gr_paged_cache."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_strides", _ll3), ("v_strides", _ll3),
+                ("dtype", ctypes.c_int), ("pages", ctypes.c_int), ("heads", ctypes.c_int),
+                ("page_size", ctypes.c_int), ("head_dim", ctypes.c_int)]
+
+
+class PagedBatch(ctypes.Structure):
+    """gr_paged_batch."""
+    _fields_ = [("table", ctypes.c_void_p), ("table_stride", ctypes.c_longlong), ("lens", ctypes.c_void_p),
+                ("starts", ctypes.c_void_p), ("B", ctypes.c_int), ("rows", ctypes.c_int), ("width", ctypes.c_int),
+                ("max_new", ctypes.c_int), ("max_len", ctypes.c_int)]
 
 
 # Every symbol the C header declares; tests check the library exports them all.
@@ -138,6 +165,7 @@ EXPORTED = (
     "gr_attn_fwd_train", "gr_attn_bwd_workspace", "gr_attn_bwd", "gr_attn_decode_noalloc",
     "gr_plan_run_args", "gr_gemm_workspace", "gr_gemm_ws", "gr_mlp_fwd_workspace", "gr_mlp_fwd_ws",
     "gr_selftest_f32_no_workspace", "gr_attn_fwd_shape", "gr_gemm_f32_groups",
+    "gr_rotary", "gr_paged_append", "gr_paged_attn_workspace", "gr_paged_attn",
 )
 
 # Bytes of the per-device scratch array behind gr_attn_decode_noalloc (GR_DECODE_SCRATCH_BYTES).
@@ -248,6 +276,31 @@ def torch_stream(stream, device):
     if handle == 0:                  # ExternalStream(0) would be a new stream of torch's pool
         return torch.cuda.default_stream(device)
     return torch.cuda.ExternalStream(handle, device=device)
+
+
+def on_device(t):
+    """Context in which the device of tensor `t` is the current one: launches
+    go to the current device, and a call's current stream is that device's."""
+    import torch
+    dev = t.device.index
+    return _NO_CHANGE if dev == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+_NO_CHANGE = contextlib.nullcontext()
+
+
+def launcher(fn, args: tuple, t, stream, what: str, out, keep):
+    """launch() that calls the C entry `fn` with `args` and the handle of `stream`
+    (the current stream of t's device if None), holding `keep` (the tensors and
+    structures that the arguments point to) as long as it lives; returns `out`."""
+    with on_device(t):
+        args += (_stream_ptr(stream),)
+
+    def launch(_keep=keep):
+        with on_device(t):
+            check(fn(*args), what)
+        return out
+    return launch
 
 
 _STREAM_PER_THREAD = 2               # hipStreamPerThread

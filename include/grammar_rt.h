@@ -225,6 +225,97 @@ int gr_attn_decode_noalloc(const void* q, const void* k, const void* v, void* o,
                            const long long* v_strides, const long long* o_strides, float scale, int splits,
                            void* stream);
 
+/* ---- positions and paged caches ------------------------------------------ */
+
+/* The rotation of queries and keys by position. No counterpart in the reference,
+ * whose attention has no positions. Pair j of a head, (x1, x2), becomes
+ * (x1 cos t - x2 sin t, x1 sin t + x2 cos t), t = position x (frequency of j).
+ *  turns: device array, per pair the frequency in units of 2^-64 turns a
+ *         position (radians / 2 pi, modulo one turn); 8-byte aligned.
+ *  axes:  device array, per pair the position axis it turns with; 8-byte
+ *         aligned; not read with naxes 1. naxes: 1 to 8.
+ *  pairs: a multiple of 8, at most head_dim / 2; the first 2 pairs elements of a
+ *         head are rotated, the others pass. head_dim: a multiple of 16 up to 256.
+ *  interleaved: pair j is elements 2j and 2j + 1, else j and j + pairs. */
+typedef struct gr_rotary_spec {
+  const uint64_t* turns;
+  const uint8_t* axes;
+  int pairs, naxes, head_dim, interleaved;
+} gr_rotary_spec;
+
+/* Rotates q [B, Hq, N, D] into q_out and, if k is not NULL, k [B, Hk, N, D] into
+ * k_out (each may be its own input: the call then works in place).
+ *  Strides {batch, token, head} in elements, non-negative multiples of 8, unit
+ *  stride along D; base pointers 16-byte aligned. dtype GR_F16, GR_BF16 (angles,
+ *  products and sums in fp32, rounded once) or GR_F32.
+ *  positions: int32, any sign; position_strides = {axis, batch, token}.
+ *  inverse != 0 rotates by -t, which is also the gradient's way back. */
+int gr_rotary(const gr_rotary_spec* rotary, const void* q, void* q_out, int Hq, const long long* q_strides,
+              const long long* q_out_strides, const void* k, void* k_out, int Hk, const long long* k_strides,
+              const long long* k_out_strides, int dtype, int B, int N, const int* positions,
+              const long long* position_strides, int inverse, void* stream);
+
+/* A key/value cache in pages. No counterpart in the reference. k and v:
+ * [pages][heads][page_size][head_dim] by strides {page, head, slot} in elements
+ * (non-negative multiples of 8, unit stride along head_dim, the slot stride below
+ * 2^26), 16-byte aligned; dtype GR_F16 or GR_BF16; head_dim 64 or 128; page_size
+ * a power of two from 16 to 2^20. */
+typedef struct gr_paged_cache {
+  void* k;
+  void* v;
+  long long k_strides[3], v_strides[3];
+  int dtype, pages, heads, page_size, head_dim;
+} gr_paged_cache;
+
+/* The sequences of a call; the arrays are int32 in device memory.
+ *  table:  [B][width] page ids by row stride table_stride: key j of sequence b is
+ *          slot j % page_size of page table[b][j / page_size].
+ *  lens:   [B] keys of each sequence, the new tokens' among them: new token i
+ *          of n stands at position len - n + i.
+ *  starts: [B + 1] first row of each sequence's new tokens in a packed batch of
+ *          `rows` tokens, rows outside of every sequence being left alone; or
+ *          NULL for a uniform batch of `rows` new tokens a sequence.
+ *  max_new, max_len: the most new tokens and keys of a sequence, where known (0:
+ *          not). They only choose how a call is shared out.
+ * What the arrays hold is bounded on the device: a page id outside of the cache,
+ * a position outside of the table or a start outside of the batch reads and
+ * writes nothing (such keys do not exist, such tokens are not stored). */
+typedef struct gr_paged_batch {
+  const int* table;
+  long long table_stride;
+  const int* lens;
+  const int* starts;
+  int B, rows, width, max_new, max_len;
+} gr_paged_batch;
+
+/* Puts the new tokens' keys and values into their pages and, with a rotation
+ * (NULL: none), turns the keys on the way, and the queries, if q is not NULL, from
+ * q into q_out (which may be q). Strides {batch, token, head}, as gr_rotary's
+ * (a packed batch's batch stride is not read). positions NULL: a token's place
+ * len - n + i in its sequence, on every axis; else int32 by {axis, batch, token}
+ * (packed: the token axis is the batch's). A page that two tokens of one call
+ * fall on at the same slot ends with either's entry. */
+int gr_paged_append(const gr_paged_cache* cache, const gr_paged_batch* batch, const gr_rotary_spec* rotary, const void* q,
+                    void* q_out, int Hq, const long long* q_strides, const long long* q_out_strides, const void* k,
+                    const void* v, const long long* k_strides, const long long* v_strides, const int* positions,
+                    const long long* position_strides, void* stream);
+
+/* Attention of the new tokens over the cache, O = softmax(scale Q K^T) V; token
+ * i sees the keys up to its own position (causal != 0) or all of its sequence's.
+ * Hq, a multiple of the cache's heads: query head h reads key head h / (Hq /
+ * heads). q, o: strides {batch, token, head} as above. lse: NULL, or [tokens][Hq]
+ * fp32 (uniform batches [B][rows][Hq]) for the log-sum-exp of the scaled scores,
+ * natural log. A row that sees no key gets 0 and -inf.
+ * workspace: device memory, 16-byte aligned, in which workgroups that share a
+ * row's keys leave partial results; gr_paged_attn_workspace names the size for a
+ * call's shapes (0 for calls that are not shared out, and for invalid ones). With
+ * less the keys are shared out less, with none not at all. The call overwrites
+ * it: calls that may overlap in time need one each. */
+size_t gr_paged_attn_workspace(const gr_paged_cache* cache, const gr_paged_batch* batch, int Hq);
+int gr_paged_attn(const gr_paged_cache* cache, const gr_paged_batch* batch, const void* q, void* o, float* lse, int Hq,
+                  const long long* q_strides, const long long* o_strides, int causal, float scale, void* workspace,
+                  size_t workspace_bytes, void* stream);
+
 /* Batched GEMM with fused epilogue, C[z] = act(alpha * A[z] @ B[z]).
  * Replaces the grammar's matmul stage (a stage whose body is matmul over a
  * contraction axis, optionally followed by mulc and relu/silu:
