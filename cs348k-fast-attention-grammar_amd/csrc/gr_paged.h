@@ -17,8 +17,11 @@
 //    tile ahead), the lanes' offsets are constant over the whole call.
 //  * KG groups of NW waves each take every KG-th tile and merge through LDS.
 //    With NW = 1 a wave reads only tiles that it loaded itself: no barrier.
-//  * Keys of a tile are shared out over up to `parts` workgroups, of `chunk`
-//    keys at least, which leave partial results for gr_paged_merge_body.
+//  * Few tiles (`shares` > 0): the work of the call, counted in blocks of 64 keys
+//    over all tiles and key heads, is cut into equal runs, one a workgroup, by
+//    the lengths as they are on the device. A run covers a tile's end, whole
+//    tiles and a tile's start; tiles that several runs cover are merged by
+//    gr_paged_merge_body. Many tiles: a workgroup each.
 //  * Slots behind the part's last key, and pages whose id is out of range,
 //    are written to LDS as zeros: what the cache holds there (NaN, say) does not
 //    reach a product. A key that only some of a tile's rows may see, and whose
@@ -46,10 +49,9 @@ struct gr_paged_args {
   int Hq, Hkv, G;
   int causal;
   float scale_log2;
-  int tiles;                       // row tiles of a key head in the grid (an upper bound for ragged batches)
-  int parts, chunk;                // key parts in the grid; fewest keys of a part (a multiple of 64)
-  int chunk_long;                  // the same for sequences of more than one row tile
-  float* part_o;                   // [(tile Hkv + key head) parts + part][row of the tile][D]
+  int tiles;                       // row tiles of a key head (an upper bound for ragged batches)
+  int shares;                      // workgroups that share the work out; 0: a workgroup a tile
+  float* part_o;                   // [2 share + place][row of the tile][D]
   float* part_ml;                  // the same, [2]: base (in scores), row sum
 };
 
@@ -59,65 +61,122 @@ struct gr_paged_tile {
   int n, row0, nrows;              // new tokens, first row of the tile, rows n G of the sequence
   int len, keys;                   // key count as given, and those that the page table can hold
   int kend;                        // keys that the tile's last row sees
-  int per, np;                     // keys of a part, parts
+  int nb;                          // blocks of 64 keys, 1 at least
+  int block;                       // found by block: the block in the tile
+  int x0;                          // blocks of a key head before the tile's
 };
 
-// The tile-th tile of BM rows; false past the last one.
-template <int BM>
-__device__ __forceinline__ bool gr_paged_find(const gr_paged_args& a, int tile, int lane, gr_paged_tile& t) {
-  int rt = -1;
-  if (a.starts) {
-    int before = 0;
-    t.b = -1;
-    for (int b0 = 0; b0 < a.B; b0 += 64) {
-      const int b = gr_imin(b0 + lane, a.B - 1);
-      const int s0 = a.starts[b], s1 = a.starts[b + 1];
-      // starts out of order or out of the batch: no tokens
-      const int n = b0 + lane < a.B && s0 >= 0 && s1 > s0 && s1 <= a.rows ? s1 - s0 : 0;
-      const int mine = (n * a.G + BM - 1) / BM;
-      int upto = mine;                            // inclusive sum over the lanes
-#pragma unroll
-      for (int off = 1; off < 64; off <<= 1) {
-        const int x = __shfl_up(upto, off, 64);
-        if (lane >= off) upto += x;
-      }
-      const unsigned long long past = __builtin_amdgcn_ballot_w64(before + upto > tile);
-      if (past) {
-        const int l = __builtin_ctzll(past);
-        t.b = b0 + l;
-        t.n = __builtin_amdgcn_readlane(n, l);
-        t.first = __builtin_amdgcn_readlane(s0, l);
-        rt = tile - before - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(mine, l));
-        break;
-      }
-      before += __builtin_amdgcn_readlane(upto, 63);
-    }
-    if (t.b < 0) return false;
-  } else {
-    const int per = (a.rows * a.G + BM - 1) / BM;
-    t.b = tile / per;
-    rt = tile - t.b * per;
-    if (t.b >= a.B) return false;
-    t.n = a.rows;
-    t.first = 0;
-  }
-  t.nrows = t.n * a.G;
-  const int ntile = (t.nrows + BM - 1) / BM;
-  t.row0 = (ntile - 1 - rt) * BM;                 // the tiles that see the most keys first
-  t.len = a.lens[t.b];
-  const int cap = a.width << a.page_shift;
-  t.keys = t.len < 0 ? 0 : gr_imin(t.len, cap);
-  const int last = (gr_imin(t.row0 + BM, t.nrows) - 1) / a.G;
-  // (len - n + last + 1 cannot wrap: n > last, and len is compared first)
-  t.kend = a.causal ? gr_imin(t.keys, t.len < 0 ? 0 : t.len - t.n + last + 1) : t.keys;
-  if (t.kend < 0) t.kend = 0;
-  const int chunk = ntile > 1 ? a.chunk_long : a.chunk;
-  const int even = ((t.kend + a.parts - 1) / a.parts + 63) & ~63;
-  t.per = chunk > even ? chunk : even;
-  t.np = a.parts == 1 ? 1 : (t.kend + t.per - 1) / t.per;
-  if (t.np < 1) t.np = 1;
-  return true;
+// Blocks of 64 keys of a sequence, as its tiles are counted (1 for none: its
+// rows are written all the same).
+__device__ __forceinline__ int gr_paged_keys(const gr_paged_args& a, int len) {
+  return len < 0 ? 0 : gr_imin(len, a.width << a.page_shift);
 }
+__device__ __forceinline__ int gr_paged_blocks(int keys) { return keys > 64 ? (keys + 63) >> 6 : 1; }
+
+// Sequence b's new tokens and, in a packed batch, its first row. Starts out of
+// order or out of the batch: no tokens.
+__device__ __forceinline__ int gr_paged_news(const gr_paged_args& a, int b, int& first) {
+  first = 0;
+  if (!a.starts) return a.rows;
+  first = a.starts[b];
+  const int s1 = a.starts[b + 1];
+  return first >= 0 && s1 > first && s1 <= a.rows ? s1 - first : 0;
+}
+
+// Sum over lanes 0 .. l, for every lane l (DPP: a few cycles a step, a tenth of
+// what a shuffle through LDS takes).
+__device__ __forceinline__ int gr_wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);    // row_shr:1 (rows of 16 lanes)
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);    // row_shr:2
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);    // row_shr:4
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);    // row_shr:8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);   // row_bcast:15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);   // row_bcast:31 into rows 2 and 3
+  return v;
+}
+
+// 64 sequences, one a lane, and where their tiles and blocks begin.
+template <int BM>
+struct gr_paged_seqs {
+  int b0 = -1;
+  int tiles, blocks;               // before these 64
+  int first, n, len, nt, nb;       // of the lane's sequence: tiles, blocks of a tile
+  int tsum, bsum;                  // tiles and blocks of the 64 up to and with it
+  __device__ __forceinline__ void load(const gr_paged_args& a, int from, int tiles0, int blocks0, int lane) {
+    b0 = from;
+    tiles = tiles0;
+    blocks = blocks0;
+    const int b = gr_imin(from + lane, a.B - 1);
+    len = a.lens[b];
+    n = gr_paged_news(a, b, first);
+    nt = from + lane < a.B ? (n * a.G + BM - 1) / BM : 0;
+    nb = gr_paged_blocks(gr_paged_keys(a, len));
+    tsum = gr_wave_scan(nt);
+    bsum = gr_wave_scan((int)((unsigned)nt * nb));
+  }
+  __device__ __forceinline__ int tiles_after() const { return tiles + __builtin_amdgcn_readlane(tsum, 63); }
+  __device__ __forceinline__ int blocks_after() const { return blocks + __builtin_amdgcn_readlane(bsum, 63); }
+
+  // Blocks of one key head over all tiles.
+  __device__ __forceinline__ int total(const gr_paged_args& a, int lane) {
+    load(a, 0, 0, 0, lane);
+    int sum = blocks_after();
+    if (a.B > 64) {
+      gr_paged_seqs more;
+      for (int from = 64; from < a.B; from += 64) {
+        more.load(a, from, 0, sum, lane);
+        sum = more.blocks_after();
+      }
+    }
+    return sum;
+  }
+
+  // BLOCK: the tile of the at-th block of a key head, else the at-th tile;
+  // false past the last one.
+  template <bool BLOCK>
+  __device__ __forceinline__ bool find(const gr_paged_args& a, int at, int lane, gr_paged_tile& t) {
+    if (b0 < 0 || (BLOCK ? blocks : tiles) > at) load(a, 0, 0, 0, lane);
+    while ((BLOCK ? blocks_after() : tiles_after()) <= at) {
+      if (b0 + 64 >= a.B) return false;
+      load(a, b0 + 64, tiles_after(), blocks_after(), lane);
+    }
+    const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64((BLOCK ? blocks + bsum : tiles + tsum) > at));
+    t.b = b0 + l;
+    t.n = __builtin_amdgcn_readlane(n, l);
+    t.first = __builtin_amdgcn_readlane(first, l);
+    t.len = __builtin_amdgcn_readlane(len, l);
+    t.nb = __builtin_amdgcn_readlane(nb, l);
+    const int before = blocks + __builtin_amdgcn_readlane(bsum - (int)((unsigned)nt * nb), l);
+    const int rt = BLOCK ? (at - before) / t.nb : at - tiles - __builtin_amdgcn_readlane(tsum - nt, l);
+    t.x0 = before + rt * t.nb;
+    t.block = at - t.x0;
+    t.nrows = t.n * a.G;
+    const int ntile = (t.nrows + BM - 1) / BM;
+    t.row0 = (ntile - 1 - rt) * BM;               // the tiles that see the most keys first
+    t.keys = gr_paged_keys(a, t.len);
+    const int last = (gr_imin(t.row0 + BM, t.nrows) - 1) / a.G;
+    // (len - n + last + 1 cannot wrap: n > last, and len is compared first)
+    t.kend = a.causal ? gr_imin(t.keys, t.len < 0 ? 0 : t.len - t.n + last + 1) : t.keys;
+    if (t.kend < 0) t.kend = 0;
+    return true;
+  }
+};
+
+// The shares of a call's `total` blocks: as many as workgroups, fewer if a share
+// would not get 4 blocks; the first `rest` get per + 1 blocks, the others per.
+struct gr_paged_cut {
+  int W, per, rest;
+  __device__ __forceinline__ gr_paged_cut(int total, int shares) {
+    W = total >> 2 < shares ? (total + 3) >> 2 : shares;
+    per = W > 0 ? total / W : 0;
+    rest = total - per * W;
+  }
+  __device__ __forceinline__ int begin(int w) const { return w * per + gr_imin(w, rest); }
+  __device__ __forceinline__ int of(int x) const {               // the share of block x
+    const int big = rest * (per + 1);
+    return x < big ? x / (per + 1) : rest + (x - big) / per;
+  }
+};
 
 // global_load_lds_dwordx4 from a scalar base plus a lane offset in bytes (see
 // gr_g2lds16).
@@ -174,17 +233,32 @@ __device__ __forceinline__ void gr_paged_body(const gr_paged_args& a, char* lds_
   char* const ks0 = lds;
   char* const vt0 = lds + 2 * L::TILE;
 
-  // key head slowest, then the tiles: workgroups of one key head share an XCD's L2
-  const int logical = gr_xcd_remap_any((int)blockIdx.x, (int)gridDim.x);
-  const int part = logical % a.parts, ti = logical / a.parts;
-  const int hk = ti / a.tiles, tile_id = ti - hk * a.tiles;
-  gr_paged_tile t;
-  if (!gr_paged_find<BM>(a, tile_id, lane, t)) return;
-  t.b = __builtin_amdgcn_readfirstlane(t.b);
-  if (part >= t.np) return;
+  // Load instruction i of the wave: 64 / CPR rows of LDS from row r0, in block
+  // j = r0 / 16. K rows are stored with row bits 2 and 3 swapped, V rows as they
+  // are; both swizzled (gr_swz for 16-byte row reads, gr_swz_tr for gr_tr_frag).
+  unsigned koff[PER], voff[PER];              // lane byte offsets within the block's page slots
+  int krow[PER];                              // LDS row of the lane; the key of a K chunk is gr_perm32 of it
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int c = lane + (wave + i * NW) * 64, r = c / CPR, pc = c % CPR;
+    krow[i] = r;
+    koff[i] = (unsigned)((gr_perm32(r) & 15) * a.k_ss * 2) + gr_swz<CPR>(r, pc) * 16;
+    voff[i] = (unsigned)((r & 15) * a.v_ss * 2) + gr_swz_tr<CPR>(r, pc) * 16;
+  }
+  const float c = a.scale_log2;
+  // LDS addresses of the fragments: the swizzles are XORs of chunk bits, so a
+  // fragment's is a lane constant XOR an immediate, plus whole rows.
+  //  K (gr_swz): row 32 kb + l32, chunk 2 ds + g
+  //  V (gr_tr_frag): rows 16 x + 8 g + 4 h + (lane / 4) % 4, columns 32 db + ...
+  const int kbase = l32 * (D * 2) + gr_swz<CPR>(l32, g) * 16;
+  const int vcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3), vrow = 8 * g + ((lane >> 2) & 3);
+  const int vbase = vrow * (D * 2) + gr_swz_tr<CPR>(vrow, vcol >> 3) * 16 + (vcol & 7) * 2;
+  typedef __attribute__((address_space(4))) const int cint;   // the page table by scalar loads
+  const int smask = (1 << a.page_shift) - 1;
 
-  const int key0 = part * t.per;                              // multiples of 64
-  const int key1 = gr_imin(t.kend, key0 + t.per);
+  // One tile over keys [key0, key1); place: where its partial result goes, or -1
+  // for a tile that is done here.
+  auto segment = [&](const gr_paged_tile& t, int hk, int key0, int key1, int place) {
   const int rw = t.row0 + wave * 32;                          // this wave's first row
   const bool wave_live = rw < t.nrows;
   const int row = gr_imin(rw + l32, t.nrows - 1);             // rows past the end: copies of the last
@@ -202,26 +276,11 @@ __device__ __forceinline__ void gr_paged_body(const gr_paged_args& a, char* lds_
 #pragma unroll
     for (int ds = 0; ds < DS; ++ds) qf[ds] = gr_as<vec8>(gr_ld16(qp + ds * 16 + 8 * g));
   }
-
-  // Load instruction i of the wave: 64 / CPR rows of LDS from row r0, in block
-  // j = r0 / 16. K rows are stored with row bits 2 and 3 swapped, V rows as they
-  // are; both swizzled (gr_swz for 16-byte row reads, gr_swz_tr for gr_tr_frag).
-  unsigned koff[PER], voff[PER];              // lane byte offsets within the block's page slots
-  int krow[PER];                              // LDS row of the lane; the key of a K chunk is gr_perm32 of it
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int c = lane + (wave + i * NW) * 64, r = c / CPR, pc = c % CPR;
-    krow[i] = r;
-    koff[i] = (unsigned)((gr_perm32(r) & 15) * a.k_ss * 2) + gr_swz<CPR>(r, pc) * 16;
-    voff[i] = (unsigned)((r & 15) * a.v_ss * 2) + gr_swz_tr<CPR>(r, pc) * 16;
-  }
-  typedef __attribute__((address_space(4))) const int cint;   // the page table by scalar loads
   cint* const tab = (cint*)(unsigned long long)(a.table + t.b * a.table_stride);
-  const int smask = (1 << a.page_shift) - 1;
   const T* const kp = static_cast<const T*>(a.k) + hk * a.k_sh;
   const T* const vp = static_cast<const T*>(a.v) + hk * a.v_sh;
 
-  const int ntile_all = (key1 - key0 + BN - 1) / BN;
+  const int ntile_all = key1 > key0 ? (key1 - key0 + BN - 1) / BN : 0;
   const int ntile = (ntile_all - kg + KG - 1) / KG;           // of this group
   const int niter = SOLO ? ntile : (ntile_all + KG - 1) / KG; // of the workgroup (its barriers are everyone's)
   auto key_of = [&](int j) { return key0 + (j * KG + kg) * BN; };
@@ -273,53 +332,73 @@ __device__ __forceinline__ void gr_paged_body(const gr_paged_args& a, char* lds_
 #pragma unroll
   for (int db = 0; db < DB; ++db) o[db] = (gr_f32x16)(0.f);
   float m = -GR_INF, l = 0.f;
-  const float c = a.scale_log2;
 
-  // One tile's scores, softmax and P V. MASK: some row may not see all of its keys.
-  auto tile = [&](int j, int slot, unsigned bad, auto mask_tag) {
-    constexpr bool MASK = decltype(mask_tag)::value;
+  // One tile's scores, softmax and P V. masked: some row may not see all of its
+  // keys (bad: 16-key blocks of no page, a bit each). One code path for both: two
+  // copies of the products cost registers that the loop has not got.
+  auto tile = [&](int j, int slot, bool masked, unsigned bad) {
     const int k0 = key_of(j);
-    gr_f32x16 s[KB][1];
-    vec8 qv[1][DS];
+    const int ka = kbase + slot * L::TILE, va = vbase + slot * L::TILE;
+    auto vfrag = [&](int x, int db) -> vec8 {       // 16 keys x, head dims 32 db on
+      typedef short v4s __attribute__((ext_vector_type(4)));
+      typedef __attribute__((address_space(3))) v4s lds_v4s;
+      gr_u32x4 r;
 #pragma unroll
-    for (int ds = 0; ds < DS; ++ds) qv[0][ds] = qf[ds];
-    gr_flash_qk<T, D, BN, 1>(s, ks0 + slot * L::TILE, qv, l32, g);
-    bool sees = true;                                          // whether the row sees any key of the tile
-    if constexpr (MASK) {
+      for (int h = 0; h < 2; ++h) {
+        const char* p = vt0 + (va ^ (db * 64)) + (16 * x + 4 * h) * (D * 2);
+        const v4s v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(__attribute__((address_space(3))) char*)(char*)p);
+        const gr_u32x2 w = __builtin_bit_cast(gr_u32x2, v);
+        r[2 * h] = w[0];
+        r[2 * h + 1] = w[1];
+      }
+      return gr_as<vec8>(r);
+    };
+    gr_f32x16 s[KB];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) s[kb] = (gr_f32x16)(0.f);
+#pragma unroll
+    for (int ds = 0; ds < DS; ++ds)
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        // (gr_swz of 128-byte rows also takes row bit 5)
+        const int off = (ka ^ (ds * 32) ^ (CPR == 8 ? (kb & 1) * 64 : 0)) + kb * 32 * (D * 2);
+        s[kb] = MF::mma32(gr_as<vec8>(gr_ld16(ks0 + off)), qf[ds], s[kb]);
+      }
+    bool fresh = m == -GR_INF;                                // no base yet, and a key to take it from
+    if (masked) {
       // element r of key block kb is key k0 + 32 kb + 16 (r / 8) + 8 g + r % 8
       const int delta = limit - k0 - 8 * g;
-      bool any = false;
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const bool vis = 32 * kb + 16 * (r >> 3) + (r & 7) <= delta && !(bad >> (2 * kb + (r >> 3)) & 1);
-          any |= vis;
-          if (!vis) s[kb][0][r] = -GR_INF;
-        }
-      sees = any;
-    }
-    vec8 pt[KB][2];
-    float lt;
-    auto make_p = [&](float nmc) {
-      lt = 0.f;
+      bool sees = false;
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
-          gr_u32x4 pw;
+          const int d = (bad >> (2 * kb + hf)) & 1 ? -1 : delta - 32 * kb - 16 * hf;
+          sees |= d >= 0;
 #pragma unroll
-          for (int e = 0; e < 8; e += 2) {
-            const float p0 = gr_exp2(fmaf(s[kb][0][8 * hf + e], c, nmc));
-            const float p1 = gr_exp2(fmaf(s[kb][0][8 * hf + e + 1], c, nmc));
-            const vec2 pp = __builtin_convertvector((gr_f32x2){p0, p1}, vec2);
-            lt = MF::sum2(pp, lt);
-            pw[e >> 1] = __builtin_bit_cast(unsigned, pp);
-          }
-          pt[kb][hf] = gr_as<vec8>(pw);
+          for (int e = 0; e < 8; ++e) s[kb][8 * hf + e] = e <= d ? s[kb][8 * hf + e] : -GR_INF;
         }
+      fresh &= sees;
+    }
+    vec8 pt[2 * KB];
+    float lt;
+    auto make_p = [&](float nmc) {
+      lt = 0.f;
+#pragma unroll
+      for (int x = 0; x < 2 * KB; ++x) {
+        gr_u32x4 pw;
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const float p0 = gr_exp2(fmaf(s[x >> 1][8 * (x & 1) + e], c, nmc));
+          const float p1 = gr_exp2(fmaf(s[x >> 1][8 * (x & 1) + e + 1], c, nmc));
+          const vec2 pp = __builtin_convertvector((gr_f32x2){p0, p1}, vec2);
+          lt = MF::sum2(pp, lt);
+          pw[e >> 1] = __builtin_bit_cast(unsigned, pp);
+        }
+        pt[x] = gr_as<vec8>(pw);
+      }
     };
-    bool ok = !gr_any(m == -GR_INF && sees);
+    bool ok = !gr_any(fresh);
     if (ok) {
       make_p(m == -GR_INF ? 0.f : -m * c);
       ok = !gr_any(!(lt <= GR_FLASH_SUM_MAX));
@@ -329,7 +408,7 @@ __device__ __forceinline__ void gr_paged_body(const gr_paged_args& a, char* lds_
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[kb][0][r]);
+        for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[kb][r]);
       mt = fmaxf(mt, gr_xor32(mt));
       const float mn = fmaxf(m, mt);
       const float alpha = mn > m ? gr_exp2((m - mn) * c) : 1.f;   // m = -inf -> 0
@@ -340,87 +419,67 @@ __device__ __forceinline__ void gr_paged_body(const gr_paged_args& a, char* lds_
       make_p(m == -GR_INF ? 0.f : -m * c);
     }
     l += lt;
-    const char* vt = vt0 + slot * L::TILE;
-    if constexpr (MASK) {
-      // keys with a value that is not finite: exponent bits all ones
+    if (masked) {
+      // keys with a value that is not finite (exponent bits all ones), a bit each
       constexpr unsigned EXP = gr_is_same<T, _Float16>::value ? 0x7c007c00u : 0x7f807f80u;
       constexpr unsigned ONE = gr_is_same<T, _Float16>::value ? 0x04000400u : 0x00800080u;
-      gr_u32x4 flags[KB][2];
-      unsigned all = 0;
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          flags[kb][hf] = (gr_u32x4)(0u);
-#pragma unroll
-          for (int db = 0; db < DB; ++db)
-            flags[kb][hf] |= (gr_raw(gr_tr_frag<T, D, false>(vt, kb * 32 + 16 * hf, db * 32, lane)) & EXP) + ONE;
-          flags[kb][hf] &= 0x80008000u;
-          all |= flags[kb][hf][0] | flags[kb][hf][1] | flags[kb][hf][2] | flags[kb][hf][3];
-        }
-      if (__builtin_expect(gr_any(all != 0), 0)) {
-        unsigned long long odd = 0;                            // those keys, a bit each
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              // lanes 0-31 hold key e of the 16, lanes 32-63 key 8 + e
-              const unsigned long long who =
-                  __builtin_amdgcn_ballot_w64((flags[kb][hf][e >> 1] >> ((e & 1) ? 31 : 15)) & 1);
-              odd |= ((unsigned long long)((unsigned)who != 0) | (unsigned long long)((who >> 32) != 0) << 8)
-                     << (kb * 32 + 16 * hf + e);
-            }
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            const unsigned byte = (unsigned)(odd >> (kb * 32 + 16 * hf + 8 * g)) & 0xffu;
-            gr_u32x4 keep;                                     // halfwords of the keys that stay in the product
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              keep[e] = ((byte >> (2 * e)) & 1 ? 0u : 0x0000ffffu) | ((byte >> (2 * e + 1)) & 1 ? 0u : 0xffff0000u);
-#pragma unroll
-            for (int db = 0; db < DB; ++db) {
-              const gr_u32x4 w = gr_raw(gr_tr_frag<T, D, false>(vt, kb * 32 + 16 * hf, db * 32, lane));
-              o[db] = MF::mma32(gr_as<vec8>(w & keep), pt[kb][hf], o[db]);
-            }
-          }
+      unsigned long long odd = 0;
 #pragma unroll 1
-        for (; odd; odd &= odd - 1) {
-          const int key = __builtin_ctzll(odd);
-          float p = 0.f;                                       // this lane's p of the key, if its half has it
+      for (int x = 0; x < 2 * KB; ++x) {
+        gr_u32x4 f = (gr_u32x4)(0u);
 #pragma unroll
-          for (int kb = 0; kb < KB; ++kb)
+        for (int db = 0; db < DB; ++db) f |= (gr_raw(vfrag(x, db)) & EXP) + ONE;
+        f &= 0x80008000u;
+        if (gr_any((f[0] | f[1] | f[2] | f[3]) != 0)) {
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf)
+          for (int e = 0; e < 8; ++e) {
+            // lanes 0-31 hold key e of the 16, lanes 32-63 key 8 + e
+            const unsigned long long who = __builtin_amdgcn_ballot_w64((f[e >> 1] >> ((e & 1) ? 31 : 15)) & 1);
+            odd |= ((unsigned long long)((unsigned)who != 0) | (unsigned long long)((who >> 32) != 0) << 8) << (16 * x + e);
+          }
+        }
+      }
+      if (__builtin_expect(odd != 0, 0)) {
+#pragma unroll 1
+        for (int x = 0; x < 2 * KB; ++x) {
+          gr_u32x4 p = gr_raw(pt[0]);
 #pragma unroll
-              for (int e = 0; e < 8; ++e)
-                if (key == kb * 32 + 16 * hf + 8 * g + e) p = (float)pt[kb][hf][e];
-          p += gr_xor32(p);                                    // the other half's is 0
-          const bool vis = k0 + key <= limit && !(bad >> (key >> 4) & 1);
-          const char* const vr = vt + key * (D * 2);
+          for (int y = 1; y < 2 * KB; ++y) p = x == y ? gr_raw(pt[y]) : p;
+          const unsigned byte = (unsigned)(odd >> (16 * x + 8 * g)) & 0xffu;
+          gr_u32x4 keep;                                       // halfwords of the keys that stay in the product
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            keep[e] = ((byte >> (2 * e)) & 1 ? 0u : 0x0000ffffu) | ((byte >> (2 * e + 1)) & 1 ? 0u : 0xffff0000u);
 #pragma unroll
           for (int db = 0; db < DB; ++db)
+            o[db] = MF::mma32(gr_as<vec8>(gr_raw(vfrag(x, db)) & keep), gr_as<vec8>(p), o[db]);
+#pragma unroll 1
+          for (unsigned left = (unsigned)(odd >> (16 * x)) & 0xffffu; left; left &= left - 1) {
+            const int i = __builtin_ctz(left), key = 16 * x + i;   // key i of the 16: half i / 8, element i % 8
+            const unsigned w = (i & 6) == 0 ? p[0] : (i & 6) == 2 ? p[1] : (i & 6) == 4 ? p[2] : p[3];
+            const unsigned short hw = (unsigned short)((i & 1) ? w >> 16 : w & 0xffffu);
+            const float mine = g == (i >> 3) ? (float)__builtin_bit_cast(T, hw) : 0.f;
+            const float pv = mine + gr_xor32(mine);
+            const bool vis = k0 + key <= limit && !(bad >> x & 1);
+            const char* const vr = vt0 + slot * L::TILE + key * (D * 2);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const int d = db * 32 + 8 * (r >> 2) + 4 * g + (r & 3);
-              const float v = (float)*reinterpret_cast<const T*>(vr + gr_swz_tr<CPR>(key, d >> 3) * 16 + (d & 7) * 2);
-              if (vis) o[db][r] = fmaf(p, v, o[db][r]);
-              if ((r & 3) == 3) __builtin_amdgcn_sched_barrier(0);   // not all reads at once: they would spill
-            }
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+              for (int r = 0; r < 16; ++r) {
+                const int d = db * 32 + 8 * (r >> 2) + 4 * g + (r & 3);
+                const float v = (float)*reinterpret_cast<const T*>(vr + gr_swz_tr<CPR>(key, d >> 3) * 16 + (d & 7) * 2);
+                if (vis) o[db][r] = fmaf(pv, v, o[db][r]);
+                if ((r & 3) == 3) __builtin_amdgcn_sched_barrier(0);   // (all reads at once would spill)
+              }
+          }
         }
         return;
       }
     }
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
+    for (int x = 0; x < 2 * KB; ++x)
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-        for (int db = 0; db < DB; ++db)
-          o[db] = MF::mma32(gr_tr_frag<T, D, false>(vt, kb * 32 + 16 * hf, db * 32, lane), pt[kb][hf], o[db]);
+      for (int db = 0; db < DB; ++db) o[db] = MF::mma32(vfrag(x, db), pt[x], o[db]);
   };
 
   // Iteration j reads slot j & 1; tile j + 1 is on its way to the other. A
@@ -458,8 +517,7 @@ __device__ __forceinline__ void gr_paged_body(const gr_paged_args& a, char* lds_
     if (j + 2 < ntile) nxt = ids_of(j + 2);
     const int k0 = key_of(j);
     if (wave_live && j < ntile && k0 <= lim_hi) {
-      if (k0 + BN - 1 <= lim_lo && bad_now == 0) tile(j, slot, 0u, gr_ic<0>{});
-      else tile(j, slot, bad_now, gr_ic<1>{});
+      tile(j, slot, k0 + BN - 1 > lim_lo || bad_now != 0, bad_now);
     }
   };
 #pragma unroll 1
@@ -512,9 +570,9 @@ __device__ __forceinline__ void gr_paged_body(const gr_paged_args& a, char* lds_
 
   const bool live = rw + l32 < t.nrows;
   const float lt = l + gr_xor32(l);
-  if (t.np > 1) {
-    // unnormalised O and (base, row sum) of this part
-    const long long at = ((long long)(tile_id * a.Hkv + hk) * a.parts + part) * BM + wave * 32 + l32;
+  if (place >= 0) {
+    // unnormalised O and (base, row sum) of these keys
+    const long long at = (long long)place * BM + wave * 32 + l32;
     if (live) {
       float* const po = a.part_o + at * D;
 #pragma unroll
@@ -544,47 +602,158 @@ __device__ __forceinline__ void gr_paged_body(const gr_paged_args& a, char* lds_
       a.lse[trow * a.Hq + head] = lt == 0.f ? -GR_INF : (m * c + __builtin_amdgcn_logf(lt)) * 0.6931471805599453f;
     }
   }
+  };   // segment
+
+  const int logical = gr_xcd_remap_any((int)blockIdx.x, (int)gridDim.x);
+  gr_paged_tile t;
+  gr_paged_seqs<BM> seqs;
+  if (a.shares == 0) {
+    // key head slowest, then the tiles: workgroups of one key head share an XCD's L2
+    const int hk = logical / a.tiles;
+    if (seqs.template find<false>(a, logical - hk * a.tiles, lane, t)) segment(t, hk, 0, t.kend, -1);
+    return;
+  }
+  const int per_head = seqs.total(a, lane);
+  const gr_paged_cut cut(per_head * a.Hkv, a.shares);
+  if (logical >= cut.W) return;
+  const int end = cut.begin(logical + 1);
+  int place = 2 * logical;
+#pragma unroll 1
+  for (int x = cut.begin(logical); x < end;) {
+    const int hk = x / per_head;
+    if (!seqs.template find<true>(a, x - hk * per_head, lane, t)) return;
+    const int left = gr_imin(end - x, t.nb - t.block);
+    segment(t, hk, t.block * 64, gr_imin(t.kend, (t.block + left) * 64), left == t.nb ? -1 : place);
+    x += left;
+    if (x < end) __syncthreads();                             // the rings are free again
+    place = 2 * logical + 1;
+  }
 }
 
-// Merges the key parts of a tile's rows, a wave to a row: O = sum_p w_p O_p /
-// sum_p w_p l_p with w_p = 2^((m_p - max m) c), the parts in order.
+// Merges the parts of a tile's rows: O = sum_p w_p O_p / sum_p w_p l_p with w_p =
+// 2^((m_p - max m) c), in an order that the cut alone decides. D / 4 lanes hold a
+// part's row. Up to 8 parts: every such group of lanes has a row of its own and
+// asks for all of its parts at once. More: the four waves share a row, 256 / D
+// parts a wave at a time, UN such loads ahead.
+constexpr int GR_PAGED_MAX_SHARES = 512;
+
 template <class T, int D, int BM>
 __device__ __forceinline__ void gr_paged_merge_body(const gr_paged_args& a) {
-  constexpr int V = D / 64;                  // floats a lane
+  constexpr int LPR = D / 4, PPW = 64 / LPR;  // lanes of a row, rows of a wave's load
+  constexpr int FEW = 8, UN = 4, NW = 4;
+  __shared__ float xm[NW][D];
   const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), nw = blockDim.x >> 6;
-  const int hk = blockIdx.x / a.tiles, tile_id = blockIdx.x - hk * a.tiles;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int hk = blockIdx.x / a.tiles;
   gr_paged_tile t;
-  if (!gr_paged_find<BM>(a, tile_id, lane, t) || t.np == 1) return;
+  gr_paged_seqs<BM> seqs;
+  const int per_head = seqs.total(a, lane);
+  if (!seqs.template find<false>(a, (int)blockIdx.x - hk * a.tiles, lane, t)) return;
+  // the shares that cover the tile's blocks; only the first may have begun in
+  // another tile, and then left this one's part in its second place
+  const gr_paged_cut cut(per_head * a.Hkv, a.shares);
+  const int x0 = hk * per_head + t.x0;
+  const int w0 = cut.of(x0), np = cut.of(x0 + t.nb - 1) - w0 + 1;
+  if (np == 1) return;
+  const int skew = cut.begin(w0) < x0 ? 1 : 0;
+  auto slot = [&](int p, int r) { return (long long)(2 * (w0 + p) + (p == 0 ? skew : 0)) * BM + r; };
   const float c = a.scale_log2;
   const int rows = gr_imin(BM, t.nrows - t.row0);
-  for (int r = (int)blockIdx.y * nw + wave; r < rows; r += nw * gridDim.y) {
-    const long long at = ((long long)(tile_id * a.Hkv + hk) * a.parts) * BM + r;
-    float mx = -GR_INF;
-    for (int p = lane; p < t.np; p += 64) mx = fmaxf(mx, a.part_ml[(at + (long long)p * BM) * 2]);
-    mx = gr_wave_max(mx);
-    const float base = mx == -GR_INF ? 0.f : mx;
-    float l = 0.f, o[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e) o[e] = 0.f;
-    for (int p = 0; p < t.np; ++p) {
-      const long long ap = at + (long long)p * BM;
-      const gr_f32x2 ml = *reinterpret_cast<const gr_f32x2*>(a.part_ml + ap * 2);
-      const float w = gr_exp2((ml[0] - base) * c);
-      l = fmaf(w, ml[1], l);
-      float x[V];
-      gr_row_load<V>(x, a.part_o + ap * D + lane * V);
-#pragma unroll
-      for (int e = 0; e < V; ++e) o[e] = fmaf(w, x[e], o[e]);
-    }
+  const int sub = lane / LPR, d4 = (lane % LPR) * 4;
+  auto put = [&](int r, gr_f32x4 o, float l, float mx) {
     const float inv = l == 0.f ? 0.f : 1.0f / l;
-#pragma unroll
-    for (int e = 0; e < V; ++e) o[e] *= inv;
     const int token = (t.row0 + r) / a.G, head = hk * a.G + (t.row0 + r) % a.G;
-    gr_row_store<V>(static_cast<T*>(a.o) + t.b * a.o_sb + (long long)(t.first + token) * a.o_st + head * a.o_sh + lane * V, o);
-    if (a.lse && lane == 0) {
+    T* const op = static_cast<T*>(a.o) + t.b * a.o_sb + (long long)(t.first + token) * a.o_st + head * a.o_sh + d4;
+    *reinterpret_cast<gr_u32x2*>(op) = (gr_u32x2){gr_pack2f<T>(o[0] * inv, o[1] * inv), gr_pack2f<T>(o[2] * inv, o[3] * inv)};
+    if (a.lse && d4 == 0) {
       const long long trow = a.starts ? t.first + token : (long long)t.b * a.rows + token;
       a.lse[trow * a.Hq + head] = l == 0.f ? -GR_INF : (mx * c + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
     }
+  };
+  if (np <= FEW) {
+    for (int r0 = ((int)blockIdx.y * NW + wave) * PPW; r0 < rows; r0 += (int)gridDim.y * NW * PPW) {
+      const int r = gr_imin(r0 + sub, rows - 1);
+      gr_f32x2 ml[FEW];
+      gr_f32x4 x[FEW];
+#pragma unroll
+      for (int p = 0; p < FEW; ++p)
+        if (p < np) {
+          ml[p] = *reinterpret_cast<const gr_f32x2*>(a.part_ml + slot(p, r) * 2);
+          x[p] = *reinterpret_cast<const gr_f32x4*>(a.part_o + slot(p, r) * D + d4);
+        }
+      float mx = -GR_INF, l = 0.f;
+#pragma unroll
+      for (int p = 0; p < FEW; ++p)
+        if (p < np) mx = fmaxf(mx, ml[p][0]);
+      const float base = mx == -GR_INF ? 0.f : mx;
+      gr_f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int p = 0; p < FEW; ++p)
+        if (p < np) {
+          const float w = gr_exp2((ml[p][0] - base) * c);
+          l = fmaf(w, ml[p][1], l);
+          o += w * x[p];
+        }
+      if (r0 + sub < rows) put(r, o, l, mx);
+    }
+    return;
+  }
+  for (int r = (int)blockIdx.y; r < rows; r += (int)gridDim.y) {
+    // part lane + 64 i: base and sum
+    float m[GR_PAGED_MAX_SHARES / 64], w[GR_PAGED_MAX_SHARES / 64];
+    float mx = -GR_INF, l = 0.f;
+#pragma unroll
+    for (int i = 0; i < GR_PAGED_MAX_SHARES / 64; ++i) {
+      const int p = lane + 64 * i;
+      m[i] = -GR_INF;
+      w[i] = 0.f;
+      if (p < np) {
+        const gr_f32x2 ml = *reinterpret_cast<const gr_f32x2*>(a.part_ml + slot(p, r) * 2);
+        m[i] = ml[0];
+        w[i] = ml[1];
+      }
+      mx = fmaxf(mx, m[i]);
+    }
+    mx = gr_wave_max(mx);
+    const float base = mx == -GR_INF ? 0.f : mx;
+#pragma unroll
+    for (int i = 0; i < GR_PAGED_MAX_SHARES / 64; ++i) {
+      const float sum = w[i];
+      w[i] = gr_exp2((m[i] - base) * c);
+      l = fmaf(w[i], sum, l);
+    }
+    l = gr_wave_sum(l);
+    gr_f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < GR_PAGED_MAX_SHARES / 64; ++i) {   // (w is indexed by constants)
+      if (64 * i >= np) break;
+      const int end = gr_imin(np - 64 * i, 64);
+      for (int p0 = wave * PPW * UN; p0 < end; p0 += NW * PPW * UN) {
+        gr_f32x4 x[UN];
+#pragma unroll
+        for (int k = 0; k < UN; ++k) {
+          const int p = gr_imin(p0 + k * PPW + sub, end - 1);
+          x[k] = *reinterpret_cast<const gr_f32x4*>(a.part_o + slot(64 * i + p, r) * D + d4);
+        }
+#pragma unroll
+        for (int k = 0; k < UN; ++k) {
+          const int p = p0 + k * PPW + sub;
+          const float f = __shfl(w[i], p & 63, 64);
+          if (p < end) o += f * x[k];
+        }
+      }
+    }
+#pragma unroll
+    for (int off = LPR; off < 64; off <<= 1)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], off, 64);
+    if (sub == 0) *reinterpret_cast<gr_f32x4*>(&xm[wave][d4]) = o;
+    __syncthreads();
+    if (wave == 0 && sub == 0) {
+#pragma unroll
+      for (int k = 1; k < NW; ++k) o += *reinterpret_cast<const gr_f32x4*>(&xm[k][d4]);
+      put(r, o, l, mx);
+    }
+    __syncthreads();
   }
 }

@@ -27,43 +27,43 @@ __global__ __launch_bounds__(256) void gr_paged_merge_kernel(gr_paged_args a) {
 struct Plan {
   int nw;                        // waves of 32 rows
   long long tiles;               // row tiles of a key head
-  int parts, chunk, chunk_long;
+  int shares;                    // 0: a workgroup a tile
 };
 
 Plan plan_of(const gr_paged_cache& c, const gr_paged_batch& b, int Hq) {
   Plan p;
-  const int G = Hq / c.heads;
+  const int G = Hq / c.heads, D = c.head_dim;
   const long long most = b.starts && b.max_new > 0 && b.max_new < b.rows ? b.max_new : b.rows;
   p.nw = most * G <= 32 ? 1 : most * G <= 64 ? 2 : 4;
   const int BM = 32 * p.nw;
   // packed rows: every sequence may have a part-filled tile
   p.tiles = b.starts ? (long long)b.rows * G / BM + b.B : (long long)b.B * (((long long)b.rows * G + BM - 1) / BM);
   const int cus = gr::cu_count() > 0 ? gr::cu_count() : 256;
+  const int resident = cus * (D == 128 && p.nw < 4 ? 1 : 2);      // workgroups (their LDS)
   const long long cap = (long long)b.width * c.page_size;
   const long long len = b.max_len > 0 && b.max_len < cap ? b.max_len : cap;
   const long long wgs = p.tiles * c.heads;
-  const long long want = 4LL * cus;
-  long long parts = wgs >= want ? 1 : (want + wgs - 1) / wgs;
-  if (parts > (len + 255) / 256) parts = (len + 255) / 256;
-  p.parts = (int)(parts < 1 ? 1 : parts > 256 ? 256 : parts);
-  p.chunk = p.parts == 1 ? 1 << 30 : (int)(((len + p.parts - 1) / p.parts + 63) / 64 * 64);
-  p.chunk_long = p.chunk;
+  p.shares = wgs >= (p.nw < 4 ? 4LL : 1LL) * resident || len <= 512 || p.tiles * c.heads * (cap / 64 + 1) > 0x7fffffffLL ? 0
+             : resident < GR_PAGED_MAX_SHARES ? resident : GR_PAGED_MAX_SHARES;
   return p;
 }
 
-size_t part_bytes(const Plan& p, int heads, int D, int parts) {
-  return parts <= 1 ? 0 : (size_t)p.tiles * heads * parts * 32 * p.nw * (D + 2) * sizeof(float);
-}
+size_t share_bytes(const Plan& p, int D) { return (size_t)2 * 32 * p.nw * (D + 2) * sizeof(float); }
 
 template <class T, int D, int BN, int NW, int KG>
 int launch_tiles(const gr_paged_args& a, hipStream_t st) {
   constexpr int BM = 32 * NW;
   const long long wgs = (long long)a.tiles * a.Hkv;
-  hipLaunchKernelGGL((gr_paged_kernel<T, D, BN, NW, KG>), dim3((unsigned)(wgs * a.parts)), dim3(64 * NW * KG),
+  hipLaunchKernelGGL((gr_paged_kernel<T, D, BN, NW, KG>), dim3((unsigned)(a.shares ? a.shares : wgs)), dim3(64 * NW * KG),
                      (gr_paged_lds<D, BN, NW, KG>::BYTES), st, a);
   int rc = gr::hip_check(hipGetLastError(), GR_E_LAUNCH, "gr_paged_attn launch");
-  if (rc || a.parts == 1) return rc;
-  hipLaunchKernelGGL((gr_paged_merge_kernel<T, D, BM>), dim3((unsigned)wgs, NW), dim3(256), 0, st, a);
+  if (rc || a.shares < 2) return rc;
+  const int rows = a.starts ? BM : (a.rows * a.G < BM ? a.rows * a.G : BM);      // of a tile, at most
+  // workgroups of a tile: one pass over its rows where it has few parts, and a
+  // row each where few tiles of many parts would leave CUs idle
+  const int few = (rows * D + 1023) / 1024, spare = (int)(1024 / wgs);
+  const int y = few > spare ? few : spare < rows ? spare : rows;
+  hipLaunchKernelGGL((gr_paged_merge_kernel<T, D, BM>), dim3((unsigned)wgs, y), dim3(256), 0, st, a);
   return gr::hip_check(hipGetLastError(), GR_E_LAUNCH, "gr_paged_attn merge launch");
 }
 
@@ -87,7 +87,7 @@ int check_heads(const gr_paged_cache* c, const gr_paged_batch* b, int Hq) {
 extern "C" size_t gr_paged_attn_workspace(const gr_paged_cache* cache, const gr_paged_batch* batch, int Hq) {
   if (gr::check_paged(cache, batch, "gr_paged_attn_workspace") || check_heads(cache, batch, Hq) || batch->rows == 0) return 0;
   const Plan p = plan_of(*cache, *batch, Hq);
-  return part_bytes(p, cache->heads, cache->head_dim, p.parts);
+  return p.shares * share_bytes(p, cache->head_dim);
 }
 
 extern "C" int gr_paged_attn(const gr_paged_cache* cache, const gr_paged_batch* batch, const void* q, void* o, float* lse,
@@ -105,9 +105,10 @@ extern "C" int gr_paged_attn(const gr_paged_cache* cache, const gr_paged_batch* 
       return gr::fail(GR_E_ARG, "gr_paged_attn: strides must be non-negative multiples of 8 elements");
   if (!(scale > 0.f)) return gr::fail(GR_E_ARG, "gr_paged_attn: scale must be positive");
   Plan p = plan_of(*cache, *batch, Hq);
-  // the most parts that the workspace holds
-  while (p.parts > 1 && part_bytes(p, cache->heads, cache->head_dim, p.parts) > (workspace ? workspace_bytes : 0)) --p.parts;
-  if (p.tiles * cache->heads * p.parts > 0x7fffffffLL / 256) return gr::fail(GR_E_ARG, "gr_paged_attn: grid out of range");
+  // as many shares as the workspace holds
+  const size_t fit = workspace ? workspace_bytes / share_bytes(p, cache->head_dim) : 0;
+  if ((size_t)p.shares > fit) p.shares = fit < 2 ? 0 : (int)fit;
+  if (p.tiles * cache->heads > 0x7fffffffLL / 512) return gr::fail(GR_E_ARG, "gr_paged_attn: grid out of range");
   gr_paged_args a = {};
   a.q = q;
   a.o = o;
@@ -133,12 +134,10 @@ extern "C" int gr_paged_attn(const gr_paged_cache* cache, const gr_paged_batch* 
   a.causal = causal;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.tiles = (int)p.tiles;
-  a.parts = p.parts;
-  a.chunk = p.chunk;
-  a.chunk_long = p.chunk_long;
-  if (p.parts > 1) {
+  a.shares = p.shares;
+  if (p.shares) {
     a.part_o = static_cast<float*>(workspace);
-    a.part_ml = a.part_o + (size_t)p.tiles * cache->heads * p.parts * 32 * p.nw * cache->head_dim;
+    a.part_ml = a.part_o + (size_t)p.shares * 2 * 32 * p.nw * cache->head_dim;
   }
   hipStream_t st = (hipStream_t)stream;
   if (cache->dtype == GR_F16)

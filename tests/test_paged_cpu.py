@@ -116,7 +116,7 @@ def test_workspace_is_what_the_parts_need():
     size = rt.lib().gr_paged_attn_workspace
     batch.B, batch.width = 1, 4096                      # one sequence of up to 65,536 keys: shared out
     one = size(ctypes.addressof(cache), ctypes.addressof(batch), 8)
-    assert one > 0 and one % (4 * 32 * 66 * 4) == 0     # parts of 4 key heads x 32 rows x (64 + 2) floats
+    assert one > 0 and one % (2 * 32 * 66 * 4) == 0     # two tiles of 32 rows x (64 + 2) floats a workgroup
     batch.max_len = 200                                 # too few keys to share
     assert size(ctypes.addressof(cache), ctypes.addressof(batch), 8) == 0
 

@@ -198,8 +198,8 @@ def test_whole_prompts(dtype, D):
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("n", [1, 40])
 def test_long_contexts_share_their_keys_out(D, n):
-    """Keys over several workgroups and merged: as many parts as the default takes, fewer with a smaller workspace,
-    none with an empty one; each twice, bit for bit the same."""
+    """Keys over several workgroups and merged: as many as the default takes, fewer with a smaller workspace, none
+    with an empty one; each twice, bit for bit the same."""
     from grammar import runtime as rt
     from grammar.paged import paged_attention
     lens = [20_011, 3, 5000]
@@ -211,7 +211,7 @@ def test_long_contexts_share_their_keys_out(D, n):
     batch = rt.PagedBatch(s.table.data_ptr(), s.width, s.lens.data_ptr(), None, 3, n, s.width, 0, 0)
     need = int(rt.lib().gr_paged_attn_workspace(s.cache.ref, ctypes.addressof(batch), 8))
     assert need > 0
-    for size in (need, need // 2, need // 4, 16, 0):
+    for size in (need, need // 2, need // 5, need // 100, 16, 0):
         ws = torch.empty(size, dtype=torch.uint8, device=s.dev)
         a, b = (paged_attention(q, s.cache, s.table, s.lens, workspace=ws) for _ in range(2))
         assert torch.equal(a, b)
