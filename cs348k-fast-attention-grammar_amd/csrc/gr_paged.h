@@ -62,9 +62,15 @@ struct gr_paged_tile {
   int len, keys;                   // key count as given, and those that the page table can hold
   int kend;                        // keys that the tile's last row sees
   int nb;                          // blocks of 64 keys, 1 at least
-  int block;                       // found by block: the block in the tile
+  int block;                       // found by block: the block in the tile (from nb on: its cost)
   int x0;                          // blocks of a key head before the tile's
 };
+
+// What a tile costs beside its keys (page ids, Q, the first tile's way, the
+// merge), in blocks of 64 keys: counted behind its last block.
+#ifndef GR_PAGED_COST
+#define GR_PAGED_COST 5
+#endif
 
 // Blocks of 64 keys of a sequence, as its tiles are counted (1 for none: its
 // rows are written all the same).
@@ -112,7 +118,7 @@ struct gr_paged_seqs {
     nt = from + lane < a.B ? (n * a.G + BM - 1) / BM : 0;
     nb = gr_paged_blocks(gr_paged_keys(a, len));
     tsum = gr_wave_scan(nt);
-    bsum = gr_wave_scan((int)((unsigned)nt * nb));
+    bsum = gr_wave_scan((int)((unsigned)nt * (nb + GR_PAGED_COST)));
   }
   __device__ __forceinline__ int tiles_after() const { return tiles + __builtin_amdgcn_readlane(tsum, 63); }
   __device__ __forceinline__ int blocks_after() const { return blocks + __builtin_amdgcn_readlane(bsum, 63); }
@@ -146,9 +152,10 @@ struct gr_paged_seqs {
     t.first = __builtin_amdgcn_readlane(first, l);
     t.len = __builtin_amdgcn_readlane(len, l);
     t.nb = __builtin_amdgcn_readlane(nb, l);
-    const int before = blocks + __builtin_amdgcn_readlane(bsum - (int)((unsigned)nt * nb), l);
-    const int rt = BLOCK ? (at - before) / t.nb : at - tiles - __builtin_amdgcn_readlane(tsum - nt, l);
-    t.x0 = before + rt * t.nb;
+    const int before = blocks + __builtin_amdgcn_readlane(bsum - (int)((unsigned)nt * (nb + GR_PAGED_COST)), l);
+    const int per = t.nb + GR_PAGED_COST;
+    const int rt = BLOCK ? (at - before) / per : at - tiles - __builtin_amdgcn_readlane(tsum - nt, l);
+    t.x0 = before + rt * per;
     t.block = at - t.x0;
     t.nrows = t.n * a.G;
     const int ntile = (t.nrows + BM - 1) / BM;
@@ -210,7 +217,7 @@ struct gr_paged_lds {
   static constexpr int BYTES = KG * RING > MERGE ? KG * RING : MERGE;
 };
 
-template <class T, int D, int BN, int NW, int KG>
+template <class T, int D, int BN, int NW, int KG, bool SHARED>
 __device__ __forceinline__ void gr_paged_body(const gr_paged_args& a, char* lds_all) {
   typedef gr_mfma<T> MF;
   typedef typename MF::vec8 vec8;
@@ -489,12 +496,15 @@ __device__ __forceinline__ void gr_paged_body(const gr_paged_args& a, char* lds_
   if (ntile > 0) {
     cur = ids_of(0);
     bad = bad_blocks(cur);
-    load(0, 0, cur);
     if (ntile > 1) nxt = ids_of(1);
   }
-  // Q has landed before the loop: the compiler cannot see that through the
-  // loop's back edge and would wait for every load in flight in each tile
-  __builtin_amdgcn_s_waitcnt(0);
+  // Q has landed (beside the page ids) before the first tile is asked for: its
+  // registers taken here, the compiler waits for them here, and not again for
+  // every load in flight at each tile's first product, as it cannot see through
+  // the loop's back edge that they came
+#pragma unroll
+  for (int ds = 0; ds < DS; ++ds) asm volatile("" : "+v"(qf[ds]));
+  if (ntile > 0) load(0, 0, cur);
   auto step = [&](int j, int slot) {
     if constexpr (SOLO) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // the slot's last reads are over
@@ -607,26 +617,29 @@ __device__ __forceinline__ void gr_paged_body(const gr_paged_args& a, char* lds_
   const int logical = gr_xcd_remap_any((int)blockIdx.x, (int)gridDim.x);
   gr_paged_tile t;
   gr_paged_seqs<BM> seqs;
-  if (a.shares == 0) {
+  if constexpr (!SHARED) {
     // key head slowest, then the tiles: workgroups of one key head share an XCD's L2
     const int hk = logical / a.tiles;
     if (seqs.template find<false>(a, logical - hk * a.tiles, lane, t)) segment(t, hk, 0, t.kend, -1);
-    return;
-  }
-  const int per_head = seqs.total(a, lane);
-  const gr_paged_cut cut(per_head * a.Hkv, a.shares);
-  if (logical >= cut.W) return;
-  const int end = cut.begin(logical + 1);
-  int place = 2 * logical;
+  } else {
+    const int per_head = seqs.total(a, lane);
+    const gr_paged_cut cut(per_head * a.Hkv, a.shares);
+    if (logical >= cut.W) return;
+    const int end = cut.begin(logical + 1);
+    int place = 2 * logical;
 #pragma unroll 1
-  for (int x = cut.begin(logical); x < end;) {
-    const int hk = x / per_head;
-    if (!seqs.template find<true>(a, x - hk * per_head, lane, t)) return;
-    const int left = gr_imin(end - x, t.nb - t.block);
-    segment(t, hk, t.block * 64, gr_imin(t.kend, (t.block + left) * 64), left == t.nb ? -1 : place);
-    x += left;
-    if (x < end) __syncthreads();                             // the rings are free again
-    place = 2 * logical + 1;
+    for (int x = cut.begin(logical); x < end;) {
+      const int hk = x / per_head;
+      if (!seqs.template find<true>(a, x - hk * per_head, lane, t)) return;
+      const int left = gr_imin(end - x, t.nb + GR_PAGED_COST - t.block);
+      const int to = gr_imin(t.block + left, t.nb);
+      if (t.block < to) {
+        segment(t, hk, t.block * 64, gr_imin(t.kend, to * 64), to - t.block == t.nb ? -1 : place);
+        if (x + left < end) __syncthreads();                  // the rings are free again
+      }
+      x += left;
+      place = 2 * logical + 1;
+    }
   }
 }
 

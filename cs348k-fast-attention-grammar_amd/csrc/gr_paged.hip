@@ -11,11 +11,11 @@
 
 namespace {
 
-template <class T, int D, int BN, int NW, int KG>
+template <class T, int D, int BN, int NW, int KG, bool SHARED>
 __global__ __launch_bounds__(64 * NW * KG) __attribute__((amdgpu_waves_per_eu(NW* KG == 4 && KG > 1 && D == 128 ? 1 : 2)))
 void gr_paged_kernel(gr_paged_args a) {
   extern __shared__ __attribute__((aligned(16))) char gr_lds[];
-  gr_paged_body<T, D, BN, NW, KG>(a, gr_lds);
+  gr_paged_body<T, D, BN, NW, KG, SHARED>(a, gr_lds);
 }
 
 template <class T, int D, int BM>
@@ -43,7 +43,7 @@ Plan plan_of(const gr_paged_cache& c, const gr_paged_batch& b, int Hq) {
   const long long cap = (long long)b.width * c.page_size;
   const long long len = b.max_len > 0 && b.max_len < cap ? b.max_len : cap;
   const long long wgs = p.tiles * c.heads;
-  p.shares = wgs >= (p.nw < 4 ? 4LL : 1LL) * resident || len <= 512 || p.tiles * c.heads * (cap / 64 + 1) > 0x7fffffffLL ? 0
+  p.shares = wgs >= (p.nw < 4 ? 4LL : 1LL) * resident || len <= 512 || p.tiles * c.heads * (cap / 64 + 1 + GR_PAGED_COST) > 0x7fffffffLL ? 0
              : resident < GR_PAGED_MAX_SHARES ? resident : GR_PAGED_MAX_SHARES;
   return p;
 }
@@ -54,10 +54,14 @@ template <class T, int D, int BN, int NW, int KG>
 int launch_tiles(const gr_paged_args& a, hipStream_t st) {
   constexpr int BM = 32 * NW;
   const long long wgs = (long long)a.tiles * a.Hkv;
-  hipLaunchKernelGGL((gr_paged_kernel<T, D, BN, NW, KG>), dim3((unsigned)(a.shares ? a.shares : wgs)), dim3(64 * NW * KG),
-                     (gr_paged_lds<D, BN, NW, KG>::BYTES), st, a);
-  int rc = gr::hip_check(hipGetLastError(), GR_E_LAUNCH, "gr_paged_attn launch");
-  if (rc || a.shares < 2) return rc;
+  constexpr int LDS = gr_paged_lds<D, BN, NW, KG>::BYTES;
+  if (a.shares == 0) {
+    hipLaunchKernelGGL((gr_paged_kernel<T, D, BN, NW, KG, false>), dim3((unsigned)wgs), dim3(64 * NW * KG), LDS, st, a);
+    return gr::hip_check(hipGetLastError(), GR_E_LAUNCH, "gr_paged_attn launch");
+  }
+  hipLaunchKernelGGL((gr_paged_kernel<T, D, BN, NW, KG, true>), dim3((unsigned)a.shares), dim3(64 * NW * KG), LDS, st, a);
+  const int rc = gr::hip_check(hipGetLastError(), GR_E_LAUNCH, "gr_paged_attn launch");
+  if (rc) return rc;
   const int rows = a.starts ? BM : (a.rows * a.G < BM ? a.rows * a.G : BM);      // of a tile, at most
   // workgroups of a tile: one pass over its rows where it has few parts, and a
   // row each where few tiles of many parts would leave CUs idle

@@ -45,7 +45,7 @@ class PagedCache:
             raise ValueError("PagedCache: fp16 or bf16")
         if D not in (64, 128) or size < 16 or size & (size - 1) or size > 1 << 20:
             raise ValueError(f"PagedCache: D {D} must be 64 or 128 and page_size {size} a power of two from 16 to 2^20")
-        self.k, self.v = k, v
+        self.k, self.v, self.dtype, self.index = k, v, k.dtype, k.get_device()
         self.pages, self.heads, self.page_size, self.head_dim = pages, heads, size, D
         self.desc = rt.PagedCacheDesc(k.data_ptr(), v.data_ptr(), rt._ll3(*k.stride()[:3]), rt._ll3(*v.stride()[:3]),
                                       rt.dtype_code(k.dtype), pages, heads, size, D)
@@ -64,12 +64,12 @@ def _batch(cache, table, lens, starts, x, name, max_new, max_len, who):
     """(gr_paged_batch, leading sizes of the tokens) of a call on `x`: [B, heads,
     n, D] or, with starts, [rows, heads, D]."""
     import torch
-    dev = cache.k.device
+    index, int32 = cache.index, torch.int32
     for n, t, dim in (("table", table, 2), ("lens", lens, 1), ("starts", starts, 1)):
         if t is None and n == "starts":
             continue
-        if t.dtype != torch.int32 or t.dim() != dim or t.device != dev or (t.shape[dim - 1] > 1 and t.stride(dim - 1) != 1):
-            raise ValueError(f"{who}: {n} must be a {dim}-D int32 tensor on {dev} with unit stride")
+        if t.dtype != int32 or t.dim() != dim or t.get_device() != index or (t.stride(-1) != 1 and t.shape[-1] > 1):
+            raise ValueError(f"{who}: {n} must be a {dim}-D int32 tensor on {cache.k.device} with unit stride")
     B, width = table.shape
     if lens.shape[0] != B or B == 0 or width == 0:
         raise ValueError(f"{who}: table {tuple(table.shape)} and lens {tuple(lens.shape)} do not describe a batch")
@@ -86,11 +86,10 @@ def _batch(cache, table, lens, starts, x, name, max_new, max_len, who):
 
 
 def _heads_ok(t, name, lead, heads, cache, who):
-    if not t.is_cuda:
-        raise ValueError(f"{who}: {name} must be a GPU tensor (no CPU path)")
     want = (lead[0], heads, lead[1], cache.head_dim) if len(lead) == 2 else (lead[0], heads, cache.head_dim)
-    if tuple(t.shape) != want or t.dtype != cache.k.dtype or t.device != cache.k.device:
-        raise ValueError(f"{who}: {name} must be {want} of the cache's dtype and device, not {tuple(t.shape)} {t.dtype}")
+    if t.shape != want or t.dtype != cache.dtype or t.get_device() != cache.index:
+        raise ValueError(f"{who}: {name} must be {want} {cache.dtype} on {cache.k.device} (no CPU path), not "
+                         f"{tuple(t.shape)} {t.dtype} on {t.device}")
 
 
 def _append_args(k, v, cache, table, lens, starts, q, rotary, positions, max_new, out):
@@ -99,7 +98,7 @@ def _append_args(k, v, cache, table, lens, starts, q, rotary, positions, max_new
     _heads_ok(k, "k", lead, cache.heads, cache, who)
     _heads_ok(v, "v", lead, cache.heads, cache, who)
     head = (cache.ref, ctypes.addressof(desc), rotary.ref if rotary is not None else None)
-    if rotary is not None and (rotary.head_dim != cache.head_dim or rotary.device != cache.k.device):
+    if rotary is not None and (rotary.head_dim != cache.head_dim or rotary.index != cache.index):
         raise ValueError(f"{who}: the rotation is for heads of {rotary.head_dim} on {rotary.device}")
     if q is None:
         if out is not None:
@@ -136,8 +135,7 @@ def paged_append(k, v, cache: PagedCache, table, lens, *, starts=None, q=None, r
     outside of the table or on a page id outside of the cache is not stored.
     max_new: the most new tokens of a sequence, where known."""
     args, out, keep = _append_args(k, v, cache, table, lens, starts, q, rotary, positions, max_new, out)
-    with rt.on_device(k):
-        rt.check(rt.lib().gr_paged_append(*args, rt._stream_ptr(stream)), "gr_paged_append")
+    rt.launch(rt.lib().gr_paged_append, args, k, stream, "gr_paged_append")
     return out
 
 
@@ -160,7 +158,7 @@ def _attn_args(q, cache, table, lens, starts, causal, scale, max_new, max_len, o
     out = check_out(out, q, "out", who)
     if lse is not None:
         want = (lead[0], lead[1], Hq) if len(lead) == 2 else (lead[0], Hq)
-        if tuple(lse.shape) != want or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != q.device:
+        if tuple(lse.shape) != want or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.get_device() != cache.index:
             raise ValueError(f"{who}: lse must be a contiguous {want} float32 tensor")
     if scale is None:
         scale = 1.0 / math.sqrt(cache.head_dim)
@@ -192,8 +190,7 @@ def paged_attention(q, cache: PagedCache, table, lens, *, starts=None, causal: b
     Returns the result, laid out as q, or `out`."""
     args, out, keep = _attn_args(q, cache, table, lens, starts, causal, scale, max_new, max_len, out, lse, workspace,
                                  stream)
-    with rt.on_device(q):
-        rt.check(rt.lib().gr_paged_attn(*args, rt._stream_ptr(stream)), "gr_paged_attn")
+    rt.launch(rt.lib().gr_paged_attn, args, q, stream, "gr_paged_attn")
     return out
 
 

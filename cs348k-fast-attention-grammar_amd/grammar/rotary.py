@@ -63,38 +63,52 @@ class Rotary:
         whole = [round(math.ldexp((f / (2 * math.pi)) % 1.0, 64)) % (1 << 64) for f in freqs]
         self.turns = torch.tensor([w - (1 << 64) if w >> 63 else w for w in whole], dtype=torch.int64, device=device)
         self.axes = torch.tensor(axes, dtype=torch.uint8, device=device)
-        self.device = self.turns.device
+        self.device, self.index = self.turns.device, self.turns.get_device()
         self.desc = rt.RotarySpec(self.turns.data_ptr(), self.axes.data_ptr(), pairs, self.naxes, self.head_dim,
                                   int(self.interleaved))
         self.ref = ctypes.addressof(self.desc)
+
+
+@functools.lru_cache(maxsize=1024)
+def _position_strides(naxes: int, shape: tuple, st: tuple, lead: tuple):
+    """{axis, batch, token} strides of positions of `shape`, None if it does not fit the tokens `lead`."""
+    axis = 0
+    if naxes > 1:
+        if shape[:1] != (naxes,):
+            return None
+        axis, shape, st = st[0], shape[1:], st[1:]
+    if shape == lead:
+        return _pair(axis, *((0,) * (2 - len(st))), *st)
+    return _pair(axis, 0, st[0]) if len(lead) == 2 and shape == lead[1:] else None
 
 
 def check_positions(positions, rot, lead: tuple, who: str):
     """The strides {axis, batch, token} of int32 `positions`: [*lead] or, with
     several axes, [axes, *lead]; a batch of positions may be left out."""
     import torch
-    if positions.dtype != torch.int32 or positions.device != rot.device:
+    if positions.dtype != torch.int32 or positions.get_device() != rot.index:
         raise ValueError(f"{who}: positions must be an int32 tensor on {rot.device}")
-    shape, st = tuple(positions.shape), positions.stride()
-    if rot.naxes > 1:
-        if shape[:1] != (rot.naxes,):
-            raise ValueError(f"{who}: positions {shape} must lead with the {rot.naxes} axes")
-        axis, shape, st = st[0], shape[1:], st[1:]
-    else:
-        axis = 0
-    if shape == lead:
-        return _pair(axis, *((0,) * (2 - len(st))), *st)
-    if len(lead) == 2 and shape == lead[1:]:
-        return _pair(axis, 0, st[0])
-    raise ValueError(f"{who}: positions {tuple(positions.shape)} do not match the tokens {lead}")
+    ps = _position_strides(rot.naxes, positions.shape, positions.stride(), lead)
+    if ps is None:
+        raise ValueError(f"{who}: positions {tuple(positions.shape)} do not match the tokens {lead}"
+                         + (f" led by the {rot.naxes} axes" if rot.naxes > 1 else ""))
+    return ps
+
+
+@functools.lru_cache(maxsize=1024)
+def _head_strides(shape: tuple, st: tuple):
+    if st[-1] != 1:
+        return None
+    st = [s if n > 1 else 0 for s, n in zip(st, shape)]                # a single row's stride says nothing
+    return _pair(st[0], st[2], st[1]) if len(st) == 4 else _pair(0, st[0], st[1])
 
 
 def head_strides(t, name: str, who: str):
     """{batch, token, head} strides of [B, H, N, D] or packed [T, H, D] heads."""
-    if t.stride(-1) != 1:
+    st = _head_strides(t.shape, t.stride())
+    if st is None:
         raise ValueError(f"{who}: {name} must have unit stride on its last dimension")
-    st = [s if n > 1 else 0 for s, n in zip(t.stride(), t.shape)]      # a single row's stride says nothing
-    return _pair(st[0], st[2], st[1]) if len(st) == 4 else _pair(0, st[0], st[1])
+    return st
 
 
 def check_out(out, like, name: str, who: str):
@@ -102,7 +116,7 @@ def check_out(out, like, name: str, who: str):
     import torch
     if out is None:
         return torch.empty_like(like)
-    if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device:
+    if out.shape != like.shape or out.dtype != like.dtype or out.get_device() != like.get_device():
         raise ValueError(f"{who}: bad `{name}` tensor")
     return out
 
@@ -114,42 +128,42 @@ def rotary_fwd(q, k, positions, rot: Rotary, *, inverse: bool = False, out=None,
     Returns (q', k'), new tensors laid out as the given ones, or `out` and
     `k_out`, which may be q and k themselves. inverse=True rotates back."""
     who = "rotary"
-    for name, t in (("q", q), ("k", k)):
-        if t is None:
-            if name == "k":
-                continue
-            raise ValueError(f"{who}: q must be given")
-        if not t.is_cuda:
-            raise ValueError(f"{who}: {name} must be a GPU tensor (no CPU path)")
-        if t.dim() != 4 or t.shape[3] != rot.head_dim or t.dtype != q.dtype or t.device != rot.device:
-            raise ValueError(f"{who}: {name} must be [B, H, N, {rot.head_dim}] of q's dtype on {rot.device}")
+    if q is None:
+        raise ValueError(f"{who}: q must be given")
+    dtype, dim, index = q.dtype, rot.head_dim, rot.index
+    for t in (q,) if k is None else (q, k):
+        if t.get_device() != index or t.dtype != dtype or t.dim() != 4 or t.shape[3] != dim:
+            raise ValueError(f"{who}: q and k must be [B, H, N, {dim}] tensors of one dtype on {rot.device} (no CPU path)")
     B, Hq, N, _ = q.shape
-    if k is not None and (k.shape[0] != B or k.shape[2] != N):
-        raise ValueError(f"{who}: k {tuple(k.shape)} does not match q {tuple(q.shape)}")
     ps = check_positions(positions, rot, (B, N), who)
     out = check_out(out, q, "out", who)
-    if k is not None:
+    head = (rot.ref, q.data_ptr(), out.data_ptr(), Hq, head_strides(q, "q", who), head_strides(out, "out", who))
+    if k is None:
+        head += (None, None, 0, None, None)
+    else:
+        if k.shape[0] != B or k.shape[2] != N:
+            raise ValueError(f"{who}: k {tuple(k.shape)} does not match q {tuple(q.shape)}")
         k_out = check_out(k_out, k, "k_out", who)
+        head += (k.data_ptr(), k_out.data_ptr(), k.shape[1], head_strides(k, "k", who), head_strides(k_out, "k_out", who))
     if B == 0 or N == 0:
         return out, k_out
-    args = (rot.ref, q.data_ptr(), out.data_ptr(), Hq, head_strides(q, "q", who), head_strides(out, "out", who))
-    if k is None:
-        args += (None, None, 0, None, None)
-    else:
-        args += (k.data_ptr(), k_out.data_ptr(), k.shape[1], head_strides(k, "k", who), head_strides(k_out, "k_out", who))
-    with rt.on_device(q):
-        rt.check(rt.lib().gr_rotary(*args, rt.dtype_code(q.dtype), B, N, positions.data_ptr(), ps, int(bool(inverse)),
-                                    rt._stream_ptr(stream)), "gr_rotary")
+    rt.launch(rt.lib().gr_rotary, head + (rt.dtype_code(q.dtype), B, N, positions.data_ptr(), ps, int(bool(inverse))),
+              q, stream, "gr_rotary")
     return out, k_out
+
+
+@functools.lru_cache(maxsize=1024)
+def _is_dense(shape: tuple, st: tuple) -> bool:
+    return st[3] == 1 and all(n == 1 or (s > 0 and s % 8 == 0) for s, n in zip(st, shape[:3]))
 
 
 def _dense(t):
     """t with strides the kernels take: itself, or a contiguous copy (the
     gradient of a sum is a broadcast one, of a slice a strided one)."""
+    if t.dim() != 4 or (_is_dense(t.shape, t.stride()) and t.data_ptr() % 16 == 0):
+        return t
     import torch
-    st = t.stride()
-    ok = st[3] == 1 and t.data_ptr() % 16 == 0 and all(n == 1 or (s > 0 and s % 8 == 0) for s, n in zip(st, t.shape[:3]))
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _autograd_function():
@@ -166,17 +180,22 @@ def _autograd_function():
         @staticmethod
         def backward(ctx, dq, dk):
             # a rotation's gradient is the rotation back, of the queries' and
-            # the keys' gradients in one launch where both came
+            # the keys' gradients in one launch where both came; itself
+            # differentiable where the backward pass is recorded
             positions, = ctx.saved_tensors
-            dq = dq if ctx.needs_input_grad[0] else None
-            dk = dk if ctx.needs_input_grad[1] else None
+            need_q, need_k = ctx.needs_input_grad[:2]
+            if not need_q:
+                dq = None
+            if not need_k:
+                dk = None
             if dq is None and dk is None:
                 return None, None, None, None, None
-            apply = RotaryFunction.apply
-            if dq is None:
-                return None, apply(dk, None, positions, ctx.rot, not ctx.inverse)[0], None, None, None
-            dq, dk = apply(dq, dk, positions, ctx.rot, not ctx.inverse)
-            return dq, dk, None, None, None
+            a, b = (dq, dk) if dq is not None else (dk, None)
+            if torch.is_grad_enabled():
+                a, b = RotaryFunction.apply(a, b, positions, ctx.rot, not ctx.inverse)
+            else:
+                a, b = rotary_fwd(_dense(a), None if b is None else _dense(b), positions, ctx.rot, inverse=not ctx.inverse)
+            return (a, b, None, None, None) if dq is not None else (None, a, None, None, None)
     return RotaryFunction
 
 

@@ -10,7 +10,6 @@ loading fails loudly otherwise -- there is no CPU fallback on this path.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import functools
 import os
@@ -278,29 +277,41 @@ def torch_stream(stream, device):
     return torch.cuda.ExternalStream(handle, device=device)
 
 
-def on_device(t):
-    """Context in which the device of tensor `t` is the current one: launches
-    go to the current device, and a call's current stream is that device's."""
+def launch(fn, args: tuple, t, stream, what: str) -> None:
+    """fn(*args, handle) with the handle of `stream` (if None, the current stream of
+    t's device) and the device of tensor `t` the current one: launches go to the
+    current device."""
     import torch
     dev = t.device.index
-    return _NO_CHANGE if dev == torch.cuda.current_device() else torch.cuda.device(dev)
-
-
-_NO_CHANGE = contextlib.nullcontext()
+    handle = torch._C._cuda_getCurrentRawStream(dev) if stream is None else _stream_ptr(stream)
+    if dev == torch._C._cuda_getDevice():
+        rc = fn(*args, handle)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, handle)
+    if rc != 0:
+        check(rc, what)
 
 
 def launcher(fn, args: tuple, t, stream, what: str, out, keep):
-    """launch() that calls the C entry `fn` with `args` and the handle of `stream`
-    (the current stream of t's device if None), holding `keep` (the tensors and
-    structures that the arguments point to) as long as it lives; returns `out`."""
-    with on_device(t):
-        args += (_stream_ptr(stream),)
+    """A function that makes launch()'s call on the stream that is meant now,
+    holding `keep` (the tensors and structures that the arguments point to) as
+    long as it lives, and returns `out`."""
+    import torch
+    dev = t.device.index
+    args += (torch._C._cuda_getCurrentRawStream(dev) if stream is None else _stream_ptr(stream),)
+    current = torch._C._cuda_getDevice
 
-    def launch(_keep=keep):
-        with on_device(t):
-            check(fn(*args), what)
+    def call(_keep=keep):
+        if dev == current():
+            rc = fn(*args)
+        else:
+            with torch.cuda.device(dev):
+                rc = fn(*args)
+        if rc != 0:
+            check(rc, what)
         return out
-    return launch
+    return call
 
 
 _STREAM_PER_THREAD = 2               # hipStreamPerThread
