@@ -102,7 +102,7 @@ __device__ __forceinline__ int gr_wave_scan(int v) {
 }
 
 // 64 sequences, one a lane, and where their tiles and blocks begin.
-template <int BM>
+template <int BM, bool SMALL>
 struct gr_paged_seqs {
   int b0 = -1;
   int tiles, blocks;               // before these 64
@@ -115,7 +115,8 @@ struct gr_paged_seqs {
     const int b = gr_imin(from + lane, a.B - 1);
     len = a.lens[b];
     n = gr_paged_news(a, b, first);
-    nt = from + lane < a.B ? (n * a.G + BM - 1) / BM : 0;
+    const int rows = n * a.G;
+    nt = from + lane >= a.B || rows == 0 ? 0 : SMALL && rows <= 32 ? 1 : (rows + BM - 1) / BM;
     nb = gr_paged_blocks(gr_paged_keys(a, len));
     tsum = gr_wave_scan(nt);
     bsum = gr_wave_scan((int)((unsigned)nt * (nb + GR_PAGED_COST)));
@@ -158,7 +159,7 @@ struct gr_paged_seqs {
     t.x0 = before + rt * per;
     t.block = at - t.x0;
     t.nrows = t.n * a.G;
-    const int ntile = (t.nrows + BM - 1) / BM;
+    const int ntile = (t.nrows + BM - 1) / BM;    // (one, whatever its size, for at most 32 rows)
     t.row0 = (ntile - 1 - rt) * BM;               // the tiles that see the most keys first
     t.keys = gr_paged_keys(a, t.len);
     const int last = (gr_imin(t.row0 + BM, t.nrows) - 1) / a.G;
@@ -186,26 +187,23 @@ struct gr_paged_cut {
 };
 
 // global_load_lds_dwordx4 from a scalar base plus a lane offset in bytes (see
-// gr_g2lds16).
-__device__ __forceinline__ void gr_g2lds16s(const void* base, unsigned off, unsigned lds) {
-  unsigned saved;
+// gr_g2lds16); M0 holds the LDS address.
+__device__ __forceinline__ void gr_g2lds16s(unsigned long long base, unsigned off, unsigned lds) {
   asm volatile(
-      "s_mov_b32 %0, m0\n\t"
-      "s_mov_b32 m0, %3\n\t"
+      "s_mov_b32 m0, %2\n\t"
       "s_nop 0\n\t"
-      "global_load_lds_dwordx4 %1, %2\n\t"
-      "s_mov_b32 m0, %0"
-      : "=&s"(saved)
+      "global_load_lds_dwordx4 %0, %1"
+      :
       : "v"(off), "s"(base), "s"(lds)
-      : "memory");
+      : "memory", "m0");
 }
 
-// A pointer that is the same in every lane, in scalar registers.
-template <class P>
-__device__ __forceinline__ P gr_uniform(P p) {
-  const unsigned long long u = (unsigned long long)p;
-  const unsigned lo = __builtin_amdgcn_readfirstlane((int)(unsigned)u), hi = __builtin_amdgcn_readfirstlane((int)(unsigned)(u >> 32));
-  return (P)((unsigned long long)hi << 32 | lo);
+// XOR swizzle of K's 16-byte chunks for reads of consecutive rows at one logical
+// chunk: 8 and 16 rows of an aligned 16 fall on distinct bank groups, as with
+// gr_swz, by row bits 0 to 3 only.
+template <int CPR>
+__device__ __forceinline__ int gr_paged_swz(int row, int chunk) {
+  return CPR >= 16 ? chunk ^ (row & 15) : chunk ^ ((row & 7) ^ ((row >> 3) & 1));
 }
 
 template <int D, int BN, int NW, int KG>
@@ -217,55 +215,63 @@ struct gr_paged_lds {
   static constexpr int BYTES = KG * RING > MERGE ? KG * RING : MERGE;
 };
 
-template <class T, int D, int BN, int NW, int KG, bool SHARED>
-__device__ __forceinline__ void gr_paged_body(const gr_paged_args& a, char* lds_all) {
+// One tile over keys [key0, key1), by NW KG waves of the workgroup's WAVES; place:
+// where its partial result of BM rows goes, or -1 for a tile that is done here.
+template <class T, int D, int BN, int NW, int KG, int WAVES, int BM>
+__device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* lds_all, const gr_paged_tile& t, int hk,
+                                                 int key0, int key1, int place) {
   typedef gr_mfma<T> MF;
   typedef typename MF::vec8 vec8;
   typedef typename MF::vec2 vec2;
   typedef gr_paged_lds<D, BN, NW, KG> L;
-  constexpr int BM = 32 * NW, NT = 64 * NW;
+  constexpr bool SOLO = NW == 1;             // waves independent until the merge
   constexpr int KB = BN / 32, DB = D / 32, DS = D / 16;
   constexpr int CPR = D / 8;                 // 16-byte chunks of a row
   constexpr int BLOCKS = BN / 16;            // 16-row blocks of a tile
   constexpr int IPB = 16 * CPR / 64;         // load instructions of a block
   constexpr int PER = BLOCKS * IPB / NW;     // of a wave, for K and for V
   static_assert(BLOCKS * IPB % NW == 0, "whole load instructions");
-  constexpr bool SOLO = NW == 1;             // waves independent until the merge
 
   const int lane = threadIdx.x & 63;
   const int wave_all = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int kg = wave_all / NW, wave = wave_all % NW;
+  if (NW * KG < WAVES && kg >= KG) {          // a wave without a part: the merge's barriers only
+    if constexpr (KG > 1) {
+      __syncthreads();
+      __syncthreads();
+    }
+    return;
+  }
+  static_assert(NW * KG == WAVES || SOLO, "the loop's barriers are every wave's");
   const int g = lane >> 5, l32 = lane & 31;
   char* const lds = lds_all + kg * L::RING;
   char* const ks0 = lds;
   char* const vt0 = lds + 2 * L::TILE;
 
-  // Load instruction i of the wave: 64 / CPR rows of LDS from row r0, in block
-  // j = r0 / 16. K rows are stored with row bits 2 and 3 swapped, V rows as they
-  // are; both swizzled (gr_swz for 16-byte row reads, gr_swz_tr for gr_tr_frag).
-  unsigned koff[PER], voff[PER];              // lane byte offsets within the block's page slots
-  int krow[PER];                              // LDS row of the lane; the key of a K chunk is gr_perm32 of it
+  // Load instruction i of the wave is number wave + i NW of the tile: 64 / CPR
+  // rows of LDS, part `sub` of the IPB of a block of 16 rows. K rows are stored
+  // with row bits 2 and 3 swapped, V rows as they are; both swizzled (gr_paged_swz
+  // for 16-byte row reads, gr_swz_tr for gr_tr_frag) by row bits 0 to 3, so that a
+  // lane's offset from its block's first slot depends on sub alone.
+  constexpr int SUBS = IPB > NW ? IPB / NW : 1;
+  auto block_row = [&](int i) { return lane / CPR + ((wave + i * NW) % IPB) * (64 / CPR); };
+  unsigned koff[SUBS], voff[SUBS];            // bytes
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int c = lane + (wave + i * NW) * 64, r = c / CPR, pc = c % CPR;
-    krow[i] = r;
-    koff[i] = (unsigned)((gr_perm32(r) & 15) * a.k_ss * 2) + gr_swz<CPR>(r, pc) * 16;
-    voff[i] = (unsigned)((r & 15) * a.v_ss * 2) + gr_swz_tr<CPR>(r, pc) * 16;
+  for (int i = 0; i < SUBS; ++i) {
+    const int r = block_row(i), pc = lane % CPR;
+    koff[i] = (unsigned)((gr_perm32(r) & 15) * a.k_ss * 2) + gr_paged_swz<CPR>(r, pc) * 16;
+    voff[i] = (unsigned)(r * a.v_ss * 2) + gr_swz_tr<CPR>(r, pc) * 16;
   }
   const float c = a.scale_log2;
   // LDS addresses of the fragments: the swizzles are XORs of chunk bits, so a
   // fragment's is a lane constant XOR an immediate, plus whole rows.
-  //  K (gr_swz): row 32 kb + l32, chunk 2 ds + g
+  //  K (gr_paged_swz): row 32 kb + l32, chunk 2 ds + g
   //  V (gr_tr_frag): rows 16 x + 8 g + 4 h + (lane / 4) % 4, columns 32 db + ...
-  const int kbase = l32 * (D * 2) + gr_swz<CPR>(l32, g) * 16;
+  const int kbase = l32 * (D * 2) + gr_paged_swz<CPR>(l32, g) * 16;
   const int vcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3), vrow = 8 * g + ((lane >> 2) & 3);
   const int vbase = vrow * (D * 2) + gr_swz_tr<CPR>(vrow, vcol >> 3) * 16 + (vcol & 7) * 2;
-  typedef __attribute__((address_space(4))) const int cint;   // the page table by scalar loads
   const int smask = (1 << a.page_shift) - 1;
 
-  // One tile over keys [key0, key1); place: where its partial result goes, or -1
-  // for a tile that is done here.
-  auto segment = [&](const gr_paged_tile& t, int hk, int key0, int key1, int place) {
   const int rw = t.row0 + wave * 32;                          // this wave's first row
   const bool wave_live = rw < t.nrows;
   const int row = gr_imin(rw + l32, t.nrows - 1);             // rows past the end: copies of the last
@@ -276,14 +282,7 @@ __device__ __forceinline__ void gr_paged_body(const gr_paged_args& a, char* lds_
   const int lim_lo = a.causal ? gr_imin(base_pos + gr_imin(rw, t.nrows - 1) / a.G, t.keys - 1) : t.keys - 1;
   const int lim_hi = a.causal ? gr_imin(base_pos + gr_imin(rw + 31, t.nrows - 1) / a.G, t.keys - 1) : t.keys - 1;
 
-  // this lane's Q row, 8 consecutive dims of every 16
-  vec8 qf[DS];
-  {
-    const T* qp = static_cast<const T*>(a.q) + t.b * a.q_sb + (long long)(t.first + token) * a.q_st + head * a.q_sh;
-#pragma unroll
-    for (int ds = 0; ds < DS; ++ds) qf[ds] = gr_as<vec8>(gr_ld16(qp + ds * 16 + 8 * g));
-  }
-  cint* const tab = (cint*)(unsigned long long)(a.table + t.b * a.table_stride);
+  const int* const tab = a.table + t.b * a.table_stride;
   const T* const kp = static_cast<const T*>(a.k) + hk * a.k_sh;
   const T* const vp = static_cast<const T*>(a.v) + hk * a.v_sh;
 
@@ -291,50 +290,57 @@ __device__ __forceinline__ void gr_paged_body(const gr_paged_args& a, char* lds_
   const int ntile = (ntile_all - kg + KG - 1) / KG;           // of this group
   const int niter = SOLO ? ntile : (ntile_all + KG - 1) / KG; // of the workgroup (its barriers are everyone's)
   auto key_of = [&](int j) { return key0 + (j * KG + kg) * BN; };
-  struct Ids { int id[BLOCKS]; };
-  auto ids_of = [&](int j) {
-    Ids x;
-#pragma unroll
-    for (int bl = 0; bl < BLOCKS; ++bl) x.id[bl] = tab[gr_imin((key_of(j) + 16 * bl) >> a.page_shift, a.width - 1)];
-    return x;
+  // Where the blocks of this group's tiles are: lane l has block l % BLOCKS of
+  // tile j0 + l / BLOCKS, its K and V addresses and (a bit each) whether its page
+  // exists; refilled every 64 / BLOCKS tiles, the page ids read a window ahead. A
+  // tile's loads take their scalar bases from it by lane reads (worked out by
+  // scalar multiplications they cost more than the loads).
+  constexpr int WIN = 64 / BLOCKS;
+  auto id_of = [&](int j0) {
+    const long long key = key0 + ((long long)(j0 + lane / BLOCKS) * KG + kg) * BN + 16 * (lane % BLOCKS);
+    return tab[key >> a.page_shift < a.width ? (int)(key >> a.page_shift) : a.width - 1];
   };
-  auto bad_blocks = [&](const Ids& x) {       // blocks whose page id is out of range, a bit each
-    unsigned m = 0;
-#pragma unroll
-    for (int bl = 0; bl < BLOCKS; ++bl) m |= ((unsigned)x.id[bl] >= (unsigned)a.pages ? 1u : 0u) << bl;
-    return m;
+  unsigned long long kwin = 0, vwin = 0, badwin = 0;
+  int next_id = 0;
+  auto refill = [&](int j0, int id) {
+    const int slot = (key0 + ((j0 + lane / BLOCKS) * KG + kg) * BN + 16 * (lane % BLOCKS)) & smask;
+    const bool ok = (unsigned)id < (unsigned)a.pages;
+    kwin = (unsigned long long)(kp + (ok ? id : 0) * a.k_sp + slot * a.k_ss);
+    vwin = (unsigned long long)(vp + (ok ? id : 0) * a.v_sp + slot * a.v_ss);
+    badwin = __builtin_amdgcn_ballot_w64(!ok);
+    if (j0 + WIN < ntile) next_id = id_of(j0 + WIN);
   };
-  auto load = [&](int j, int slot, const Ids& x) {
+  auto bad_of = [&](int j) { return (unsigned)(badwin >> ((j % WIN) * BLOCKS)) & ((1u << BLOCKS) - 1); };
+  auto lane64 = [&](unsigned long long w, int l) {
+    return (unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)(w >> 32), l) << 32
+           | (unsigned)__builtin_amdgcn_readlane((int)(unsigned)w, l);
+  };
+  const unsigned kring = __builtin_amdgcn_readfirstlane((int)gr_lds_addr(ks0));
+  auto load = [&](int j, int slot) {
     const int k0 = key_of(j);
-    const unsigned bad = bad_blocks(x);
+    const unsigned bad = bad_of(j);
     const bool whole = bad == 0 && k0 + BN <= key1;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int instr = wave + i * NW, bl = instr / IPB;
-      int id = x.id[0];                       // (bl depends on the wave: a select, not an indexed read)
-#pragma unroll
-      for (int e = 1; e < BLOCKS; ++e) id = bl == e ? x.id[e] : id;
-      char* const kd = ks0 + slot * L::TILE + instr * 1024;
-      char* const vd = vt0 + slot * L::TILE + instr * 1024;
-      const long long s = (k0 + 16 * bl) & smask;
-      const bool ok = (unsigned)id < (unsigned)a.pages;
-      const T* const kb = gr_uniform(kp + (ok ? id : 0) * a.k_sp + s * a.k_ss);
-      const T* const vb = gr_uniform(vp + (ok ? id : 0) * a.v_sp + s * a.v_ss);
-      const unsigned kl = __builtin_amdgcn_readfirstlane((int)gr_lds_addr(kd));
-      const unsigned vl = __builtin_amdgcn_readfirstlane((int)gr_lds_addr(vd));
+      const unsigned long long kb = lane64(kwin, (j % WIN) * BLOCKS + bl), vb = lane64(vwin, (j % WIN) * BLOCKS + bl);
+      const unsigned kl = kring + slot * L::TILE + instr * 1024, vl = kl + 2 * L::TILE;
       if (whole) {
-        gr_g2lds16s(kb, koff[i], kl);
-        gr_g2lds16s(vb, voff[i], vl);
+        gr_g2lds16s(kb, koff[i % SUBS], kl);
+        gr_g2lds16s(vb, voff[i % SUBS], vl);
       } else {
-        const int r = krow[i];
-        if (ok && k0 + gr_perm32(r) < key1) gr_g2lds16s(kb, koff[i], kl);
-        else gr_st16(kd + lane * 16, (gr_u32x4){0, 0, 0, 0});
-        if (ok && k0 + r < key1) gr_g2lds16s(vb, voff[i], vl);
-        else gr_st16(vd + lane * 16, (gr_u32x4){0, 0, 0, 0});
+        char* const kd = ks0 + slot * L::TILE + instr * 1024 + lane * 16;
+        const int r = block_row(i), kblk = k0 + 16 * bl;
+        const bool ok = !(bad >> bl & 1);
+        if (ok && kblk + gr_perm32(r) < key1) gr_g2lds16s(kb, koff[i % SUBS], kl);
+        else gr_st16(kd, (gr_u32x4){0, 0, 0, 0});
+        if (ok && kblk + r < key1) gr_g2lds16s(vb, voff[i % SUBS], vl);
+        else gr_st16(kd + 2 * L::TILE, (gr_u32x4){0, 0, 0, 0});
       }
     }
   };
 
+  vec8 qf[DS];
   gr_f32x16 o[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db) o[db] = (gr_f32x16)(0.f);
@@ -367,9 +373,7 @@ __device__ __forceinline__ void gr_paged_body(const gr_paged_args& a, char* lds_
     for (int ds = 0; ds < DS; ++ds)
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
-        // (gr_swz of 128-byte rows also takes row bit 5)
-        const int off = (ka ^ (ds * 32) ^ (CPR == 8 ? (kb & 1) * 64 : 0)) + kb * 32 * (D * 2);
-        s[kb] = MF::mma32(gr_as<vec8>(gr_ld16(ks0 + off)), qf[ds], s[kb]);
+        s[kb] = MF::mma32(gr_as<vec8>(gr_ld16(ks0 + (ka ^ (ds * 32)) + kb * 32 * (D * 2))), qf[ds], s[kb]);
       }
     bool fresh = m == -GR_INF;                                // no base yet, and a key to take it from
     if (masked) {
@@ -491,44 +495,43 @@ __device__ __forceinline__ void gr_paged_body(const gr_paged_args& a, char* lds_
 
   // Iteration j reads slot j & 1; tile j + 1 is on its way to the other. A
   // part-filled tile's zeros are LDS stores, so a wave alone also waits on them.
-  Ids cur = {}, nxt = {};
-  unsigned bad = 0;
-  if (ntile > 0) {
-    cur = ids_of(0);
-    bad = bad_blocks(cur);
-    if (ntile > 1) nxt = ids_of(1);
+  // the page ids first, then this lane's Q row (8 consecutive dims of every 16)
+  const int first_id = ntile > 0 ? id_of(0) : 0;
+  {
+    const T* qp = static_cast<const T*>(a.q) + t.b * a.q_sb + (long long)(t.first + token) * a.q_st + head * a.q_sh;
+#pragma unroll
+    for (int ds = 0; ds < DS; ++ds) qf[ds] = gr_as<vec8>(gr_ld16(qp + ds * 16 + 8 * g));
   }
+  if (ntile > 0) refill(0, first_id);
   // Q has landed (beside the page ids) before the first tile is asked for: its
   // registers taken here, the compiler waits for them here, and not again for
   // every load in flight at each tile's first product, as it cannot see through
   // the loop's back edge that they came
 #pragma unroll
   for (int ds = 0; ds < DS; ++ds) asm volatile("" : "+v"(qf[ds]));
-  if (ntile > 0) load(0, 0, cur);
+  unsigned bad_next = 0;                      // bad blocks of the tile last asked for
+  auto ask = [&](int j) {
+    if (j > 0 && j % WIN == 0) refill(j, next_id);
+    load(j, j & 1);
+    bad_next = bad_of(j);
+  };
+  if (ntile > 0) ask(0);
   auto step = [&](int j, int slot) {
+    const unsigned bad = bad_next;
     if constexpr (SOLO) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // the slot's last reads are over
-      if (j + 1 < ntile) load(j + 1, slot ^ 1, nxt);
-      if (j + 1 < ntile && key_of(j + 1) + BN <= key1) {
-        // (a part-filled or bad next tile issues fewer loads: then all are waited for)
-        if (bad_blocks(nxt) == 0) gr_wait_vmcnt<2 * PER>();
-        else gr_wait_vmcnt<0>();
-      } else {
-        gr_wait_vmcnt<0>();
-      }
+      if (j + 1 < ntile) ask(j + 1);
+      // (a part-filled or bad next tile issues fewer loads: then all are waited for)
+      if (j + 1 < ntile && key_of(j + 1) + BN <= key1 && bad_next == 0) gr_wait_vmcnt<2 * PER>();
+      else gr_wait_vmcnt<0>();
       asm volatile("" ::: "memory");
     } else {
       gr_wait_vmcnt<0>();
       __syncthreads();                                         // tile j is there, and the other slot free
-      if (j + 1 < ntile) load(j + 1, slot ^ 1, nxt);
+      if (j + 1 < ntile) ask(j + 1);
     }
-    const unsigned bad_now = bad;
-    if (j + 1 < ntile) bad = bad_blocks(nxt);
-    if (j + 2 < ntile) nxt = ids_of(j + 2);
     const int k0 = key_of(j);
-    if (wave_live && j < ntile && k0 <= lim_hi) {
-      tile(j, slot, k0 + BN - 1 > lim_lo || bad_now != 0, bad_now);
-    }
+    if (wave_live && j < ntile && k0 <= lim_hi) tile(j, slot, k0 + BN - 1 > lim_lo || bad != 0, bad);
   };
 #pragma unroll 1
   for (int j = 0; j < niter; ++j) step(j, j & 1);
@@ -612,15 +615,28 @@ __device__ __forceinline__ void gr_paged_body(const gr_paged_args& a, char* lds_
       a.lse[trow * a.Hq + head] = lt == 0.f ? -GR_INF : (m * c + __builtin_amdgcn_logf(lt)) * 0.6931471805599453f;
     }
   }
-  };   // segment
+}
 
+// A workgroup of WAVES waves. Tiles of BM rows: NW waves by row, KG groups by
+// key, BN keys a step. KGS > 0: sequences of at most 32 rows (single tokens in a
+// batch with long chunks) take tiles of 32, KGS waves sharing out the keys, 32 a step.
+template <class T, int D, int BN, int NW, int KG, int KGS, bool SHARED>
+__device__ __forceinline__ void gr_paged_body(const gr_paged_args& a, char* lds) {
+  constexpr int BM = 32 * NW, WAVES = NW * KG;
+  const int lane = threadIdx.x & 63;
   const int logical = gr_xcd_remap_any((int)blockIdx.x, (int)gridDim.x);
   gr_paged_tile t;
-  gr_paged_seqs<BM> seqs;
+  gr_paged_seqs<BM, (KGS > 0)> seqs;
+  auto segment = [&](int hk, int key0, int key1, int place) {
+    if constexpr (KGS > 0) {
+      if (t.nrows <= 32) return gr_paged_segment<T, D, 32, 1, KGS, WAVES, BM>(a, lds, t, hk, key0, key1, place);
+    }
+    gr_paged_segment<T, D, BN, NW, KG, WAVES, BM>(a, lds, t, hk, key0, key1, place);
+  };
   if constexpr (!SHARED) {
     // key head slowest, then the tiles: workgroups of one key head share an XCD's L2
     const int hk = logical / a.tiles;
-    if (seqs.template find<false>(a, logical - hk * a.tiles, lane, t)) segment(t, hk, 0, t.kend, -1);
+    if (seqs.template find<false>(a, logical - hk * a.tiles, lane, t)) segment(hk, 0, t.kend, -1);
   } else {
     const int per_head = seqs.total(a, lane);
     const gr_paged_cut cut(per_head * a.Hkv, a.shares);
@@ -634,7 +650,7 @@ __device__ __forceinline__ void gr_paged_body(const gr_paged_args& a, char* lds_
       const int left = gr_imin(end - x, t.nb + GR_PAGED_COST - t.block);
       const int to = gr_imin(t.block + left, t.nb);
       if (t.block < to) {
-        segment(t, hk, t.block * 64, gr_imin(t.kend, to * 64), to - t.block == t.nb ? -1 : place);
+        segment(hk, t.block * 64, gr_imin(t.kend, to * 64), to - t.block == t.nb ? -1 : place);
         if (x + left < end) __syncthreads();                  // the rings are free again
       }
       x += left;
@@ -645,12 +661,13 @@ __device__ __forceinline__ void gr_paged_body(const gr_paged_args& a, char* lds_
 
 // Merges the parts of a tile's rows: O = sum_p w_p O_p / sum_p w_p l_p with w_p =
 // 2^((m_p - max m) c), in an order that the cut alone decides. D / 4 lanes hold a
-// part's row. Up to 8 parts: every such group of lanes has a row of its own and
-// asks for all of its parts at once. More: the four waves share a row, 256 / D
-// parts a wave at a time, UN such loads ahead.
+// part's row. Up to two parts for each row of the tile: every such group of lanes
+// has a row of its own and asks for 8 of its parts at once. More (few rows, long
+// contexts): the four waves share a row, 256 / D parts a wave at a time, UN such
+// loads ahead.
 constexpr int GR_PAGED_MAX_SHARES = 512;
 
-template <class T, int D, int BM>
+template <class T, int D, int BM, bool SMALL>
 __device__ __forceinline__ void gr_paged_merge_body(const gr_paged_args& a) {
   constexpr int LPR = D / 4, PPW = 64 / LPR;  // lanes of a row, rows of a wave's load
   constexpr int FEW = 8, UN = 4, NW = 4;
@@ -659,7 +676,7 @@ __device__ __forceinline__ void gr_paged_merge_body(const gr_paged_args& a) {
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int hk = blockIdx.x / a.tiles;
   gr_paged_tile t;
-  gr_paged_seqs<BM> seqs;
+  gr_paged_seqs<BM, SMALL> seqs;
   const int per_head = seqs.total(a, lane);
   if (!seqs.template find<false>(a, (int)blockIdx.x - hk * a.tiles, lane, t)) return;
   // the shares that cover the tile's blocks; only the first may have begun in
@@ -683,30 +700,37 @@ __device__ __forceinline__ void gr_paged_merge_body(const gr_paged_args& a) {
       a.lse[trow * a.Hq + head] = l == 0.f ? -GR_INF : (mx * c + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
     }
   };
-  if (np <= FEW) {
+  if (np <= 2 * rows) {
     for (int r0 = ((int)blockIdx.y * NW + wave) * PPW; r0 < rows; r0 += (int)gridDim.y * NW * PPW) {
       const int r = gr_imin(r0 + sub, rows - 1);
-      gr_f32x2 ml[FEW];
-      gr_f32x4 x[FEW];
-#pragma unroll
-      for (int p = 0; p < FEW; ++p)
-        if (p < np) {
-          ml[p] = *reinterpret_cast<const gr_f32x2*>(a.part_ml + slot(p, r) * 2);
-          x[p] = *reinterpret_cast<const gr_f32x4*>(a.part_o + slot(p, r) * D + d4);
-        }
       float mx = -GR_INF, l = 0.f;
-#pragma unroll
-      for (int p = 0; p < FEW; ++p)
-        if (p < np) mx = fmaxf(mx, ml[p][0]);
-      const float base = mx == -GR_INF ? 0.f : mx;
       gr_f32x4 o = {0.f, 0.f, 0.f, 0.f};
+      for (int p0 = 0; p0 < np; p0 += FEW) {
+        gr_f32x2 ml[FEW];
+        gr_f32x4 x[FEW];
 #pragma unroll
-      for (int p = 0; p < FEW; ++p)
-        if (p < np) {
-          const float w = gr_exp2((ml[p][0] - base) * c);
-          l = fmaf(w, ml[p][1], l);
-          o += w * x[p];
-        }
+        for (int p = 0; p < FEW; ++p)
+          if (p0 + p < np) {
+            ml[p] = *reinterpret_cast<const gr_f32x2*>(a.part_ml + slot(p0 + p, r) * 2);
+            x[p] = *reinterpret_cast<const gr_f32x4*>(a.part_o + slot(p0 + p, r) * D + d4);
+          }
+        float mn = mx;
+#pragma unroll
+        for (int p = 0; p < FEW; ++p)
+          if (p0 + p < np) mn = fmaxf(mn, ml[p][0]);
+        const float base = mn == -GR_INF ? 0.f : mn;
+        const float old = gr_exp2((mx - base) * c);       // 0 before the first part
+        mx = mn;
+        l *= old;
+        o *= old;
+#pragma unroll
+        for (int p = 0; p < FEW; ++p)
+          if (p0 + p < np) {
+            const float w = gr_exp2((ml[p][0] - base) * c);
+            l = fmaf(w, ml[p][1], l);
+            o += w * x[p];
+          }
+      }
       if (r0 + sub < rows) put(r, o, l, mx);
     }
     return;

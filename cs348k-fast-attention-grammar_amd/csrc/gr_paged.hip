@@ -11,16 +11,26 @@
 
 namespace {
 
-template <class T, int D, int BN, int NW, int KG, bool SHARED>
-__global__ __launch_bounds__(64 * NW * KG) __attribute__((amdgpu_waves_per_eu(NW* KG == 4 && KG > 1 && D == 128 ? 1 : 2)))
+constexpr int imax(int a, int b) { return a > b ? a : b; }
+
+template <int D, int BN, int NW, int KG, int KGS>
+struct Lds {
+  static constexpr int BYTES = imax(gr_paged_lds<D, BN, NW, KG>::BYTES, gr_paged_lds<D, 32, 1, KGS ? KGS : 1>::BYTES);
+};
+
+// One workgroup of four waves a CU where its LDS allows no two, else (and with
+// eight waves) two waves a SIMD.
+template <class T, int D, int BN, int NW, int KG, int KGS, bool SHARED>
+__global__ __launch_bounds__(64 * NW * KG)
+__attribute__((amdgpu_waves_per_eu(NW* KG == 4 && Lds<D, BN, NW, KG, KGS>::BYTES > 80 * 1024 ? 1 : 2)))
 void gr_paged_kernel(gr_paged_args a) {
   extern __shared__ __attribute__((aligned(16))) char gr_lds[];
-  gr_paged_body<T, D, BN, NW, KG, SHARED>(a, gr_lds);
+  gr_paged_body<T, D, BN, NW, KG, KGS, SHARED>(a, gr_lds);
 }
 
-template <class T, int D, int BM>
+template <class T, int D, int BM, bool SMALL>
 __global__ __launch_bounds__(256) void gr_paged_merge_kernel(gr_paged_args a) {
-  gr_paged_merge_body<T, D, BM>(a);
+  gr_paged_merge_body<T, D, BM, SMALL>(a);
 }
 
 // How a call is cut into workgroups.
@@ -50,16 +60,16 @@ Plan plan_of(const gr_paged_cache& c, const gr_paged_batch& b, int Hq) {
 
 size_t share_bytes(const Plan& p, int D) { return (size_t)2 * 32 * p.nw * (D + 2) * sizeof(float); }
 
-template <class T, int D, int BN, int NW, int KG>
+template <class T, int D, int BN, int NW, int KG, int KGS>
 int launch_tiles(const gr_paged_args& a, hipStream_t st) {
-  constexpr int BM = 32 * NW;
+  constexpr int BM = 32 * NW, LDS = Lds<D, BN, NW, KG, KGS>::BYTES;
   const long long wgs = (long long)a.tiles * a.Hkv;
-  constexpr int LDS = gr_paged_lds<D, BN, NW, KG>::BYTES;
+  const dim3 block(64 * NW * KG);
   if (a.shares == 0) {
-    hipLaunchKernelGGL((gr_paged_kernel<T, D, BN, NW, KG, false>), dim3((unsigned)wgs), dim3(64 * NW * KG), LDS, st, a);
+    hipLaunchKernelGGL((gr_paged_kernel<T, D, BN, NW, KG, KGS, false>), dim3((unsigned)wgs), block, LDS, st, a);
     return gr::hip_check(hipGetLastError(), GR_E_LAUNCH, "gr_paged_attn launch");
   }
-  hipLaunchKernelGGL((gr_paged_kernel<T, D, BN, NW, KG, true>), dim3((unsigned)a.shares), dim3(64 * NW * KG), LDS, st, a);
+  hipLaunchKernelGGL((gr_paged_kernel<T, D, BN, NW, KG, KGS, true>), dim3((unsigned)a.shares), block, LDS, st, a);
   const int rc = gr::hip_check(hipGetLastError(), GR_E_LAUNCH, "gr_paged_attn launch");
   if (rc) return rc;
   const int rows = a.starts ? BM : (a.rows * a.G < BM ? a.rows * a.G : BM);      // of a tile, at most
@@ -67,15 +77,15 @@ int launch_tiles(const gr_paged_args& a, hipStream_t st) {
   // row each where few tiles of many parts would leave CUs idle
   const int few = (rows * D + 1023) / 1024, spare = (int)(1024 / wgs);
   const int y = few > spare ? few : spare < rows ? spare : rows;
-  hipLaunchKernelGGL((gr_paged_merge_kernel<T, D, BM>), dim3((unsigned)wgs, y), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((gr_paged_merge_kernel<T, D, BM, (KGS > 0)>), dim3((unsigned)wgs, y), dim3(256), 0, st, a);
   return gr::hip_check(hipGetLastError(), GR_E_LAUNCH, "gr_paged_attn merge launch");
 }
 
 template <class T, int D>
 int launch(const gr_paged_args& a, int nw, hipStream_t st) {
-  if (nw == 1) return launch_tiles<T, D, 32, 1, 4>(a, st);
-  if (nw == 2) return launch_tiles<T, D, 32, 2, 4>(a, st);
-  return launch_tiles<T, D, 64, 4, 1>(a, st);
+  if (nw == 1) return launch_tiles<T, D, 32, 1, 4, 0>(a, st);
+  if (nw == 2) return launch_tiles<T, D, 32, 2, 4, 0>(a, st);
+  return launch_tiles<T, D, 64, 4, 1, D == 64 ? 4 : 2>(a, st);
 }
 
 int check_heads(const gr_paged_cache* c, const gr_paged_batch* b, int Hq) {
