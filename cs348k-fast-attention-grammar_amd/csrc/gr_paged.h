@@ -206,10 +206,10 @@ __device__ __forceinline__ int gr_paged_swz(int row, int chunk) {
   return CPR >= 16 ? chunk ^ (row & 15) : chunk ^ ((row & 7) ^ ((row >> 3) & 1));
 }
 
-template <int D, int BN, int NW, int KG>
+template <int D, int BN, int NW, int KG, int NS>
 struct gr_paged_lds {
   static constexpr int TILE = BN * D * 2;
-  static constexpr int RING = 4 * TILE;                       // two slots of K and of V
+  static constexpr int RING = 2 * NS * TILE;                  // NS slots of K, then of V
   static constexpr int PART = 32 * D * 4 + 64 * 8;            // a wave's O, base and sum
   static constexpr int MERGE = (KG - 1) * NW * PART;
   static constexpr int BYTES = KG * RING > MERGE ? KG * RING : MERGE;
@@ -217,13 +217,13 @@ struct gr_paged_lds {
 
 // One tile over keys [key0, key1), by NW KG waves of the workgroup's WAVES; place:
 // where its partial result of BM rows goes, or -1 for a tile that is done here.
-template <class T, int D, int BN, int NW, int KG, int WAVES, int BM>
+template <class T, int D, int BN, int NW, int KG, int NS, int WAVES, int BM>
 __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* lds_all, const gr_paged_tile& t, int hk,
                                                  int key0, int key1, int place) {
   typedef gr_mfma<T> MF;
   typedef typename MF::vec8 vec8;
   typedef typename MF::vec2 vec2;
-  typedef gr_paged_lds<D, BN, NW, KG> L;
+  typedef gr_paged_lds<D, BN, NW, KG, NS> L;
   constexpr bool SOLO = NW == 1;             // waves independent until the merge
   constexpr int KB = BN / 32, DB = D / 32, DS = D / 16;
   constexpr int CPR = D / 8;                 // 16-byte chunks of a row
@@ -246,7 +246,7 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
   const int g = lane >> 5, l32 = lane & 31;
   char* const lds = lds_all + kg * L::RING;
   char* const ks0 = lds;
-  char* const vt0 = lds + 2 * L::TILE;
+  char* const vt0 = lds + NS * L::TILE;
 
   // Load instruction i of the wave is number wave + i NW of the tile: 64 / CPR
   // rows of LDS, part `sub` of the IPB of a block of 16 rows. K rows are stored
@@ -324,7 +324,7 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
     for (int i = 0; i < PER; ++i) {
       const int instr = wave + i * NW, bl = instr / IPB;
       const unsigned long long kb = lane64(kwin, (j % WIN) * BLOCKS + bl), vb = lane64(vwin, (j % WIN) * BLOCKS + bl);
-      const unsigned kl = kring + slot * L::TILE + instr * 1024, vl = kl + 2 * L::TILE;
+      const unsigned kl = kring + slot * L::TILE + instr * 1024, vl = kl + NS * L::TILE;
       if (whole) {
         gr_g2lds16s(kb, koff[i % SUBS], kl);
         gr_g2lds16s(vb, voff[i % SUBS], vl);
@@ -335,7 +335,7 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
         if (ok && kblk + gr_perm32(r) < key1) gr_g2lds16s(kb, koff[i % SUBS], kl);
         else gr_st16(kd, (gr_u32x4){0, 0, 0, 0});
         if (ok && kblk + r < key1) gr_g2lds16s(vb, voff[i % SUBS], vl);
-        else gr_st16(kd + 2 * L::TILE, (gr_u32x4){0, 0, 0, 0});
+        else gr_st16(kd + NS * L::TILE, (gr_u32x4){0, 0, 0, 0});
       }
     }
   };
@@ -346,10 +346,10 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
   for (int db = 0; db < DB; ++db) o[db] = (gr_f32x16)(0.f);
   float m = -GR_INF, l = 0.f;
 
-  // One tile's scores, softmax and P V. masked: some row may not see all of its
-  // keys (bad: 16-key blocks of no page, a bit each). One code path for both: two
-  // copies of the products cost registers that the loop has not got.
-  auto tile = [&](int j, int slot, bool masked, unsigned bad) {
+  // One tile's scores, softmax and P V. MASKED: some row may not see all of its
+  // keys (bad: 16-key blocks of no page, a bit each).
+  auto tile = [&](int j, int slot, unsigned bad, auto masked_tag) {
+    constexpr bool MASKED = decltype(masked_tag)::value;
     const int k0 = key_of(j);
     const int ka = kbase + slot * L::TILE, va = vbase + slot * L::TILE;
     auto vfrag = [&](int x, int db) -> vec8 {       // 16 keys x, head dims 32 db on
@@ -376,7 +376,7 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
         s[kb] = MF::mma32(gr_as<vec8>(gr_ld16(ks0 + (ka ^ (ds * 32)) + kb * 32 * (D * 2))), qf[ds], s[kb]);
       }
     bool fresh = m == -GR_INF;                                // no base yet, and a key to take it from
-    if (masked) {
+    if constexpr (MASKED) {
       // element r of key block kb is key k0 + 32 kb + 16 (r / 8) + 8 g + r % 8
       const int delta = limit - k0 - 8 * g;
       bool sees = false;
@@ -430,7 +430,7 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
       make_p(m == -GR_INF ? 0.f : -m * c);
     }
     l += lt;
-    if (masked) {
+    if constexpr (MASKED) {
       // keys with a value that is not finite (exponent bits all ones), a bit each
       constexpr unsigned EXP = gr_is_same<T, _Float16>::value ? 0x7c007c00u : 0x7f807f80u;
       constexpr unsigned ONE = gr_is_same<T, _Float16>::value ? 0x04000400u : 0x00800080u;
@@ -493,8 +493,8 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
       for (int db = 0; db < DB; ++db) o[db] = MF::mma32(vfrag(x, db), pt[x], o[db]);
   };
 
-  // Iteration j reads slot j & 1; tile j + 1 is on its way to the other. A
-  // part-filled tile's zeros are LDS stores, so a wave alone also waits on them.
+  // Iteration j reads slot j % NS; the tiles up to j + NS - 1 are on their way to
+  // the others. A part-filled tile's zeros are LDS stores.
   // the page ids first, then this lane's Q row (8 consecutive dims of every 16)
   const int first_id = ntile > 0 ? id_of(0) : 0;
   {
@@ -509,32 +509,62 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
   // the loop's back edge that they came
 #pragma unroll
   for (int ds = 0; ds < DS; ++ds) asm volatile("" : "+v"(qf[ds]));
-  unsigned bad_next = 0;                      // bad blocks of the tile last asked for
-  auto ask = [&](int j) {
-    if (j > 0 && j % WIN == 0) refill(j, next_id);
-    load(j, j & 1);
-    bad_next = bad_of(j);
+  // A tile that is part-filled or has a bad page issues fewer loads than 2 PER:
+  // from the first such one on, every load is waited for.
+  bool uneven = false;
+  int asked = 0, to = 0;                      // tiles asked for; the next one's slot
+  unsigned long long bads = 0;                // bad blocks of the last tiles asked for, newest first
+  auto ask = [&]() {
+    if (asked >= ntile) return;
+    if (asked > 0 && asked % WIN == 0) refill(asked, next_id);
+    load(asked, to);
+    uneven |= bad_of(asked) != 0 || key_of(asked) + BN > key1;
+    bads = bads << BLOCKS | bad_of(asked);
+    ++asked;
+    to = to + 1 == NS ? 0 : to + 1;
   };
-  if (ntile > 0) ask(0);
-  auto step = [&](int j, int slot) {
-    const unsigned bad = bad_next;
+  // Waits for all but the tiles behind tile j.
+  auto arrived = [&](int j) {
+    const int behind = uneven ? 0 : asked - 1 - j;
+    if (NS > 3 && behind >= 3) gr_wait_vmcnt<(NS > 3 ? 6 * PER : 0)>();
+    else if (NS > 2 && behind >= 2) gr_wait_vmcnt<(NS > 2 ? 4 * PER : 0)>();
+    else if (behind >= 1) gr_wait_vmcnt<2 * PER>();
+    else gr_wait_vmcnt<0>();
+    asm volatile("" ::: "memory");
+  };
+  static_assert(NS <= 4 && 2 * (NS - 1) * PER < 64 && NS * BLOCKS <= 64, "load counters");
+#pragma unroll
+  for (int j = 0; j < NS - 1; ++j) ask();
+  int slot = 0;
+  auto enter = [&](int j) {
     if constexpr (SOLO) {
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // the slot's last reads are over
-      if (j + 1 < ntile) ask(j + 1);
-      // (a part-filled or bad next tile issues fewer loads: then all are waited for)
-      if (j + 1 < ntile && key_of(j + 1) + BN <= key1 && bad_next == 0) gr_wait_vmcnt<2 * PER>();
-      else gr_wait_vmcnt<0>();
-      asm volatile("" ::: "memory");
+      // the slot's last reads are over (no other wave reads it)
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      ask();
+      arrived(j);
     } else {
-      gr_wait_vmcnt<0>();
-      __syncthreads();                                         // tile j is there, and the other slot free
-      if (j + 1 < ntile) ask(j + 1);
+      arrived(j);
+      __syncthreads();                                         // tile j is there, and its predecessor's slot free
+      ask();
     }
-    const int k0 = key_of(j);
-    if (wave_live && j < ntile && k0 <= lim_hi) tile(j, slot, k0 + BN - 1 > lim_lo || bad != 0, bad);
   };
+  auto bad_at = [&](int j) { return (unsigned)(bads >> ((asked - 1 - j) * BLOCKS)) & ((1u << BLOCKS) - 1); };
+  // Tiles that every row of the wave sees in full, then the others (they end a
+  // row's keys): two loops, for a join of both kinds in one made the compiler
+  // copy the accumulators in every tile. The iterations' barriers are alike.
+  int j = 0;
 #pragma unroll 1
-  for (int j = 0; j < niter; ++j) step(j, j & 1);
+  for (; j < ntile && wave_live && key_of(j) + BN - 1 <= lim_lo && !uneven; ++j) {
+    enter(j);
+    tile(j, slot, 0u, gr_ic<0>{});
+    slot = slot + 1 == NS ? 0 : slot + 1;
+  }
+#pragma unroll 1
+  for (; j < niter; ++j) {
+    enter(j);
+    if (wave_live && j < ntile && key_of(j) <= lim_hi) tile(j, slot, bad_at(j), gr_ic<1>{});
+    slot = slot + 1 == NS ? 0 : slot + 1;
+  }
 
   if constexpr (KG > 1) {
     // the groups' partials through LDS: O as 4 DB quads of floats per lane,
@@ -617,10 +647,10 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
   }
 }
 
-// A workgroup of WAVES waves. Tiles of BM rows: NW waves by row, KG groups by
-// key, BN keys a step. KGS > 0: sequences of at most 32 rows (single tokens in a
+// Tiles of BM rows: NW waves by row, KG groups by key, BN keys a step, NS steps in
+// LDS. KGS > 0: sequences of at most 32 rows (single tokens in a
 // batch with long chunks) take tiles of 32, KGS waves sharing out the keys, 32 a step.
-template <class T, int D, int BN, int NW, int KG, int KGS, bool SHARED>
+template <class T, int D, int BN, int NW, int KG, int NS, int KGS, bool SHARED>
 __device__ __forceinline__ void gr_paged_body(const gr_paged_args& a, char* lds) {
   constexpr int BM = 32 * NW, WAVES = NW * KG;
   const int lane = threadIdx.x & 63;
@@ -629,9 +659,9 @@ __device__ __forceinline__ void gr_paged_body(const gr_paged_args& a, char* lds)
   gr_paged_seqs<BM, (KGS > 0)> seqs;
   auto segment = [&](int hk, int key0, int key1, int place) {
     if constexpr (KGS > 0) {
-      if (t.nrows <= 32) return gr_paged_segment<T, D, 32, 1, KGS, WAVES, BM>(a, lds, t, hk, key0, key1, place);
+      if (t.nrows <= 32) return gr_paged_segment<T, D, 32, 1, KGS, 2, WAVES, BM>(a, lds, t, hk, key0, key1, place);
     }
-    gr_paged_segment<T, D, BN, NW, KG, WAVES, BM>(a, lds, t, hk, key0, key1, place);
+    gr_paged_segment<T, D, BN, NW, KG, NS, WAVES, BM>(a, lds, t, hk, key0, key1, place);
   };
   if constexpr (!SHARED) {
     // key head slowest, then the tiles: workgroups of one key head share an XCD's L2

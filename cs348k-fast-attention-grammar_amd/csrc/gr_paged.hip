@@ -13,19 +13,19 @@ namespace {
 
 constexpr int imax(int a, int b) { return a > b ? a : b; }
 
-template <int D, int BN, int NW, int KG, int KGS>
+template <int D, int BN, int NW, int KG, int NS, int KGS>
 struct Lds {
-  static constexpr int BYTES = imax(gr_paged_lds<D, BN, NW, KG>::BYTES, gr_paged_lds<D, 32, 1, KGS ? KGS : 1>::BYTES);
+  static constexpr int BYTES = imax(gr_paged_lds<D, BN, NW, KG, NS>::BYTES, KGS ? gr_paged_lds<D, 32, 1, KGS ? KGS : 1, 2>::BYTES : 0);
 };
 
 // One workgroup of four waves a CU where its LDS allows no two, else (and with
 // eight waves) two waves a SIMD.
-template <class T, int D, int BN, int NW, int KG, int KGS, bool SHARED>
+template <class T, int D, int BN, int NW, int KG, int NS, int KGS, bool SHARED>
 __global__ __launch_bounds__(64 * NW * KG)
-__attribute__((amdgpu_waves_per_eu(NW* KG == 4 && Lds<D, BN, NW, KG, KGS>::BYTES > 80 * 1024 ? 1 : 2)))
+__attribute__((amdgpu_waves_per_eu(NW* KG == 4 && Lds<D, BN, NW, KG, NS, KGS>::BYTES > 80 * 1024 ? 1 : 2)))
 void gr_paged_kernel(gr_paged_args a) {
   extern __shared__ __attribute__((aligned(16))) char gr_lds[];
-  gr_paged_body<T, D, BN, NW, KG, KGS, SHARED>(a, gr_lds);
+  gr_paged_body<T, D, BN, NW, KG, NS, KGS, SHARED>(a, gr_lds);
 }
 
 template <class T, int D, int BM, bool SMALL>
@@ -52,24 +52,35 @@ Plan plan_of(const gr_paged_cache& c, const gr_paged_batch& b, int Hq) {
   const int resident = cus * (D == 128 && p.nw < 4 ? 1 : 2);      // workgroups (their LDS)
   const long long cap = (long long)b.width * c.page_size;
   const long long len = b.max_len > 0 && b.max_len < cap ? b.max_len : cap;
+  // Work is shared out from a length on that grows with the workgroups that one a
+  // tile would make: in brackets shared / a workgroup a tile, lengths spread by a
+  // half around the mean. One token, D 128: 64 tiles, mean 600 keys 13.8 / 15.5 us,
+  // 400 13.7 / 12.8; 256 tiles, 2,400 52.0 / 55.4, 1,200 32.5 / 31.2. D 64: 64
+  // tiles, 1,200 12.7 / 16.3, 600 12.3 / 10.6; 512 tiles, 4,800 115.7 / 114.7. Chunks
+  // of 128-row tiles: 12 tiles, D 128, 1,024 keys 24.7 / 30.8, 512 20.6 / 19.2; 528
+  // tiles, 16,384 keys 612 / 578.
   const long long wgs = p.tiles * c.heads;
-  p.shares = wgs >= (p.nw < 4 ? 4LL : 1LL) * resident || len <= 512 || p.tiles * c.heads * (cap / 64 + 1 + GR_PAGED_COST) > 0x7fffffffLL ? 0
-             : resident < GR_PAGED_MAX_SHARES ? resident : GR_PAGED_MAX_SHARES;
+  const double fill = wgs < resident ? (double)wgs / resident : 1.0;
+  const double least = p.nw == 4 ? 1000 : D == 64 ? 1200 : 900, slope = p.nw == 4 ? 6500 : D == 64 ? 7000 : 3000;
+  const double from = slope * fill > least ? slope * fill : least;
+  const bool shared = (double)len > from && !(p.nw == 4 && wgs >= resident)
+                      && p.tiles * c.heads * (cap / 64 + 1 + GR_PAGED_COST) <= 0x7fffffffLL;
+  p.shares = !shared ? 0 : resident < GR_PAGED_MAX_SHARES ? resident : GR_PAGED_MAX_SHARES;
   return p;
 }
 
 size_t share_bytes(const Plan& p, int D) { return (size_t)2 * 32 * p.nw * (D + 2) * sizeof(float); }
 
-template <class T, int D, int BN, int NW, int KG, int KGS>
+template <class T, int D, int BN, int NW, int KG, int NS, int KGS>
 int launch_tiles(const gr_paged_args& a, hipStream_t st) {
-  constexpr int BM = 32 * NW, LDS = Lds<D, BN, NW, KG, KGS>::BYTES;
+  constexpr int BM = 32 * NW, LDS = Lds<D, BN, NW, KG, NS, KGS>::BYTES;
   const long long wgs = (long long)a.tiles * a.Hkv;
   const dim3 block(64 * NW * KG);
   if (a.shares == 0) {
-    hipLaunchKernelGGL((gr_paged_kernel<T, D, BN, NW, KG, KGS, false>), dim3((unsigned)wgs), block, LDS, st, a);
+    hipLaunchKernelGGL((gr_paged_kernel<T, D, BN, NW, KG, NS, KGS, false>), dim3((unsigned)wgs), block, LDS, st, a);
     return gr::hip_check(hipGetLastError(), GR_E_LAUNCH, "gr_paged_attn launch");
   }
-  hipLaunchKernelGGL((gr_paged_kernel<T, D, BN, NW, KG, KGS, true>), dim3((unsigned)a.shares), block, LDS, st, a);
+  hipLaunchKernelGGL((gr_paged_kernel<T, D, BN, NW, KG, NS, KGS, true>), dim3((unsigned)a.shares), block, LDS, st, a);
   const int rc = gr::hip_check(hipGetLastError(), GR_E_LAUNCH, "gr_paged_attn launch");
   if (rc) return rc;
   const int rows = a.starts ? BM : (a.rows * a.G < BM ? a.rows * a.G : BM);      // of a tile, at most
@@ -83,9 +94,9 @@ int launch_tiles(const gr_paged_args& a, hipStream_t st) {
 
 template <class T, int D>
 int launch(const gr_paged_args& a, int nw, hipStream_t st) {
-  if (nw == 1) return launch_tiles<T, D, 32, 1, 4, 0>(a, st);
-  if (nw == 2) return launch_tiles<T, D, 32, 2, 4, 0>(a, st);
-  return launch_tiles<T, D, 64, 4, 1, D == 64 ? 4 : 2>(a, st);
+  if (nw == 1) return launch_tiles<T, D, 32, 1, 4, 2, 0>(a, st);
+  if (nw == 2) return launch_tiles<T, D, 32, 2, 4, 2, 0>(a, st);
+  return launch_tiles<T, D, 64, 4, 1, 2, D == 64 ? 4 : 2>(a, st);
 }
 
 int check_heads(const gr_paged_cache* c, const gr_paged_batch* b, int Hq) {
