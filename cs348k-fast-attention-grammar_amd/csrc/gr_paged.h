@@ -409,12 +409,8 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
         pt[x] = gr_as<vec8>(pw);
       }
     };
-    bool ok = !gr_any(fresh);
-    if (ok) {
-      make_p(m == -GR_INF ? 0.f : -m * c);
-      ok = !gr_any(!(lt <= GR_FLASH_SUM_MAX));
-    }
-    if (!ok) {
+    make_p(m == -GR_INF ? 0.f : -m * c);
+    if (gr_any(fresh || !(lt <= GR_FLASH_SUM_MAX))) {
       float mt = -GR_INF;
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
@@ -533,9 +529,10 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
     asm volatile("" ::: "memory");
   };
   static_assert(NS <= 4 && 2 * (NS - 1) * PER < 64 && NS * BLOCKS <= 64, "load counters");
+  auto barrier = [&] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+  int j = 0, slot = 0;
 #pragma unroll
-  for (int j = 0; j < NS - 1; ++j) ask();
-  int slot = 0;
+  for (int i = 0; i < NS - 1; ++i) ask();
   auto enter = [&](int j) {
     if constexpr (SOLO) {
       // the slot's last reads are over (no other wave reads it)
@@ -544,7 +541,7 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
       arrived(j);
     } else {
       arrived(j);
-      __syncthreads();                                         // tile j is there, and its predecessor's slot free
+      barrier();                                               // tile j is there, and its predecessor's slot free
       ask();
     }
   };
@@ -552,7 +549,6 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
   // Tiles that every row of the wave sees in full, then the others (they end a
   // row's keys): two loops, for a join of both kinds in one made the compiler
   // copy the accumulators in every tile. The iterations' barriers are alike.
-  int j = 0;
 #pragma unroll 1
   for (; j < ntile && wave_live && key_of(j) + BN - 1 <= lim_lo && !uneven; ++j) {
     enter(j);

@@ -206,6 +206,9 @@ def rotary(q, k, positions, rot: Rotary):
     """rotary_fwd, differentiable in q and k (either may need no gradient; k
     may be None): both rotations are one launch of gr_rotary, and so are their
     gradients."""
+    import torch
+    if not torch.is_grad_enabled() or not (q.requires_grad or (k is not None and k.requires_grad)):
+        return rotary_fwd(_dense(q), None if k is None else _dense(k), positions, rot)
     global _ROTARY_FN
     if _ROTARY_FN is None:
         _ROTARY_FN = _autograd_function()

@@ -195,21 +195,49 @@ def test_whole_prompts(dtype, D):
     _run(s, [1111, 130], 8, ragged=True)
 
 
+def _needs_workspace(s, rows, Hq, starts=None):
+    import ctypes
+    from grammar import runtime as rt
+    batch = rt.PagedBatch(s.table.data_ptr(), s.width, s.lens.data_ptr(), starts, len(s.lens_host), rows, s.width, 0, 0)
+    return int(rt.lib().gr_paged_attn_workspace(s.cache.ref, ctypes.addressof(batch), Hq))
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n,G,Hkv", [(1, 4, 2), (1, 1, 3), (5, 7, 1), (3, 20, 1), (50, 4, 1)])
+def test_shared_work_of_ragged_lengths(dtype, D, n, G, Hkv):
+    """A table with room for long contexts, so that the work is shared out, over short, empty and long sequences:
+    shares that end in a tile's first, last and only blocks, and tiles of one share and of many."""
+    lens = [m + n - 1 for m in LENS] + [0, 3000, 64, 128, 5000, n]
+    s = Setup(lens, Hkv, 16, D, dtype, seed=n, width=1024)
+    print(f"[case] shared {dtype} D{D} n{n} G{G} Hkv{Hkv}", flush=True)
+    assert _needs_workspace(s, n, G * Hkv) > 0
+    _run(s, [n] * len(lens), G * Hkv, hints=False, strided=True)
+
+
+@pytest.mark.parametrize("dtype,D,G,Hkv", [("bf16", 128, 4, 2), ("fp16", 64, 1, 4)])
+def test_shared_mixed_batches(dtype, D, G, Hkv):
+    news = [1, 0, 150, 1, 7, 0, 1, 301, 1, 0] + [1] * 70
+    lens = [40, 99, 150, 4000, 7, 0, 1, 900, 0, 5] + [3 * i for i in range(70)]
+    s = Setup(lens, Hkv, 16, D, dtype, seed=D, width=2048)
+    print(f"[case] shared mixed {dtype} D{D} G{G}", flush=True)
+    assert _needs_workspace(s, sum(news) + 5, G * Hkv, s.lens.data_ptr()) > 0
+    for causal in (True, False):
+        _run(s, news, G * Hkv, causal=causal, ragged=True, pad=5, hints=False)
+
+
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("n", [1, 40])
 def test_long_contexts_share_their_keys_out(D, n):
     """Keys over several workgroups and merged: as many as the default takes, fewer with a smaller workspace, none
     with an empty one; each twice, bit for bit the same."""
-    from grammar import runtime as rt
     from grammar.paged import paged_attention
     lens = [20_011, 3, 5000]
     s = Setup(lens, 2, 32, D, "bf16", seed=D)
     print(f"[case] long D{D} n{n}", flush=True)
     _run(s, [n] * 3, 8)
     q = s.randn(3, 8, n, D)
-    import ctypes
-    batch = rt.PagedBatch(s.table.data_ptr(), s.width, s.lens.data_ptr(), None, 3, n, s.width, 0, 0)
-    need = int(rt.lib().gr_paged_attn_workspace(s.cache.ref, ctypes.addressof(batch), 8))
+    need = _needs_workspace(s, n, 8)
     assert need > 0
     for size in (need, need // 2, need // 5, need // 100, 16, 0):
         ws = torch.empty(size, dtype=torch.uint8, device=s.dev)
@@ -222,11 +250,12 @@ def test_long_contexts_share_their_keys_out(D, n):
 
 @pytest.mark.parametrize("dtype,D", [("bf16", 128), ("fp16", 64), ("fp16", 128)])
 @pytest.mark.parametrize("n,G", [(1, 4), (9, 4), (70, 2)])
-def test_hidden_entries_may_hold_anything(dtype, D, n, G):
+@pytest.mark.parametrize("width", [None, 2048], ids=["tile", "shared"])
+def test_hidden_entries_may_hold_anything(dtype, D, n, G, width):
     """Stale slots and pages of other sequences hold NaN; a value that only later tokens see holds inf or NaN, and
     so do they, but no earlier row."""
     lens = [n, n + 7, n + 100, 200 + n]
-    s = Setup(lens, 2, 16, D, dtype, seed=n)
+    s = Setup(lens, 2, 16, D, dtype, seed=n, width=width)
     nan = float("nan")
     live = torch.zeros(s.k.shape[0], s.S, dtype=torch.bool)
     for b, m in enumerate(lens):
@@ -235,8 +264,8 @@ def test_hidden_entries_may_hold_anything(dtype, D, n, G):
     dead = (~live).to(s.dev)[:, None, :, None]
     s.k.masked_fill_(dead, nan)
     s.v.masked_fill_(dead, nan)
-    print(f"[case] hidden {dtype} D{D} n{n}", flush=True)
-    assert _run(s, [n] * 4, 2 * G).isfinite().all()
+    print(f"[case] hidden {dtype} D{D} n{n} width {width}", flush=True)
+    assert _run(s, [n] * 4, 2 * G, hints=False).isfinite().all()
     if n == 1:
         return
     # the last token's entries: NaN key in head 0; inf and NaN values in head 1, and a finite huge one
@@ -244,21 +273,22 @@ def test_hidden_entries_may_hold_anything(dtype, D, n, G):
         page, slot = int(s.table[b, (m - 1) // s.S]), (m - 1) % s.S
         s.k[page, 0, slot, 3] = nan
         s.v[page, 1, slot, 5], s.v[page, 1, slot, D - 1] = float("inf"), nan
-    out = _run(s, [n] * 4, 2 * G)
+    out = _run(s, [n] * 4, 2 * G, hints=False)
     assert out[:3, :, :-1].isfinite().all()                     # earlier rows
     assert out[:3, :G, -1].isnan().all() and out[:3, G:, -1, 5].isinf().all() and out[:3, G:, -1, D - 1].isnan().all()
 
 
-def test_pages_that_do_not_exist():
+@pytest.mark.parametrize("width", [None, 2048], ids=["tile", "shared"])
+def test_pages_that_do_not_exist(width):
     """Page ids out of range, keys behind the table and starts out of the batch read nothing."""
     from grammar.paged import paged_attention
-    s = Setup([100, 100, 64], 2, 16, 64, "bf16", seed=1)
+    s = Setup([100, 100, 64], 2, 16, 64, "bf16", seed=1, width=width)
     s.table[0, 2], s.table[0, 6], s.table[1, 0] = -1, s.k.shape[0], 2 ** 31 - 1
     s.table[2, :4] = -7
     for n in (1, 20):
-        out = _run(s, [n] * 3, 4)
+        out = _run(s, [n] * 3, 4, hints=False)
         assert not out[2].any()
-    s.lens_host[1] = 10_000                                     # more keys than the table holds
+    s.lens_host[1] = 50_000                                     # more keys than the table holds
     s.lens.copy_(torch.tensor(s.lens_host, dtype=torch.int32))
     _run(s, [1] * 3, 4, hints=False)
     s.lens_host[1] = -5
@@ -537,7 +567,6 @@ def test_bound_steps_on_streams_and_in_graphs():
 
 
 def test_scratch_goes_back_to_the_launch_stream():
-    from grammar import runtime as rt
     from grammar.paged import paged_attention
     s = Setup([60_000], 1, 64, 128, "fp16", seed=1)
     q = s.randn(1, 8, 40, 128)
@@ -549,9 +578,7 @@ def test_scratch_goes_back_to_the_launch_stream():
     def free():
         return sum(b["size"] for seg in torch.cuda.memory_snapshot() if seg["stream"] == side.cuda_stream
                    for b in seg["blocks"] if b["state"] == "inactive")
-    import ctypes
-    batch = rt.PagedBatch(s.table.data_ptr(), s.width, s.lens.data_ptr(), None, 1, 40, s.width, 0, 0)
-    need = int(rt.lib().gr_paged_attn_workspace(s.cache.ref, ctypes.addressof(batch), 8))
+    need = _needs_workspace(s, 40, 8)
     before = free()
     got = paged_attention(q, s.cache, s.table, s.lens, stream=side)
     torch.cuda.synchronize()
