@@ -292,45 +292,44 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
   auto key_of = [&](int j) { return key0 + (j * KG + kg) * BN; };
   // Where the blocks of this group's tiles are: lane l has block l % BLOCKS of
   // tile j0 + l / BLOCKS, its K and V addresses and (a bit each) whether its page
-  // exists; refilled every 64 / BLOCKS tiles, the page ids read a window ahead. A
-  // tile's loads take their scalar bases from it by lane reads (worked out by
-  // scalar multiplications they cost more than the loads).
+  // exists; refilled every 64 / BLOCKS tiles. A tile's loads take their scalar
+  // bases from it by lane reads (worked out by scalar multiplications they cost more
+  // than the loads). The page ids are read when a window begins, not ahead: kept
+  // over the tiles in a register, they made the compiler wait for all loads in
+  // every tile.
   constexpr int WIN = 64 / BLOCKS;
   auto id_of = [&](int j0) {
     const long long key = key0 + ((long long)(j0 + lane / BLOCKS) * KG + kg) * BN + 16 * (lane % BLOCKS);
     return tab[key >> a.page_shift < a.width ? (int)(key >> a.page_shift) : a.width - 1];
   };
   unsigned long long kwin = 0, vwin = 0, badwin = 0;
-  int next_id = 0;
   auto refill = [&](int j0, int id) {
-    const int slot = (key0 + ((j0 + lane / BLOCKS) * KG + kg) * BN + 16 * (lane % BLOCKS)) & smask;
+    const int key = key0 + ((j0 + lane / BLOCKS) * KG + kg) * BN + 16 * (lane % BLOCKS), slot = key & smask;
     const bool ok = (unsigned)id < (unsigned)a.pages;
     kwin = (unsigned long long)(kp + (ok ? id : 0) * a.k_sp + slot * a.k_ss);
     vwin = (unsigned long long)(vp + (ok ? id : 0) * a.v_sp + slot * a.v_ss);
-    badwin = __builtin_amdgcn_ballot_w64(!ok);
-    if (j0 + WIN < ntile) next_id = id_of(j0 + WIN);
+    badwin = __builtin_amdgcn_ballot_w64(!ok && key < key1);
   };
-  auto bad_of = [&](int j) { return (unsigned)(badwin >> ((j % WIN) * BLOCKS)) & ((1u << BLOCKS) - 1); };
   auto lane64 = [&](unsigned long long w, int l) {
     return (unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)(w >> 32), l) << 32
            | (unsigned)__builtin_amdgcn_readlane((int)(unsigned)w, l);
   };
   const unsigned kring = __builtin_amdgcn_readfirstlane((int)gr_lds_addr(ks0));
-  auto load = [&](int j, int slot) {
-    const int k0 = key_of(j);
-    const unsigned bad = bad_of(j);
-    const bool whole = bad == 0 && k0 + BN <= key1;
+  // Asks for tile j: 2 PER loads of the wave if all of its keys are there.
+  auto load = [&](int j, int slot, auto whole_tag, unsigned bad) {
+    constexpr bool WHOLE = decltype(whole_tag)::value;
+    const int at = (j & (WIN - 1)) * BLOCKS;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int instr = wave + i * NW, bl = instr / IPB;
-      const unsigned long long kb = lane64(kwin, (j % WIN) * BLOCKS + bl), vb = lane64(vwin, (j % WIN) * BLOCKS + bl);
+      const unsigned long long kb = lane64(kwin, at + bl), vb = lane64(vwin, at + bl);
       const unsigned kl = kring + slot * L::TILE + instr * 1024, vl = kl + NS * L::TILE;
-      if (whole) {
+      if constexpr (WHOLE) {
         gr_g2lds16s(kb, koff[i % SUBS], kl);
         gr_g2lds16s(vb, voff[i % SUBS], vl);
       } else {
         char* const kd = ks0 + slot * L::TILE + instr * 1024 + lane * 16;
-        const int r = block_row(i), kblk = k0 + 16 * bl;
+        const int r = block_row(i), kblk = key_of(j) + 16 * bl;
         const bool ok = !(bad >> bl & 1);
         if (ok && kblk + gr_perm32(r) < key1) gr_g2lds16s(kb, koff[i % SUBS], kl);
         else gr_st16(kd, (gr_u32x4){0, 0, 0, 0});
@@ -505,30 +504,46 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
   // the loop's back edge that they came
 #pragma unroll
   for (int ds = 0; ds < DS; ++ds) asm volatile("" : "+v"(qf[ds]));
+  // Leading tiles of the group that end before key `end`.
+  auto tiles_before = [&](int end) { return end - key0 < (kg + 1) * BN ? 0 : ((end - key0) / BN - kg + KG - 1) / KG; };
+  const int nwhole = gr_imin(ntile, tiles_before(key1));
+  // Tiles are asked for in order. Up to `plain` they are whole and their pages
+  // are in the window and exist; the next one is looked at closer.
+  int asked = 0, to = 0, plain = 0;           // (to: the next one's slot)
+  unsigned long long bads = 0;                // bad blocks of the last tiles asked for, newest first
   // A tile that is part-filled or has a bad page issues fewer loads than 2 PER:
   // from the first such one on, every load is waited for.
   bool uneven = false;
-  int asked = 0, to = 0;                      // tiles asked for; the next one's slot
-  unsigned long long bads = 0;                // bad blocks of the last tiles asked for, newest first
   auto ask = [&]() {
-    if (asked >= ntile) return;
-    if (asked > 0 && asked % WIN == 0) refill(asked, next_id);
-    load(asked, to);
-    uneven |= bad_of(asked) != 0 || key_of(asked) + BN > key1;
-    bads = bads << BLOCKS | bad_of(asked);
+    if (asked < plain) {
+      load(asked, to, gr_ic<1>{}, 0u);
+      bads <<= BLOCKS;
+    } else {
+      if (asked >= ntile) return;
+      if (asked > 0 && (asked & (WIN - 1)) == 0) refill(asked, id_of(asked));
+      const unsigned bad = (unsigned)(badwin >> ((asked & (WIN - 1)) * BLOCKS)) & ((1u << BLOCKS) - 1);
+      bads = bads << BLOCKS | bad;
+      if (bad == 0 && asked < nwhole) {
+        load(asked, to, gr_ic<1>{}, 0u);
+      } else {
+        load(asked, to, gr_ic<0>{}, bad);
+        uneven = true;
+      }
+      plain = badwin == 0 ? gr_imin(nwhole, (asked & ~(WIN - 1)) + WIN) : 0;
+    }
     ++asked;
     to = to + 1 == NS ? 0 : to + 1;
   };
-  // Waits for all but the tiles behind tile j.
+  // Waits for all but the tiles behind tile j (a barrier's waves wait before they ask on).
+  constexpr int AHEAD = SOLO ? NS - 1 : NS - 2;
   auto arrived = [&](int j) {
     const int behind = uneven ? 0 : asked - 1 - j;
-    if (NS > 3 && behind >= 3) gr_wait_vmcnt<(NS > 3 ? 6 * PER : 0)>();
-    else if (NS > 2 && behind >= 2) gr_wait_vmcnt<(NS > 2 ? 4 * PER : 0)>();
-    else if (behind >= 1) gr_wait_vmcnt<2 * PER>();
+    if (AHEAD >= 2 && behind >= 2) gr_wait_vmcnt<(AHEAD >= 2 ? 4 * PER : 0)>();
+    else if (AHEAD >= 1 && behind >= 1) gr_wait_vmcnt<2 * PER>();
     else gr_wait_vmcnt<0>();
     asm volatile("" ::: "memory");
   };
-  static_assert(NS <= 4 && 2 * (NS - 1) * PER < 64 && NS * BLOCKS <= 64, "load counters");
+  static_assert(NS <= 3 && 2 * (NS - 1) * PER < 64 && NS * BLOCKS <= 64, "load counters");
   auto barrier = [&] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
   int j = 0, slot = 0;
 #pragma unroll
@@ -549,8 +564,9 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
   // Tiles that every row of the wave sees in full, then the others (they end a
   // row's keys): two loops, for a join of both kinds in one made the compiler
   // copy the accumulators in every tile. The iterations' barriers are alike.
+  const int nclean = wave_live ? gr_imin(nwhole, tiles_before(lim_lo + 1)) : 0;
 #pragma unroll 1
-  for (; j < ntile && wave_live && key_of(j) + BN - 1 <= lim_lo && !uneven; ++j) {
+  for (; j < nclean && !uneven; ++j) {
     enter(j);
     tile(j, slot, 0u, gr_ic<0>{});
     slot = slot + 1 == NS ? 0 : slot + 1;

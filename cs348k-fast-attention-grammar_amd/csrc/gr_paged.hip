@@ -44,14 +44,21 @@ Plan plan_of(const gr_paged_cache& c, const gr_paged_batch& b, int Hq) {
   Plan p;
   const int G = Hq / c.heads, D = c.head_dim;
   const long long most = b.starts && b.max_new > 0 && b.max_new < b.rows ? b.max_new : b.rows;
+  const int cus = gr::cu_count() > 0 ? gr::cu_count() : 256;
+  const long long cap = (long long)b.width * c.page_size;
+  const long long len = b.max_len > 0 && b.max_len < cap ? b.max_len : cap;
   p.nw = most * G <= 32 ? 1 : most * G <= 64 ? 2 : 4;
+  // Chunks whose tiles of 128 rows would leave most CUs idle take tiles of 64
+  // with four key groups: 16 or 64 tiles (one chunk of 512, 4 key heads, G 1 or 4)
+  // at 512 keys 13.0 us to 9.4 and 13.0 to 9.8 (D 64), 18.1 to 13.4 and 18.5 to
+  // 14.1 (D 128). Over longer contexts, where keys are shared out anyway, only at D
+  // 128 (16 tiles, 2,048 keys 30 to 22 us, 64 tiles, 8,192 keys 62 to 71).
+  const long long rows128 = (b.starts ? (long long)b.rows : (long long)b.B * b.rows) * G / 128 * c.heads;
+  if (p.nw == 4 && (len <= 1000 ? 4 * rows128 <= cus : D == 128 && 4 * rows128 < cus)) p.nw = 2;
   const int BM = 32 * p.nw;
   // packed rows: every sequence may have a part-filled tile
   p.tiles = b.starts ? (long long)b.rows * G / BM + b.B : (long long)b.B * (((long long)b.rows * G + BM - 1) / BM);
-  const int cus = gr::cu_count() > 0 ? gr::cu_count() : 256;
   const int resident = cus * (D == 128 && p.nw < 4 ? 1 : 2);      // workgroups (their LDS)
-  const long long cap = (long long)b.width * c.page_size;
-  const long long len = b.max_len > 0 && b.max_len < cap ? b.max_len : cap;
   // Work is shared out from a length on that grows with the workgroups that one a
   // tile would make: in brackets shared / a workgroup a tile, lengths spread by a
   // half around the mean. One token, D 128: 64 tiles, mean 600 keys 13.8 / 15.5 us,
