@@ -85,39 +85,38 @@ def _batch(cache, table, lens, starts, x, name, max_new, max_len, who):
                          B, lead[-1], width, int(max_new), int(max_len)), lead
 
 
-def _heads_ok(t, name, lead, heads, cache, who):
+def _heads(t, name, lead, heads, cache, who):
+    """The strides of `heads` heads of the tokens `lead`, checked."""
     want = (lead[0], heads, lead[1], cache.head_dim) if len(lead) == 2 else (lead[0], heads, cache.head_dim)
     if t.shape != want or t.dtype != cache.dtype or t.get_device() != cache.index:
         raise ValueError(f"{who}: {name} must be {want} {cache.dtype} on {cache.k.device} (no CPU path), not "
                          f"{tuple(t.shape)} {t.dtype} on {t.device}")
+    return head_strides(t, name, who)
 
 
 def _append_args(k, v, cache, table, lens, starts, q, rotary, positions, max_new, out):
     who = "paged_append"
     desc, lead = _batch(cache, table, lens, starts, k, "k", max_new, 0, who)
-    _heads_ok(k, "k", lead, cache.heads, cache, who)
-    _heads_ok(v, "v", lead, cache.heads, cache, who)
-    head = (cache.ref, ctypes.addressof(desc), rotary.ref if rotary is not None else None)
-    if rotary is not None and (rotary.head_dim != cache.head_dim or rotary.index != cache.index):
+    ks, vs = _heads(k, "k", lead, cache.heads, cache, who), _heads(v, "v", lead, cache.heads, cache, who)
+    if rotary is None:
+        if q is not None or positions is not None:
+            raise ValueError(f"{who}: q is only rotated here, and positions only turn: both need `rotary`")
+        ref = None
+    elif rotary.head_dim != cache.head_dim or rotary.index != cache.index:
         raise ValueError(f"{who}: the rotation is for heads of {rotary.head_dim} on {rotary.device}")
-    if q is None:
-        if out is not None:
-            raise ValueError(f"{who}: `out` is the queries' and needs q")
-        head += (None, None, 0, None, None)
     else:
-        if rotary is None:
-            raise ValueError(f"{who}: q is only rotated here, which needs `rotary`")
+        ref = rotary.ref
+    if q is not None:
         Hq = q.shape[1] if q.dim() >= 3 else 0
-        _heads_ok(q, "q", lead, Hq, cache, who)
-        out = check_out(out, q, "out", who)
-        head += (q.data_ptr(), out.data_ptr(), Hq, head_strides(q, "q", who), head_strides(out, "out", who))
-    if positions is None:
-        place = (None, None)
+        qs, out = _heads(q, "q", lead, Hq, cache, who), check_out(out, q, "out", who)
+        qp, op, os = q.data_ptr(), out.data_ptr(), head_strides(out, "out", who)
+    elif out is None:
+        qp = op = qs = os = None
+        Hq = 0
     else:
-        if rotary is None:
-            raise ValueError(f"{who}: positions need `rotary`")
-        place = (positions.data_ptr(), check_positions(positions, rotary, lead, who))
-    args = head + (k.data_ptr(), v.data_ptr(), head_strides(k, "k", who), head_strides(v, "v", who)) + place
+        raise ValueError(f"{who}: `out` is the queries' and needs q")
+    pp, ps = (None, None) if positions is None else (positions.data_ptr(), check_positions(positions, rotary, lead, who))
+    args = (cache.ref, ctypes.addressof(desc), ref, qp, op, Hq, qs, os, k.data_ptr(), v.data_ptr(), ks, vs, pp, ps)
     return args, out, (desc, k, v, cache, table, lens, starts, q, rotary, positions, out)
 
 
@@ -152,7 +151,7 @@ def _attn_args(q, cache, table, lens, starts, causal, scale, max_new, max_len, o
     who = "paged_attention"
     desc, lead = _batch(cache, table, lens, starts, q, "q", max_new, max_len, who)
     Hq = q.shape[1]
-    _heads_ok(q, "q", lead, Hq, cache, who)
+    qs = _heads(q, "q", lead, Hq, cache, who)
     if Hq == 0 or Hq % cache.heads:
         raise ValueError(f"{who}: {Hq} query heads are not a multiple of the cache's {cache.heads}")
     out = check_out(out, q, "out", who)
@@ -168,7 +167,7 @@ def _attn_args(q, cache, table, lens, starts, causal, scale, max_new, max_len, o
         workspace = rt.workspace(need, q.device, stream)
     size = workspace.numel() * workspace.element_size() if workspace is not None else 0
     args = (cache.ref, ref, q.data_ptr(), out.data_ptr(), lse.data_ptr() if lse is not None else None, Hq,
-            head_strides(q, "q", who), head_strides(out, "out", who), int(bool(causal)), float(scale),
+            qs, head_strides(out, "out", who), int(bool(causal)), float(scale),
             workspace.data_ptr() if workspace is not None else None, size)
     return args, out, (desc, q, cache, table, lens, starts, out, lse, workspace)
 

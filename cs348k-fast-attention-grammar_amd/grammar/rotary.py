@@ -95,7 +95,7 @@ def check_positions(positions, rot, lead: tuple, who: str):
     return ps
 
 
-@functools.lru_cache(maxsize=1024)
+@functools.lru_cache(maxsize=4096)
 def _head_strides(shape: tuple, st: tuple):
     if st[-1] != 1:
         return None
