@@ -186,16 +186,70 @@ struct gr_paged_cut {
   }
 };
 
-// global_load_lds_dwordx4 from a scalar base plus a lane offset in bytes (see
-// gr_g2lds16); M0 holds the LDS address.
+// global_load_lds_dwordx4 from scalar bases plus lane offsets in bytes (see
+// gr_g2lds16); M0 holds the LDS address. The bases come from lane reads, which are
+// vector instructions: a memory instruction may read a scalar register no sooner
+// than five wait states after one wrote it. The compiler cannot see these loads,
+// so the wait (s_nop 4) is part of each group.
 __device__ __forceinline__ void gr_g2lds16s(unsigned long long base, unsigned off, unsigned lds) {
   asm volatile(
       "s_mov_b32 m0, %2\n\t"
-      "s_nop 0\n\t"
+      "s_nop 4\n\t"
       "global_load_lds_dwordx4 %0, %1"
       :
       : "v"(off), "s"(base), "s"(lds)
       : "memory", "m0");
+}
+
+// N loads of K and N of V, the K loads STEP bytes of LDS apart, V's VOFF behind.
+template <int N, int STEP, int VOFF>
+__device__ __forceinline__ void gr_g2lds16_kv(unsigned long long kb, unsigned long long vb, const unsigned* koff,
+                                              const unsigned* voff, unsigned lds) {
+  static_assert(N == 1 || N == 2 || N == 4, "loads of a group");
+  if constexpr (N == 1)
+    asm volatile(
+        "s_mov_b32 m0, %4\n\ts_nop 4\n\t"
+        "global_load_lds_dwordx4 %0, %2\n\t"
+        "s_add_u32 m0, m0, %5\n\ts_nop 0\n\t"
+        "global_load_lds_dwordx4 %1, %3"
+        :
+        : "v"(koff[0]), "v"(voff[0]), "s"(kb), "s"(vb), "s"(lds), "n"(VOFF)
+        : "memory", "m0", "scc");
+  else if constexpr (N == 2)
+    asm volatile(
+        "s_mov_b32 m0, %6\n\ts_nop 4\n\t"
+        "global_load_lds_dwordx4 %0, %4\n\t"
+        "s_add_u32 m0, m0, %7\n\ts_nop 0\n\t"
+        "global_load_lds_dwordx4 %1, %4\n\t"
+        "s_add_u32 m0, m0, %8\n\ts_nop 0\n\t"
+        "global_load_lds_dwordx4 %2, %5\n\t"
+        "s_add_u32 m0, m0, %7\n\ts_nop 0\n\t"
+        "global_load_lds_dwordx4 %3, %5"
+        :
+        : "v"(koff[0]), "v"(koff[1]), "v"(voff[0]), "v"(voff[1]), "s"(kb), "s"(vb), "s"(lds), "n"(STEP), "n"(VOFF - STEP)
+        : "memory", "m0", "scc");
+  else
+    asm volatile(
+        "s_mov_b32 m0, %10\n\ts_nop 4\n\t"
+        "global_load_lds_dwordx4 %0, %8\n\t"
+        "s_add_u32 m0, m0, %11\n\ts_nop 0\n\t"
+        "global_load_lds_dwordx4 %1, %8\n\t"
+        "s_add_u32 m0, m0, %11\n\ts_nop 0\n\t"
+        "global_load_lds_dwordx4 %2, %8\n\t"
+        "s_add_u32 m0, m0, %11\n\ts_nop 0\n\t"
+        "global_load_lds_dwordx4 %3, %8\n\t"
+        "s_add_u32 m0, m0, %12\n\ts_nop 0\n\t"
+        "global_load_lds_dwordx4 %4, %9\n\t"
+        "s_add_u32 m0, m0, %11\n\ts_nop 0\n\t"
+        "global_load_lds_dwordx4 %5, %9\n\t"
+        "s_add_u32 m0, m0, %11\n\ts_nop 0\n\t"
+        "global_load_lds_dwordx4 %6, %9\n\t"
+        "s_add_u32 m0, m0, %11\n\ts_nop 0\n\t"
+        "global_load_lds_dwordx4 %7, %9"
+        :
+        : "v"(koff[0]), "v"(koff[1]), "v"(koff[2]), "v"(koff[3]), "v"(voff[0]), "v"(voff[1]), "v"(voff[2]), "v"(voff[3]),
+          "s"(kb), "s"(vb), "s"(lds), "n"(STEP), "n"(VOFF - 3 * STEP)
+        : "memory", "m0", "scc");
 }
 
 // XOR swizzle of K's 16-byte chunks for reads of consecutive rows at one logical
@@ -315,26 +369,29 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
            | (unsigned)__builtin_amdgcn_readlane((int)(unsigned)w, l);
   };
   const unsigned kring = __builtin_amdgcn_readfirstlane((int)gr_lds_addr(ks0));
-  // Asks for tile j: 2 PER loads of the wave if all of its keys are there.
+  // Asks for tile j: 2 PER loads of the wave if all of its keys are there, SUBS of
+  // K and of V for each block that it has a part of.
   auto load = [&](int j, int slot, auto whole_tag, unsigned bad) {
     constexpr bool WHOLE = decltype(whole_tag)::value;
     const int at = (j & (WIN - 1)) * BLOCKS;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int instr = wave + i * NW, bl = instr / IPB;
+    for (int n = 0; n < PER / SUBS; ++n) {
+      const int instr = wave + n * SUBS * NW, bl = instr / IPB;
       const unsigned long long kb = lane64(kwin, at + bl), vb = lane64(vwin, at + bl);
-      const unsigned kl = kring + slot * L::TILE + instr * 1024, vl = kl + NS * L::TILE;
+      const unsigned kl = kring + slot * L::TILE + instr * 1024;
       if constexpr (WHOLE) {
-        gr_g2lds16s(kb, koff[i % SUBS], kl);
-        gr_g2lds16s(vb, voff[i % SUBS], vl);
+        gr_g2lds16_kv<SUBS, NW * 1024, NS * L::TILE>(kb, vb, koff, voff, kl);
       } else {
-        char* const kd = ks0 + slot * L::TILE + instr * 1024 + lane * 16;
-        const int r = block_row(i), kblk = key_of(j) + 16 * bl;
         const bool ok = !(bad >> bl & 1);
-        if (ok && kblk + gr_perm32(r) < key1) gr_g2lds16s(kb, koff[i % SUBS], kl);
-        else gr_st16(kd, (gr_u32x4){0, 0, 0, 0});
-        if (ok && kblk + r < key1) gr_g2lds16s(vb, voff[i % SUBS], vl);
-        else gr_st16(kd + NS * L::TILE, (gr_u32x4){0, 0, 0, 0});
+#pragma unroll
+        for (int i = 0; i < SUBS; ++i) {
+          char* const kd = ks0 + slot * L::TILE + (instr + i * NW) * 1024 + lane * 16;
+          const int r = block_row(i), kblk = key_of(j) + 16 * bl;
+          if (ok && kblk + gr_perm32(r) < key1) gr_g2lds16s(kb, koff[i], kl + i * NW * 1024);
+          else gr_st16(kd, (gr_u32x4){0, 0, 0, 0});
+          if (ok && kblk + r < key1) gr_g2lds16s(vb, voff[i], kl + i * NW * 1024 + NS * L::TILE);
+          else gr_st16(kd + NS * L::TILE, (gr_u32x4){0, 0, 0, 0});
+        }
       }
     }
   };
