@@ -40,6 +40,8 @@ class PagedCache:
             if t.dim() != 4 or t.shape != k.shape or t.dtype != k.dtype or t.device != k.device or t.stride(3) != 1:
                 raise ValueError("PagedCache: k and v must be [pages, heads, page_size, D] of one shape, dtype and "
                                  "device with unit stride on D")
+            if t.shape[0] and any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride())):
+                raise ValueError("PagedCache: pages of k and v must not overlap (a stride of 0)")
         pages, heads, size, D = k.shape
         if rt.dtype_code(k.dtype) == rt.GR_F32:
             raise ValueError("PagedCache: fp16 or bf16")
@@ -163,6 +165,8 @@ def _attn_args(q, cache, table, lens, starts, causal, scale, max_new, max_len, o
         scale = 1.0 / math.sqrt(cache.head_dim)
     ref = ctypes.addressof(desc)
     need = int(rt.lib().gr_paged_attn_workspace(cache.ref, ref, Hq))
+    if workspace is not None and (workspace.get_device() != cache.index or not workspace.is_contiguous()):
+        raise ValueError(f"{who}: workspace must be a contiguous tensor on {cache.k.device}")
     if need and workspace is None:
         workspace = rt.workspace(need, q.device, stream)
     size = workspace.numel() * workspace.element_size() if workspace is not None else 0

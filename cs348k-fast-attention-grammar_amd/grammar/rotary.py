@@ -111,12 +111,18 @@ def head_strides(t, name: str, who: str):
     return st
 
 
+@functools.lru_cache(maxsize=4096)
+def _overlaps(shape: tuple, st: tuple) -> bool:
+    return any(s == 0 and n > 1 for s, n in zip(st, shape))
+
+
 def check_out(out, like, name: str, who: str):
     """`out`, checked, or a new tensor laid out as `like`."""
     import torch
     if out is None:
         return torch.empty_like(like)
-    if out.shape != like.shape or out.dtype != like.dtype or out.get_device() != like.get_device():
+    if out.shape != like.shape or out.dtype != like.dtype or out.get_device() != like.get_device() \
+            or _overlaps(out.shape, out.stride()):
         raise ValueError(f"{who}: bad `{name}` tensor")
     return out
 
@@ -132,7 +138,7 @@ def rotary_fwd(q, k, positions, rot: Rotary, *, inverse: bool = False, out=None,
         raise ValueError(f"{who}: q must be given")
     dtype, dim, index = q.dtype, rot.head_dim, rot.index
     for t in (q,) if k is None else (q, k):
-        if t.get_device() != index or t.dtype != dtype or t.dim() != 4 or t.shape[3] != dim:
+        if index < 0 or t.get_device() != index or t.dtype != dtype or t.dim() != 4 or t.shape[3] != dim:
             raise ValueError(f"{who}: q and k must be [B, H, N, {dim}] tensors of one dtype on {rot.device} (no CPU path)")
     B, Hq, N, _ = q.shape
     ps = check_positions(positions, rot, (B, N), who)
@@ -205,7 +211,9 @@ _ROTARY_FN = None
 def rotary(q, k, positions, rot: Rotary):
     """rotary_fwd, differentiable in q and k (either may need no gradient; k
     may be None): both rotations are one launch of gr_rotary, and so are their
-    gradients."""
+    gradients. A backward pass captured into a graph takes
+    torch.autograd.grad: an eager backward of the same leaves on another stream,
+    still alive, must not be joined by a captured one (torch's own rule)."""
     import torch
     if not torch.is_grad_enabled() or not (q.requires_grad or (k is not None and k.requires_grad)):
         return rotary_fwd(_dense(q), None if k is None else _dense(k), positions, rot)

@@ -603,7 +603,8 @@ def test_refusals():
                 lambda: attend(q[:1]), lambda: attend(table=s.table.long()), lambda: attend(lens=s.lens.long()),
                 lambda: attend(lens=s.lens[:1]), lambda: attend(table=s.table[0]), lambda: attend(lens=s.lens.cpu()),
                 lambda: attend(starts=starts), lambda: attend(q[:, :, 0], starts=starts[:2]), lambda: attend(q[:, :, 0]),
-                lambda: attend(out=q[:, :2]), lambda: attend(lse=torch.empty(2, 4, device=s.dev)),
+                lambda: attend(out=q[:, :2]), lambda: attend(workspace=torch.empty(64, dtype=torch.uint8)),
+                lambda: attend(out=q[:, :1].expand(2, 4, 1, 64)), lambda: PagedCache(s.k[:1].expand(4, 2, 16, 64), s.v[:4]), lambda: attend(lse=torch.empty(2, 4, device=s.dev)),
                 lambda: attend(q.transpose(1, 3).contiguous().transpose(1, 3)),
                 lambda: append(k=k[:, :1]), lambda: append(v=k.bfloat16()), lambda: append(q=q), lambda: append(out=q),
                 lambda: append(positions=s.lens), lambda: append(q=q, rotary=Rotary(128, device=s.dev)),

@@ -172,6 +172,20 @@ def test_broadcast_missing_and_partial_gradients():
     assert ((q1.grad.double() - 3 * one).abs() <= 3 * 2.0 ** -8 * 3 * one.abs() + 1e-5).all()
 
 
+def test_gradient_of_the_gradient():
+    """The gradient is linear in the one that comes in: differentiated again it is the forward rotation."""
+    dev = _cuda()
+    from grammar.rotary import Rotary, rotary
+    rot = Rotary(32, device=dev)
+    pos = torch.arange(5, dtype=torch.int32, device=dev)
+    q, k, w = (torch.randn((1, 2, 5, 32), device=dev).requires_grad_() for _ in range(3))
+    qo, ko = rotary(q, k, pos, rot)
+    dq, dk = torch.autograd.grad((qo * w).sum() + ko.sum(), (q, k), create_graph=True)
+    u = torch.randn_like(q)
+    dw, = torch.autograd.grad(dq, w, u)
+    _check(dw, *_exact(u, pos, rot), "d dq / d w")
+
+
 def test_rotated_training_attention_gradients():
     """rotary and flash_attention as a training step runs them, against 64 bits."""
     dev = _cuda()
@@ -195,7 +209,7 @@ def test_rotated_training_attention_gradients():
     # fp16 rounds q and k once more than the oracle (2^-11 of scores up to 6 or
     # so), then P, dS and the results: a few 2^-11 of the largest entry
     for got, w in zip((o, *grads), (ro, *want)):
-        assert (got.double() - w).abs().max() <= 8 * 2.0 ** -11 * max(1.0, float(w.abs().max()))
+        assert (got.double() - w).detach().abs().max() <= 8 * 2.0 ** -11 * max(1.0, float(w.detach().abs().max()))
 
 
 def test_other_streams_and_graph_replays():
@@ -248,6 +262,11 @@ def test_refusals():
                 lambda: rotary_fwd(q.double(), None, pos, rot)):
         with pytest.raises(ValueError):
             bad()
+    on_cpu = Rotary(64, device="cpu")
+    with pytest.raises(ValueError, match="GPU|CPU"):
+        rotary_fwd(q.cpu(), None, pos.cpu(), on_cpu)
+    with pytest.raises(ValueError):
+        rotary_fwd(q, None, pos, rot, out=q[:, :1].expand(1, 2, 8, 64))
     odd = torch.randn(1 * 2 * 8 * 64 + 4, device=dev).half()[4:].view(1, 2, 8, 64)
     with pytest.raises(rt.GrError, match="aligned"):
         rotary_fwd(odd, None, pos, rot)
