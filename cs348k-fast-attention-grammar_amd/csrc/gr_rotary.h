@@ -12,9 +12,21 @@
 //
 // Layout: a wave takes one token and ITER passes over its head rows. A head is
 // D / 16 units of 8 + 8 elements (two 16-byte accesses in fp16 / bf16): 8 pairs,
-// or 16 elements behind the rotated part. Lane l has unit l % (D / 16) of row
-// l / (D / 16) of every pass, so its 8 sines and cosines serve all of its rows.
-// The rows of all passes are requested before the angles are computed.
+// or 8 elements of each half of what is behind the rotated part. Lane l has unit
+// l % (D / 16) of row l / (D / 16) of every pass, so its 8 sines and cosines serve
+// all of its rows. The rows of all passes are requested before the angles are
+// computed.
+//
+// Bound by memory once there are tokens enough: 2 x 4,096 tokens of 32 + 32 heads
+// of 128 (268 MB, bf16) take 43-52 us, 5.2-6.2 TB/s, where a large copy reaches
+// 5.15; 320 tokens of 4 + 4 heads of 64 take 4.0 us, a launch and two trips to
+// memory.
+//
+// Stores that write whole lines go past the caches, where the attention that
+// reads the rows runs on other XCDs: 8,193 tokens of 32 + 8 + 8 heads of 128 into
+// pages 45.5 us to 41.3, 1,024 tokens 7.6 to 6.6, and the attention behind takes as
+// long. Stores of parts of lines stay in them: 2 x 4,096 tokens of 32 + 32 heads of
+// 32 take 15.0 us, past the caches 30; of 128 with neighbours as pairs 45.5 and 76.
 #pragma once
 #include "gr_common.h"
 
@@ -68,9 +80,14 @@ struct gr_rope8 {
 #pragma unroll
     for (int i = 0; i < W; ++i) w[i] = gr_ld16(reinterpret_cast<const char*>(p) + 16 * i);
   }
+  template <bool PAST>
   __device__ __forceinline__ void store(T* p) const {
 #pragma unroll
-    for (int i = 0; i < W; ++i) gr_st16(reinterpret_cast<char*>(p) + 16 * i, w[i]);
+    for (int i = 0; i < W; ++i) {
+      char* const at = reinterpret_cast<char*>(p) + 16 * i;
+      if constexpr (PAST) __builtin_nontemporal_store(w[i], reinterpret_cast<gr_u32x4*>(at));
+      else gr_st16(at, w[i]);
+    }
   }
   __device__ __forceinline__ float get(int e) const {
     if constexpr (W == 2) {
@@ -92,7 +109,8 @@ struct gr_rope8 {
   }
 };
 
-template <class T, bool APPEND, bool INTER, int ITER>
+// PAST: stores go past the caches (of whole 128-byte lines only)
+template <class T, bool APPEND, bool INTER, int ITER, bool PAST>
 __device__ __forceinline__ void gr_rope_body(const gr_rope_args& a, bool inverse) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)((blockIdx.x * blockDim.x + threadIdx.x) >> 6));
@@ -105,8 +123,8 @@ __device__ __forceinline__ void gr_rope_body(const gr_rope_args& a, bool inverse
   const int row0 = (wave - tok * groups) * ITER * rpp + lane / units, u = lane % units;
   const int ru = a.pairs >> 3;                   // rotated units
   const bool lane_live = lane < rpp * units;
-  const int lo = u < ru ? (INTER ? 16 * u : 8 * u) : 2 * a.pairs + 16 * (u - ru);
-  const int hi = u < ru ? (INTER ? 16 * u + 8 : a.pairs + 8 * u) : lo + 8;
+  const int lo = u < ru ? (INTER ? 16 * u : 8 * u) : 2 * a.pairs + 8 * (u - ru);
+  const int hi = u < ru ? (INTER ? 16 * u + 8 : a.pairs + 8 * u) : lo + 8 * (units - ru);
 
   // the token's sequence and index in it
   int b, i, at = 0;
@@ -201,7 +219,7 @@ __device__ __forceinline__ void gr_rope_body(const gr_rope_args& a, bool inverse
     }
     if (APPEND && r >= h0 && page < 0) continue;
     T* d = r < h0 ? dq + r * a.q.dh : !APPEND || r < h1 ? dk + (r - h0) * a.k.dh : dv + (r - h1) * a.v.dh;
-    x[p].store(d + lo);
-    y[p].store(d + hi);
+    x[p].template store<PAST>(d + lo);
+    y[p].template store<PAST>(d + hi);
   }
 }

@@ -11,31 +11,45 @@
 
 namespace {
 
-template <class T, bool APPEND, bool INTER, int ITER>
+template <class T, bool APPEND, bool INTER, int ITER, bool PAST>
 __global__ __launch_bounds__(256) void gr_rope_kernel(gr_rope_args a, int inverse) {
-  gr_rope_body<T, APPEND, INTER, ITER>(a, inverse != 0);
+  gr_rope_body<T, APPEND, INTER, ITER, PAST>(a, inverse != 0);
 }
 
-template <class T, bool APPEND, bool INTER>
+template <class T, bool APPEND, bool INTER, bool PAST>
 int launch(const gr_rope_args& a, int inverse, const char* who, hipStream_t st) {
   const int rows = a.q.heads + a.k.heads + a.v.heads;
   const int rpp = 64 / (a.D / 16), passes = (rows + rpp - 1) / rpp;
-  // As many passes to a wave as leave every CU 8 waves, at most 4
+  // Passes to a wave. One while two would leave a CU fewer than 4 waves (128 tokens
+  // of 64 heads of 128 3.8 us, two 4.0; 1,024 tokens of 48 7.8 and 6.8). Else four,
+  // or two of 16-bit rows of 128 and more (two / four, 8,192 tokens: 64 heads of 96
+  // 42.5 / 33.8 us, 48 of 64 22.3 / 19.2, 32 of 128 in fp32 46.6 / 43.9; 64 of 128
+  // 43.3 / 49.0, 48 of 128 33.2 / 32.7).
   const long long full = (long long)a.tokens * passes;
   const int cus = gr::cu_count() > 0 ? gr::cu_count() : 256;
-  const int iter = passes >= 4 && full >= 32LL * cus ? 4 : passes >= 2 && full >= 16LL * cus ? 2 : 1;
+  const int iter = passes < 2 || full < 8LL * cus ? 1 : passes == 2 || (sizeof(T) == 2 && a.D >= 128) ? 2 : 4;
   const long long waves = (long long)a.tokens * ((passes + iter - 1) / iter);
   if (waves > 0x7fffffffLL / 64) return gr::fail(GR_E_ARG, "%s: %d tokens of %d head rows are too many for one call", who, a.tokens, rows);
   const dim3 grid((unsigned)((waves + 3) / 4));
-  if (iter == 4) hipLaunchKernelGGL((gr_rope_kernel<T, APPEND, INTER, 4>), grid, dim3(256), 0, st, a, inverse);
-  else if (iter == 2) hipLaunchKernelGGL((gr_rope_kernel<T, APPEND, INTER, 2>), grid, dim3(256), 0, st, a, inverse);
-  else hipLaunchKernelGGL((gr_rope_kernel<T, APPEND, INTER, 1>), grid, dim3(256), 0, st, a, inverse);
+  if constexpr (!PAST) {
+    if (iter == 4) {
+      hipLaunchKernelGGL((gr_rope_kernel<T, APPEND, INTER, 4, false>), grid, dim3(256), 0, st, a, inverse);
+      return gr::hip_check(hipGetLastError(), GR_E_LAUNCH, who);
+    }
+  }
+  if (iter == 2) hipLaunchKernelGGL((gr_rope_kernel<T, APPEND, INTER, 2, PAST>), grid, dim3(256), 0, st, a, inverse);
+  else hipLaunchKernelGGL((gr_rope_kernel<T, APPEND, INTER, 1, PAST>), grid, dim3(256), 0, st, a, inverse);
   return gr::hip_check(hipGetLastError(), GR_E_LAUNCH, who);
 }
 
 template <class T, bool APPEND>
 int launch_inter(const gr_rope_args& a, bool inter, int inverse, const char* who, hipStream_t st) {
-  return inter ? launch<T, APPEND, true>(a, inverse, who, st) : launch<T, APPEND, false>(a, inverse, who, st);
+  if (inter) return launch<T, APPEND, true, false>(a, inverse, who, st);
+  if constexpr (sizeof(T) == 2) {
+    // 8 lanes of 16 bytes side by side, in the rotated part and behind it
+    if (2 * a.pairs % 128 == 0 && a.D % 128 == 0) return launch<T, APPEND, false, true>(a, inverse, who, st);
+  }
+  return launch<T, APPEND, false, false>(a, inverse, who, st);
 }
 
 // The rotation's own arguments: head_dim a multiple of 16 up to 256, at most 8 axes.
