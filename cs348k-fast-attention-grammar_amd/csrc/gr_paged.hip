@@ -37,6 +37,7 @@ __global__ __launch_bounds__(256) void gr_paged_merge_kernel(gr_paged_args a) {
 struct Plan {
   int nw;                        // waves of 32 rows
   long long tiles;               // row tiles of a key head
+  int groups;                    // key groups of a tile of 128 rows
   int shares;                    // 0: a workgroup a tile
 };
 
@@ -59,37 +60,54 @@ Plan plan_of(const gr_paged_cache& c, const gr_paged_batch& b, int Hq) {
   // packed rows: every sequence may have a part-filled tile
   p.tiles = b.starts ? (long long)b.rows * G / BM + b.B : (long long)b.B * (((long long)b.rows * G + BM - 1) / BM);
   const int resident = cus * (D == 128 && p.nw < 4 ? 1 : 2);      // workgroups (their LDS)
+  // Tiles of 128 rows that leave a CU at most one of them halve the chain of their
+  // key steps, with two key groups of four waves: 175 or 176 tiles, 1,500 keys 27.0
+  // us to 23.0 (D 64), 44.5 to 36.0 (D 128); 256 tiles, 2,048 keys 33.8 to 28.8 and 57.0
+  // to 46.2; 1,024 tiles 83.6 to 93.6 and 145 to 170. Single tokens beside them, which
+  // take a workgroup each too, count by three quarters more.
+  const long long wgs = p.tiles * c.heads;
+  p.groups = p.nw == 4 && rows128 <= cus && 4 * wgs <= 7LL * cus ? 2 : 1;
   // Work is shared out from a length on that grows with the workgroups that one a
   // tile would make: in brackets shared / a workgroup a tile, lengths spread by a
   // half around the mean. One token, D 128: 64 tiles, mean 600 keys 13.8 / 15.5 us,
   // 400 13.7 / 12.8; 256 tiles, 2,400 52.0 / 55.4, 1,200 32.5 / 31.2. D 64: 64
-  // tiles, 1,200 12.7 / 16.3, 600 12.3 / 10.6; 512 tiles, 4,800 115.7 / 114.7. Chunks
-  // of 128-row tiles: 12 tiles, D 128, 1,024 keys 24.7 / 30.8, 512 20.6 / 19.2; 528
-  // tiles, 16,384 keys 612 / 578.
-  const long long wgs = p.tiles * c.heads;
+  // tiles, 1,200 12.7 / 16.3, 600 12.3 / 10.6; 512 tiles, 4,800 115.7 / 114.7. Tiles
+  // of 128 rows in two groups: D 64, 16 tiles, 1,600 keys 18.8 / 21.7, 1,100 20.1 /
+  // 18.1; 128 tiles, 4,500 44.4 / 49.4, 2,400 34.3 / 30.7; D 128, 96 tiles, 2,400 42.6 /
+  // 49.5, 1,100 35.2 / 28.7; from three quarters of the CUs on not at all (176 tiles,
+  // 8,000 87.8 / 82.7 and 162 / 144). In one group: 528 tiles, 16,384 keys 612 / 578.
   const double fill = wgs < resident ? (double)wgs / resident : 1.0;
-  const double least = p.nw == 4 ? 1000 : D == 64 ? 1200 : 900, slope = p.nw == 4 ? 6500 : D == 64 ? 7000 : 3000;
+  double least = D == 64 ? 1200 : 900, slope = D == 64 ? 7000 : 3000;
+  bool can = true;
+  if (p.nw == 4) {
+    least = 1300;
+    slope = p.groups == 1 ? 6500 : D == 64 ? 12500 : 8000;
+    can = p.groups == 1 ? wgs < resident : 4 * wgs < 3LL * cus;
+  }
   const double from = slope * fill > least ? slope * fill : least;
-  const bool shared = (double)len > from && !(p.nw == 4 && wgs >= resident)
-                      && p.tiles * c.heads * (cap / 64 + 1 + GR_PAGED_COST) <= 0x7fffffffLL;
+  const bool shared = can && (double)len > from && wgs * (cap / 64 + 1 + GR_PAGED_COST) <= 0x7fffffffLL;
   p.shares = !shared ? 0 : resident < GR_PAGED_MAX_SHARES ? resident : GR_PAGED_MAX_SHARES;
   return p;
 }
 
 size_t share_bytes(const Plan& p, int D) { return (size_t)2 * 32 * p.nw * (D + 2) * sizeof(float); }
 
+// A workgroup a tile.
 template <class T, int D, int BN, int NW, int KG, int NS, int KGS>
-int launch_tiles(const gr_paged_args& a, hipStream_t st) {
+int launch_alone(const gr_paged_args& a, hipStream_t st) {
+  constexpr int LDS = Lds<D, BN, NW, KG, NS, KGS>::BYTES;
+  hipLaunchKernelGGL((gr_paged_kernel<T, D, BN, NW, KG, NS, KGS, false>), dim3((unsigned)((long long)a.tiles * a.Hkv)),
+                     dim3(64 * NW * KG), LDS, st, a);
+  return gr::hip_check(hipGetLastError(), GR_E_LAUNCH, "gr_paged_attn launch");
+}
+
+template <class T, int D, int BN, int NW, int KG, int NS, int KGS>
+int launch_shared(const gr_paged_args& a, hipStream_t st) {
   constexpr int BM = 32 * NW, LDS = Lds<D, BN, NW, KG, NS, KGS>::BYTES;
-  const long long wgs = (long long)a.tiles * a.Hkv;
-  const dim3 block(64 * NW * KG);
-  if (a.shares == 0) {
-    hipLaunchKernelGGL((gr_paged_kernel<T, D, BN, NW, KG, NS, KGS, false>), dim3((unsigned)wgs), block, LDS, st, a);
-    return gr::hip_check(hipGetLastError(), GR_E_LAUNCH, "gr_paged_attn launch");
-  }
-  hipLaunchKernelGGL((gr_paged_kernel<T, D, BN, NW, KG, NS, KGS, true>), dim3((unsigned)a.shares), block, LDS, st, a);
+  hipLaunchKernelGGL((gr_paged_kernel<T, D, BN, NW, KG, NS, KGS, true>), dim3((unsigned)a.shares), dim3(64 * NW * KG), LDS, st, a);
   const int rc = gr::hip_check(hipGetLastError(), GR_E_LAUNCH, "gr_paged_attn launch");
   if (rc) return rc;
+  const long long wgs = (long long)a.tiles * a.Hkv;
   const int rows = a.starts ? BM : (a.rows * a.G < BM ? a.rows * a.G : BM);      // of a tile, at most
   // workgroups of a tile: one pass over its rows where it has few parts, and a
   // row each where few tiles of many parts would leave CUs idle
@@ -100,10 +118,13 @@ int launch_tiles(const gr_paged_args& a, hipStream_t st) {
 }
 
 template <class T, int D>
-int launch(const gr_paged_args& a, int nw, hipStream_t st) {
-  if (nw == 1) return launch_tiles<T, D, 32, 1, 4, 2, 0>(a, st);
-  if (nw == 2) return launch_tiles<T, D, 32, 2, 4, 2, 0>(a, st);
-  return launch_tiles<T, D, 64, 4, 1, 2, D == 64 ? 4 : 2>(a, st);
+int launch(const gr_paged_args& a, const Plan& p, hipStream_t st) {
+  if (p.nw == 1) return a.shares ? launch_shared<T, D, 32, 1, 4, 2, 0>(a, st) : launch_alone<T, D, 32, 1, 4, 2, 0>(a, st);
+  if (p.nw == 2) return a.shares ? launch_shared<T, D, 32, 2, 4, 2, 0>(a, st) : launch_alone<T, D, 32, 2, 4, 2, 0>(a, st);
+  // (keys 32 a step in two groups at D 128: two rings of 64 would take a CU's LDS)
+  if (a.shares) return launch_shared<T, D, 64, 4, 1, 2, D == 64 ? 4 : 2>(a, st);
+  if (p.groups == 2) return launch_alone<T, D, D == 64 ? 64 : 32, 4, 2, 2, 4>(a, st);
+  return launch_alone<T, D, 64, 4, 1, 2, D == 64 ? 4 : 2>(a, st);
 }
 
 int check_heads(const gr_paged_cache* c, const gr_paged_batch* b, int Hq) {
@@ -173,6 +194,6 @@ extern "C" int gr_paged_attn(const gr_paged_cache* cache, const gr_paged_batch* 
   }
   hipStream_t st = (hipStream_t)stream;
   if (cache->dtype == GR_F16)
-    return cache->head_dim == 64 ? launch<_Float16, 64>(a, p.nw, st) : launch<_Float16, 128>(a, p.nw, st);
-  return cache->head_dim == 64 ? launch<__bf16, 64>(a, p.nw, st) : launch<__bf16, 128>(a, p.nw, st);
+    return cache->head_dim == 64 ? launch<_Float16, 64>(a, p, st) : launch<_Float16, 128>(a, p, st);
+  return cache->head_dim == 64 ? launch<__bf16, 64>(a, p, st) : launch<__bf16, 128>(a, p, st);
 }

@@ -215,7 +215,7 @@ def test_shared_work_of_ragged_lengths(dtype, D, n, G, Hkv):
     _run(s, [n] * len(lens), G * Hkv, hints=False, strided=True)
 
 
-@pytest.mark.parametrize("dtype,D,G,Hkv", [("bf16", 128, 4, 2), ("fp16", 64, 1, 4)])
+@pytest.mark.parametrize("dtype,D,G,Hkv", [("bf16", 128, 4, 2), ("fp16", 64, 1, 2)])
 def test_shared_mixed_batches(dtype, D, G, Hkv):
     news = [1, 0, 150, 1, 7, 0, 1, 301, 1, 0] + [1] * 70
     lens = [40, 99, 150, 4000, 7, 0, 1, 900, 0, 5] + [3 * i for i in range(70)]
@@ -224,6 +224,19 @@ def test_shared_mixed_batches(dtype, D, G, Hkv):
     assert _needs_workspace(s, sum(news) + 5, G * Hkv, s.lens.data_ptr()) > 0
     for causal in (True, False):
         _run(s, news, G * Hkv, causal=causal, ragged=True, pad=5, hints=False)
+
+
+@pytest.mark.parametrize("dtype,D", [("bf16", 128), ("fp16", 64)])
+@pytest.mark.parametrize("G,Hkv", [(8, 16), (4, 8)], ids=["many", "few"])
+def test_mixed_batches_of_a_workgroup_a_tile(dtype, D, G, Hkv):
+    """Grids that fill the GPU and grids that do not (their tiles' keys in two groups), single tokens among them."""
+    news = [1, 130, 0, 33, 300, 1, 16]
+    lens = [260, 131, 9, 33, 449, 0, 80]
+    s = Setup(lens, Hkv, 32, D, dtype, seed=G)
+    print(f"[case] tiles {dtype} D{D} G{G} Hkv{Hkv}", flush=True)
+    assert _needs_workspace(s, sum(news) + 3, G * Hkv, s.lens.data_ptr()) == 0
+    for causal in (True, False):
+        _run(s, news, G * Hkv, causal=causal, ragged=True, pad=3, hints=False)
 
 
 @pytest.mark.parametrize("D", [64, 128])
