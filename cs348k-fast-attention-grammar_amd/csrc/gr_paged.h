@@ -104,6 +104,7 @@ __device__ __forceinline__ int gr_wave_scan(int v) {
 template <int BM, bool SMALL>
 struct gr_paged_seqs {
   int b0 = -1;
+  int only = 0;                    // SMALL: 1 and 2 leave out sequences of at most and of more than 32 rows
   int tiles, blocks;               // before these 64
   int first, n, len, nt, nb;       // of the lane's sequence: tiles, blocks of a tile
   int tsum, bsum;                  // tiles and blocks of the 64 up to and with it
@@ -116,12 +117,28 @@ struct gr_paged_seqs {
     n = gr_paged_news(a, b, first);
     const int rows = n * a.G;
     nt = from + lane >= a.B || rows == 0 ? 0 : SMALL && rows <= 32 ? 1 : (rows + BM - 1) / BM;
+    if (SMALL && only == (rows <= 32 ? 1 : 2)) nt = 0;
     nb = gr_paged_blocks(gr_paged_keys(a, len));
     tsum = gr_wave_scan(nt);
     bsum = gr_wave_scan((int)((unsigned)nt * (nb + GR_PAGED_COST)));
   }
   __device__ __forceinline__ int tiles_after() const { return tiles + __builtin_amdgcn_readlane(tsum, 63); }
   __device__ __forceinline__ int blocks_after() const { return blocks + __builtin_amdgcn_readlane(bsum, 63); }
+
+  // Tiles of one key head.
+  __device__ __forceinline__ int count(const gr_paged_args& a, int lane) {
+    load(a, 0, 0, 0, lane);
+    int sum = tiles_after();
+    if (a.B > 64) {
+      gr_paged_seqs more;
+      more.only = only;
+      for (int from = 64; from < a.B; from += 64) {
+        more.load(a, from, sum, 0, lane);
+        sum = more.tiles_after();
+      }
+    }
+    return sum;
+  }
 
   // Blocks of one key head over all tiles.
   __device__ __forceinline__ int total(const gr_paged_args& a, int lane) {
@@ -733,8 +750,28 @@ __device__ __forceinline__ void gr_paged_body(const gr_paged_args& a, char* lds)
   };
   if constexpr (!SHARED) {
     // key head slowest, then the tiles: workgroups of one key head share an XCD's L2
-    const int hk = logical / a.tiles;
-    if (seqs.template find<false>(a, logical - hk * a.tiles, lane, t)) segment(hk, 0, t.kend, -1);
+    int at = logical, per = a.tiles;          // tile of all heads' and their tiles
+    if constexpr (KGS > 0 && D == 64) {
+      // in packed batches the tiles of long chunks of all key heads first, so that
+      // they spread over the CUs and single tokens fill up: two chunks of 423 and 17
+      // tokens, 16 heads 45.7 us to 37.6, three of 800 and 29 77.3 to 68.9, but two of
+      // 400 with short contexts and 18 33 to 36 (D 128: 43.9 to 47.4, 124.9 to 131.9)
+      if (a.starts) {
+        seqs.only = 1;
+        const int large = gr_imin(seqs.count(a, lane), a.tiles), first = large * a.Hkv;
+        if ((int)blockIdx.x < first) {
+          at = gr_xcd_remap_any((int)blockIdx.x, first);
+          per = large;
+        } else {
+          at = gr_xcd_remap_any((int)blockIdx.x - first, (int)gridDim.x - first);
+          per = a.tiles - large;
+          seqs.only = 2;
+          seqs.b0 = -1;
+        }
+      }
+    }
+    const int hk = at / per;
+    if (seqs.template find<false>(a, at - hk * per, lane, t)) segment(hk, 0, t.kend, -1);
   } else {
     const int per_head = seqs.total(a, lane);
     const gr_paged_cut cut(per_head * a.Hkv, a.shares);

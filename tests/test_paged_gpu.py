@@ -230,8 +230,8 @@ def test_shared_mixed_batches(dtype, D, G, Hkv):
 @pytest.mark.parametrize("G,Hkv", [(8, 16), (4, 8)], ids=["many", "few"])
 def test_mixed_batches_of_a_workgroup_a_tile(dtype, D, G, Hkv):
     """Grids that fill the GPU and grids that do not (their tiles' keys in two groups), single tokens among them."""
-    news = [1, 130, 0, 33, 300, 1, 16]
-    lens = [260, 131, 9, 33, 449, 0, 80]
+    news = [1, 130, 0, 33, 300, 1, 16] + [1, 0, 2] * 25 + [34]
+    lens = [260, 131, 9, 33, 449, 0, 80] + [5 * i for i in range(75)] + [70]
     s = Setup(lens, Hkv, 32, D, dtype, seed=G)
     print(f"[case] tiles {dtype} D{D} G{G} Hkv{Hkv}", flush=True)
     assert _needs_workspace(s, sum(news) + 3, G * Hkv, s.lens.data_ptr()) == 0
