@@ -27,6 +27,13 @@
 //    reach a product. A key that only some of a tile's rows may see, and whose
 //    value is not finite, is taken out of the matrix product and added on the
 //    vector unit to the rows that see it: 0 x inf would be NaN in the others.
+//
+// Measured (bf16, 32 / 8 heads of 128). A token each of 48 sequences of 150 to 8,000
+// keys (848 MB): 147-150 us, 5.7 TB/s, bound by memory (matrix cores 8 % busy), and
+// 4.8 for the merge. 4,096 tokens onto 4,096: 410 us, 1,007 TFLOP/s, bound by the
+// MFMAs and the softmax of two waves a SIMD taking turns (matrix cores 49 % busy, no
+// LDS conflicts). Small grids are bound by a workgroup's chain of steps, 1.2-1.3 us
+// for 64 keys of 128 rows: 419 keys of one token (16 heads of 64) take 7.2 us.
 #pragma once
 #include "gr_flash_fwd.h"
 #include "gr_gemm.h"
