@@ -150,7 +150,10 @@ def rotary_fwd(q, k, positions, rot: Rotary, *, inverse: bool = False, out=None,
         if k.shape[0] != B or k.shape[2] != N:
             raise ValueError(f"{who}: k {tuple(k.shape)} does not match q {tuple(q.shape)}")
         k_out = check_out(k_out, k, "k_out", who)
-        head += (k.data_ptr(), k_out.data_ptr(), k.shape[1], head_strides(k, "k", who), head_strides(k_out, "k_out", who))
+        k_to = k_out.data_ptr()
+        if k_to == head[2] and k_to:
+            raise ValueError(f"{who}: `out` and `k_out` must be two tensors")
+        head += (k.data_ptr(), k_to, k.shape[1], head_strides(k, "k", who), head_strides(k_out, "k_out", who))
     if B == 0 or N == 0:
         return out, k_out
     rt.launch(rt.lib().gr_rotary, head + (rt.dtype_code(q.dtype), B, N, positions.data_ptr(), ps, int(bool(inverse))),

@@ -291,6 +291,33 @@ def test_hidden_entries_may_hold_anything(dtype, D, n, G, width):
     assert out[:3, :G, -1].isnan().all() and out[:3, G:, -1, 5].isinf().all() and out[:3, G:, -1, D - 1].isnan().all()
 
 
+@pytest.mark.parametrize("dtype,D", [("bf16", 128), ("fp16", 64)])
+@pytest.mark.parametrize("G,Hkv", [(8, 24), (4, 12)], ids=["many", "few"])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_hidden_entries_of_chunks(dtype, D, G, Hkv, ragged):
+    """The same in tiles of 128 rows (grids that fill the GPU and grids that do not), and pages that do not exist
+    at a chunk's start, middle and end."""
+    n, S = 90, 16
+    lens = [n, n + 7, n + 100, 300 + n]
+    s = Setup(lens, Hkv, S, D, dtype, seed=G)
+    live = torch.zeros(s.k.shape[0], S, dtype=torch.bool)
+    for b, m in enumerate(lens):
+        for j in range(m):
+            live[int(s.table[b, j // S]), j % S] = True
+    dead = (~live).to(s.dev)[:, None, :, None]
+    s.k.masked_fill_(dead, float("nan"))
+    s.v.masked_fill_(dead, float("nan"))
+    for b, m in enumerate(lens):
+        page, slot = int(s.table[b, (m - 1) // S]), (m - 1) % S
+        s.k[page, 0, slot, 3] = float("nan")
+        s.v[page, 1, slot, 5], s.v[page, 1, slot, D - 1] = float("inf"), float("nan")
+    s.table[1, 3], s.table[2, 0], s.table[3, 5], s.table[3, 17] = -1, s.k.shape[0], -9, 2 ** 31 - 1
+    print(f"[case] hidden chunks {dtype} D{D} G{G} Hkv{Hkv} ragged {ragged}", flush=True)
+    out = _run(s, [n] * 4, G * Hkv, ragged=ragged, pad=3 * ragged, hints=False)
+    if not ragged:
+        assert out[:, :, :-1].isfinite().all() and out[:, 2 * G:].isfinite().all()
+
+
 @pytest.mark.parametrize("width", [None, 2048], ids=["tile", "shared"])
 def test_pages_that_do_not_exist(width):
     """Page ids out of range, keys behind the table and starts out of the batch read nothing."""

@@ -267,6 +267,9 @@ def test_refusals():
         rotary_fwd(q.cpu(), None, pos.cpu(), on_cpu)
     with pytest.raises(ValueError):
         rotary_fwd(q, None, pos, rot, out=q[:, :1].expand(1, 2, 8, 64))
+    to = torch.empty_like(q)
+    with pytest.raises(ValueError, match="two tensors"):
+        rotary_fwd(q, q, pos, rot, out=to, k_out=to)
     odd = torch.randn(1 * 2 * 8 * 64 + 4, device=dev).half()[4:].view(1, 2, 8, 64)
     with pytest.raises(rt.GrError, match="aligned"):
         rotary_fwd(odd, None, pos, rot)
