@@ -419,6 +419,8 @@ APPENDS = [
     ([9] * 2, [9, 30], 4, 4, 64, 16, 64, [10, 11, 11], False, "fp16", False),
     ([1, 0, 40, 1, 17], [3, 8, 40, 99, 50], 6, 3, 128, 16, 64, None, False, "bf16", True),
     ([300, 2], [310, 2], 32, 8, 128, 64, 128, [16, 24, 24], True, "bf16", True),
+    ([500, 1, 60], [700, 90, 60], 32, 8, 128, 16, 128, None, False, "bf16", True),
+    ([600, 1, 500], [610, 20, 500], 35, 7, 64, 32, 32, None, False, "fp16", True),
     ([2, 30], [1, 25], 2, 1, 64, 16, 64, None, False, "fp16", True),          # more tokens than keys: places below 0
 ]
 

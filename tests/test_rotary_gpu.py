@@ -57,6 +57,11 @@ CASES = [
     (1, 7, 4, 1, 256, 256, [16] * 8, False, False, "bf16"),
     (4, 1000, 12, 4, 96, 96, None, False, False, "fp32"),
     (2, 2048, 32, 8, 128, 64, None, False, True, "bf16"),
+    # several passes of a wave, the last one part-filled; stores of whole lines and of parts
+    (2, 701, 33, 8, 128, 128, None, False, False, "bf16"),
+    (1, 700, 13, 6, 256, 128, None, False, False, "fp16"),
+    (3, 900, 25, 12, 64, 32, None, False, False, "fp16"),
+    (1, 1500, 17, 3, 128, 96, [20, 28], False, False, "fp32"),
 ]
 
 
