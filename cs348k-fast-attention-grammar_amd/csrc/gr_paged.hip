@@ -63,8 +63,9 @@ Plan plan_of(const gr_paged_cache& c, const gr_paged_batch& b, int Hq) {
   // Tiles of 128 rows that leave a CU at most one of them halve the chain of their
   // key steps, with two key groups of four waves: 175 or 176 tiles, 1,500 keys 27.0
   // us to 23.0 (D 64), 44.5 to 36.0 (D 128); 256 tiles, 2,048 keys 33.8 to 28.8 and 57.0
-  // to 46.2; 1,024 tiles 83.6 to 93.6 and 145 to 170. Single tokens beside them, which
-  // take a workgroup each too, count by three quarters more.
+  // to 46.2; 1,024 tiles 83.6 to 93.6 and 145 to 170. Single tokens beside them take a
+  // workgroup each too: up to 7/4 of the CUs in all (400, D 64, 49.5 to 45.7; 528 24.0
+  // to 27.0).
   const long long wgs = p.tiles * c.heads;
   p.groups = p.nw == 4 && rows128 <= cus && 4 * wgs <= 7LL * cus ? 2 : 1;
   // Work is shared out from a length on that grows with the workgroups that one a
