@@ -21,10 +21,11 @@ raise.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 from . import runtime as rt
-from .rotary import Rotary, _pair, check_out, check_positions, head_strides
+from .rotary import Rotary, _head_strides, check_out, check_positions, head_strides
 
 
 class PagedCache:
@@ -62,43 +63,63 @@ class PagedCache:
         return cls(torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device))
 
 
-def _batch(cache, table, lens, starts, x, name, max_new, max_len, who):
+@functools.lru_cache(maxsize=4096)
+def _batch_sizes(table: tuple, table_st: tuple, lens: tuple, lens_st: tuple, starts, starts_st, x: tuple):
+    """(B, width, leading sizes of the tokens) of a call's shapes and strides, or what is wrong with them."""
+    for n, shape, st, dim in (("table", table, table_st, 2), ("lens", lens, lens_st, 1), ("starts", starts, starts_st, 1)):
+        if shape is not None and (len(shape) != dim or (st[-1] != 1 and shape[-1] > 1)):
+            return f"{n} must be a {dim}-D int32 tensor with unit stride"
+    B, width = table
+    if lens[0] != B or B == 0 or width == 0:
+        return f"table {tuple(table)} and lens {tuple(lens)} do not describe a batch"
+    if starts is None:
+        return (B, width, (B, x[2])) if len(x) == 4 and x[0] == B else \
+            f"the tokens must be [{B}, heads, n, D] (packed rows need starts), not {tuple(x)}"
+    return (B, width, (x[0],)) if len(x) == 3 and starts[0] == B + 1 else \
+        f"with starts [{B + 1}] the tokens must be packed [rows, heads, D], not {tuple(x)}"
+
+
+def _batch(cache, table, lens, starts, x, max_new, max_len, who):
     """(gr_paged_batch, leading sizes of the tokens) of a call on `x`: [B, heads,
     n, D] or, with starts, [rows, heads, D]."""
     import torch
     index, int32 = cache.index, torch.int32
-    for n, t, dim in (("table", table, 2), ("lens", lens, 1), ("starts", starts, 1)):
-        if t is None and n == "starts":
-            continue
-        if t.dtype != int32 or t.dim() != dim or t.get_device() != index or (t.stride(-1) != 1 and t.shape[-1] > 1):
-            raise ValueError(f"{who}: {n} must be a {dim}-D int32 tensor on {cache.k.device} with unit stride")
-    B, width = table.shape
-    if lens.shape[0] != B or B == 0 or width == 0:
-        raise ValueError(f"{who}: table {tuple(table.shape)} and lens {tuple(lens.shape)} do not describe a batch")
     if starts is None:
-        if x.dim() != 4 or x.shape[0] != B:
-            raise ValueError(f"{who}: {name} must be [{B}, heads, n, D] (packed rows need starts)")
-        lead = (B, x.shape[2])
+        sizes = _batch_sizes(table.shape, table.stride(), lens.shape, lens.stride(), None, None, x.shape)
+        at, ok = None, True
     else:
-        if x.dim() != 3 or starts.shape[0] != B + 1:
-            raise ValueError(f"{who}: with starts [{B + 1}], {name} must be packed [rows, heads, D]")
-        lead = (x.shape[0],)
-    return rt.PagedBatch(table.data_ptr(), table.stride(0), lens.data_ptr(), starts.data_ptr() if starts is not None else None,
-                         B, lead[-1], width, int(max_new), int(max_len)), lead
+        sizes = _batch_sizes(table.shape, table.stride(), lens.shape, lens.stride(), starts.shape, starts.stride(), x.shape)
+        at, ok = starts.data_ptr(), starts.dtype == int32 and starts.get_device() == index
+    if not ok or table.dtype != int32 or lens.dtype != int32 or table.get_device() != index or lens.get_device() != index:
+        raise ValueError(f"{who}: table, lens and starts must be int32 tensors on {cache.k.device}")
+    if type(sizes) is str:
+        raise ValueError(f"{who}: {sizes}")
+    B, width, lead = sizes
+    return rt.PagedBatch(table.data_ptr(), table.stride(0), lens.data_ptr(), at, B, lead[-1], width, int(max_new),
+                         int(max_len)), lead
+
+
+@functools.lru_cache(maxsize=4096)
+def _heads_strides(shape: tuple, st: tuple, lead: tuple, heads: int, dim: int):
+    """{batch, token, head} strides of `heads` heads of the tokens `lead`; None: another shape."""
+    if shape != ((lead[0], heads, lead[1], dim) if len(lead) == 2 else (lead[0], heads, dim)):
+        return None
+    return _head_strides(shape, st) or "stride"
 
 
 def _heads(t, name, lead, heads, cache, who):
     """The strides of `heads` heads of the tokens `lead`, checked."""
-    want = (lead[0], heads, lead[1], cache.head_dim) if len(lead) == 2 else (lead[0], heads, cache.head_dim)
-    if t.shape != want or t.dtype != cache.dtype or t.get_device() != cache.index:
+    st = _heads_strides(t.shape, t.stride(), lead, heads, cache.head_dim)
+    if st is None or t.dtype != cache.dtype or t.get_device() != cache.index:
+        want = (*lead[:1], heads, *lead[1:], cache.head_dim)
         raise ValueError(f"{who}: {name} must be {want} {cache.dtype} on {cache.k.device} (no CPU path), not "
                          f"{tuple(t.shape)} {t.dtype} on {t.device}")
-    return head_strides(t, name, who)
+    return st if st != "stride" else head_strides(t, name, who)
 
 
 def _append_args(k, v, cache, table, lens, starts, q, rotary, positions, max_new, out):
     who = "paged_append"
-    desc, lead = _batch(cache, table, lens, starts, k, "k", max_new, 0, who)
+    desc, lead = _batch(cache, table, lens, starts, k, max_new, 0, who)
     ks, vs = _heads(k, "k", lead, cache.heads, cache, who), _heads(v, "v", lead, cache.heads, cache, who)
     if rotary is None:
         if q is not None or positions is not None:
@@ -151,7 +172,7 @@ def bind_paged_append(k, v, cache: PagedCache, table, lens, *, starts=None, q=No
 def _attn_args(q, cache, table, lens, starts, causal, scale, max_new, max_len, out, lse, workspace, stream):
     import torch
     who = "paged_attention"
-    desc, lead = _batch(cache, table, lens, starts, q, "q", max_new, max_len, who)
+    desc, lead = _batch(cache, table, lens, starts, q, max_new, max_len, who)
     Hq = q.shape[1]
     qs = _heads(q, "q", lead, Hq, cache, who)
     if Hq == 0 or Hq % cache.heads:

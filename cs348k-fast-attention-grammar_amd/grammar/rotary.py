@@ -112,8 +112,8 @@ def head_strides(t, name: str, who: str):
 
 
 @functools.lru_cache(maxsize=4096)
-def _overlaps(shape: tuple, st: tuple) -> bool:
-    return any(s == 0 and n > 1 for s, n in zip(st, shape))
+def _takes(shape: tuple, st: tuple, like: tuple) -> bool:
+    return shape == like and not any(s == 0 and n > 1 for s, n in zip(st, shape))
 
 
 def check_out(out, like, name: str, who: str):
@@ -121,8 +121,7 @@ def check_out(out, like, name: str, who: str):
     import torch
     if out is None:
         return torch.empty_like(like)
-    if out.shape != like.shape or out.dtype != like.dtype or out.get_device() != like.get_device() \
-            or _overlaps(out.shape, out.stride()):
+    if not _takes(out.shape, out.stride(), like.shape) or out.dtype != like.dtype or out.get_device() != like.get_device():
         raise ValueError(f"{who}: bad `{name}` tensor")
     return out
 
