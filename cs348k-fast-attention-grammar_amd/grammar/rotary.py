@@ -126,6 +126,15 @@ def check_out(out, like, name: str, who: str):
     return out
 
 
+@functools.lru_cache(maxsize=4096)
+def _tokens(q: tuple, q_st: tuple, k, k_st, dim: int):
+    """(B, N, query heads, their strides, key heads, theirs) of a call's shapes and strides, None if they do not fit."""
+    for shape, st in ((q, q_st), (k, k_st)):
+        if shape is not None and (len(shape) != 4 or shape[3] != dim or st[3] != 1 or shape[0] != q[0] or shape[2] != q[2]):
+            return None
+    return (q[0], q[2], q[1], _head_strides(q, q_st)) + ((0, None) if k is None else (k[1], _head_strides(k, k_st)))
+
+
 def rotary_fwd(q, k, positions, rot: Rotary, *, inverse: bool = False, out=None, k_out=None, stream=None):
     """q [B, Hq, N, D] and k [B, Hk, N, D] (or None) rotated to `positions`: int32,
     [N] or [B, N], with several axes [axes, N] or [axes, B, N]. fp16, bf16 or
@@ -135,24 +144,28 @@ def rotary_fwd(q, k, positions, rot: Rotary, *, inverse: bool = False, out=None,
     who = "rotary"
     if q is None:
         raise ValueError(f"{who}: q must be given")
-    dtype, dim, index = q.dtype, rot.head_dim, rot.index
-    for t in (q,) if k is None else (q, k):
-        if index < 0 or t.get_device() != index or t.dtype != dtype or t.dim() != 4 or t.shape[3] != dim:
-            raise ValueError(f"{who}: q and k must be [B, H, N, {dim}] tensors of one dtype on {rot.device} (no CPU path)")
-    B, Hq, N, _ = q.shape
+    index = rot.index
+    ok = index >= 0 and q.get_device() == index
+    if k is None:
+        sizes = _tokens(q.shape, q.stride(), None, None, rot.head_dim)
+    else:
+        sizes = _tokens(q.shape, q.stride(), k.shape, k.stride(), rot.head_dim)
+        ok = ok and k.get_device() == index and k.dtype == q.dtype
+    if sizes is None or not ok:
+        raise ValueError(f"{who}: q and k must be [B, H, N, {rot.head_dim}] tensors of one dtype, B and N on {rot.device} "
+                         "(no CPU path) with unit stride on their last dimension")
+    B, N, Hq, qs, Hk, ks = sizes
     ps = check_positions(positions, rot, (B, N), who)
     out = check_out(out, q, "out", who)
-    head = (rot.ref, q.data_ptr(), out.data_ptr(), Hq, head_strides(q, "q", who), head_strides(out, "out", who))
+    head = (rot.ref, q.data_ptr(), out.data_ptr(), Hq, qs, head_strides(out, "out", who))
     if k is None:
         head += (None, None, 0, None, None)
     else:
-        if k.shape[0] != B or k.shape[2] != N:
-            raise ValueError(f"{who}: k {tuple(k.shape)} does not match q {tuple(q.shape)}")
         k_out = check_out(k_out, k, "k_out", who)
         k_to = k_out.data_ptr()
         if k_to == head[2] and k_to:
             raise ValueError(f"{who}: `out` and `k_out` must be two tensors")
-        head += (k.data_ptr(), k_to, k.shape[1], head_strides(k, "k", who), head_strides(k_out, "k_out", who))
+        head += (k.data_ptr(), k_to, Hk, ks, head_strides(k_out, "k_out", who))
     if B == 0 or N == 0:
         return out, k_out
     rt.launch(rt.lib().gr_rotary, head + (rt.dtype_code(q.dtype), B, N, positions.data_ptr(), ps, int(bool(inverse))),
