@@ -283,6 +283,24 @@ __device__ __forceinline__ int gr_paged_swz(int row, int chunk) {
   return CPR >= 16 ? chunk ^ (row & 15) : chunk ^ ((row & 7) ^ ((row >> 3) & 1));
 }
 
+// P is rounded to the type before its product with V, as in the flash body, and the
+// row sum is taken of the rounded ones, so that what a rounding adds to a key's weight
+// divides out in part; sums, bases and partial results are fp32. fp16 alone would
+// drop weights below 2^-25 of the base (the row's max when its base was taken)
+// and round those below 2^-14 to whole steps of 2^-24, which many alike keys add
+// up (131,072 keys of 2^-25.05 beside one of 1: 0.7 % of the result). So fp16's P, row
+// sums and O carry a factor of 2^shift, which divides out of O and leaves the
+// log-sum-exp at the end, by the sequence's keys: N keys lose N 2^-(25 + shift) of
+// the base at most, 2^-14 (an eighth of a rounding of P) for up to 2^26 keys. P then
+// overflows 16 - shift powers of two above the base, and the tile is redone from a
+// new one: no more shift than is needed (4,096 tokens onto 4,096, 16 heads of 64 with
+// scores of deviation 3: 162 us with 0 or the 2 that it takes, 171 with 8, 183 with 12).
+template <class T>
+__device__ __forceinline__ float gr_paged_shift(int keys) {
+  if (!gr_is_same<T, _Float16>::value || keys <= 2048) return 0.f;
+  return (float)gr_imin(32 - __builtin_clz((unsigned)(keys - 1)) - 11, 15);
+}
+
 template <int D, int BN, int NW, int KG, int NS>
 struct gr_paged_lds {
   static constexpr int TILE = BN * D * 2;
@@ -302,6 +320,7 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
   typedef typename MF::vec2 vec2;
   typedef gr_paged_lds<D, BN, NW, KG, NS> L;
   constexpr bool SOLO = NW == 1;             // waves independent until the merge
+  constexpr bool HALF = gr_is_same<T, _Float16>::value;
   constexpr int KB = BN / 32, DB = D / 32, DS = D / 16;
   constexpr int CPR = D / 8;                 // 16-byte chunks of a row
   constexpr int BLOCKS = BN / 16;            // 16-row blocks of a tile
@@ -339,7 +358,7 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
     koff[i] = (unsigned)((gr_perm32(r) & 15) * a.k_ss * 2) + gr_paged_swz<CPR>(r, pc) * 16;
     voff[i] = (unsigned)(r * a.v_ss * 2) + gr_swz_tr<CPR>(r, pc) * 16;
   }
-  const float c = a.scale_log2;
+  const float c = a.scale_log2, shift = gr_paged_shift<T>(t.keys);
   // LDS addresses of the fragments: the swizzles are XORs of chunk bits, so a
   // fragment's is a lane constant XOR an immediate, plus whole rows.
   //  K (gr_paged_swz): row 32 kb + l32, chunk 2 ds + g
@@ -423,7 +442,7 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
   gr_f32x16 o[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db) o[db] = (gr_f32x16)(0.f);
-  float m = -GR_INF, l = 0.f;
+  float m = -GR_INF, l = 0.f, base = shift;    // the row's base, its sum, shift - m c (no base yet: shift)
 
   // One tile's scores, softmax and P V. MASKED: some row may not see all of its
   // keys (bad: 16-key blocks of no page, a bit each).
@@ -472,7 +491,10 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
     }
     vec8 pt[2 * KB];
     float lt;
-    auto make_p = [&](float nmc) {
+    auto make_p = [&]() {
+      // (kept over the tiles for fp16 alone: without the shift it costs more than it
+      // saves, 4,096 tokens onto 4,096, 16 heads of 64 in bf16 152 us to 158)
+      const float nmc = HALF ? base : m == -GR_INF ? 0.f : -m * c;
       lt = 0.f;
 #pragma unroll
       for (int x = 0; x < 2 * KB; ++x) {
@@ -488,7 +510,7 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
         pt[x] = gr_as<vec8>(pw);
       }
     };
-    make_p(m == -GR_INF ? 0.f : -m * c);
+    make_p();
     if (gr_any(fresh || !(lt <= GR_FLASH_SUM_MAX))) {
       float mt = -GR_INF;
 #pragma unroll
@@ -502,7 +524,8 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
 #pragma unroll
       for (int db = 0; db < DB; ++db) o[db] *= alpha;
       m = mn;
-      make_p(m == -GR_INF ? 0.f : -m * c);
+      if (HALF) base = m == -GR_INF ? shift : fmaf(-m, c, shift);
+      make_p();
     }
     l += lt;
     if constexpr (MASKED) {
@@ -682,15 +705,15 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
       ml[k] = *reinterpret_cast<const gr_f32x2*>(at(k) + DB * 4096 - lane * 8);
       mx = fmaxf(mx, ml[k][0]);
     }
-    const float base = mx == -GR_INF ? 0.f : mx;
-    const float w0 = gr_exp2((m - base) * c);
+    const float to = mx == -GR_INF ? 0.f : mx;
+    const float w0 = gr_exp2((m - to) * c);
     l *= w0;
 #pragma unroll
     for (int db = 0; db < DB; ++db) o[db] *= w0;
     m = mx;
 #pragma unroll
     for (int k = 1; k < KG; ++k) {
-      const float wk = gr_exp2((ml[k][0] - base) * c);
+      const float wk = gr_exp2((ml[k][0] - to) * c);
       l = fmaf(wk, ml[k][1], l);
 #pragma unroll
       for (int db = 0; db < DB; ++db)
@@ -734,7 +757,7 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
       }
     if (a.lse && g == 0) {
       const long long trow = a.starts ? t.first + token : (long long)t.b * a.rows + token;
-      a.lse[trow * a.Hq + head] = lt == 0.f ? -GR_INF : (m * c + __builtin_amdgcn_logf(lt)) * 0.6931471805599453f;
+      a.lse[trow * a.Hq + head] = lt == 0.f ? -GR_INF : (m * c + (__builtin_amdgcn_logf(lt) - shift)) * 0.6931471805599453f;
     }
   }
 }
@@ -831,7 +854,7 @@ __device__ __forceinline__ void gr_paged_merge_body(const gr_paged_args& a) {
   if (w0 < 0 || np <= 1) return;
   const int skew = cut.begin(w0) < x0 ? 1 : 0;
   auto slot = [&](int p, int r) { return (long long)(2 * (w0 + p) + (p == 0 ? skew : 0)) * BM + r; };
-  const float c = a.scale_log2;
+  const float c = a.scale_log2, shift = gr_paged_shift<T>(t.keys);
   const int rows = gr_imin(BM, t.nrows - t.row0);
   const int sub = lane / LPR, d4 = (lane % LPR) * 4;
   auto put = [&](int r, gr_f32x4 o, float l, float mx) {
@@ -841,7 +864,7 @@ __device__ __forceinline__ void gr_paged_merge_body(const gr_paged_args& a) {
     *reinterpret_cast<gr_u32x2*>(op) = (gr_u32x2){gr_pack2f<T>(o[0] * inv, o[1] * inv), gr_pack2f<T>(o[2] * inv, o[3] * inv)};
     if (a.lse && d4 == 0) {
       const long long trow = a.starts ? t.first + token : (long long)t.b * a.rows + token;
-      a.lse[trow * a.Hq + head] = l == 0.f ? -GR_INF : (mx * c + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+      a.lse[trow * a.Hq + head] = l == 0.f ? -GR_INF : (mx * c + (__builtin_amdgcn_logf(l) - shift)) * 0.6931471805599453f;
     }
   };
   if (np <= 2 * rows) {

@@ -1,0 +1,47 @@
+"""Paged attention and appending at the edges of what they promise."""
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+from test_paged_gpu import Setup  # noqa: E402
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("w", [23.4, 24.6, 25.05, 26.5])
+@pytest.mark.parametrize("n,G,D,alone", [(1, 4, 64, False), (1, 4, 128, True), (5, 7, 64, True), (200, 2, 64, True),
+                                         (200, 2, 128, False), (4100, 8, 64, True), (4100, 8, 128, True)])
+def test_many_small_weights_add_up(dtype, w, n, G, D, alone):
+    """One key of weight 1 and value 1, then N of about 2^-w and value -1: a row that sees M' = N p of the latter is
+    (1 - M') / (1 + M'), its log-sum-exp log(1 + M'). In tiles of all sizes, a workgroup a tile and shared out."""
+    from grammar.paged import paged_attention
+    N = 50_001
+    print(f"[case] small weights {dtype} w {w} n{n} G{G} D{D} alone={alone}", flush=True)
+    s = Setup([N], 1, 64, D, dtype)
+    s.k.zero_()
+    s.k[..., 0] = -w * math.log(2)
+    s.v.fill_(-1.0)
+    first = int(s.table[0, 0])
+    x = float(s.k[first, 0, 1, 0])                               # the score as it is stored
+    s.k[first, 0, 0] = 0
+    s.v[first, 0, 0] = 1
+    q = torch.zeros(1, G, n, D, dtype=s.dtype, device=s.dev)
+    q[..., 0] = 1
+    lse = torch.empty(1, n, G, device=s.dev)
+    got = paged_attention(q, s.cache, s.table, s.lens, scale=1.0, lse=lse,
+                          workspace=torch.empty(0, dtype=torch.uint8, device=s.dev) if alone else None)
+    m = (N - n + torch.arange(n, dtype=torch.float64, device=s.dev)) * math.exp(x)
+    want = ((1 - m) / (1 + m))[None, None, :, None]
+    # p rounds by half a step of itself and is off by its exponent's rounding (2^-24 of 40) and 2^-22, which is what M'
+    # and log(1 + M') are off by, and half of what (1 - M') / (1 + M') is; in fp16 all keys far below the base lose 2^-14
+    # of it at most. fp32 sums: a rounding for each 4 keys at least, 2^-24 of a sum of about 1. The result rounds once.
+    u = torch.finfo(s.dtype).eps / 2
+    sums = N / 4 * 2.0 ** -24
+    off = float(m.max()) * (u + 40 * 2.0 ** -24 + 2.0 ** -22) + (2.0 ** -14 if dtype == "fp16" else 0)
+    assert ((got.double() - want).abs() <= 2 * off + sums + u * want.abs()).all(), \
+        float((got.double() - want).abs().max())
+    assert ((lse.double() - torch.log1p(m)[None, :, None]).abs() <= off + sums + 2.0 ** -22).all(), \
+        float((lse.double() - torch.log1p(m)[None, :, None]).abs().max())
