@@ -135,7 +135,7 @@ __device__ __forceinline__ void gr_rope_body(const gr_rope_args& a, bool inverse
     if (ends >= a.B) return;                     // behind the last sequence
     b = ends;
     const int s0 = a.starts[b], s1 = a.starts[b + 1];
-    if (tok < s0 || tok >= s1) return;
+    if (tok < s0 || tok >= s1 || s0 < 0 || s1 > a.tokens) return;   // (a sequence out of the batch has no tokens)
     i = tok - s0;
     at = a.lens[b] - (s1 - s0) + i;
   } else {

@@ -45,3 +45,32 @@ def test_many_small_weights_add_up(dtype, w, n, G, D, alone):
         float((got.double() - want).abs().max())
     assert ((lse.double() - torch.log1p(m)[None, :, None]).abs() <= off + sums + 2.0 ** -22).all(), \
         float((lse.double() - torch.log1p(m)[None, :, None]).abs().max())
+
+
+@pytest.mark.parametrize("starts,rows_of", [([0, 3, 9], {0: (0, 3)}), ([-2, 3, 6], {1: (3, 6)}), ([-1, 7, 8], {}),
+                                            ([0, 0, 7], {})])
+def test_sequences_out_of_the_batch_append_nothing(starts, rows_of):
+    """A sequence whose rows are not all in the batch has no new tokens, to appends as to attention."""
+    from grammar.paged import paged_append, paged_attention
+    from grammar.rotary import Rotary
+    s = Setup([40, 50], 2, 16, 64, "fp16", seed=5)
+    rot = Rotary(64, device=s.dev)
+    print(f"[case] starts {starts}", flush=True)
+    q, k, v = s.randn(6, 4, 64), s.randn(6, 2, 64), s.randn(6, 2, 64)
+    at = torch.tensor(starts, dtype=torch.int32, device=s.dev)
+    before = s.k.clone(), s.v.clone()
+    out, o = torch.full_like(q, 5.0), torch.full_like(q, 5.0)
+    paged_append(k, v, s.cache, s.table, s.lens, starts=at, q=q, rotary=rot, out=out)
+    paged_attention(q, s.cache, s.table, s.lens, starts=at, out=o)
+    written = torch.zeros(s.k.shape[0], s.S, dtype=torch.bool, device=s.dev)
+    rows = torch.zeros(6, dtype=torch.bool, device=s.dev)
+    for b, (r0, r1) in rows_of.items():
+        place = torch.arange(s.lens_host[b] - (r1 - r0), s.lens_host[b], device=s.dev)
+        page, slot = s.table[b].long()[place // s.S], place % s.S
+        written[page, slot] = True
+        rows[r0:r1] = True
+        assert torch.equal(s.v[page, :, slot], v[r0:r1])
+    for now, old in zip((s.k, s.v), before):
+        assert torch.equal(now.transpose(1, 2)[~written], old.transpose(1, 2)[~written])
+    for x in (out, o):
+        assert (x[~rows] == 5.0).all() and (x[rows] != 5.0).any(-1).all()
