@@ -126,7 +126,16 @@ struct gr_paged_seqs {
     nt = from + lane >= a.B || rows == 0 ? 0 : SMALL && rows <= 32 ? 1 : (rows + BM - 1) / BM;
     if (SMALL && only == (rows <= 32 ? 1 : 2)) nt = 0;
     nb = gr_paged_blocks(gr_paged_keys(a, len));
+    // Starts that overlap could make more tiles than the grid, and more blocks than 32
+    // bits count (a head's number from them could then be below 0): tiles past the
+    // grid's are left out. Starts in order never make them.
+    nt = gr_imin(nt, a.tiles);
     tsum = gr_wave_scan(nt);
+    if (__builtin_expect(tiles_after() > a.tiles, 0)) {
+      const int over = tiles + tsum - a.tiles;
+      nt = over <= 0 ? nt : nt > over ? nt - over : 0;
+      tsum -= over > 0 ? over : 0;
+    }
     bsum = gr_wave_scan((int)((unsigned)nt * (nb + GR_PAGED_COST)));
   }
   __device__ __forceinline__ int tiles_after() const { return tiles + __builtin_amdgcn_readlane(tsum, 63); }
@@ -848,10 +857,8 @@ __device__ __forceinline__ void gr_paged_merge_body(const gr_paged_args& a) {
   // another tile, and then left this one's part in its second place
   const gr_paged_cut cut(per_head * a.Hkv, a.shares);
   const int x0 = hk * per_head + t.x0;
-  // (the bounds: starts that overlap can make more blocks than 32 bits count)
-  const int w0 = gr_imin(cut.of(x0), cut.W - 1);
-  const int np = gr_imin(cut.of(x0 + t.nb - 1) + 1, cut.W) - w0;
-  if (w0 < 0 || np <= 1) return;
+  const int w0 = cut.of(x0), np = cut.of(x0 + t.nb - 1) + 1 - w0;
+  if (np <= 1) return;
   const int skew = cut.begin(w0) < x0 ? 1 : 0;
   auto slot = [&](int p, int r) { return (long long)(2 * (w0 + p) + (p == 0 ? skew : 0)) * BM + r; };
   const float c = a.scale_log2, shift = gr_paged_shift<T>(t.keys);

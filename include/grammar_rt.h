@@ -278,8 +278,10 @@ typedef struct gr_paged_cache {
  *  max_new, max_len: the most new tokens and keys of a sequence, where known (0:
  *          not). They only choose how a call is shared out.
  * What the arrays hold is bounded on the device: a page id outside of the cache,
- * a position outside of the table or a start outside of the batch reads and
- * writes nothing (such keys do not exist, such tokens are not stored). */
+ * a position outside of the table or a sequence whose starts are not both in
+ * the batch reads and writes nothing (such keys do not exist, such tokens are not
+ * stored). Starts are to be in order: where they overlap, nothing else is touched, but
+ * which of the sequences a row belongs to is not defined. */
 typedef struct gr_paged_batch {
   const int* table;
   long long table_stride;

@@ -74,3 +74,22 @@ def test_sequences_out_of_the_batch_append_nothing(starts, rows_of):
         assert torch.equal(now.transpose(1, 2)[~written], old.transpose(1, 2)[~written])
     for x in (out, o):
         assert (x[~rows] == 5.0).all() and (x[rows] != 5.0).any(-1).all()
+
+
+@pytest.mark.parametrize("D,hint", [(64, 1), (64, 0), (128, 1), (128, 0)])
+def test_overlapping_starts_stay_in_bounds(D, hint):
+    """Every second sequence claims all of the batch's rows: more tiles than the grid has, and more blocks of keys than
+    32 bits count. The rows of no other call are touched, and every row gets the result that any of them would give."""
+    from grammar.paged import paged_attention
+    B, rows, W = 512, 16_384, 65_536
+    print(f"[case] overlapping starts D{D} hint {hint}", flush=True)
+    s = Setup([16], 2, 16, D, "bf16")
+    table = torch.full((1, W), -1, dtype=torch.int32, device=s.dev).expand(B, W)
+    lens = torch.full((B,), W * 16, dtype=torch.int32, device=s.dev)
+    starts = torch.tensor([0, rows] * (B // 2) + [0], dtype=torch.int32, device=s.dev)
+    q = s.randn(rows, 2, D)
+    for ws in (None, torch.empty(0, dtype=torch.uint8, device=s.dev)):
+        out = torch.full((rows + 64, 2, D), 5.0, dtype=s.dtype, device=s.dev)
+        paged_attention(q, s.cache, table, lens, starts=starts, max_new=hint, out=out[32:-32], workspace=ws)
+        torch.cuda.synchronize()
+        assert not out[32:-32].any() and (out[:32] == 5.0).all() and (out[-32:] == 5.0).all()
