@@ -220,17 +220,26 @@ def _autograd_function():
     return RotaryFunction
 
 
+def _has_tangent(*tensors) -> bool:
+    """Whether one of them is a dual tensor of forward-mode differentiation."""
+    import torch.autograd.forward_ad as forward_ad
+    return forward_ad._current_level >= 0 and \
+        any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 _ROTARY_FN = None
 
 
 def rotary(q, k, positions, rot: Rotary):
     """rotary_fwd, differentiable in q and k (either may need no gradient; k
     may be None): both rotations are one launch of gr_rotary, and so are their
-    gradients. A backward pass captured into a graph takes
+    gradients. Forward-mode tangents are refused (NotImplementedError), as by
+    flash_attention. A backward pass captured into a graph takes
     torch.autograd.grad: an eager backward of the same leaves on another stream,
     still alive, must not be joined by a captured one (torch's own rule)."""
     import torch
-    if not torch.is_grad_enabled() or not (q.requires_grad or (k is not None and k.requires_grad)):
+    recorded = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))
+    if not recorded and not _has_tangent(q, k):
         return rotary_fwd(_dense(q), None if k is None else _dense(k), positions, rot)
     global _ROTARY_FN
     if _ROTARY_FN is None:
