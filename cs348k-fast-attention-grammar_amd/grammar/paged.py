@@ -117,7 +117,7 @@ def _heads(t, name, lead, heads, cache, who):
     return st if st != "stride" else head_strides(t, name, who)
 
 
-def _append_args(k, v, cache, table, lens, starts, q, rotary, positions, max_new, out):
+def _append_args(k, v, cache, table, lens, starts, q, rotary, positions, max_new, out, stream):
     who = "paged_append"
     desc, lead = _batch(cache, table, lens, starts, k, max_new, 0, who)
     ks, vs = _heads(k, "k", lead, cache.heads, cache, who), _heads(v, "v", lead, cache.heads, cache, who)
@@ -131,7 +131,7 @@ def _append_args(k, v, cache, table, lens, starts, q, rotary, positions, max_new
         ref = rotary.ref
     if q is not None:
         Hq = q.shape[1] if q.dim() >= 3 else 0
-        qs, out = _heads(q, "q", lead, Hq, cache, who), check_out(out, q, "out", who)
+        qs, out = _heads(q, "q", lead, Hq, cache, who), check_out(out, q, "out", who, stream)
         qp, op, os = q.data_ptr(), out.data_ptr(), head_strides(out, "out", who)
     elif out is None:
         qp = op = qs = os = None
@@ -156,7 +156,7 @@ def paged_append(k, v, cache: PagedCache, table, lens, *, starts=None, q=None, r
     Returns the rotated queries, or None without q. A token whose place is
     outside of the table or on a page id outside of the cache is not stored.
     max_new: the most new tokens of a sequence, where known."""
-    args, out, keep = _append_args(k, v, cache, table, lens, starts, q, rotary, positions, max_new, out)
+    args, out, keep = _append_args(k, v, cache, table, lens, starts, q, rotary, positions, max_new, out, stream)
     rt.launch(rt.lib().gr_paged_append, args, k, stream, "gr_paged_append")
     return out
 
@@ -165,7 +165,7 @@ def bind_paged_append(k, v, cache: PagedCache, table, lens, *, starts=None, q=No
                       positions=None, max_new: int = 0, out=None, stream=None):
     """Validate once and return (launch, out): launch() enqueues gr_paged_append
     on these tensors with pre-packed arguments; arguments as paged_append."""
-    args, out, keep = _append_args(k, v, cache, table, lens, starts, q, rotary, positions, max_new, out)
+    args, out, keep = _append_args(k, v, cache, table, lens, starts, q, rotary, positions, max_new, out, stream)
     return rt.launcher(rt.lib().gr_paged_append, args, k, stream, "gr_paged_append", out, keep), out
 
 
@@ -177,7 +177,7 @@ def _attn_args(q, cache, table, lens, starts, causal, scale, max_new, max_len, o
     qs = _heads(q, "q", lead, Hq, cache, who)
     if Hq == 0 or Hq % cache.heads:
         raise ValueError(f"{who}: {Hq} query heads are not a multiple of the cache's {cache.heads}")
-    out = check_out(out, q, "out", who)
+    out = check_out(out, q, "out", who, stream)
     if lse is not None:
         want = (lead[0], lead[1], Hq) if len(lead) == 2 else (lead[0], Hq)
         if tuple(lse.shape) != want or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.get_device() != cache.index:

@@ -116,11 +116,10 @@ def _takes(shape: tuple, st: tuple, like: tuple) -> bool:
     return shape == like and not any(s == 0 and n > 1 for s, n in zip(st, shape))
 
 
-def check_out(out, like, name: str, who: str):
-    """`out`, checked, or a new tensor laid out as `like`."""
-    import torch
+def check_out(out, like, name: str, who: str, stream):
+    """`out`, checked, or a new tensor laid out as `like` for a launch on `stream`."""
     if out is None:
-        return torch.empty_like(like)
+        return rt.empty_like(like, stream)
     if not _takes(out.shape, out.stride(), like.shape) or out.dtype != like.dtype or out.get_device() != like.get_device():
         raise ValueError(f"{who}: bad `{name}` tensor")
     return out
@@ -156,12 +155,12 @@ def rotary_fwd(q, k, positions, rot: Rotary, *, inverse: bool = False, out=None,
                          "(no CPU path) with unit stride on their last dimension")
     B, N, Hq, qs, Hk, ks = sizes
     ps = check_positions(positions, rot, (B, N), who)
-    out = check_out(out, q, "out", who)
+    out = check_out(out, q, "out", who, stream)
     head = (rot.ref, q.data_ptr(), out.data_ptr(), Hq, qs, head_strides(out, "out", who))
     if k is None:
         head += (None, None, 0, None, None)
     else:
-        k_out = check_out(k_out, k, "k_out", who)
+        k_out = check_out(k_out, k, "k_out", who, stream)
         k_to = k_out.data_ptr()
         if k_to == head[2] and k_to:
             raise ValueError(f"{who}: `out` and `k_out` must be two tensors")

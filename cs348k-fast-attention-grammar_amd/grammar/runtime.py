@@ -317,6 +317,22 @@ def launcher(fn, args: tuple, t, stream, what: str, out, keep):
 _STREAM_PER_THREAD = 2               # hipStreamPerThread
 
 
+def _allocate(make, device, stream):
+    """make() for a launch on `stream`: once dropped, the memory is only reused
+    by work queued there later."""
+    import torch
+    s = torch_stream(stream, device)
+    if s.cuda_stream == _STREAM_PER_THREAD:
+        # One handle for another stream in every host thread: memory kept by
+        # handle would pass between them. The current stream's, ordered by events.
+        t = make()
+        s.wait_stream(torch.cuda.current_stream(device))
+        t.record_stream(s)
+        return t
+    with torch.cuda.stream(s):
+        return make()
+
+
 def empty(shape, dtype, device, stream=None):
     """torch.empty for a launch on `stream` (the current stream if None),
     allocated for that stream: once dropped it is only reused by work queued
@@ -324,16 +340,19 @@ def empty(shape, dtype, device, stream=None):
     import torch
     if stream is None:
         return torch.empty(shape, dtype=dtype, device=device)
-    s = torch_stream(stream, device)
-    if s.cuda_stream == _STREAM_PER_THREAD:
-        # One handle for another stream in every host thread: memory kept by
-        # handle would pass between them. The current stream's, ordered by events.
-        t = torch.empty(shape, dtype=dtype, device=device)
-        s.wait_stream(torch.cuda.current_stream(device))
-        t.record_stream(s)
-        return t
-    with torch.cuda.stream(s):
-        return torch.empty(shape, dtype=dtype, device=device)
+    return _allocate(lambda: torch.empty(shape, dtype=dtype, device=device), device, stream)
+
+
+def empty_like(t, stream=None):
+    """torch.empty_like for the result of a launch on `stream`: as empty(), and
+    what the current stream has queued when it is dropped (a caller's reads)
+    comes before its reuse too."""
+    import torch
+    if stream is None:
+        return torch.empty_like(t)
+    r = _allocate(lambda: torch.empty_like(t), t.device, stream)
+    r.record_stream(torch.cuda.current_stream(t.device))
+    return r
 
 
 def workspace(nbytes: int, device, stream=None):
