@@ -50,7 +50,6 @@ def picked_shape(B: int, H: int, N: int, D: int, dtype: str, *, causal: bool = F
 def _fwd_args(q, k, v, lse, causal, scale, k_transposed, block_m, block_n, out, stream):
     """(C arguments, out) of gr_attn_fwd, or (lse given) of gr_attn_fwd_train,
     after checking the operands."""
-    import torch
     dtype = q.dtype
     for name, t in (("q", q), ("k", k), ("v", v)):
         if not t.is_cuda:
@@ -69,7 +68,7 @@ def _fwd_args(q, k, v, lse, causal, scale, k_transposed, block_m, block_n, out, 
     if q.stride(3) != 1 or v.stride(3) != 1 or k.stride(3) != 1:
         raise ValueError("flash_attention_fwd: innermost dimension must be contiguous")
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=q.device)
+        out = rt.result(shape, dtype, q.device, stream)
     elif out.shape != shape or out.dtype != dtype or out.stride(3) != 1:
         raise ValueError("flash_attention_fwd: bad `out` tensor")
     if scale is None:
@@ -112,12 +111,12 @@ def flash_attention_fwd(q, k, v, *, causal: bool = False, scale: float | None = 
     return out
 
 
-def _train_lse(q, lse):
+def _train_lse(q, lse, stream):
     """The [B, H, N] float32 row log-sum-exp to write: `lse`, checked, or a new one."""
     import torch
     shape = q.shape[:3]
     if lse is None:
-        return torch.empty(shape, dtype=torch.float32, device=q.device)
+        return rt.result(shape, torch.float32, q.device, stream)
     if lse.shape != shape or lse.dtype != torch.float32 or not lse.is_contiguous():
         raise ValueError("flash_attention_fwd_train: bad `lse` tensor")
     return lse
@@ -130,7 +129,7 @@ def bind_flash_attention_train(q, k, v, *, causal: bool = False, scale: float | 
     the scaled scores ([B, H, N] fp32, natural log). K in [B, H, N, D]."""
     if q.dim() != 4:
         raise ValueError("flash_attention_fwd: q must be 4-D")
-    lse = _train_lse(q, lse)
+    lse = _train_lse(q, lse, stream)
     args, out = _fwd_args(q, k, v, lse, causal, scale, False, block_m, block_n, out, stream)
     fn = rt.lib().gr_attn_fwd_train
     keep = (q, k, v, out, lse)
@@ -148,7 +147,7 @@ def flash_attention_fwd_train(q, k, v, *, causal: bool = False, scale: float | N
     K in [B, H, N, D] layout. Returns (out, lse)."""
     if q.dim() != 4:
         raise ValueError("flash_attention_fwd: q must be 4-D")
-    lse = _train_lse(q, lse)
+    lse = _train_lse(q, lse, stream)
     args, out = _fwd_args(q, k, v, lse, causal, scale, False, block_m, block_n, out, stream)
     rt.check(rt.lib().gr_attn_fwd_train(*args), "gr_attn_fwd_train")
     return out, lse
@@ -175,7 +174,7 @@ def _bwd_args(q, k, v, o, do, lse, causal, scale, workspace, grads, stream):
     elif workspace.numel() * workspace.element_size() < need:
         raise ValueError(f"flash_attention_bwd: workspace of {need} bytes needed")
     if grads is None:
-        grads = (torch.empty_like(q), torch.empty_like(q), torch.empty_like(q))
+        grads = tuple(rt.empty_like(q, stream) for _ in range(3))
     else:
         for t in grads:
             if t.shape != shape or t.dtype != dtype or not t.is_contiguous():
@@ -318,7 +317,6 @@ def decode_splits_noalloc(B: int, H: int, Nq: int, N: int, D: int, cu_count: int
 
 def _decode_args(q, k, v, scale, splits, out, workspace, stream):
     """(C arguments, out, workspace) of gr_attn_decode after checking the operands."""
-    import torch
     dtype = q.dtype
     for name, t in (("q", q), ("k", k), ("v", v)):
         if not t.is_cuda:
@@ -330,7 +328,7 @@ def _decode_args(q, k, v, scale, splits, out, workspace, stream):
     if k.shape != (B, H, N, D) or v.shape != (B, H, N, D):
         raise ValueError(f"flash_attention_decode: k {tuple(k.shape)} / v {tuple(v.shape)} do not match q {tuple(q.shape)}")
     if out is None:
-        out = torch.empty((B, H, Nq, D), dtype=dtype, device=q.device)
+        out = rt.result((B, H, Nq, D), dtype, q.device, stream)
     elif out.shape != (B, H, Nq, D) or out.dtype != dtype or out.stride(3) != 1:
         raise ValueError("flash_attention_decode: bad `out` tensor")
     if scale is None:
@@ -372,7 +370,6 @@ def bind_flash_attention_decode_noalloc(q, k, v, *, scale: float | None = None, 
     that overlap on one device race on that array. Raises if the split needs
     more than rt.DECODE_SCRATCH_BYTES; splits = 0 picks the largest split
     decode_splits allows that fits it (decode_splits_noalloc)."""
-    import torch
     for name, t in (("q", q), ("k", k), ("v", v)):
         if not t.is_cuda:
             raise ValueError(f"flash_attention_decode_noalloc: {name} must be a GPU tensor (no CPU path)")
@@ -383,7 +380,7 @@ def bind_flash_attention_decode_noalloc(q, k, v, *, scale: float | None = None, 
     if tuple(k.shape) != (B, H, N, D) or tuple(v.shape) != (B, H, N, D):
         raise ValueError("flash_attention_decode_noalloc: k / v do not match q")
     if out is None:
-        out = torch.empty((B, H, Nq, D), dtype=q.dtype, device=q.device)
+        out = rt.result((B, H, Nq, D), q.dtype, q.device, stream)
     elif tuple(out.shape) != (B, H, Nq, D) or out.dtype != q.dtype or out.stride(3) != 1:
         raise ValueError("flash_attention_decode_noalloc: bad `out` tensor")
     if scale is None:

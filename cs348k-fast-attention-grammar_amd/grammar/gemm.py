@@ -50,7 +50,6 @@ def gemm(a, b, *, epilogue: str = "none", alpha: float = 1.0, b_kmajor: bool = F
     a: [..., M, K]; b: [..., K, N], or [..., N, K] with b_kmajor=True (b used
     transposed). Leading dims are a batch (b may have none: broadcast).
     Returns [..., M, N] in a's dtype (or writes `out`)."""
-    import torch
     for name, t in (("a", a), ("b", b)):
         if not t.is_cuda:
             raise ValueError(f"gemm: {name} must be a GPU tensor (no CPU path)")
@@ -69,7 +68,7 @@ def gemm(a, b, *, epilogue: str = "none", alpha: float = 1.0, b_kmajor: bool = F
         b_sb = 0
     shape = tuple(a.shape[:-2]) + (M, N)
     if out is None:
-        out = torch.empty(shape, dtype=a.dtype, device=a.device)
+        out = rt.result(shape, a.dtype, a.device, stream)
     elif tuple(out.shape) != shape or out.dtype != a.dtype:
         raise ValueError("gemm: bad `out` tensor")
     zc, _, _, c_sb, c_sm = _batch_view(out, "out")
@@ -98,7 +97,6 @@ def mlp_fwd(x, w1, w2, *, block_m: int = 0, block_n: int = 0, h=None, out=None, 
     """Y = SiLU(X @ W1) @ W2 with X [M, D], W1 [D, F], W2 [F, D] contiguous
     fp16/bf16 GPU tensors. `h` ([M, F]) is the intermediate buffer (allocated
     if not given). Returns Y [M, D]."""
-    import torch
     for name, t in (("x", x), ("w1", w1), ("w2", w2)):
         if not t.is_cuda:
             raise ValueError(f"mlp_fwd: {name} must be a GPU tensor (no CPU path)")
@@ -111,7 +109,7 @@ def mlp_fwd(x, w1, w2, *, block_m: int = 0, block_n: int = 0, h=None, out=None, 
     if h is None:
         h = rt.empty((M, F), x.dtype, x.device, stream)
     if out is None:
-        out = torch.empty((M, D), dtype=x.dtype, device=x.device)
+        out = rt.result((M, D), x.dtype, x.device, stream)
     for name, t, shp in (("h", h, (M, F)), ("out", out, (M, D))):
         if tuple(t.shape) != shp or not t.is_contiguous() or t.dtype != x.dtype:
             raise ValueError(f"mlp_fwd: bad `{name}` tensor")

@@ -343,16 +343,30 @@ def empty(shape, dtype, device, stream=None):
     return _allocate(lambda: torch.empty(shape, dtype=dtype, device=device), device, stream)
 
 
+def _result(make, device, stream):
+    """make() for what a launch on `stream` returns: allocated for that stream,
+    and what the current stream has queued when it is dropped (a caller's
+    reads) comes before its reuse too."""
+    import torch
+    t = _allocate(make, device, stream)
+    t.record_stream(torch.cuda.current_stream(device))
+    return t
+
+
+def result(shape, dtype, device, stream=None):
+    """torch.empty for the result of a launch on `stream` (_result)."""
+    import torch
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    return _result(lambda: torch.empty(shape, dtype=dtype, device=device), device, stream)
+
+
 def empty_like(t, stream=None):
-    """torch.empty_like for the result of a launch on `stream`: as empty(), and
-    what the current stream has queued when it is dropped (a caller's reads)
-    comes before its reuse too."""
+    """torch.empty_like for the result of a launch on `stream` (_result)."""
     import torch
     if stream is None:
         return torch.empty_like(t)
-    r = _allocate(lambda: torch.empty_like(t), t.device, stream)
-    r.record_stream(torch.cuda.current_stream(t.device))
-    return r
+    return _result(lambda: torch.empty_like(t), t.device, stream)
 
 
 def workspace(nbytes: int, device, stream=None):

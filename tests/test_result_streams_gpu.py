@@ -42,6 +42,56 @@ def _paged_attention(stream):
     return _paged(stream, True)
 
 
+def _heads(*shape):
+    return torch.randn(*shape, device="cuda").half()
+
+
+def _flash(stream):
+    from grammar.attention import flash_attention_fwd
+    q = _heads(2, 8, 1024, 64)
+    return lambda: flash_attention_fwd(q, q, q, stream=stream)
+
+
+def _flash_train(stream):
+    from grammar.attention import flash_attention_fwd_train
+    q = _heads(2, 8, 1024, 64)
+    return lambda: flash_attention_fwd_train(q, q, q, stream=stream)
+
+
+def _flash_bwd(stream):
+    from grammar.attention import flash_attention_bwd, flash_attention_fwd_train
+    q = _heads(2, 8, 1024, 64)
+    o, lse = flash_attention_fwd_train(q, q, q)
+    return lambda: flash_attention_bwd(q, q, q, o, o, lse, stream=stream)
+
+
+def _decode(stream):
+    from grammar.attention import flash_attention_decode
+    q, kv = _heads(4, 64, 64, 128), _heads(4, 64, 256, 128)
+    return lambda: flash_attention_decode(q, kv, kv, stream=stream)
+
+
+def _bound_decode(stream):
+    from grammar.attention import bind_flash_attention_decode_noalloc
+    q, kv = _heads(4, 64, 64, 128), _heads(4, 64, 256, 128)
+    return lambda: bind_flash_attention_decode_noalloc(q, kv, kv, splits=1, stream=stream)[0]()
+
+
+def _gemm(stream):
+    from grammar.gemm import gemm
+    a, b = _heads(1024, 256), _heads(256, 2048)
+    return lambda: gemm(a, b, stream=stream)
+
+
+def _mlp(stream):
+    from grammar.gemm import mlp_fwd
+    x, w1, w2 = _heads(2048, 1024), _heads(1024, 512) / 16, _heads(512, 1024) / 16
+    return lambda: mlp_fwd(x, w1, w2, stream=stream)
+
+
+CALLS = [_rotary, _paged_append, _paged_attention, _flash, _flash_train, _flash_bwd, _decode, _bound_decode, _gemm, _mlp]
+
+
 def _stream_of(t):
     """The handle of the stream whose pool a tensor's memory is from."""
     return next(seg["stream"] for seg in torch.cuda.memory_snapshot()
@@ -49,7 +99,7 @@ def _stream_of(t):
 
 
 @pytest.mark.parametrize("raw", [False, True], ids=["stream", "handle"])
-@pytest.mark.parametrize("call", [_rotary, _paged_append, _paged_attention], ids=lambda f: f.__name__[1:])
+@pytest.mark.parametrize("call", CALLS, ids=lambda f: f.__name__[1:])
 def test_results_belong_to_the_launch_stream(call, raw):
     """A result is memory of the stream that its launch writes it on: no work of another stream can still be reading
     what was there before. Dropped, it also waits for what the current stream has queued by then."""
