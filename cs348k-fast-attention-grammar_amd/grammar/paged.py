@@ -54,6 +54,10 @@ class PagedCache:
                                       rt.dtype_code(k.dtype), pages, heads, size, D)
         self.ref = ctypes.addressof(self.desc)
 
+    def __reduce__(self):
+        """For copies and pickles: the descriptor points at this object's pages."""
+        return type(self), (self.k, self.v)
+
     @classmethod
     def empty(cls, pages: int, heads: int, page_size: int, head_dim: int, dtype, device="cuda"):
         """A cache of unwritten pages (their contents are never read before

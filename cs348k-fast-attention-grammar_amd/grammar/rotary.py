@@ -63,10 +63,21 @@ class Rotary:
         whole = [round(math.ldexp((f / (2 * math.pi)) % 1.0, 64)) % (1 << 64) for f in freqs]
         self.turns = torch.tensor([w - (1 << 64) if w >> 63 else w for w in whole], dtype=torch.int64, device=device)
         self.axes = torch.tensor(axes, dtype=torch.uint8, device=device)
+        self._describe()
+
+    def _describe(self):
         self.device, self.index = self.turns.device, self.turns.get_device()
-        self.desc = rt.RotarySpec(self.turns.data_ptr(), self.axes.data_ptr(), pairs, self.naxes, self.head_dim,
-                                  int(self.interleaved))
+        self.desc = rt.RotarySpec(self.turns.data_ptr(), self.axes.data_ptr(), self.rotary_dim // 2, self.naxes,
+                                  self.head_dim, int(self.interleaved))
         self.ref = ctypes.addressof(self.desc)
+
+    def __getstate__(self):
+        """For copies and pickles: without what points at this object's tables."""
+        return {n: v for n, v in self.__dict__.items() if n not in ("device", "index", "desc", "ref")}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self._describe()
 
 
 @functools.lru_cache(maxsize=1024)

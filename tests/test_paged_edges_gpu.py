@@ -93,3 +93,28 @@ def test_overlapping_starts_stay_in_bounds(D, hint):
         paged_attention(q, s.cache, table, lens, starts=starts, max_new=hint, out=out[32:-32], workspace=ws)
         torch.cuda.synchronize()
         assert not out[32:-32].any() and (out[:32] == 5.0).all() and (out[-32:] == 5.0).all()
+
+
+def test_caches_and_rotations_can_be_copied_and_pickled():
+    import copy
+    import pickle
+    from grammar.paged import PagedCache, paged_append, paged_attention
+    from grammar.rotary import Rotary
+    s = Setup([40, 50], 2, 16, 64, "fp16", seed=6)
+    rot = Rotary(64, device=s.dev)
+    both = torch.stack((s.k, s.v), 1)                            # keys and values in one tensor
+    q, k, v = s.randn(2, 4, 1, 64), s.randn(2, 2, 1, 64), s.randn(2, 2, 1, 64)
+    for cache in (s.cache, PagedCache(both[:, 0], both[:, 1])):
+        for make in (copy.deepcopy, lambda x: pickle.loads(pickle.dumps(x))):
+            c, r = make((cache, rot))
+            assert type(c) is PagedCache and c.desc.k == c.k.data_ptr() != cache.k.data_ptr()
+            assert torch.equal(c.k, cache.k) and torch.equal(c.v, cache.v) and c.k.stride() == cache.k.stride()
+            old = cache.k.clone()
+            qr = paged_append(k, v, c, s.table, s.lens, q=q, rotary=r)
+            got = paged_attention(qr, c, s.table, s.lens)
+            assert torch.equal(cache.k, old)                     # the copy's pages are its own
+            there = make(cache)
+            assert torch.equal(paged_append(k, v, there, s.table, s.lens, q=q, rotary=rot), qr)
+            assert torch.equal(paged_attention(qr, there, s.table, s.lens), got)
+        shared = copy.copy(cache)
+        assert shared.k is cache.k and shared.ref != cache.ref

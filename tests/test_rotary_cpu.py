@@ -33,3 +33,28 @@ def test_forward_mode_tangents_are_refused(launches, which, grad):
         assert torch.equal(plain[0], q) and torch.equal(plain[1], k)
     assert rotary(q, None, pos, None)[1] is None
     assert launches[-2:] == [False, False]
+
+
+@pytest.mark.parametrize("how", ["copy", "deepcopy", "pickle", "save"])
+def test_rotary_can_be_copied_and_pickled(how):
+    """As part of a model that is copied or saved whole; a copy points at tables of its own."""
+    import copy
+    import io
+    import pickle
+    from grammar.rotary import Rotary
+    r = Rotary(64, rotary_dim=48, sections=[4, 8, 12], base=500.0, interleaved=True, device="cpu")
+
+    def saved(x):
+        file = io.BytesIO()
+        torch.save({"rotary": x}, file)
+        file.seek(0)
+        return torch.load(file, weights_only=False)["rotary"]          # (its own file, just written)
+    c = {"copy": copy.copy, "deepcopy": copy.deepcopy, "pickle": lambda x: pickle.loads(pickle.dumps(x)),
+         "save": saved}[how](r)
+    assert type(c) is Rotary and c is not r and c.ref != r.ref
+    for name in ("head_dim", "rotary_dim", "interleaved", "sections", "naxes", "inv_freq", "device", "index"):
+        assert getattr(c, name) == getattr(r, name), name
+    assert torch.equal(c.turns, r.turns) and torch.equal(c.axes, r.axes)
+    assert c.desc.turns == c.turns.data_ptr() and c.desc.axes == c.axes.data_ptr()
+    assert how == "copy" or c.turns.data_ptr() != r.turns.data_ptr()
+    assert (c.desc.pairs, c.desc.naxes, c.desc.head_dim, c.desc.interleaved) == (24, 3, 64, 1)
