@@ -4,9 +4,10 @@
 // Pair j of a head, (x1, x2), becomes (x1 cos t - x2 sin t, x1 sin t + x2 cos t)
 // with t = pos f_j, f_j an angle per position; the gradient is the rotation by
 // -t. Nothing is tabulated: f_j comes as a whole number of 2^-64 turns, so that
-// pos f_j modulo a turn is one wrapping integer product, exact but for f_j's own
-// rounding (pos 2^-65 turns: 2^-34 of a turn at position 2^31; in fp32 the
-// angle of position 200,000 would be off by 2^-7 radians). A table of sines
+// pos f_j modulo a turn is one wrapping integer product, off by what f_j was rounded
+// to that whole number (pos 2^-65 turns: 2^-34 of a turn at position 2^31), of which
+// the upper 32 bits are used (less than 2^-32 of a turn, 1.5e-9 radians, at any
+// position). In fp32 the angle of position 200,000 would be off by 2^-7. A table of sines
 // would be read once a token, as this is computed once a token, but holds a
 // fixed number of positions per axis.
 //

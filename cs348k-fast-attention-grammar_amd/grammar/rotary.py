@@ -21,6 +21,33 @@ from . import runtime as rt
 _pair = functools.lru_cache(maxsize=1024)(lambda *s: (ctypes.c_longlong * len(s))(*s))
 
 
+_PI_BITS = 1216
+
+
+@functools.lru_cache(maxsize=None)
+def _pi() -> int:
+    """pi 2^1216, by Machin's formula pi / 4 = 4 arctan(1/5) - arctan(1/239) in
+    integers with 32 bits more (a few hundred terms, each off by less than 2)."""
+    def arctan(x):
+        term = (1 << (_PI_BITS + 32)) // x
+        total, n, sign = term, 1, 1
+        while term:
+            term //= x * x
+            n, sign = n + 2, -sign
+            total += sign * (term // n)
+        return total
+    return 4 * (4 * arctan(5) - arctan(239)) >> 32
+
+
+def _turns(f: float) -> int:
+    """f radians as a whole number of 2^-64 turns, modulo one turn: the nearest
+    to the double's own value, whatever its size (a quotient in doubles would be
+    off by 2^-56 of a turn at 1 radian, which position 2^31 makes 2^-25)."""
+    n, d = f.as_integer_ratio()
+    num, den = n << (63 + _PI_BITS), d * _pi()                # f 2^64 / (2 pi)
+    return (2 * num + den) // (2 * den) % (1 << 64)
+
+
 class Rotary:
     """The rotation of heads of `head_dim` elements.
 
@@ -60,7 +87,7 @@ class Rotary:
         self.sections, self.naxes = tuple(sections), len(sections)
         self.inv_freq = tuple(freqs)
         # turns a position, modulo one, as whole numbers of 2^-64 (two's complement)
-        whole = [round(math.ldexp((f / (2 * math.pi)) % 1.0, 64)) % (1 << 64) for f in freqs]
+        whole = [_turns(f) for f in freqs]
         self.turns = torch.tensor([w - (1 << 64) if w >> 63 else w for w in whole], dtype=torch.int64, device=device)
         self.axes = torch.tensor(axes, dtype=torch.uint8, device=device)
         self._describe()

@@ -58,3 +58,20 @@ def test_rotary_can_be_copied_and_pickled(how):
     assert c.desc.turns == c.turns.data_ptr() and c.desc.axes == c.axes.data_ptr()
     assert how == "copy" or c.turns.data_ptr() != r.turns.data_ptr()
     assert (c.desc.pairs, c.desc.naxes, c.desc.head_dim, c.desc.interleaved) == (24, 3, 64, 1)
+
+
+def test_turns_are_the_nearest_to_the_frequency():
+    """To a unit of 2^-64 turns, against 60-digit decimals (pi by its published digits), for tiny and huge ones too."""
+    import math
+    from decimal import Decimal, getcontext
+    from grammar.rotary import Rotary
+    getcontext().prec = 120
+    pi = Decimal("3.14159265358979323846264338327950288419716939937510582097494459230781640628620899862803482534211706798")
+    freqs = [1.0, 0.5, 10000.0 ** -0.25, 500.0 ** -0.9, math.pi, 2 * math.pi, 1e-30, 5e-324, -1.0, -1e-9, 9.0, 12345.678,
+             2.0 ** 53, 1e15, -1e15, 0.0]
+    r = Rotary(32, inv_freq=freqs, device="cpu")
+    for f, t in zip(freqs, r.turns.tolist()):
+        want = Decimal(f) / (2 * pi) * 2 ** 64
+        off = (Decimal(t) - want) % 2 ** 64
+        assert min(abs(off), abs(2 ** 64 - abs(off))) <= Decimal("0.51"), (f, t, off)
+    assert Rotary(32, inv_freq=[1e308] * 16, device="cpu").inv_freq[0] == 1e308
