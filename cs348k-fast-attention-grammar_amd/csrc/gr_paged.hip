@@ -5,6 +5,7 @@
 #include <cstdint>
 
 #include "gr_host.h"
+#include "gr_overlap.h"
 #include "gr_paged.h"
 #include "gr_paged_host.h"
 #include "grammar_rt.h"
@@ -158,6 +159,17 @@ extern "C" int gr_paged_attn(const gr_paged_cache* cache, const gr_paged_batch* 
     if (q_strides[i] < 0 || q_strides[i] % 8 || o_strides[i] < 0 || o_strides[i] % 8)
       return gr::fail(GR_E_ARG, "gr_paged_attn: strides must be non-negative multiples of 8 elements");
   if (!(scale > 0.f)) return gr::fail(GR_E_ARG, "gr_paged_attn: scale must be positive");
+  {
+    // o may be q (a tile's rows are read before its result is written) and nothing else
+    const int B = batch->starts ? 1 : batch->B, N = batch->rows, D = cache->head_dim;
+    const gr::strided qi = gr::heads_of(q, B, N, Hq, D, q_strides), oo = gr::heads_of(o, B, N, Hq, D, o_strides);
+    const long long ks[3] = {cache->k_strides[0], cache->k_strides[2], cache->k_strides[1]};
+    const long long vs[3] = {cache->v_strides[0], cache->v_strides[2], cache->v_strides[1]};
+    if ((!gr::same_array(oo, qi) && gr::overlap(oo, qi, 2)) ||
+        gr::overlap(oo, gr::heads_of(cache->k, cache->pages, cache->page_size, cache->heads, D, ks), 2) ||
+        gr::overlap(oo, gr::heads_of(cache->v, cache->pages, cache->page_size, cache->heads, D, vs), 2))
+      return gr::fail(GR_E_ARG, "gr_paged_attn: o shares memory with the cache or with q (it may be q, by the same strides)");
+  }
   Plan p = plan_of(*cache, *batch, Hq);
   // as many shares as the workspace holds
   const size_t fit = workspace ? workspace_bytes / share_bytes(p, cache->head_dim) : 0;

@@ -5,6 +5,7 @@
 #include <cstdint>
 
 #include "gr_host.h"
+#include "gr_overlap.h"
 #include "gr_paged_host.h"
 #include "gr_rotary.h"
 #include "grammar_rt.h"
@@ -52,6 +53,16 @@ int launch_inter(const gr_rope_args& a, bool inter, int inverse, const char* who
   return launch<T, APPEND, false, false>(a, inverse, who, st);
 }
 
+// An output may be its own input, and shares no other memory with the call's
+// arrays: the waves of a token read and write its heads in no order.
+int check_apart(const gr::strided& out, const gr::strided& own, const gr::strided* others, int n, int size, const char* name,
+                const char* who) {
+  bool bad = !gr::same_array(out, own) && gr::overlap(out, own, size);
+  for (int i = 0; i < n; ++i) bad |= gr::overlap(out, others[i], size);
+  return bad ? gr::fail(GR_E_ARG, "%s: %s shares memory with another array (it may be its own input, by the same strides)", who, name)
+             : GR_OK;
+}
+
 // The rotation's own arguments: head_dim a multiple of 16 up to 256, at most 8 axes.
 int take_rotary(gr_rope_args& a, const gr_rotary_spec* r, const char* who) {
   if (!r->turns || ((uintptr_t)r->turns & 7)) return gr::fail(GR_E_ARG, "%s: the rotation's turns must be an 8-byte aligned buffer", who);
@@ -96,6 +107,15 @@ extern "C" int gr_rotary(const gr_rotary_spec* rotary, const void* q, void* q_ou
   if (rc) return rc;
   if ((rc = take_rows(a.q, q, q_out, Hq, q_strides, q_out_strides, "q", who))) return rc;
   if (k && (rc = take_rows(a.k, k, k_out, Hk, k_strides, k_out_strides, "k", who))) return rc;
+  const int D = rotary->head_dim, size = dtype == GR_F32 ? 4 : 2;
+  const gr::strided qi = gr::heads_of(q, B, N, Hq, D, q_strides), qo = gr::heads_of(q_out, B, N, Hq, D, q_out_strides);
+  if (!k) {
+    if ((rc = check_apart(qo, qi, nullptr, 0, size, "q_out", who))) return rc;
+  } else {
+    const gr::strided ki = gr::heads_of(k, B, N, Hk, D, k_strides), ko = gr::heads_of(k_out, B, N, Hk, D, k_out_strides);
+    const gr::strided not_q[2] = {ki, ko};
+    if ((rc = check_apart(qo, qi, not_q, 2, size, "q_out", who)) || (rc = check_apart(ko, ki, &qi, 1, size, "k_out", who))) return rc;
+  }
   a.tokens = B * N;
   a.per_seq = N;
   a.pos = positions;
@@ -132,6 +152,16 @@ extern "C" int gr_paged_append(const gr_paged_cache* cache, const gr_paged_batch
   const long long vd[3] = {cache->v_strides[0], cache->v_strides[2], cache->v_strides[1]};
   if ((rc = take_rows(a.k, k, cache->k, cache->heads, k_strides, kd, "k", who))) return rc;
   if ((rc = take_rows(a.v, v, cache->v, cache->heads, v_strides, vd, "v", who))) return rc;
+  if (q) {
+    const int B = batch->starts ? 1 : batch->B, N = batch->rows, D = cache->head_dim;
+    const gr::strided others[4] = {
+        gr::heads_of(k, B, N, cache->heads, D, k_strides), gr::heads_of(v, B, N, cache->heads, D, v_strides),
+        gr::heads_of(cache->k, cache->pages, cache->page_size, cache->heads, D, kd),
+        gr::heads_of(cache->v, cache->pages, cache->page_size, cache->heads, D, vd)};
+    if ((rc = check_apart(gr::heads_of(q_out, B, N, Hq, D, q_out_strides), gr::heads_of(q, B, N, Hq, D, q_strides), others, 4, 2,
+                          "q_out", who)))
+      return rc;
+  }
   a.tokens = batch->starts ? batch->rows : batch->B * batch->rows;
   a.per_seq = batch->starts ? 1 : batch->rows;
   a.pos = positions;
@@ -149,4 +179,14 @@ extern "C" int gr_paged_append(const gr_paged_cache* cache, const gr_paged_batch
   const bool inter = r->interleaved != 0;
   if (cache->dtype == GR_F16) return launch_inter<_Float16, true>(a, inter, 0, who, st);
   return launch_inter<__bf16, true>(a, inter, 0, who, st);
+}
+
+extern "C" int gr_selftest_overlap(const void* a, const long long* a_sizes, const long long* a_strides, const void* b,
+                                   const long long* b_sizes, const long long* b_strides, int size) {
+  gr::strided x = {a, {}, {}}, y = {b, {}, {}};
+  for (int i = 0; i < 4; ++i) {
+    x.n[i] = a_sizes[i]; x.s[i] = a_strides[i];
+    y.n[i] = b_sizes[i]; y.s[i] = b_strides[i];
+  }
+  return gr::overlap(x, y, size);
 }

@@ -154,7 +154,9 @@ def paged_append(k, v, cache: PagedCache, table, lens, *, starts=None, q=None, r
     k, v: [B, heads, n, D], or [rows, heads, D] with `starts`; any strides that
     are multiples of 8, unit on D (slices of a projection's output serve).
     rotary: a `Rotary` that turns the keys on the way, and q ([.., Hq, .., D]) if
-    given, into a new tensor laid out as q or into `out` (which may be q).
+    given, into a new tensor laid out as q or into `out` (which may be q and
+    shares no other memory with the call's tensors; nor do k and v lie in pages
+    that the call writes).
     positions: int32, [B, n], [n] or (packed) [rows], with several axes led by
     them; default: each token's place len - n + i, on every axis.
     Returns the rotated queries, or None without q. A token whose place is
@@ -215,7 +217,8 @@ def paged_attention(q, cache: PagedCache, table, lens, *, starts=None, causal: b
     scores (natural log). workspace: device memory for calls whose keys are
     shared out (allocated here unless given; rt.lib().gr_paged_attn_workspace
     names the size; with less the keys are shared out less).
-    Returns the result, laid out as q, or `out`."""
+    Returns the result, laid out as q, or `out`, which may be q and shares no
+    other memory with the call's tensors."""
     args, out, keep = _attn_args(q, cache, table, lens, starts, causal, scale, max_new, max_len, out, lse, workspace,
                                  stream)
     rt.launch(rt.lib().gr_paged_attn, args, q, stream, "gr_paged_attn")

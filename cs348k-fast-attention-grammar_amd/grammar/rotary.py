@@ -177,7 +177,8 @@ def rotary_fwd(q, k, positions, rot: Rotary, *, inverse: bool = False, out=None,
     [N] or [B, N], with several axes [axes, N] or [axes, B, N]. fp16, bf16 or
     fp32 on the GPU, any strides that are multiples of 8 with a unit one on D.
     Returns (q', k'), new tensors laid out as the given ones, or `out` and
-    `k_out`, which may be q and k themselves. inverse=True rotates back."""
+    `k_out`, which may be q and k themselves and share no other memory with them
+    or each other. inverse=True rotates back."""
     who = "rotary"
     if q is None:
         raise ValueError(f"{who}: q must be given")

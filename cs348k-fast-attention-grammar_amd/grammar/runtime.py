@@ -128,6 +128,7 @@ def lib() -> ctypes.CDLL:
         pll = ctypes.POINTER(ctypes.c_longlong)
         L.gr_rotary.argtypes = [vp, vp, vp, i32, pll, pll, vp, vp, i32, pll, pll, i32, i32, i32, vp, pll, i32, vp]
         L.gr_paged_append.argtypes = [vp, vp, vp, vp, vp, i32, pll, pll, vp, vp, pll, pll, vp, pll, vp]
+        L.gr_selftest_overlap.argtypes = [vp, pll, pll, vp, pll, pll, i32]
         L.gr_paged_attn_workspace.argtypes = [vp, vp, i32]
         L.gr_paged_attn_workspace.restype = sz
         L.gr_paged_attn.argtypes = [vp, vp, vp, vp, vp, i32, pll, pll, i32, ctypes.c_float, vp, sz, vp]
@@ -164,7 +165,7 @@ EXPORTED = (
     "gr_attn_fwd_train", "gr_attn_bwd_workspace", "gr_attn_bwd", "gr_attn_decode_noalloc",
     "gr_plan_run_args", "gr_gemm_workspace", "gr_gemm_ws", "gr_mlp_fwd_workspace", "gr_mlp_fwd_ws",
     "gr_selftest_f32_no_workspace", "gr_attn_fwd_shape", "gr_gemm_f32_groups",
-    "gr_rotary", "gr_paged_append", "gr_paged_attn_workspace", "gr_paged_attn",
+    "gr_rotary", "gr_paged_append", "gr_paged_attn_workspace", "gr_paged_attn", "gr_selftest_overlap",
 )
 
 # Bytes of the per-device scratch array behind gr_attn_decode_noalloc (GR_DECODE_SCRATCH_BYTES).

@@ -244,7 +244,8 @@ typedef struct gr_rotary_spec {
 } gr_rotary_spec;
 
 /* Rotates q [B, Hq, N, D] into q_out and, if k is not NULL, k [B, Hk, N, D] into
- * k_out (each may be its own input: the call then works in place).
+ * k_out (each may be its own input, by the same strides: the call then works in
+ * place; outputs share no other memory with inputs or each other).
  *  Strides {batch, token, head} in elements, non-negative multiples of 8, unit
  *  stride along D; base pointers 16-byte aligned. dtype GR_F16, GR_BF16 (angles,
  *  products and sums in fp32, rounded once) or GR_F32.
@@ -295,8 +296,9 @@ typedef struct gr_paged_batch {
  * q into q_out (which may be q). Strides {batch, token, head}, as gr_rotary's
  * (a packed batch's batch stride is not read). positions NULL: a token's place
  * len - n + i in its sequence, on every axis; else int32 by {axis, batch, token}
- * (packed: the token axis is the batch's). A page that two tokens of one call
- * fall on at the same slot ends with either's entry. */
+ * (packed: the token axis is the batch's). q_out shares no memory with k, v or
+ * the cache, and k and v lie in no page that the call writes. A slot that two
+ * tokens of one call fall on ends with either's entry or parts of both. */
 int gr_paged_append(const gr_paged_cache* cache, const gr_paged_batch* batch, const gr_rotary_spec* rotary, const void* q,
                     void* q_out, int Hq, const long long* q_strides, const long long* q_out_strides, const void* k,
                     const void* v, const long long* k_strides, const long long* v_strides, const int* positions,
@@ -307,7 +309,8 @@ int gr_paged_append(const gr_paged_cache* cache, const gr_paged_batch* batch, co
  * Hq, a multiple of the cache's heads: query head h reads key head h / (Hq /
  * heads). q, o: strides {batch, token, head} as above. lse: NULL, or [tokens][Hq]
  * fp32 (uniform batches [B][rows][Hq]) for the log-sum-exp of the scaled scores,
- * natural log. A row that sees no key gets 0 and -inf.
+ * natural log. A row that sees no key gets 0 and -inf. o may be q, by the same
+ * strides; outputs and workspace share no other memory with the call's arrays.
  * workspace: device memory, 16-byte aligned, in which workgroups that share a
  * row's keys leave partial results; gr_paged_attn_workspace names the size for a
  * call's shapes (0 for calls that are not shared out, and for invalid ones). With
@@ -391,6 +394,12 @@ int gr_selftest_mfma32(const void* a, const void* b, float* d, void* stream);
  * `lookups` key-split workspaces fail to allocate (each asks the device for
  * more memory than it has), whether or not the stream has one already. */
 int gr_selftest_f32_no_workspace(int lookups);
+
+/* Self-test of the check for outputs that overlap inputs, on the host: 1 if two
+ * arrays of `size`-byte elements, of 4 sizes and non-negative strides in
+ * elements each, share memory, else 0. The addresses are not followed. */
+int gr_selftest_overlap(const void* a, const long long* a_sizes, const long long* a_strides, const void* b,
+                        const long long* b_sizes, const long long* b_strides, int size);
 
 #ifdef __cplusplus
 }

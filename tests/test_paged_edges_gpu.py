@@ -118,3 +118,41 @@ def test_caches_and_rotations_can_be_copied_and_pickled():
             assert torch.equal(paged_attention(qr, there, s.table, s.lens), got)
         shared = copy.copy(cache)
         assert shared.k is cache.k and shared.ref != cache.ref
+
+
+def test_outputs_share_memory_with_their_own_input_only():
+    from grammar import runtime as rt
+    from grammar.paged import paged_append, paged_attention
+    from grammar.rotary import Rotary, rotary_fwd
+    s = Setup([40, 50, 300], 2, 16, 64, "fp16", seed=7)
+    rot = Rotary(64, device=s.dev)
+    n, starts = 9, torch.tensor([0, 9, 18, 27], dtype=torch.int32, device=s.dev)
+    rows = s.randn(27, 14, 64)                                   # a projection's rows: 8 q, 2 k, 2 v heads and 2 more
+    q, k, v = rows[:, :8], rows[:, 8:10], rows[:, 10:12]
+    args = (s.cache, s.table, s.lens)
+    for bad in (lambda: paged_append(k, v, *args, starts=starts, q=q, rotary=rot, out=rows[:, 4:12]),
+                lambda: paged_append(k, v, *args, starts=starts, q=k, rotary=rot, out=v),
+                lambda: paged_append(k, v, *args, starts=starts, q=q, rotary=rot, out=rows.view(-1)[:27 * 512].view(27, 8, 64)),
+                lambda: paged_attention(q, *args, starts=starts, out=rows[:, 6:14]),
+                lambda: paged_attention(q, *args, starts=starts, out=s.k.view(-1)[:27 * 512].view(27, 8, 64)),
+                lambda: rotary_fwd(q[None].transpose(1, 2), k[None].transpose(1, 2), starts[:1].expand(27), rot,
+                                   out=rows[None, :, 2:10].transpose(1, 2))):
+        before = rows.clone(), s.k.clone()
+        with pytest.raises(rt.GrError, match="shares memory"):
+            bad()
+        assert torch.equal(rows, before[0]) and torch.equal(s.k, before[1])
+    # in place, and into other heads of the same rows
+    want = paged_append(k, v, *args, starts=starts, q=q, rotary=rot)
+    wide = s.randn(27, 24, 64)
+    wide[:, :14] = rows
+    got = paged_append(wide[:, 8:10], wide[:, 10:12], *args, starts=starts, q=wide[:, :8], rotary=rot, out=wide[:, 16:])
+    assert torch.equal(got, want) and torch.equal(wide[:, :14], rows)
+    paged_append(k, v, *args, starts=starts, q=q, rotary=rot, out=q)
+    assert torch.equal(q, want)
+    # attention in place: in tiles of 32, 64 and 128 rows, a workgroup a tile and shared out
+    for m, lens, width in ((1, [40, 50, 3000], None), (9, [40, 50, 300], None), (150, [150, 500, 4000], None),
+                           (1, [40, 50, 3000], 2048), (150, [150, 500, 4000], 2048)):
+        t = Setup(lens, 2, 16, 64, "fp16", seed=m, width=width)
+        x = t.randn(3, 8, m, 64)
+        o = paged_attention(x, t.cache, t.table, t.lens)
+        assert paged_attention(x, t.cache, t.table, t.lens, out=x) is x and torch.equal(x, o)
