@@ -156,8 +156,9 @@ def _takes(shape: tuple, st: tuple, like: tuple) -> bool:
 
 def check_out(out, like, name: str, who: str, stream):
     """`out`, checked, or a new tensor laid out as `like` for a launch on `stream`."""
+    import torch
     if out is None:
-        return rt.empty_like(like, stream)
+        return rt.empty_like(like, stream) if stream is not None else torch.empty_like(like)
     if not _takes(out.shape, out.stride(), like.shape) or out.dtype != like.dtype or out.get_device() != like.get_device():
         raise ValueError(f"{who}: bad `{name}` tensor")
     return out
@@ -258,11 +259,9 @@ def _autograd_function():
     return RotaryFunction
 
 
-def _has_tangent(*tensors) -> bool:
+def _has_tangent(forward_ad, *tensors) -> bool:
     """Whether one of them is a dual tensor of forward-mode differentiation."""
-    import torch.autograd.forward_ad as forward_ad
-    return forward_ad._current_level >= 0 and \
-        any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 _ROTARY_FN = None
@@ -277,7 +276,8 @@ def rotary(q, k, positions, rot: Rotary):
     still alive, must not be joined by a captured one (torch's own rule)."""
     import torch
     recorded = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))
-    if not recorded and not _has_tangent(q, k):
+    forward_ad = torch.autograd.forward_ad
+    if not recorded and (forward_ad._current_level < 0 or not _has_tangent(forward_ad, q, k)):
         return rotary_fwd(_dense(q), None if k is None else _dense(k), positions, rot)
     global _ROTARY_FN
     if _ROTARY_FN is None:
