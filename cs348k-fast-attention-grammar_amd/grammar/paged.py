@@ -161,7 +161,8 @@ def paged_append(k, v, cache: PagedCache, table, lens, *, starts=None, q=None, r
     them; default: each token's place len - n + i, on every axis.
     Returns the rotated queries, or None without q. A token whose place is
     outside of the table or on a page id outside of the cache is not stored.
-    max_new: the most new tokens of a sequence, where known."""
+    max_new: as paged_attention takes it, so that one set of arguments serves
+    both; an append is shared out alike whatever it is."""
     args, out, keep = _append_args(k, v, cache, table, lens, starts, q, rotary, positions, max_new, out, stream)
     rt.launch(rt.lib().gr_paged_append, args, k, stream, "gr_paged_append")
     return out

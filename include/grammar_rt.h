@@ -277,7 +277,7 @@ typedef struct gr_paged_cache {
  *          `rows` tokens, rows outside of every sequence being left alone; or
  *          NULL for a uniform batch of `rows` new tokens a sequence.
  *  max_new, max_len: the most new tokens and keys of a sequence, where known (0:
- *          not). They only choose how a call is shared out.
+ *          not). They only choose how an attention is shared out.
  * What the arrays hold is bounded on the device: a page id outside of the cache,
  * a position outside of the table or a sequence whose starts are not both in
  * the batch reads and writes nothing (such keys do not exist, such tokens are not

@@ -7,7 +7,7 @@ pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
 
-from test_paged_gpu import Setup  # noqa: E402
+from test_paged_gpu import Setup, _attention, _check, _check_lse  # noqa: E402
 
 
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
@@ -156,3 +156,36 @@ def test_outputs_share_memory_with_their_own_input_only():
         x = t.randn(3, 8, m, 64)
         o = paged_attention(x, t.cache, t.table, t.lens)
         assert paged_attention(x, t.cache, t.table, t.lens, out=x) is x and torch.equal(x, o)
+
+
+HINTS = [dict(max_new=1, max_len=1), dict(max_new=1), dict(max_len=1), dict(max_new=20, max_len=700),
+         dict(max_new=2 ** 31 - 1, max_len=2 ** 31 - 1), dict(max_new=-5, max_len=-5)]
+
+
+@pytest.mark.parametrize("hints", HINTS, ids=lambda h: "-".join(f"{k[4:]}{v}" for k, v in h.items()))
+@pytest.mark.parametrize("dtype,D,G,Hkv", [("bf16", 128, 4, 2), ("fp16", 64, 1, 4)])
+@pytest.mark.parametrize("width", [None, 2048], ids=["fit", "roomy"])
+def test_hints_that_do_not_hold(hints, dtype, D, G, Hkv, width):
+    """max_new and max_len only choose how the work is shared out: a bound loop outgrows them. A packed batch of chunks
+    and single tokens, decode steps over long contexts and a chunk of its own, with hints too small and too large."""
+    from grammar.paged import paged_append, paged_attention
+    print(f"[case] hints {hints} {dtype} D{D} width {width}", flush=True)
+    for news, lens, ragged in (([1, 0, 150, 1, 7, 301, 1], [40, 99, 150, 700, 7, 900, 0], True),
+                               ([1, 1, 1], [20_011, 3, 5000], False), ([200], [5000], False)):
+        s = Setup(lens, Hkv, 16, D, dtype, seed=D, width=width)
+        T, B, Hq = sum(news) + 3 * ragged, len(news), G * Hkv
+        q = s.randn(T, Hq, D) if ragged else s.randn(B, Hq, news[0], D)
+        starts = torch.tensor([sum(news[:b]) for b in range(B + 1)], dtype=torch.int32, device=s.dev) if ragged else None
+        out, lse = torch.full_like(q, 5.0), torch.full((T, Hq) if ragged else (B, news[0], Hq), 7.0, device=s.dev)
+        paged_attention(q, s.cache, s.table, s.lens, starts=starts, out=out, lse=lse, **hints)
+        for b, n in enumerate(news):
+            pick = (lambda x: x[sum(news[:b]):sum(news[:b + 1])]) if ragged else (lambda x: x[b].transpose(0, 1))
+            o, ls, size = _attention(s, b, pick(q))
+            _check(pick(out), o, size, f"{n} of {lens[b]} keys")
+            _check_lse(pick(lse) if ragged else lse[b], ls, s.dtype, f"lse of {b}")
+        if ragged:
+            assert (out[sum(news):] == 5.0).all() and (lse[sum(news):] == 7.0).all()
+            k, v = s.randn(T, Hkv, D), s.randn(T, Hkv, D)
+            paged_append(k, v, s.cache, s.table, s.lens, starts=starts, max_new=hints.get("max_new", 0))
+            page, slot = int(s.table[5, 899 // 16]), 899 % 16
+            assert torch.equal(s.k[page, :, slot], k[459]) and torch.equal(s.v[page, :, slot], v[459])
