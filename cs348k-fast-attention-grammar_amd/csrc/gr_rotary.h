@@ -27,7 +27,8 @@
 // reads the rows runs on other XCDs: 8,193 tokens of 32 + 8 + 8 heads of 128 into
 // pages 45.5 us to 41.3, 1,024 tokens 7.6 to 6.6, and the attention behind takes as
 // long. Stores of parts of lines stay in them: 2 x 4,096 tokens of 32 + 32 heads of
-// 32 take 15.0 us, past the caches 30; of 128 with neighbours as pairs 45.5 and 76.
+// 32 take 15.0 us, past the caches 30; of 128 with neighbours as pairs 45.5 and 76, in
+// rows that begin 16 bytes off a line 50.5 and 93.5.
 #pragma once
 #include "gr_common.h"
 

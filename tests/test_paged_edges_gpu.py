@@ -189,3 +189,35 @@ def test_hints_that_do_not_hold(hints, dtype, D, G, Hkv, width):
             paged_append(k, v, s.cache, s.table, s.lens, starts=starts, max_new=hints.get("max_new", 0))
             page, slot = int(s.table[5, 899 // 16]), 899 % 16
             assert torch.equal(s.k[page, :, slot], k[459]) and torch.equal(s.v[page, :, slot], v[459])
+
+
+@pytest.mark.parametrize("pad,off", [(128, 8), (128, 32), (136, 0), (192, 0)])
+def test_destinations_off_a_line(pad, off):
+    """Results in rows that begin off a 128-byte line, and pages with padded slots: bit for bit the packed ones, and
+    nothing behind a row is written."""
+    from grammar.paged import PagedCache, paged_append
+    from grammar.rotary import Rotary, rotary_fwd
+    s = Setup([700, 900], 8, 16, 128, "bf16", seed=8)
+    rot = Rotary(128, device=s.dev)
+    print(f"[case] rows of {pad}, {off} off", flush=True)
+
+    def rows(*shape):
+        n = math.prod(shape)
+        x = torch.full((n * pad + 64,), 5.0, dtype=s.dtype, device=s.dev)
+        whole = x[off:off + n * pad].view(*shape, pad)
+        return whole[..., :128], lambda: (whole[..., 128:] == 5.0).all() and (x[:off] == 5.0).all() and (x[off + n * pad:] == 5.0).all()
+    q, k = s.randn(1, 32, 600, 128), s.randn(1, 8, 600, 128)
+    pos = torch.arange(600, dtype=torch.int32, device=s.dev)
+    (o, o_kept), (ko, ko_kept) = rows(1, 32, 600), rows(1, 8, 600)
+    want = rotary_fwd(q, k, pos, rot)
+    rotary_fwd(q, k, pos, rot, out=o, k_out=ko)
+    assert torch.equal(o, want[0]) and torch.equal(ko, want[1]) and o_kept() and ko_kept()
+    q, k = s.randn(2, 32, 600, 128), s.randn(2, 8, 600, 128)
+    pages = [rows(s.k.shape[0], 8, 16) for _ in range(2)]
+    for (p, _), x in zip(pages, (s.k, s.v)):
+        p.copy_(x)
+    cache, (o, o_kept) = PagedCache(pages[0][0], pages[1][0]), rows(2, 32, 600)
+    want = paged_append(k, k, s.cache, s.table, s.lens, q=q, rotary=rot)
+    paged_append(k, k, cache, s.table, s.lens, q=q, rotary=rot, out=o)
+    assert torch.equal(o, want) and torch.equal(cache.k, s.k) and torch.equal(cache.v, s.v)
+    assert o_kept() and pages[0][1]() and pages[1][1]()
