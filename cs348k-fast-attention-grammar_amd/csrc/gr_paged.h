@@ -30,9 +30,9 @@
 //
 // Measured (bf16, 32 / 8 heads of 128). A token each of 48 sequences of 150 to 8,000
 // keys (848 MB): 147-150 us, 5.7 TB/s, bound by memory (matrix cores 8 % busy), and
-// 4.8 for the merge. 4,096 tokens onto 4,096: 410 us, 1,007 TFLOP/s, bound by the
-// MFMAs and the softmax of two waves a SIMD taking turns (matrix cores 49 % busy, no
-// LDS conflicts). Small grids are bound by a workgroup's chain of steps, 1.2-1.3 us
+// 4.8 for the merge. 4,096 tokens onto 4,096: 403-440 us by clocks, 940-1,020 TFLOP/s,
+// bound by the MFMAs and the softmax of two waves a SIMD taking turns (matrix cores
+// 49 % busy, no LDS conflicts). Small grids are bound by a workgroup's chain of steps, 1.2-1.3 us
 // for 64 keys of 128 rows: 419 keys of one token (16 heads of 64) take 7.2 us.
 #pragma once
 #include "gr_flash_fwd.h"

@@ -15,8 +15,8 @@ keys as queries, run_attention_search.py:34-114).
 
 Lengths, starts and page ids are read on the GPU, so one bound or captured call
 serves every step. What lies outside of the cache or the table is not touched:
-such keys do not exist. There is no CPU path: CPU tensors or a missing library
-raise.
+such keys do not exist. The results carry no gradient. There is no CPU path: CPU
+tensors or a missing library raise.
 """
 from __future__ import annotations
 
