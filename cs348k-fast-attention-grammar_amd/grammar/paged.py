@@ -46,6 +46,8 @@ class PagedCache:
         pages, heads, size, D = k.shape
         if rt.dtype_code(k.dtype) == rt.GR_F32:
             raise ValueError("PagedCache: fp16 or bf16")
+        if max(pages, heads) >= 1 << 31:
+            raise ValueError(f"PagedCache: {pages} pages of {heads} heads are too many (2^31)")
         if D not in (64, 128) or size < 16 or size & (size - 1) or size > 1 << 20:
             raise ValueError(f"PagedCache: D {D} must be 64 or 128 and page_size {size} a power of two from 16 to 2^20")
         self.k, self.v, self.dtype, self.index = k, v, k.dtype, k.get_device()
@@ -74,6 +76,8 @@ def _batch_sizes(table: tuple, table_st: tuple, lens: tuple, lens_st: tuple, sta
         if shape is not None and (len(shape) != dim or (st[-1] != 1 and shape[-1] > 1)):
             return f"{n} must be a {dim}-D int32 tensor with unit stride"
     B, width = table
+    if max(B, width, *x) >= 1 << 31:                                                # (C integers would wrap)
+        return f"{tuple(x)} by a table {tuple(table)} is too large for one call (2^31)"
     if lens[0] != B or B == 0 or width == 0:
         return f"table {tuple(table)} and lens {tuple(lens)} do not describe a batch"
     if starts is None:

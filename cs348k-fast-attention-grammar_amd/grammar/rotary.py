@@ -170,6 +170,8 @@ def _tokens(q: tuple, q_st: tuple, k, k_st, dim: int):
     for shape, st in ((q, q_st), (k, k_st)):
         if shape is not None and (len(shape) != 4 or shape[3] != dim or st[3] != 1 or shape[0] != q[0] or shape[2] != q[2]):
             return None
+        if shape is not None and max(shape[0] * shape[2], shape[1]) >= 1 << 31:     # (C integers would wrap)
+            return "too many"
     return (q[0], q[2], q[1], _head_strides(q, q_st)) + ((0, None) if k is None else (k[1], _head_strides(k, k_st)))
 
 
@@ -193,6 +195,8 @@ def rotary_fwd(q, k, positions, rot: Rotary, *, inverse: bool = False, out=None,
     if sizes is None or not ok:
         raise ValueError(f"{who}: q and k must be [B, H, N, {rot.head_dim}] tensors of one dtype, B and N on {rot.device} "
                          "(no CPU path) with unit stride on their last dimension")
+    if sizes == "too many":
+        raise ValueError(f"{who}: {tuple(q.shape)} is too many tokens or heads for one call (2^31)")
     B, N, Hq, qs, Hk, ks = sizes
     ps = check_positions(positions, rot, (B, N), who)
     out = check_out(out, q, "out", who, stream)

@@ -75,3 +75,28 @@ def test_turns_are_the_nearest_to_the_frequency():
         off = (Decimal(t) - want) % 2 ** 64
         assert min(abs(off), abs(2 ** 64 - abs(off))) <= Decimal("0.51"), (f, t, off)
     assert Rotary(32, inv_freq=[1e308] * 16, device="cpu").inv_freq[0] == 1e308
+
+
+def test_sizes_past_32_bits_are_refused():
+    """The library takes 32-bit counts, and ctypes would pass 2^32 + 5 tokens as 5. (A head of 16 in fp16 is 32 bytes:
+    such tensors fit a GPU. Shapes alone here.)"""
+    from grammar.paged import _batch_sizes
+    from grammar.rotary import Rotary, _tokens, rotary_fwd
+    n = 2 ** 32 + 5
+    for shape, st in (((1, 1, n, 16), (n * 16, 16, 16, 1)), ((n, 1, 1, 16), (16, 16, 16, 1)), ((1, n, 1, 16), (0, 16, 0, 1)),
+                      ((2 ** 16, 1, 2 ** 16, 16), (2 ** 20, 16, 16, 1)), ((1, 1, 2 ** 31, 16), (0, 0, 16, 1))):
+        assert _tokens(shape, st, None, None, 16) == "too many"
+        assert _tokens((shape[0], 1, shape[2], 16), st, shape, st, 16) == "too many"
+    assert _tokens((1, 1, 2 ** 31 - 1, 16), (0, 0, 16, 1), None, None, 16)[:3] == (1, 2 ** 31 - 1, 1)
+    for table, x in (((1, n), (1, 1, 1, 64)), ((1, 4), (1, 1, n, 64)), ((1, 4), (1, n, 1, 64)), ((n, 4), (n, 1, 1, 64))):
+        assert "too large" in _batch_sizes(table, (table[1], 1), (table[0],), (1,), None, None, x)
+    assert "too large" in _batch_sizes((1, 4), (4, 1), (1,), (1,), (2,), (1,), (n, 1, 64))
+
+    class Far:                                                        # the shape of a tensor that no test can hold
+        shape, dtype = torch.Size((1, 1, n, 16)), torch.float16
+        stride = staticmethod(lambda: (0, 0, 16, 1))
+        get_device = staticmethod(lambda: 0)
+    rot = Rotary(16, device="cpu")
+    rot.index = 0
+    with pytest.raises(ValueError, match="too many tokens"):
+        rotary_fwd(Far(), None, None, rot)
