@@ -221,3 +221,40 @@ def test_destinations_off_a_line(pad, off):
     paged_append(k, k, cache, s.table, s.lens, q=q, rotary=rot, out=o)
     assert torch.equal(o, want) and torch.equal(cache.k, s.k) and torch.equal(cache.v, s.v)
     assert o_kept() and pages[0][1]() and pages[1][1]()
+
+
+def test_calls_of_two_threads_at_once():
+    """Two host threads, each with a stream and a cache of its own and calls whose work is shared out, in flight at once."""
+    import threading
+    from grammar.paged import paged_append, paged_attention
+    from grammar.rotary import Rotary
+    rot = Rotary(128, device=torch.device("cuda:0"))
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    cases = []
+    for i in range(2):
+        s = Setup([4000 + 900 * i, 70, 2500], 2, 16, 128, "bf16", seed=20 + i, width=400)
+        q, k, v = s.randn(3, 8, 5, 128), s.randn(3, 2, 5, 128), s.randn(3, 2, 5, 128)
+        qr = paged_append(k, v, s.cache, s.table, s.lens, q=q, rotary=rot)
+        cases.append((s, q, k, v, qr, paged_attention(qr, s.cache, s.table, s.lens)))
+    torch.cuda.synchronize()
+    got, errors, start = [[], []], [], threading.Barrier(2)
+
+    def loop(i):
+        try:
+            s, q, k, v, *_ = cases[i]
+            start.wait(30)
+            with torch.cuda.stream(sides[i]):
+                for _ in range(40):
+                    qr = paged_append(k, v, s.cache, s.table, s.lens, q=q, rotary=rot)
+                    got[i].append((qr, paged_attention(qr, s.cache, s.table, s.lens)))
+        except Exception as e:                                   # shown below: a thread's own would be lost
+            errors.append(e)
+    threads = [threading.Thread(target=loop, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    torch.cuda.synchronize()
+    assert not errors
+    for (*_, qr, o), results in zip(cases, got):
+        assert len(results) == 40 and all(torch.equal(a, qr) and torch.equal(b, o) for a, b in results)
