@@ -50,7 +50,8 @@ COMMON = [
 # accumulators on the vector ALU the same way.
 EXTRA = {"gr_attn_bwd128.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
          "gr_attn_f32.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
-         "gr_paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+         "gr_paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+         "gr_paged8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 
 def _sources() -> list[str]:

@@ -35,6 +35,7 @@
 // 49 % busy, no LDS conflicts). Small grids are bound by a workgroup's chain of steps, 1.2-1.3 us
 // for 64 keys of 128 rows: 419 keys of one token (16 heads of 64) take 7.2 us.
 #pragma once
+#include "gr_e4m3.h"
 #include "gr_flash_fwd.h"
 #include "gr_gemm.h"
 
@@ -48,6 +49,8 @@ struct gr_paged_args {
   const void* v;
   long long k_sp, k_sh, k_ss;      // page, head, slot
   long long v_sp, v_sh, v_ss;
+  const unsigned char* scales;     // Q8: of the cache's rows, unit stride along the slots
+  long long s_sp, s_sh, s_kind;    // page, head, from a key's to a value's
   const int* table;
   long long table_stride;
   const int* lens;
@@ -321,7 +324,14 @@ struct gr_paged_lds {
 
 // One tile over keys [key0, key1), by NW KG waves of the workgroup's WAVES; place:
 // where its partial result of BM rows goes, or -1 for a tile that is done here.
-template <class T, int D, int BN, int NW, int KG, int NS, int WAVES, int BM>
+//
+// Q8: the cache holds e4m3 bytes and power-of-two scales. A tile's bytes come
+// through registers, are turned into T exactly (gr_from_e4m3) and written to LDS where
+// the 16-bit tile's loads would have put them, once for all waves that read them: from there
+// on the two are alike. Loads are a tile ahead of the one being written, which is
+// a tile ahead of the products where waves share it (NS 2), and the products' own
+// where a wave has it alone (NS 1).
+template <class T, int D, int BN, int NW, int KG, int NS, int WAVES, int BM, bool Q8>
 __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* lds_all, const gr_paged_tile& t, int hk,
                                                  int key0, int key1, int place) {
   typedef gr_mfma<T> MF;
@@ -336,6 +346,7 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
   constexpr int IPB = 16 * CPR / 64;         // load instructions of a block
   constexpr int PER = BLOCKS * IPB / NW;     // of a wave, for K and for V
   static_assert(BLOCKS * IPB % NW == 0, "whole load instructions");
+  typedef typename gr_bytes<Q8>::type E;     // element of the cache
 
   const int lane = threadIdx.x & 63;
   const int wave_all = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -358,11 +369,27 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
   // with row bits 2 and 3 swapped, V rows as they are; both swizzled (gr_paged_swz
   // for 16-byte row reads, gr_swz_tr for gr_tr_frag) by row bits 0 to 3, so that a
   // lane's offset from its block's first slot depends on sub alone.
-  constexpr int SUBS = IPB > NW ? IPB / NW : 1;
+  //
+  // Q8: instructions of 64 / CPR8 rows of 16 bytes a lane; koff and voff are offsets
+  // in the cache, kdst and vdst in LDS, where the second half of a lane's numbers is
+  // the neighbouring chunk.
+  constexpr int CPR8 = D / 16, IPB8 = CPR8 / 4, PER8 = Q8 ? BLOCKS * IPB8 / NW : 1;
+  static_assert(!Q8 || BLOCKS * IPB8 % NW == 0, "whole load instructions");
+  constexpr int SUBS = Q8 ? (IPB8 > NW ? IPB8 / NW : 1) : IPB > NW ? IPB / NW : 1;
+  auto block_row8 = [&](int i) { return lane / CPR8 + ((wave + i * NW) % IPB8) * (64 / CPR8); };
+  int kdst[SUBS], vdst[SUBS];
   auto block_row = [&](int i) { return lane / CPR + ((wave + i * NW) % IPB) * (64 / CPR); };
   unsigned koff[SUBS], voff[SUBS];            // bytes
 #pragma unroll
   for (int i = 0; i < SUBS; ++i) {
+    if constexpr (Q8) {
+      const int r = block_row8(i), c8 = lane % CPR8, pr = gr_perm32(r);
+      koff[i] = (unsigned)(r * a.k_ss) + c8 * 16;
+      voff[i] = (unsigned)(r * a.v_ss) + c8 * 16;
+      kdst[i] = pr * (D * 2) + gr_paged_swz<CPR>(pr, 2 * c8) * 16;
+      vdst[i] = r * (D * 2) + gr_swz_tr<CPR>(r, 2 * c8) * 16;
+      continue;
+    }
     const int r = block_row(i), pc = lane % CPR;
     koff[i] = (unsigned)((gr_perm32(r) & 15) * a.k_ss * 2) + gr_paged_swz<CPR>(r, pc) * 16;
     voff[i] = (unsigned)(r * a.v_ss * 2) + gr_swz_tr<CPR>(r, pc) * 16;
@@ -388,8 +415,8 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
   const int lim_hi = a.causal ? gr_imin(base_pos + gr_imin(rw + 31, t.nrows - 1) / a.G, t.keys - 1) : t.keys - 1;
 
   const int* const tab = a.table + t.b * a.table_stride;
-  const T* const kp = static_cast<const T*>(a.k) + hk * a.k_sh;
-  const T* const vp = static_cast<const T*>(a.v) + hk * a.v_sh;
+  const E* const kp = static_cast<const E*>(a.k) + hk * a.k_sh;
+  const E* const vp = static_cast<const E*>(a.v) + hk * a.v_sh;
 
   const int ntile_all = key1 > key0 ? (key1 - key0 + BN - 1) / BN : 0;
   const int ntile = (ntile_all - kg + KG - 1) / KG;           // of this group
@@ -407,12 +434,13 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
     const long long key = key0 + ((long long)(j0 + lane / BLOCKS) * KG + kg) * BN + 16 * (lane % BLOCKS);
     return tab[key >> a.page_shift < a.width ? (int)(key >> a.page_shift) : a.width - 1];
   };
-  unsigned long long kwin = 0, vwin = 0, badwin = 0;
+  unsigned long long kwin = 0, vwin = 0, swin = 0, badwin = 0;
   auto refill = [&](int j0, int id) {
     const int key = key0 + ((j0 + lane / BLOCKS) * KG + kg) * BN + 16 * (lane % BLOCKS), slot = key & smask;
     const bool ok = (unsigned)id < (unsigned)a.pages;
     kwin = (unsigned long long)(kp + (ok ? id : 0) * a.k_sp + slot * a.k_ss);
     vwin = (unsigned long long)(vp + (ok ? id : 0) * a.v_sp + slot * a.v_ss);
+    if (Q8) swin = (unsigned long long)(a.scales + (ok ? id : 0) * a.s_sp + hk * a.s_sh + slot);
     badwin = __builtin_amdgcn_ballot_w64(!ok && key < key1);
   };
   auto lane64 = [&](unsigned long long w, int l) {
@@ -444,6 +472,50 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
           else gr_st16(kd + NS * L::TILE, (gr_u32x4){0, 0, 0, 0});
         }
       }
+    }
+  };
+
+  // Q8: the bytes and scales of the next tile, and their way into a slot. Rows that
+  // are not there are zeros.
+  typedef const __attribute__((address_space(1))) gr_u32x4 global_u32x4;
+  typedef const __attribute__((address_space(1))) unsigned char global_u8;
+  gr_u32x4 kr[PER8], vr[PER8];
+  unsigned ksb[PER8], vsb[PER8];
+  auto load8 = [&](int j, auto whole_tag, unsigned bad) {
+    constexpr bool WHOLE = decltype(whole_tag)::value;
+    const int at = (j & (WIN - 1)) * BLOCKS;
+#pragma unroll
+    for (int n = 0; n < PER8; ++n) {
+      const int bl = (wave + n * NW) / IPB8, i = n % SUBS, r = block_row8(i);
+      const unsigned long long kb = lane64(kwin, at + bl), vb = lane64(vwin, at + bl), sb = lane64(swin, at + bl);
+      auto get = [&] {
+        kr[n] = *(global_u32x4*)(kb + koff[i]);
+        vr[n] = *(global_u32x4*)(vb + voff[i]);
+        ksb[n] = *(global_u8*)(sb + (unsigned)r);
+        vsb[n] = *(global_u8*)(sb + a.s_kind + (unsigned)r);
+      };
+      if constexpr (WHOLE) {
+        get();
+      } else {
+        kr[n] = vr[n] = (gr_u32x4){0, 0, 0, 0};
+        ksb[n] = vsb[n] = 0;
+        if (!(bad >> bl & 1) && key_of(j) + 16 * bl + r < key1) get();
+      }
+    }
+  };
+  auto store8 = [&](int slot) {
+#pragma unroll
+    for (int n = 0; n < PER8; ++n) {
+      const int bl = (wave + n * NW) / IPB8, i = n % SUBS;
+      auto put = [&](char* base, int at, gr_u32x4 w, unsigned sb) {
+        const float f = gr_e8m0(sb);
+        gr_st16(base + at, (gr_u32x4){gr_from_e4m3<T, false>(w[0], f), gr_from_e4m3<T, true>(w[0], f),
+                                      gr_from_e4m3<T, false>(w[1], f), gr_from_e4m3<T, true>(w[1], f)});
+        gr_st16(base + (at ^ 16), (gr_u32x4){gr_from_e4m3<T, false>(w[2], f), gr_from_e4m3<T, true>(w[2], f),
+                                             gr_from_e4m3<T, false>(w[3], f), gr_from_e4m3<T, true>(w[3], f)});
+      };
+      put(ks0 + slot * L::TILE + bl * (16 * D * 2), kdst[i], kr[n], ksb[n]);
+      put(vt0 + slot * L::TILE + bl * (16 * D * 2), vdst[i], vr[n], vsb[n]);
     }
   };
 
@@ -624,18 +696,26 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
   int asked = 0, to = 0, plain = 0;           // (to: the next one's slot)
   unsigned long long bads = 0;                // bad blocks of the last tiles asked for, newest first
   // A tile that is part-filled or has a bad page issues fewer loads than 2 PER:
-  // from the first such one on, every load is waited for.
+  // from the first such one on, every load is waited for, and every tile masked.
   bool uneven = false;
   auto ask = [&]() {
     if (asked < plain) {
-      load(asked, to, gr_ic<1>{}, 0u);
+      if constexpr (Q8) load8(asked, gr_ic<1>{}, 0u);
+      else load(asked, to, gr_ic<1>{}, 0u);
       bads <<= BLOCKS;
     } else {
       if (asked >= ntile) return;
       if (asked > 0 && (asked & (WIN - 1)) == 0) refill(asked, id_of(asked));
       const unsigned bad = (unsigned)(badwin >> ((asked & (WIN - 1)) * BLOCKS)) & ((1u << BLOCKS) - 1);
       bads = bads << BLOCKS | bad;
-      if (bad == 0 && asked < nwhole) {
+      if constexpr (Q8) {
+        if (bad == 0 && asked < nwhole) {
+          load8(asked, gr_ic<1>{}, 0u);
+        } else {
+          load8(asked, gr_ic<0>{}, bad);
+          uneven = true;
+        }
+      } else if (bad == 0 && asked < nwhole) {
         load(asked, to, gr_ic<1>{}, 0u);
       } else {
         load(asked, to, gr_ic<0>{}, bad);
@@ -644,6 +724,14 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
       plain = badwin == 0 ? gr_imin(nwhole, (asked & ~(WIN - 1)) + WIN) : 0;
     }
     ++asked;
+    if (!Q8) to = to + 1 == NS ? 0 : to + 1;
+  };
+  // Q8: the tile asked for last, from registers into its slot
+  int stored = 0;
+  auto put = [&]() {
+    if (stored >= ntile) return;
+    store8(to);
+    ++stored;
     to = to + 1 == NS ? 0 : to + 1;
   };
   // Waits for all but the tiles behind tile j (a barrier's waves wait before they ask on).
@@ -655,13 +743,26 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
     else gr_wait_vmcnt<0>();
     asm volatile("" ::: "memory");
   };
-  static_assert(NS <= 3 && 2 * (NS - 1) * PER < 64 && NS * BLOCKS <= 64, "load counters");
+  static_assert(NS <= 3 && 2 * (NS - 1) * PER < 64 && (NS + 1) * BLOCKS <= 64, "load counters");
+  static_assert(!Q8 || NS == (SOLO ? 1 : 2), "a wave's own slot, or one to read and one to write");
   auto barrier = [&] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
   int j = 0, slot = 0;
+  if constexpr (Q8) {
+    ask();
+    if constexpr (!SOLO) {
+      put();
+      ask();
+    }
+  } else {
 #pragma unroll
-  for (int i = 0; i < NS - 1; ++i) ask();
+    for (int i = 0; i < NS - 1; ++i) ask();
+  }
   auto enter = [&](int j) {
-    if constexpr (SOLO) {
+    if constexpr (Q8) {
+      if constexpr (!SOLO) barrier();                          // tile j is there, and its predecessor's slot free
+      put();
+      ask();
+    } else if constexpr (SOLO) {
       // the slot's last reads are over (no other wave reads it)
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       ask();
@@ -774,7 +875,7 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
 // Tiles of BM rows: NW waves by row, KG groups by key, BN keys a step, NS steps in
 // LDS. KGS > 0: sequences of at most 32 rows (single tokens in a
 // batch with long chunks) take tiles of 32, KGS waves sharing out the keys, 32 a step.
-template <class T, int D, int BN, int NW, int KG, int NS, int KGS, bool SHARED>
+template <class T, int D, int BN, int NW, int KG, int NS, int KGS, bool SHARED, bool Q8>
 __device__ __forceinline__ void gr_paged_body(const gr_paged_args& a, char* lds) {
   constexpr int BM = 32 * NW, WAVES = NW * KG;
   const int lane = threadIdx.x & 63;
@@ -783,9 +884,9 @@ __device__ __forceinline__ void gr_paged_body(const gr_paged_args& a, char* lds)
   gr_paged_seqs<BM, (KGS > 0)> seqs;
   auto segment = [&](int hk, int key0, int key1, int place) {
     if constexpr (KGS > 0) {
-      if (t.nrows <= 32) return gr_paged_segment<T, D, 32, 1, KGS, 2, WAVES, BM>(a, lds, t, hk, key0, key1, place);
+      if (t.nrows <= 32) return gr_paged_segment<T, D, 32, 1, KGS, Q8 ? 1 : 2, WAVES, BM, Q8>(a, lds, t, hk, key0, key1, place);
     }
-    gr_paged_segment<T, D, BN, NW, KG, NS, WAVES, BM>(a, lds, t, hk, key0, key1, place);
+    gr_paged_segment<T, D, BN, NW, KG, NS, WAVES, BM, Q8>(a, lds, t, hk, key0, key1, place);
   };
   if constexpr (!SHARED) {
     // key head slowest, then the tiles: workgroups of one key head share an XCD's L2

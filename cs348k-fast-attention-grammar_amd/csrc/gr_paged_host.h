@@ -1,9 +1,10 @@
 // gr_paged_host.h -- host-side checks shared by the entry points over a paged
-// cache (gr_paged_append, gr_paged_attn).
+// cache, of 16-bit rows or quantised.
 #pragma once
 #include <cstdint>
 
 #include "gr_host.h"
+#include "gr_overlap.h"
 #include "grammar_rt.h"
 
 namespace gr {
@@ -37,6 +38,27 @@ inline int check_paged(const gr_paged_cache* c, const gr_paged_batch* b, const c
   if ((long long)b->width * c->page_size > (1LL << 30))
     return fail(GR_E_ARG, "%s: a page table of %d pages of %d holds more than 2^30 keys", who, b->width, c->page_size);
   return GR_OK;
+}
+
+// The scales of a quantised cache, whose rows are bytes.
+inline int check_scales(const gr_paged_cache* c, const gr_paged_scales* s, const char* who) {
+  if (!s->scales) return fail(GR_E_ARG, "%s: null argument (scales)", who);
+  for (int i = 0; i < 3; ++i) {
+    if (s->strides[i] < 0) return fail(GR_E_ARG, "%s: strides must be non-negative (scales)", who);
+    if (c->k_strides[i] % 16 || c->v_strides[i] % 16)
+      return fail(GR_E_ARG, "%s: strides must be multiples of 16 elements (quantised cache)", who);
+  }
+  return GR_OK;
+}
+
+// The same memory in single bytes, and a quantised cache's scales.
+inline strided bytes_of(strided a, int size) {
+  for (int i = 0; i < 3; ++i) a.s[i] *= size;
+  a.n[3] *= size;
+  return a;
+}
+inline strided scales_of(const gr_paged_cache* c, const gr_paged_scales* s) {
+  return {s->scales, {c->pages, c->heads, 2, c->page_size}, {s->strides[0], s->strides[1], s->strides[2], 1}};
 }
 
 }  // namespace gr

@@ -1,5 +1,6 @@
 // gr_rotary.h -- rotation of query and key heads by position, alone or on the
-// way into a paged key/value cache.
+// way into a paged key/value cache, behind a norm of each head or not, the cache's
+// rows quantised or not.
 //
 // Pair j of a head, (x1, x2), becomes (x1 cos t - x2 sin t, x1 sin t + x2 cos t)
 // with t = pos f_j, f_j an angle per position; the gradient is the rotation by
@@ -55,6 +56,13 @@ struct gr_rope_args {
   int width, pages, page_shift, B;
   const int* lens;
   const int* starts;             // nullptr: uniform batch
+  // NORM: weights of the queries' and keys' rows (nullptr: ones), in fp32 or the rows' type
+  const void *wq, *wk;
+  int w32;
+  float eps;
+  // Q8: the E8M0 scales of the cache's rows, unit stride along the slots
+  unsigned char* scales;
+  long long sp, sh, skind;       // page, head, from a key's to a value's
 };
 
 // sin and cos of 2 pi h 2^-32: the nearest quarter turn off exactly in
@@ -111,20 +119,150 @@ struct gr_rope8 {
   }
 };
 
-// PAST: stores go past the caches (of whole 128-byte lines only)
-template <class T, bool APPEND, bool INTER, int ITER, bool PAST>
+// Sines and cosines of the 8 pairs of unit `u0` of a token: its position on each axis
+// from `pos`, or `at` on every axis. (a: gr_rope_args, or what has its members.)
+template <class A>
+__device__ __forceinline__ void gr_unit_angles(const A& a, const int* pos, int at, int u0, int lane, bool inverse, float (&sn)[8],
+                                               float (&cs)[8]) {
+  int p1 = at, plane = 0;
+  if (pos) {
+    if (a.naxes == 1) p1 = pos[0];
+    else if (lane < a.naxes) plane = pos[lane * a.ps[0]];
+  }
+  unsigned long long ax = 0;
+  if (a.naxes > 1) ax = *reinterpret_cast<const unsigned long long*>(a.axes + 8 * u0);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    int pe = p1;
+    if (a.naxes > 1 && pos) pe = __shfl(plane, (int)(ax >> (8 * e)) & 63, 64);
+    const unsigned long long t = (unsigned long long)(long long)pe * a.turns[8 * u0 + e];
+    gr_turn_sincos((unsigned)(t >> 32), sn[e], cs[e]);
+    if (inverse) sn[e] = -sn[e];
+  }
+}
+
+// Sum, and largest as whole numbers, over the 1, 2, 4, 8 or 16 lanes of a group (a power of
+// two, aligned), for all of them: within four lanes, then by mirrors of 8 and 16, whose
+// halves are alike by then.
+template <int CTRL>
+__device__ __forceinline__ unsigned gr_dpp(unsigned v) {
+  return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
+__device__ __forceinline__ float gr_group_sum(float v, int lanes) {
+  if (lanes > 1) v += __builtin_bit_cast(float, gr_dpp<0xb1>(__builtin_bit_cast(unsigned, v)));    // quad_perm 1 0 3 2
+  if (lanes > 2) v += __builtin_bit_cast(float, gr_dpp<0x4e>(__builtin_bit_cast(unsigned, v)));    // quad_perm 2 3 0 1
+  if (lanes > 4) v += __builtin_bit_cast(float, gr_dpp<0x141>(__builtin_bit_cast(unsigned, v)));   // row_half_mirror
+  if (lanes > 8) v += __builtin_bit_cast(float, gr_dpp<0x140>(__builtin_bit_cast(unsigned, v)));   // row_mirror
+  return v;
+}
+__device__ __forceinline__ unsigned gr_umax(unsigned a, unsigned b) { return a > b ? a : b; }
+__device__ __forceinline__ unsigned gr_group_umax(unsigned v, int lanes) {
+  if (lanes > 1) v = gr_umax(v, gr_dpp<0xb1>(v));
+  if (lanes > 2) v = gr_umax(v, gr_dpp<0x4e>(v));
+  if (lanes > 4) v = gr_umax(v, gr_dpp<0x141>(v));
+  if (lanes > 8) v = gr_umax(v, gr_dpp<0x140>(v));
+  return v;
+}
+
+// Lanes of a head row that is reduced: its units, up to a power of two.
+__device__ __forceinline__ int gr_row_lanes(int units) { return units > 1 ? 1 << (32 - __builtin_clz(units - 1)) : 1; }
+
+// 16 weights of a lane's unit, from elements lo and hi on.
+template <class T>
+__device__ __forceinline__ void gr_unit_weights(const void* w, int w32, int lo, int hi, float (&f)[16]) {
+  if (w == nullptr) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) f[e] = 1.f;
+  } else if (sizeof(T) == 4 || w32) {
+    gr_rope8<float> a, b;
+    a.load(static_cast<const float*>(w) + lo);
+    b.load(static_cast<const float*>(w) + hi);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      f[e] = a.get(e);
+      f[8 + e] = b.get(e);
+    }
+  } else {
+    gr_rope8<T> a, b;
+    a.load(static_cast<const T*>(w) + lo);
+    b.load(static_cast<const T*>(w) + hi);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      f[e] = a.get(e);
+      f[8 + e] = b.get(e);
+    }
+  }
+}
+
+// Rotates a unit's 8 pairs by its sines and cosines: elements e and 8 + e, or 2e and 2e + 1.
+template <bool INTER>
+__device__ __forceinline__ void gr_turn_unit(float (&f)[16], const float (&sn)[8], const float (&cs)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    float &x = f[INTER ? 2 * e : e], &y = f[INTER ? 2 * e + 1 : 8 + e];
+    const float a = x, b = y;
+    x = fmaf(a, cs[e], -b * sn[e]);
+    y = fmaf(a, sn[e], b * cs[e]);
+  }
+}
+
+// Stores a unit of a key's (hr below their heads) or value's row as e4m3 numbers
+// with the row's scale; the lanes of a row call it together.
+template <class T>
+__device__ __forceinline__ void gr_store_e4m3(const gr_rope_args& a, float (&f)[16], int hr, int lanes, int u, bool live, int lo,
+                                              int hi, long long page, int slot) {
+  unsigned top = 0;                              // the largest magnitude's bits
+#pragma unroll
+  for (int e = 0; e < 16; ++e) top = gr_umax(top, __builtin_bit_cast(unsigned, f[e]) & 0x7fffffffu);
+  top = gr_group_umax(top, lanes);
+  const bool finite = top < 0x7f800000u;
+  // the largest number of four significant bits in T, 15 2^12 or 15 2^124
+  constexpr float MOST = __is_same(T, _Float16) ? 61440.f : 0x1.ep+127f;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) f[e] = __builtin_amdgcn_fmed3f(f[e], -MOST, MOST);
+  top = top < __builtin_bit_cast(unsigned, MOST) ? top : __builtin_bit_cast(unsigned, MOST);
+  // 1.m 2^e <= 1.75 2^8 2^k: k = e - 8, or one more where 1.m is above 1.75
+  int sb = (int)(top >> 23) - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
+  sb = !finite ? 255 : sb < 0 ? 0 : sb;
+  const float by = __builtin_bit_cast(float, (unsigned)(finite ? 254 - sb : 127) << 23);
+  gr_u32x4 w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int half = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i] * by, f[4 * i + 1] * by, 0, false);
+    w[i] = finite ? (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i + 2] * by, f[4 * i + 3] * by, half, true) : 0x7f7f7f7fu;
+  }
+  if (!live || page < 0) return;
+  const bool key = hr < a.k.heads;
+  const gr_rope_rows& k = key ? a.k : a.v;
+  const int h = key ? hr : hr - a.k.heads;
+  unsigned char* const d = static_cast<unsigned char*>(k.dst) + page * k.db + slot * k.dt + h * k.dh;
+  *reinterpret_cast<gr_u32x2*>(d + lo) = (gr_u32x2){w[0], w[1]};
+  *reinterpret_cast<gr_u32x2*>(d + hi) = (gr_u32x2){w[2], w[3]};
+  if (u == 0) a.scales[page * a.sp + h * a.sh + (key ? 0 : a.skind) + slot] = (unsigned char)sb;
+}
+
+// PAST: stores go past the caches (of whole 128-byte lines only). NORM: query and
+// key rows are divided by their root mean square and multiplied by their
+// weights, in fp32, before they are rotated. Q8: key and value rows are stored as
+// e4m3 numbers z 2^-k, k the least power (-127 at least) by which the row's
+// largest magnitude is at most 448, and k + 127 beside them. z 2^-k is exact, so the only rounding is
+// the one to e4m3's four bits, and an attention gets the value back in bf16 or
+// fp16 as it is: rows are clamped to the largest such number of the type first, 61,440
+// in fp16 and 15 2^124 in bf16. A row with a value that is not finite is NaN all over.
+template <class T, bool APPEND, bool INTER, int ITER, bool PAST, bool NORM = false, bool Q8 = false>
 __device__ __forceinline__ void gr_rope_body(const gr_rope_args& a, bool inverse) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)((blockIdx.x * blockDim.x + threadIdx.x) >> 6));
   const int units = a.D >> 4;                    // of a head row
-  const int rpp = 64 / units;                    // rows a pass
+  const int lanes = NORM || Q8 ? gr_row_lanes(units) : units;
+  const int rpp = 64 / lanes;                    // rows a pass
   const int h0 = a.q.heads, h1 = h0 + a.k.heads, rows = h1 + (APPEND ? a.v.heads : 0);
   const int passes = (rows + rpp - 1) / rpp, groups = (passes + ITER - 1) / ITER;
   const int tok = wave / groups;
   if (tok >= a.tokens) return;
-  const int row0 = (wave - tok * groups) * ITER * rpp + lane / units, u = lane % units;
+  const int row0 = (wave - tok * groups) * ITER * rpp + lane / lanes, u = lane % lanes;
   const int ru = a.pairs >> 3;                   // rotated units
-  const bool lane_live = lane < rpp * units;
+  const bool lane_live = lane < rpp * lanes && u < units;
   const int lo = u < ru ? (INTER ? 16 * u : 8 * u) : 2 * a.pairs + 8 * (u - ru);
   const int hi = u < ru ? (INTER ? 16 * u + 8 : a.pairs + 8 * u) : lo + 8 * (units - ru);
 
@@ -155,6 +293,7 @@ __device__ __forceinline__ void gr_rope_body(const gr_rope_args& a, bool inverse
 #pragma unroll
   for (int p = 0; p < ITER; ++p) {
     const int r = row0 + p * rpp;
+    if (NORM || Q8) x[p] = y[p] = {};            // (lanes without elements add nothing to their row's sum)
     if (lane_live && r < rows) {
       const T* s = r < h0 ? sq + r * a.q.sh : !APPEND || r < h1 ? sk + (r - h0) * a.k.sh : sv + (r - h1) * a.v.sh;
       x[p].load(s + lo);
@@ -175,30 +314,59 @@ __device__ __forceinline__ void gr_rope_body(const gr_rope_args& a, bool inverse
   }
 
   float sn[8] = {}, cs[8] = {};
-  if (a.pairs > 0) {
-    int p1 = at, plane = 0;
-    if (a.pos) {
-      const int* pp = a.pos + brow * a.ps[1] + trow * a.ps[2];
-      if (a.naxes == 1) p1 = pp[0];
-      else if (lane < a.naxes) plane = pp[lane * a.ps[0]];
-    }
-    const int u0 = u < ru ? u : 0;
-    unsigned long long ax = 0;
-    if (a.naxes > 1) ax = *reinterpret_cast<const unsigned long long*>(a.axes + 8 * u0);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      int pe = p1;
-      if (a.naxes > 1 && a.pos) pe = __shfl(plane, (int)(ax >> (8 * e)) & 63, 64);
-      const unsigned long long t = (unsigned long long)(long long)pe * a.turns[8 * u0 + e];
-      gr_turn_sincos((unsigned)(t >> 32), sn[e], cs[e]);
-      if (inverse) sn[e] = -sn[e];
-    }
-  }
+  if (a.pairs > 0)
+    gr_unit_angles(a, a.pos ? a.pos + brow * a.ps[1] + trow * a.ps[2] : nullptr, at, u < ru ? u : 0, lane, inverse, sn, cs);
 
   auto target = [&](const gr_rope_rows& k, bool cached) {
     return static_cast<T*>(k.dst) + (cached ? page * k.db + slot * k.dt : brow * k.db + trow * k.dt);
   };
-  T *dq = target(a.q, false), *dk = target(a.k, APPEND), *dv = APPEND ? target(a.v, true) : nullptr;
+  T* dq = target(a.q, false);
+  if constexpr (NORM || Q8) {
+    const bool unit = u < units;
+    float wq[16], wk[16];
+    if constexpr (NORM) {
+      gr_unit_weights<T>(a.wq, a.w32, unit ? lo : 0, unit ? hi : 0, wq);
+      gr_unit_weights<T>(a.wk, a.w32, unit ? lo : 0, unit ? hi : 0, wk);
+    }
+#pragma unroll
+    for (int p = 0; p < ITER; ++p) {
+      const int r = row0 + p * rpp;
+      float f[16];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        f[e] = x[p].get(e);
+        f[8 + e] = y[p].get(e);
+      }
+      if constexpr (NORM) {
+        float ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) ss = fmaf(f[e], f[e], ss);
+        const float rms = rsqrtf(gr_group_sum(ss, lanes) / (float)a.D + a.eps);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) f[e] = APPEND && r >= h1 ? f[e] : f[e] * rms * (r < h0 ? wq[e] : wk[e]);
+      }
+      if ((!APPEND || r < h1) && u < ru) gr_turn_unit<INTER>(f, sn, cs);
+      if (Q8 && r >= h0) {
+        gr_store_e4m3<T>(a, f, r - h0, lanes, u, lane_live && r < rows, lo, hi, page, slot);
+      } else if (lane_live && r < rows && (!APPEND || r < h0 || page >= 0)) {
+        gr_rope8<T> s, t;
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          s.put2(e, f[e], f[e + 1]);
+          t.put2(e, f[8 + e], f[9 + e]);
+        }
+        T* d = dq + r * a.q.dh;
+        if (r >= h0) {
+          const gr_rope_rows& k = !APPEND || r < h1 ? a.k : a.v;
+          d = target(k, APPEND) + (!APPEND || r < h1 ? r - h0 : r - h1) * k.dh;
+        }
+        s.template store<PAST>(d + lo);
+        t.template store<PAST>(d + hi);
+      }
+    }
+    return;
+  }
+  T *dk = target(a.k, APPEND), *dv = APPEND ? target(a.v, true) : nullptr;
 #pragma unroll
   for (int p = 0; p < ITER; ++p) {
     const int r = row0 + p * rpp;

@@ -132,6 +132,16 @@ def lib() -> ctypes.CDLL:
         L.gr_paged_attn_workspace.argtypes = [vp, vp, i32]
         L.gr_paged_attn_workspace.restype = sz
         L.gr_paged_attn.argtypes = [vp, vp, vp, vp, vp, i32, pll, pll, i32, ctypes.c_float, vp, sz, vp]
+        L.gr_norm_rotary.argtypes = [vp, vp, vp, vp, i32, pll, pll, vp, vp, i32, pll, pll, i32, i32, i32, vp, pll, vp]
+        L.gr_norm_rotary_bwd_workspace.argtypes = [i32] * 6
+        L.gr_norm_rotary_bwd_workspace.restype = sz
+        L.gr_norm_rotary_bwd.argtypes = [vp, vp, vp, vp, vp, i32, pll, pll, pll, vp, vp, vp, i32, pll, pll, pll, i32, i32, i32,
+                                         vp, pll, vp, vp, vp, sz, vp]
+        L.gr_paged_append_with.argtypes = [vp, vp, vp, vp, vp, vp, vp, i32, pll, pll, vp, vp, pll, pll, vp, pll, vp]
+        L.gr_paged_read.argtypes = [vp, vp, vp, vp, vp, pll, pll, vp]
+        L.gr_paged_attn_scaled_workspace.argtypes = [vp, vp, vp, i32]
+        L.gr_paged_attn_scaled_workspace.restype = sz
+        L.gr_paged_attn_scaled.argtypes = [vp, vp, vp, vp, vp, vp, i32, pll, pll, i32, ctypes.c_float, vp, sz, vp]
         _lib = L
         return L
 
@@ -147,6 +157,17 @@ class PagedCacheDesc(ctypes.Structure):
     _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_strides", _ll3), ("v_strides", _ll3),
                 ("dtype", ctypes.c_int), ("pages", ctypes.c_int), ("heads", ctypes.c_int),
                 ("page_size", ctypes.c_int), ("head_dim", ctypes.c_int)]
+
+
+class HeadNormSpec(ctypes.Structure):
+    """gr_head_norm."""
+    _fields_ = [("q_weight", ctypes.c_void_p), ("k_weight", ctypes.c_void_p), ("dtype", ctypes.c_int),
+                ("eps", ctypes.c_float)]
+
+
+class PagedScales(ctypes.Structure):
+    """gr_paged_scales."""
+    _fields_ = [("scales", ctypes.c_void_p), ("strides", _ll3)]
 
 
 class PagedBatch(ctypes.Structure):
@@ -166,6 +187,8 @@ EXPORTED = (
     "gr_plan_run_args", "gr_gemm_workspace", "gr_gemm_ws", "gr_mlp_fwd_workspace", "gr_mlp_fwd_ws",
     "gr_selftest_f32_no_workspace", "gr_attn_fwd_shape", "gr_gemm_f32_groups",
     "gr_rotary", "gr_paged_append", "gr_paged_attn_workspace", "gr_paged_attn", "gr_selftest_overlap",
+    "gr_norm_rotary", "gr_norm_rotary_bwd_workspace", "gr_norm_rotary_bwd", "gr_paged_append_with",
+    "gr_paged_read", "gr_paged_attn_scaled_workspace", "gr_paged_attn_scaled",
 )
 
 # Bytes of the per-device scratch array behind gr_attn_decode_noalloc (GR_DECODE_SCRATCH_BYTES).

@@ -256,6 +256,41 @@ int gr_rotary(const gr_rotary_spec* rotary, const void* q, void* q_out, int Hq, 
               const long long* k_out_strides, int dtype, int B, int N, const int* positions,
               const long long* position_strides, int inverse, void* stream);
 
+/* A norm of query and key heads: a row x of D elements becomes w x / sqrt(mean
+ * x^2 + eps), w its D weights. q_weight, k_weight: device arrays, 16-byte aligned, of
+ * dtype GR_F32 or the rows' type; NULL: ones. eps: not negative. No counterpart in
+ * the reference. */
+typedef struct gr_head_norm {
+  const void* q_weight;
+  const void* k_weight;
+  int dtype;
+  float eps;
+} gr_head_norm;
+
+/* gr_rotary of normed heads, in one pass over them; arguments as there. Squares,
+ * norm, weights and rotation in fp32 (magnitudes up to 2^60), rounded once. */
+int gr_norm_rotary(const gr_rotary_spec* rotary, const gr_head_norm* norm, const void* q, void* q_out, int Hq,
+                   const long long* q_strides, const long long* q_out_strides, const void* k, void* k_out, int Hk,
+                   const long long* k_strides, const long long* k_out_strides, int dtype, int B, int N,
+                   const int* positions, const long long* position_strides, void* stream);
+
+/* Its gradient: from q, k as gr_norm_rotary took them and the gradients dq_out,
+ * dk_out of its results, those of q and k into dq, dk (strides of dq_out, dq, dk_out and
+ * dk as q's; dq may be dq_out by the same strides, outputs share no other memory with
+ * the call's arrays) and those of the weights, [D] of the weights' type, into dq_weight, dk_weight
+ * (NULL: not wanted). k NULL: queries alone. The weights' gradients are summed in fp32 over all
+ * tokens and heads, in an order that the sizes alone decide.
+ * workspace: device memory of at least gr_norm_rotary_bwd_workspace(...) bytes, 16-byte
+ * aligned, not read by calls to come (calls that may overlap in time need one each); not
+ * needed without dq_weight and dk_weight. */
+size_t gr_norm_rotary_bwd_workspace(int Hq, int Hk, int head_dim, int dtype, int B, int N);
+int gr_norm_rotary_bwd(const gr_rotary_spec* rotary, const gr_head_norm* norm, const void* q, const void* dq_out, void* dq,
+                       int Hq, const long long* q_strides, const long long* dq_out_strides, const long long* dq_strides,
+                       const void* k, const void* dk_out, void* dk, int Hk, const long long* k_strides,
+                       const long long* dk_out_strides, const long long* dk_strides, int dtype, int B, int N,
+                       const int* positions, const long long* position_strides, void* dq_weight, void* dk_weight,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
 /* A key/value cache in pages. No counterpart in the reference. k and v:
  * [pages][heads][page_size][head_dim] by strides {page, head, slot} in elements
  * (non-negative multiples of 8, unit stride along head_dim, the slot stride below
@@ -304,6 +339,39 @@ int gr_paged_append(const gr_paged_cache* cache, const gr_paged_batch* batch, co
                     const void* v, const long long* k_strides, const long long* v_strides, const int* positions,
                     const long long* position_strides, void* stream);
 
+/* The scales of a quantised cache. Its k and v hold bytes (e4m3: four significant
+ * bits, at most 448) by strides that are multiples of 16, and its dtype is that of the
+ * tokens, GR_F16 or GR_BF16. scales: bytes [pages][heads][2: key, value][page_size] by
+ * strides {page, head, key to value}, unit stride along the slots, each b standing for 2^(b - 127),
+ * or NaN for 255 (E8M0). A row stands for its numbers times its scale, which
+ * are numbers of the tokens' type. */
+typedef struct gr_paged_scales {
+  void* scales;
+  long long strides[3];
+} gr_paged_scales;
+
+/* gr_paged_append of normed queries and keys (norm NULL: none) into a cache that
+ * is quantised (scales NULL: it is not). A row is quantised after norm and rotation,
+ * in fp32: its scale is the least power of two, 2^-127 at least, by which its
+ * largest magnitude is at most 448, its numbers are rounded to nearest even. Rows
+ * are clamped to 61440 (fp16) or 15 2^124 (bf16) first; a row with a value that is not finite becomes
+ * NaN. Other arguments as gr_paged_append's, of which this is the general form. */
+int gr_paged_append_with(const gr_paged_cache* cache, const gr_paged_scales* scales, const gr_paged_batch* batch,
+                         const gr_rotary_spec* rotary, const gr_head_norm* norm, const void* q, void* q_out, int Hq,
+                         const long long* q_strides, const long long* q_out_strides, const void* k, const void* v,
+                         const long long* k_strides, const long long* v_strides, const int* positions,
+                         const long long* position_strides, void* stream);
+
+/* Reads the batch's sequences back as dense keys and values in the cache's dtype
+ * (scales NULL: the cache is not quantised): key j of sequence b goes to token j of
+ * batch b of k_out and v_out [B, rows, heads, D] or, with starts, to row starts[b] + j of
+ * [rows, heads, D], by strides {batch, token, head} that are multiples of 8. `rows`
+ * and `starts` of the batch count keys here, not new tokens. Rows of a sequence behind its
+ * keys, and keys whose page is not in the cache, become 0; rows of no sequence are
+ * left alone. k_out and v_out share no memory with each other or the cache. */
+int gr_paged_read(const gr_paged_cache* cache, const gr_paged_scales* scales, const gr_paged_batch* batch, void* k_out,
+                  void* v_out, const long long* k_strides, const long long* v_strides, void* stream);
+
 /* Attention of the new tokens over the cache, O = softmax(scale Q K^T) V; token
  * i sees the keys up to its own position (causal != 0) or all of its sequence's.
  * Hq, a multiple of the cache's heads: query head h reads key head h / (Hq /
@@ -320,6 +388,15 @@ size_t gr_paged_attn_workspace(const gr_paged_cache* cache, const gr_paged_batch
 int gr_paged_attn(const gr_paged_cache* cache, const gr_paged_batch* batch, const void* q, void* o, float* lse, int Hq,
                   const long long* q_strides, const long long* o_strides, int causal, float scale, void* workspace,
                   size_t workspace_bytes, void* stream);
+
+/* The same over a quantised cache: keys and values are taken as the numbers of
+ * the tokens' type that they stand for. The workspace has a size of its own. */
+size_t gr_paged_attn_scaled_workspace(const gr_paged_cache* cache, const gr_paged_scales* scales, const gr_paged_batch* batch,
+                                      int Hq);
+int gr_paged_attn_scaled(const gr_paged_cache* cache, const gr_paged_scales* scales, const gr_paged_batch* batch,
+                         const void* q, void* o, float* lse, int Hq, const long long* q_strides,
+                         const long long* o_strides, int causal, float scale, void* workspace, size_t workspace_bytes,
+                         void* stream);
 
 /* Batched GEMM with fused epilogue, C[z] = act(alpha * A[z] @ B[z]).
  * Replaces the grammar's matmul stage (a stage whose body is matmul over a
