@@ -327,10 +327,9 @@ struct gr_paged_lds {
 //
 // Q8: the cache holds e4m3 bytes and power-of-two scales. A tile's bytes come
 // through registers, are turned into T exactly (gr_from_e4m3) and written to LDS where
-// the 16-bit tile's loads would have put them, once for all waves that read them: from there
-// on the two are alike. Loads are a tile ahead of the one being written, which is
-// a tile ahead of the products where waves share it (NS 2), and the products' own
-// where a wave has it alone (NS 1).
+// the 16-bit tile's loads would have put them, once for all waves that read them:
+// from there on the two are alike. Loads are a tile ahead of the one being written, which
+// is a tile ahead of the products. (Few rows: gr_paged_rows.)
 template <class T, int D, int BN, int NW, int KG, int NS, int WAVES, int BM, bool Q8>
 __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* lds_all, const gr_paged_tile& t, int hk,
                                                  int key0, int key1, int place) {
@@ -744,22 +743,20 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
     asm volatile("" ::: "memory");
   };
   static_assert(NS <= 3 && 2 * (NS - 1) * PER < 64 && (NS + 1) * BLOCKS <= 64, "load counters");
-  static_assert(!Q8 || NS == (SOLO ? 1 : 2), "a wave's own slot, or one to read and one to write");
+  static_assert(!Q8 || (NS == 2 && !SOLO), "a slot to read and one to write");
   auto barrier = [&] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
   int j = 0, slot = 0;
   if constexpr (Q8) {
     ask();
-    if constexpr (!SOLO) {
-      put();
-      ask();
-    }
+    put();
+    ask();
   } else {
 #pragma unroll
     for (int i = 0; i < NS - 1; ++i) ask();
   }
   auto enter = [&](int j) {
     if constexpr (Q8) {
-      if constexpr (!SOLO) barrier();                          // tile j is there, and its predecessor's slot free
+      barrier();                                               // tile j is there, and its predecessor's slot free
       put();
       ask();
     } else if constexpr (SOLO) {
@@ -872,21 +869,36 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
   }
 }
 
+// Few rows over a quantised cache (gr_paged_rows.h).
+template <class T, int D, int BN, int RB, int KG, int WAVES, int BM>
+__device__ __forceinline__ void gr_paged_rows(const gr_paged_args& a, char* lds_all, const gr_paged_tile& t, int hk, int key0,
+                                              int key1, int place);
+
+// Rows of a tile of NW waves (0: one wave's 16).
+constexpr int gr_paged_rows_of(int nw) { return nw ? 32 * nw : 16; }
+
 // Tiles of BM rows: NW waves by row, KG groups by key, BN keys a step, NS steps in
 // LDS. KGS > 0: sequences of at most 32 rows (single tokens in a
 // batch with long chunks) take tiles of 32, KGS waves sharing out the keys, 32 a step.
 template <class T, int D, int BN, int NW, int KG, int NS, int KGS, bool SHARED, bool Q8>
 __device__ __forceinline__ void gr_paged_body(const gr_paged_args& a, char* lds) {
-  constexpr int BM = 32 * NW, WAVES = NW * KG;
+  constexpr int BM = gr_paged_rows_of(NW), WAVES = (NW ? NW : 1) * KG;
   const int lane = threadIdx.x & 63;
   const int logical = gr_xcd_remap_any((int)blockIdx.x, (int)gridDim.x);
   gr_paged_tile t;
   gr_paged_seqs<BM, (KGS > 0)> seqs;
   auto segment = [&](int hk, int key0, int key1, int place) {
-    if constexpr (KGS > 0) {
-      if (t.nrows <= 32) return gr_paged_segment<T, D, 32, 1, KGS, Q8 ? 1 : 2, WAVES, BM, Q8>(a, lds, t, hk, key0, key1, place);
+    if constexpr (Q8 && NW <= 1) {
+      gr_paged_rows<T, D, BN, BM / 16, KG, WAVES, BM>(a, lds, t, hk, key0, key1, place);
+    } else {
+      if constexpr (KGS > 0) {
+        if (t.nrows <= 32) {
+          if constexpr (Q8) return gr_paged_rows<T, D, 32, 2, KGS, WAVES, BM>(a, lds, t, hk, key0, key1, place);
+          else return gr_paged_segment<T, D, 32, 1, KGS, 2, WAVES, BM, Q8>(a, lds, t, hk, key0, key1, place);
+        }
+      }
+      gr_paged_segment<T, D, BN, NW, KG, NS, WAVES, BM, Q8>(a, lds, t, hk, key0, key1, place);
     }
-    gr_paged_segment<T, D, BN, NW, KG, NS, WAVES, BM, Q8>(a, lds, t, hk, key0, key1, place);
   };
   if constexpr (!SHARED) {
     // key head slowest, then the tiles: workgroups of one key head share an XCD's L2

@@ -10,6 +10,7 @@
 #include "gr_overlap.h"
 #include "gr_paged.h"
 #include "gr_paged_host.h"
+#include "gr_paged_rows.h"
 #include "grammar_rt.h"
 
 namespace {
@@ -18,15 +19,23 @@ constexpr int imax(int a, int b) { return a > b ? a : b; }
 
 template <int D, int BN, int NW, int KG, int NS, int KGS, bool Q8>
 struct Lds {
-  static constexpr int BYTES =
-      imax(gr_paged_lds<D, BN, NW, KG, NS>::BYTES, KGS ? gr_paged_lds<D, 32, 1, KGS ? KGS : 1, Q8 ? 1 : 2>::BYTES : 0);
+  static constexpr int small() {               // of sequences of few rows among others
+    if constexpr (KGS == 0) return 0;
+    else if constexpr (Q8) return gr_rows_lds<D, 32, 2, KGS>::BYTES;
+    else return gr_paged_lds<D, 32, 1, KGS, 2>::BYTES;
+  }
+  static constexpr int own() {
+    if constexpr (Q8 && NW <= 1) return gr_rows_lds<D, BN, NW + 1, KG>::BYTES;
+    else return gr_paged_lds<D, BN, NW, KG, NS>::BYTES;
+  }
+  static constexpr int BYTES = imax(own(), small());
 };
 
 // One workgroup of four waves a CU where its LDS allows no two, else (and with
 // eight waves) two waves a SIMD.
 template <class T, int D, int BN, int NW, int KG, int NS, int KGS, bool SHARED, bool Q8>
-__global__ __launch_bounds__(64 * NW * KG)
-__attribute__((amdgpu_waves_per_eu(NW* KG == 4 && Lds<D, BN, NW, KG, NS, KGS, Q8>::BYTES > 80 * 1024 ? 1 : 2)))
+__global__ __launch_bounds__(64 * imax(NW, 1) * KG)
+__attribute__((amdgpu_waves_per_eu(imax(NW, 1) * KG == 4 && Lds<D, BN, NW, KG, NS, KGS, Q8>::BYTES > 80 * 1024 ? 1 : 2)))
 void gr_paged_kernel(gr_paged_args a) {
   extern __shared__ __attribute__((aligned(16))) char gr_lds[];
   gr_paged_body<T, D, BN, NW, KG, NS, KGS, SHARED, Q8>(a, gr_lds);
@@ -52,7 +61,7 @@ inline Plan plan_of(const gr_paged_cache& c, const gr_paged_batch& b, int Hq, bo
   const int cus = gr::cu_count() > 0 ? gr::cu_count() : 256;
   const long long cap = (long long)b.width * c.page_size;
   const long long len = b.max_len > 0 && b.max_len < cap ? b.max_len : cap;
-  p.nw = most * G <= 32 ? 1 : most * G <= 64 ? 2 : 4;
+  p.nw = q8 && most * G <= 16 ? 0 : most * G <= 32 ? 1 : most * G <= 64 ? 2 : 4;
   // Chunks whose tiles of 128 rows would leave most CUs idle take tiles of 64
   // with four key groups: 16 or 64 tiles (one chunk of 512, 4 key heads, G 1 or 4)
   // at 512 keys 13.0 us to 9.4 and 13.0 to 9.8 (D 64), 18.1 to 13.4 and 18.5 to
@@ -60,10 +69,10 @@ inline Plan plan_of(const gr_paged_cache& c, const gr_paged_batch& b, int Hq, bo
   // 128 (16 tiles, 2,048 keys 30 to 22 us, 64 tiles, 8,192 keys 62 to 71).
   const long long rows128 = (b.starts ? (long long)b.rows : (long long)b.B * b.rows) * G / 128 * c.heads;
   if (p.nw == 4 && (len <= 1000 ? 4 * rows128 <= cus : D == 128 && 4 * rows128 < cus)) p.nw = 2;
-  const int BM = 32 * p.nw;
+  const int BM = gr_paged_rows_of(p.nw);
   // packed rows: every sequence may have a part-filled tile
   p.tiles = b.starts ? (long long)b.rows * G / BM + b.B : (long long)b.B * (((long long)b.rows * G + BM - 1) / BM);
-  const int resident = cus * (D == 128 && p.nw < 4 && !(q8 && p.nw == 1) ? 1 : 2);      // workgroups (their LDS)
+  const int resident = cus * (D == 128 && p.nw < 4 && !(q8 && p.nw <= 1) ? 1 : 2);      // workgroups (their LDS)
   // Tiles of 128 rows that leave a CU at most one of them halve the chain of their
   // key steps, with two key groups of four waves: 175 or 176 tiles, 1,500 keys 27.0
   // us to 23.0 (D 64), 44.5 to 36.0 (D 128); 256 tiles, 2,048 keys 33.8 to 28.8 and 57.0
@@ -95,21 +104,21 @@ inline Plan plan_of(const gr_paged_cache& c, const gr_paged_batch& b, int Hq, bo
   return p;
 }
 
-inline size_t share_bytes(const Plan& p, int D) { return (size_t)2 * 32 * p.nw * (D + 2) * sizeof(float); }
+inline size_t share_bytes(const Plan& p, int D) { return (size_t)2 * gr_paged_rows_of(p.nw) * (D + 2) * sizeof(float); }
 
 // A workgroup a tile.
 template <class T, int D, int BN, int NW, int KG, int NS, int KGS, bool Q8>
 int launch_alone(const gr_paged_args& a, hipStream_t st) {
   constexpr int LDS = Lds<D, BN, NW, KG, NS, KGS, Q8>::BYTES;
   hipLaunchKernelGGL((gr_paged_kernel<T, D, BN, NW, KG, NS, KGS, false, Q8>), dim3((unsigned)((long long)a.tiles * a.Hkv)),
-                     dim3(64 * NW * KG), LDS, st, a);
+                     dim3(64 * imax(NW, 1) * KG), LDS, st, a);
   return gr::hip_check(hipGetLastError(), GR_E_LAUNCH, "gr_paged_attn launch");
 }
 
 template <class T, int D, int BN, int NW, int KG, int NS, int KGS, bool Q8>
 int launch_shared(const gr_paged_args& a, hipStream_t st) {
-  constexpr int BM = 32 * NW, LDS = Lds<D, BN, NW, KG, NS, KGS, Q8>::BYTES;
-  hipLaunchKernelGGL((gr_paged_kernel<T, D, BN, NW, KG, NS, KGS, true, Q8>), dim3((unsigned)a.shares), dim3(64 * NW * KG), LDS, st, a);
+  constexpr int BM = gr_paged_rows_of(NW), LDS = Lds<D, BN, NW, KG, NS, KGS, Q8>::BYTES;
+  hipLaunchKernelGGL((gr_paged_kernel<T, D, BN, NW, KG, NS, KGS, true, Q8>), dim3((unsigned)a.shares), dim3(64 * imax(NW, 1) * KG), LDS, st, a);
   const int rc = gr::hip_check(hipGetLastError(), GR_E_LAUNCH, "gr_paged_attn launch");
   if (rc) return rc;
   const long long wgs = (long long)a.tiles * a.Hkv;
@@ -124,8 +133,11 @@ int launch_shared(const gr_paged_args& a, hipStream_t st) {
 
 template <class T, int D, bool Q8>
 int launch(const gr_paged_args& a, const Plan& p, hipStream_t st) {
-  constexpr int NS1 = Q8 ? 1 : 2, KGS = Q8 || D == 64 ? 4 : 2;
-  if (p.nw == 1) return a.shares ? launch_shared<T, D, 32, 1, 4, NS1, 0, Q8>(a, st) : launch_alone<T, D, 32, 1, 4, NS1, 0, Q8>(a, st);
+  constexpr int KGS = Q8 || D == 64 ? 4 : 2;
+  if constexpr (Q8) {
+    if (p.nw == 0) return a.shares ? launch_shared<T, D, 64, 0, 4, 1, 0, Q8>(a, st) : launch_alone<T, D, 32, 0, 4, 1, 0, Q8>(a, st);
+  }
+  if (p.nw == 1) return a.shares ? launch_shared<T, D, 32, 1, 4, 2, 0, Q8>(a, st) : launch_alone<T, D, 32, 1, 4, 2, 0, Q8>(a, st);
   if (p.nw == 2) return a.shares ? launch_shared<T, D, 32, 2, 4, 2, 0, Q8>(a, st) : launch_alone<T, D, 32, 2, 4, 2, 0, Q8>(a, st);
   // (keys 32 a step in two groups at D 128: two rings of 64 would take a CU's LDS)
   if (a.shares) return launch_shared<T, D, 64, 4, 1, 2, KGS, Q8>(a, st);
@@ -221,7 +233,7 @@ int attn(const gr_paged_cache* cache, const gr_paged_scales* scales, const gr_pa
   a.shares = p.shares;
   if (p.shares) {
     a.part_o = static_cast<float*>(workspace);
-    a.part_ml = a.part_o + (size_t)p.shares * 2 * 32 * p.nw * cache->head_dim;
+    a.part_ml = a.part_o + (size_t)p.shares * 2 * gr_paged_rows_of(p.nw) * cache->head_dim;
   }
   hipStream_t st = (hipStream_t)stream;
   if (cache->dtype == GR_F16)
