@@ -18,5 +18,24 @@ __device__ __forceinline__ unsigned gr_from_e4m3(unsigned w, float scale) {
     return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HIGH));
 }
 
-// A scale byte as the float whose exponent the conversion takes.
+// Where lane l's 16 bytes of a cached row go in LDS as T: a row of D / 16 pieces is
+// that many lanes wide, and a write of 16 bytes takes every second chunk of a row, so
+// that 8 lanes side by side (128 bytes, what LDS takes at a time) are two half rows, of rows
+// whose swizzles differ in the chunks' lowest bit: those that differ in bit 0 for keys
+// (gr_paged_swz) and bit 2 for values (gr_swz_v8). (All 8 of one row: every write in two.)
+template <int D>
+__device__ __forceinline__ int gr_piece8(int lane) { return D == 128 ? (lane & 3) | ((lane >> 1) & 4) : lane & 3; }
+template <int D>
+__device__ __forceinline__ int gr_key8(int lane) { return D == 128 ? ((lane >> 2) & 1) | ((lane >> 3) & 6) : lane >> 2; }
+template <int D>
+__device__ __forceinline__ int gr_value8(int lane) {
+  return D == 128 ? (lane & 4) | ((lane >> 4) & 3) : (lane & 4) | ((lane >> 3) & 3) | ((lane >> 2) & 8);
+}
+
+// A scale byte, and byte `shift` / 8 of a word of four, as the float whose exponent the
+// conversion takes. (Kept over a loop as loaded bytes, scales were masked to 8 bits in the
+// iteration that asked for them, which waited for its loads: words need no mask.)
+__device__ __forceinline__ float gr_e8m0_of(unsigned w, int shift) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_ubfe(w, shift, 8) << 23);
+}
 __device__ __forceinline__ float gr_e8m0(unsigned sb) { return __builtin_bit_cast(float, sb << 23); }

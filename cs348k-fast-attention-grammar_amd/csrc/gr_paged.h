@@ -313,6 +313,11 @@ __device__ __forceinline__ float gr_paged_shift(int keys) {
   return (float)gr_imin(32 - __builtin_clz((unsigned)(keys - 1)) - 11, 15);
 }
 
+// gr_swz_tr with row bit 2 in the chunk's lowest bit: the reads' rows of 4 differ in bits
+// 0 and 1, and take both chunks of a pair.
+template <int CPR>
+__device__ __forceinline__ int gr_swz_v8(int row, int chunk) { return gr_swz_tr<CPR>(row, chunk) ^ ((row >> 2) & 1); }
+
 template <int D, int BN, int NW, int KG, int NS>
 struct gr_paged_lds {
   static constexpr int TILE = BN * D * 2;
@@ -375,18 +380,19 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
   constexpr int CPR8 = D / 16, IPB8 = CPR8 / 4, PER8 = Q8 ? BLOCKS * IPB8 / NW : 1;
   static_assert(!Q8 || BLOCKS * IPB8 % NW == 0, "whole load instructions");
   constexpr int SUBS = Q8 ? (IPB8 > NW ? IPB8 / NW : 1) : IPB > NW ? IPB / NW : 1;
-  auto block_row8 = [&](int i) { return lane / CPR8 + ((wave + i * NW) % IPB8) * (64 / CPR8); };
+  auto key_row8 = [&](int i) { return gr_key8<D>(lane) + ((wave + i * NW) % IPB8) * (64 / CPR8); };
+  auto value_row8 = [&](int i) { return gr_value8<D>(lane) + ((wave + i * NW) % IPB8) * (64 / CPR8); };
   int kdst[SUBS], vdst[SUBS];
   auto block_row = [&](int i) { return lane / CPR + ((wave + i * NW) % IPB) * (64 / CPR); };
   unsigned koff[SUBS], voff[SUBS];            // bytes
 #pragma unroll
   for (int i = 0; i < SUBS; ++i) {
     if constexpr (Q8) {
-      const int r = block_row8(i), c8 = lane % CPR8, pr = gr_perm32(r);
-      koff[i] = (unsigned)(r * a.k_ss) + c8 * 16;
-      voff[i] = (unsigned)(r * a.v_ss) + c8 * 16;
+      const int kr = key_row8(i), vr = value_row8(i), c8 = gr_piece8<D>(lane), pr = gr_perm32(kr);
+      koff[i] = (unsigned)(kr * a.k_ss) + c8 * 16;
+      voff[i] = (unsigned)(vr * a.v_ss) + c8 * 16;
       kdst[i] = pr * (D * 2) + gr_paged_swz<CPR>(pr, 2 * c8) * 16;
-      vdst[i] = r * (D * 2) + gr_swz_tr<CPR>(r, 2 * c8) * 16;
+      vdst[i] = vr * (D * 2) + gr_swz_v8<CPR>(vr, 2 * c8) * 16;
       continue;
     }
     const int r = block_row(i), pc = lane % CPR;
@@ -400,7 +406,7 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
   //  V (gr_tr_frag): rows 16 x + 8 g + 4 h + (lane / 4) % 4, columns 32 db + ...
   const int kbase = l32 * (D * 2) + gr_paged_swz<CPR>(l32, g) * 16;
   const int vcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3), vrow = 8 * g + ((lane >> 2) & 3);
-  const int vbase = vrow * (D * 2) + gr_swz_tr<CPR>(vrow, vcol >> 3) * 16 + (vcol & 7) * 2;
+  const int vbase = vrow * (D * 2) + gr_swz_tr<CPR>(vrow, vcol >> 3) * 16 + (vcol & 7) * 2;   // (row bit 2 is 0)
   const int smask = (1 << a.page_shift) - 1;
 
   const int rw = t.row0 + wave * 32;                          // this wave's first row
@@ -477,28 +483,33 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
   // Q8: the bytes and scales of the next tile, and their way into a slot. Rows that
   // are not there are zeros.
   typedef const __attribute__((address_space(1))) gr_u32x4 global_u32x4;
-  typedef const __attribute__((address_space(1))) unsigned char global_u8;
+  typedef const __attribute__((address_space(1))) unsigned global_u32;
   gr_u32x4 kr[PER8], vr[PER8];
-  unsigned ksb[PER8], vsb[PER8];
+  unsigned ksb[PER8], vsb[PER8];               // words of four scales, the row's among them
   auto load8 = [&](int j, auto whole_tag, unsigned bad) {
     constexpr bool WHOLE = decltype(whole_tag)::value;
     const int at = (j & (WIN - 1)) * BLOCKS;
 #pragma unroll
     for (int n = 0; n < PER8; ++n) {
-      const int bl = (wave + n * NW) / IPB8, i = n % SUBS, r = block_row8(i);
+      const int bl = (wave + n * NW) / IPB8, i = n % SUBS, rk = key_row8(i), rv = value_row8(i);
       const unsigned long long kb = lane64(kwin, at + bl), vb = lane64(vwin, at + bl), sb = lane64(swin, at + bl);
       auto get = [&] {
         kr[n] = *(global_u32x4*)(kb + koff[i]);
+        ksb[n] = *(global_u32*)(sb + (unsigned)(rk & ~3));
+      };
+      auto get_v = [&] {
         vr[n] = *(global_u32x4*)(vb + voff[i]);
-        ksb[n] = *(global_u8*)(sb + (unsigned)r);
-        vsb[n] = *(global_u8*)(sb + a.s_kind + (unsigned)r);
+        vsb[n] = *(global_u32*)(sb + a.s_kind + (unsigned)(rv & ~3));
       };
       if constexpr (WHOLE) {
         get();
+        get_v();
       } else {
+        const int left = bad >> bl & 1 ? 0 : key1 - key_of(j) - 16 * bl;
         kr[n] = vr[n] = (gr_u32x4){0, 0, 0, 0};
         ksb[n] = vsb[n] = 0;
-        if (!(bad >> bl & 1) && key_of(j) + 16 * bl + r < key1) get();
+        if (rk < left) get();
+        if (rv < left) get_v();
       }
     }
   };
@@ -506,15 +517,18 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
 #pragma unroll
     for (int n = 0; n < PER8; ++n) {
       const int bl = (wave + n * NW) / IPB8, i = n % SUBS;
-      auto put = [&](char* base, int at, gr_u32x4 w, unsigned sb) {
-        const float f = gr_e8m0(sb);
+      // (scales taken here: what is made of a loaded word alone would go up to the load, in
+      // the tile before, and its wait with it)
+      asm volatile("" : "+v"(ksb[n]), "+v"(vsb[n]));
+      auto put = [&](char* base, int at, gr_u32x4 w, unsigned sb, int r) {
+        const float f = gr_e8m0_of(sb, 8 * (r & 3));
         gr_st16(base + at, (gr_u32x4){gr_from_e4m3<T, false>(w[0], f), gr_from_e4m3<T, true>(w[0], f),
                                       gr_from_e4m3<T, false>(w[1], f), gr_from_e4m3<T, true>(w[1], f)});
         gr_st16(base + (at ^ 16), (gr_u32x4){gr_from_e4m3<T, false>(w[2], f), gr_from_e4m3<T, true>(w[2], f),
                                              gr_from_e4m3<T, false>(w[3], f), gr_from_e4m3<T, true>(w[3], f)});
       };
-      put(ks0 + slot * L::TILE + bl * (16 * D * 2), kdst[i], kr[n], ksb[n]);
-      put(vt0 + slot * L::TILE + bl * (16 * D * 2), vdst[i], vr[n], vsb[n]);
+      put(ks0 + slot * L::TILE + bl * (16 * D * 2), kdst[i], kr[n], ksb[n], key_row8(i));
+      put(vt0 + slot * L::TILE + bl * (16 * D * 2), vdst[i], vr[n], vsb[n], value_row8(i));
     }
   };
 
@@ -526,7 +540,7 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
 
   // One tile's scores, softmax and P V. MASKED: some row may not see all of its
   // keys (bad: 16-key blocks of no page, a bit each).
-  auto tile = [&](int j, int slot, unsigned bad, auto masked_tag) {
+  auto tile = [&](int j, int slot, unsigned bad, auto masked_tag, auto next) {
     constexpr bool MASKED = decltype(masked_tag)::value;
     const int k0 = key_of(j);
     const int ka = kbase + slot * L::TILE, va = vbase + slot * L::TILE;
@@ -536,7 +550,7 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
       gr_u32x4 r;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const char* p = vt0 + (va ^ (db * 64)) + (16 * x + 4 * h) * (D * 2);
+        const char* p = vt0 + (va ^ (db * 64 + (Q8 ? 16 * h : 0))) + (16 * x + 4 * h) * (D * 2);
         const v4s v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(__attribute__((address_space(3))) char*)(char*)p);
         const gr_u32x2 w = __builtin_bit_cast(gr_u32x2, v);
         r[2 * h] = w[0];
@@ -553,6 +567,7 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
       for (int kb = 0; kb < KB; ++kb) {
         s[kb] = MF::mma32(gr_as<vec8>(gr_ld16(ks0 + (ka ^ (ds * 32)) + kb * 32 * (D * 2))), qf[ds], s[kb]);
       }
+    next();
     bool fresh = m == -GR_INF;                                // no base yet, and a key to take it from
     if constexpr (MASKED) {
       // element r of key block kb is key k0 + 32 kb + 16 (r / 8) + 8 g + r % 8
@@ -656,7 +671,8 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
 #pragma unroll
               for (int r = 0; r < 16; ++r) {
                 const int d = db * 32 + 8 * (r >> 2) + 4 * g + (r & 3);
-                const float v = (float)*reinterpret_cast<const T*>(vr + gr_swz_tr<CPR>(key, d >> 3) * 16 + (d & 7) * 2);
+                const int chunk = Q8 ? gr_swz_v8<CPR>(key, d >> 3) : gr_swz_tr<CPR>(key, d >> 3);
+                const float v = (float)*reinterpret_cast<const T*>(vr + chunk * 16 + (d & 7) * 2);
                 if (vis) o[db][r] = fmaf(pv, v, o[db][r]);
                 if ((r & 3) == 3) __builtin_amdgcn_sched_barrier(0);   // (all reads at once would spill)
               }
@@ -775,16 +791,44 @@ __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* l
   // row's keys): two loops, for a join of both kinds in one made the compiler
   // copy the accumulators in every tile. The iterations' barriers are alike.
   const int nclean = wave_live ? gr_imin(nwhole, tiles_before(lim_lo + 1)) : 0;
+  auto nothing = [] {};
+  if constexpr (Q8) {
+    // of the former, those before a plain tile have its loads, and the conversion of
+    // the tile between, behind the scores' products
 #pragma unroll 1
-  for (; j < nclean && !uneven; ++j) {
-    enter(j);
-    tile(j, slot, 0u, gr_ic<0>{});
-    slot = slot + 1 == NS ? 0 : slot + 1;
+    while (j < nclean && !uneven) {
+#pragma unroll 1
+      for (; j < nclean && asked < plain && !uneven; ++j) {
+        barrier();
+        tile(j, slot, 0u, gr_ic<0>{}, [&] {
+          store8(to);
+          ++stored;
+          to ^= 1;
+          load8(asked, gr_ic<1>{}, 0u);
+          bads <<= BLOCKS;
+          ++asked;
+        });
+        slot ^= 1;
+      }
+#pragma unroll 1
+      for (; j < nclean && asked >= plain && !uneven; ++j) {
+        enter(j);
+        tile(j, slot, 0u, gr_ic<0>{}, nothing);
+        slot ^= 1;
+      }
+    }
+  } else {
+#pragma unroll 1
+    for (; j < nclean && !uneven; ++j) {
+      enter(j);
+      tile(j, slot, 0u, gr_ic<0>{}, nothing);
+      slot = slot + 1 == NS ? 0 : slot + 1;
+    }
   }
 #pragma unroll 1
   for (; j < niter; ++j) {
     enter(j);
-    if (wave_live && j < ntile && key_of(j) <= lim_hi) tile(j, slot, bad_at(j), gr_ic<1>{});
+    if (wave_live && j < ntile && key_of(j) <= lim_hi) tile(j, slot, bad_at(j), gr_ic<1>{}, nothing);
     slot = slot + 1 == NS ? 0 : slot + 1;
   }
 

@@ -43,8 +43,10 @@ inline int check_paged(const gr_paged_cache* c, const gr_paged_batch* b, const c
 // The scales of a quantised cache, whose rows are bytes.
 inline int check_scales(const gr_paged_cache* c, const gr_paged_scales* s, const char* who) {
   if (!s->scales) return fail(GR_E_ARG, "%s: null argument (scales)", who);
+  if (!aligned16(s->scales)) return fail(GR_E_ARG, "%s: base pointers must be 16-byte aligned (scales)", who);
   for (int i = 0; i < 3; ++i) {
-    if (s->strides[i] < 0) return fail(GR_E_ARG, "%s: strides must be non-negative (scales)", who);
+    if (s->strides[i] < 0 || s->strides[i] % 16)
+      return fail(GR_E_ARG, "%s: strides must be non-negative multiples of 16 (scales)", who);
     if (c->k_strides[i] % 16 || c->v_strides[i] % 16)
       return fail(GR_E_ARG, "%s: strides must be multiples of 16 elements (quantised cache)", who);
   }

@@ -135,7 +135,7 @@ template <class T, int D, bool Q8>
 int launch(const gr_paged_args& a, const Plan& p, hipStream_t st) {
   constexpr int KGS = Q8 || D == 64 ? 4 : 2;
   if constexpr (Q8) {
-    if (p.nw == 0) return a.shares ? launch_shared<T, D, 64, 0, 4, 1, 0, Q8>(a, st) : launch_alone<T, D, 32, 0, 4, 1, 0, Q8>(a, st);
+    if (p.nw == 0) return a.shares ? launch_shared<T, D, 32, 0, 4, 1, 0, Q8>(a, st) : launch_alone<T, D, 32, 0, 4, 1, 0, Q8>(a, st);
   }
   if (p.nw == 1) return a.shares ? launch_shared<T, D, 32, 1, 4, 2, 0, Q8>(a, st) : launch_alone<T, D, 32, 1, 4, 2, 0, Q8>(a, st);
   if (p.nw == 2) return a.shares ? launch_shared<T, D, 32, 2, 4, 2, 0, Q8>(a, st) : launch_alone<T, D, 32, 2, 4, 2, 0, Q8>(a, st);

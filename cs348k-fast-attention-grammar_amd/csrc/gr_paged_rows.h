@@ -73,16 +73,17 @@ __device__ __forceinline__ void gr_paged_rows(const gr_paged_args& a, char* lds_
 
   // offsets: a key's row in the cache; values' rows there and in LDS; transposing reads
   const unsigned koff = (unsigned)(l16 * a.k_ss) + g * 16;
+  auto vrow = [&](int i) { return gr_value8<D>(lane) + i * (64 / CPR8); };
   unsigned voff[VI];
   int vdst[VI];
 #pragma unroll
   for (int i = 0; i < VI; ++i) {
-    const int r = lane / CPR8 + i * (64 / CPR8), c8 = lane % CPR8;
+    const int r = vrow(i), c8 = gr_piece8<D>(lane);
     voff[i] = (unsigned)(r * a.v_ss) + c8 * 16;
-    vdst[i] = r * (D * 2) + gr_swz_tr<CPR>(r, 2 * c8) * 16;
+    vdst[i] = r * (D * 2) + gr_swz_v8<CPR>(r, 2 * c8) * 16;
   }
   const int trow = 4 * g + ((lane >> 2) & 3), tcol = 4 * (lane & 3);
-  const int tbase = trow * (D * 2) + gr_swz_tr<CPR>(trow, tcol >> 3) * 16 + (tcol & 7) * 2;
+  const int tbase = trow * (D * 2) + gr_swz_v8<CPR>(trow, tcol >> 3) * 16 + (tcol & 7) * 2;
   const int smask = (1 << a.page_shift) - 1;
   const int* const tab = a.table + t.b * a.table_stride;
   const unsigned char* const kp = static_cast<const unsigned char*>(a.k) + hk * a.k_sh;
@@ -111,38 +112,46 @@ __device__ __forceinline__ void gr_paged_rows(const gr_paged_args& a, char* lds_
   };
 
   typedef const __attribute__((address_space(1))) gr_u32x4 global_u32x4;
-  typedef const __attribute__((address_space(1))) unsigned char global_u8;
+  typedef const __attribute__((address_space(1))) unsigned global_u32;
   gr_u32x4 kr[KB][KL], vr[KB][VI];
-  unsigned ksb[KB], vsb[KB][VI];
-  // Asks for tile j; rows that are not there are zeros.
-  auto load = [&](int j, auto whole_tag, unsigned bad) {
+  unsigned ksb[KB], vsb[KB][VI];               // words of four scales, the row's among them
+  const int kshift = 8 * (l16 & 3);
+  auto vshift = [&](int i) { return 8 * (vrow(i) & 3); };
+  // Asks for tile j's keys and values; rows that are not there are zeros.
+  auto load_k = [&](int j, auto whole_tag, unsigned bad) {
     constexpr bool WHOLE = decltype(whole_tag)::value;
     const int at = (j & (WIN - 1)) * KB;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
-      const unsigned long long k0 = lane64(kwin, at + kb), v0 = lane64(vwin, at + kb), s0 = lane64(swin, at + kb);
-      const int left = key1 - key_of(j) - 16 * kb;            // keys of the block that are there
-      const bool ok = !(bad >> kb & 1);
+      const unsigned long long k0 = lane64(kwin, at + kb), s0 = lane64(swin, at + kb);
       if (!WHOLE) {
         ksb[kb] = 0;
 #pragma unroll
         for (int i = 0; i < KL; ++i) kr[kb][i] = (gr_u32x4){0, 0, 0, 0};
       }
-      if (WHOLE || (ok && l16 < left)) {
+      if (WHOLE || (!(bad >> kb & 1) && l16 < key1 - key_of(j) - 16 * kb)) {
 #pragma unroll
         for (int i = 0; i < KL; ++i) kr[kb][i] = *(global_u32x4*)(k0 + koff + 64 * i);
-        ksb[kb] = *(global_u8*)(s0 + (unsigned)l16);
+        ksb[kb] = *(global_u32*)(s0 + (unsigned)(l16 & ~3));
       }
+    }
+  };
+  auto load_v = [&](int j, auto whole_tag, unsigned bad) {
+    constexpr bool WHOLE = decltype(whole_tag)::value;
+    const int at = (j & (WIN - 1)) * KB;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      const unsigned long long v0 = lane64(vwin, at + kb), s0 = lane64(swin, at + kb);
 #pragma unroll
       for (int i = 0; i < VI; ++i) {
-        const int r = lane / CPR8 + i * (64 / CPR8);
+        const int r = vrow(i);
         if (!WHOLE) {
           vsb[kb][i] = 0;
           vr[kb][i] = (gr_u32x4){0, 0, 0, 0};
         }
-        if (WHOLE || (ok && r < left)) {
+        if (WHOLE || (!(bad >> kb & 1) && r < key1 - key_of(j) - 16 * kb)) {
           vr[kb][i] = *(global_u32x4*)(v0 + voff[i]);
-          vsb[kb][i] = *(global_u8*)(s0 + a.s_kind + (unsigned)r);
+          vsb[kb][i] = *(global_u32*)(s0 + a.s_kind + (unsigned)(r & ~3));
         }
       }
     }
@@ -160,65 +169,28 @@ __device__ __forceinline__ void gr_paged_rows(const gr_paged_args& a, char* lds_
     base[rb] = shift;
   }
 
-  // Tiles are asked for in order; up to `plain` they are whole, in the window, and
-  // their pages exist.
+  // Tiles are asked for in order, keys and then values; those up to `plain` are
+  // whole, in the window, and their pages exist.
+  constexpr unsigned BLOCKS = (1u << KB) - 1;
   int asked = 0, plain = 0, nwhole = 0;
-  unsigned long long bads = 0;                // bad blocks of the last tiles asked for, newest first
-  bool uneven = false;                        // whether one of them had some: all behind it are masked
-  auto ask = [&]() {
-    if (asked < plain) {
-      load(asked, gr_ic<1>{}, 0u);
-      bads <<= KB;
-    } else {
-      if (asked >= ntile) return;
-      if (asked > 0 && (asked & (WIN - 1)) == 0) refill(asked, id_of(asked));
-      const unsigned bad = (unsigned)(badwin >> ((asked & (WIN - 1)) * KB)) & ((1u << KB) - 1);
-      bads = bads << KB | bad;
-      if (bad == 0 && asked < nwhole) {
-        load(asked, gr_ic<1>{}, 0u);
-      } else {
-        load(asked, gr_ic<0>{}, bad);
-        uneven = true;
-      }
-      plain = badwin == 0 ? gr_imin(nwhole, (asked & ~(WIN - 1)) + WIN) : 0;
-    }
-    ++asked;
+  unsigned bad = 0;                           // bad blocks of the tile asked for last
+  auto ask_k = [&]() {
+    if (asked >= ntile) return;
+    if (asked > 0 && (asked & (WIN - 1)) == 0) refill(asked, id_of(asked));
+    bad = (unsigned)(badwin >> ((asked & (WIN - 1)) * KB)) & BLOCKS;
+    load_k(asked, gr_ic<0>{}, bad);
+    plain = badwin == 0 ? gr_imin(nwhole, (asked & ~(WIN - 1)) + WIN) : 0;
+  };
+  auto ask_v = [&]() {
+    if (asked < ntile) load_v(asked++, gr_ic<0>{}, bad);
   };
 
-  auto tile = [&](int j, auto masked_tag) {
-    constexpr bool MASKED = decltype(masked_tag)::value;
+  // One tile, and the loads of the next one as its registers become free. MASKED: any
+  // tile, else one that every row sees in full. PLAIN: the next one is.
+  auto tile = [&](int j, auto masked_tag, auto plain_tag) {
+    constexpr bool MASKED = decltype(masked_tag)::value, PLAIN = decltype(plain_tag)::value;
     const int k0 = key_of(j);
-    const unsigned bad = MASKED ? (unsigned)(bads >> ((asked - 1 - j) * KB)) & ((1u << KB) - 1) : 0u;
-    // values to LDS (the slot's last reads came before in this wave's order)
-    unsigned long long odd = 0;               // MASKED: keys with a value that is not finite
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-      for (int i = 0; i < VI; ++i) {
-        const float f = gr_e8m0(vsb[kb][i]);
-        gr_u32x4 w[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          w[h] = (gr_u32x4){gr_from_e4m3<T, false>(vr[kb][i][2 * h], f), gr_from_e4m3<T, true>(vr[kb][i][2 * h], f),
-                            gr_from_e4m3<T, false>(vr[kb][i][2 * h + 1], f), gr_from_e4m3<T, true>(vr[kb][i][2 * h + 1], f)};
-        if constexpr (MASKED) {
-          constexpr unsigned EXP = HALF ? 0x7c007c00u : 0x7f807f80u, ONE = HALF ? 0x04000400u : 0x00800080u;
-          gr_u32x4 x = ((w[0] & EXP) + ONE) | ((w[1] & EXP) + ONE);
-          unsigned long long who = __builtin_amdgcn_ballot_w64(((x[0] | x[1] | x[2] | x[3]) & 0x80008000u) != 0);
-          if (__builtin_expect(who != 0, 0)) {
-            bool row_odd = false;
-#pragma unroll 1
-            for (int r = 0; r < 64 / CPR8; ++r, who >>= CPR8)
-              if (who & ((1ull << CPR8) - 1)) {
-                odd |= 1ull << (16 * kb + i * (64 / CPR8) + r);
-                row_odd |= lane / CPR8 == r;
-              }
-            if (row_odd) w[0] = w[1] = (gr_u32x4){0, 0, 0, 0};   // taken out of the product
-          }
-        }
-        gr_st16(vt + kb * (16 * D * 2) + vdst[i], w[0]);
-        gr_st16(vt + kb * (16 * D * 2) + (vdst[i] ^ 16), w[1]);
-      }
+    const unsigned mine = bad;
     gr_f32x4 s[RB][KB];
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb)
@@ -226,7 +198,10 @@ __device__ __forceinline__ void gr_paged_rows(const gr_paged_args& a, char* lds_
       for (int kb = 0; kb < KB; ++kb) s[rb][kb] = (gr_f32x4)(0.f);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
-      const float f = gr_e8m0(ksb[kb]);
+      // (taken here: what is made of a loaded word alone would go up to the load, in the
+      // tile before, and its wait with it)
+      asm volatile("" : "+v"(ksb[kb]));
+      const float f = gr_e8m0_of(ksb[kb], kshift);
 #pragma unroll
       for (int ds = 0; ds < DS; ++ds) {
         const gr_u32x4 r = kr[kb][ds >> 1];
@@ -237,7 +212,41 @@ __device__ __forceinline__ void gr_paged_rows(const gr_paged_args& a, char* lds_
         for (int rb = 0; rb < RB; ++rb) s[rb][kb] = MF::mma16(kf, qf[rb][ds], s[rb][kb]);
       }
     }
-    ask();                                    // the next tile's bytes take this one's registers
+    if constexpr (!PLAIN) ask_k();
+    else load_k(asked, gr_ic<1>{}, 0u);
+    // values to LDS (the slot's last reads came before in this wave's order)
+    unsigned long long odd = 0;               // MASKED: keys with a value that is not finite
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int i = 0; i < VI; ++i) {
+        asm volatile("" : "+v"(vsb[kb][i]));
+        const float f = gr_e8m0_of(vsb[kb][i], vshift(i));
+        gr_u32x4 w[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          w[h] = (gr_u32x4){gr_from_e4m3<T, false>(vr[kb][i][2 * h], f), gr_from_e4m3<T, true>(vr[kb][i][2 * h], f),
+                            gr_from_e4m3<T, false>(vr[kb][i][2 * h + 1], f), gr_from_e4m3<T, true>(vr[kb][i][2 * h + 1], f)};
+        if constexpr (MASKED) {
+          constexpr unsigned EXP = HALF ? 0x7c007c00u : 0x7f807f80u, ONE = HALF ? 0x04000400u : 0x00800080u;
+          gr_u32x4 x = ((w[0] & EXP) + ONE) | ((w[1] & EXP) + ONE);
+          const bool mine = ((x[0] | x[1] | x[2] | x[3]) & 0x80008000u) != 0;
+          if (__builtin_expect(gr_any(mine), 0)) {
+            bool row_odd = false;
+#pragma unroll 1
+            for (int r = 0; r < 16; ++r)      // (rows of this instruction: some of the 16)
+              if (gr_any(mine && vrow(i) == r)) {
+                odd |= 1ull << (16 * kb + r);
+                row_odd |= vrow(i) == r;
+              }
+            if (row_odd) w[0] = w[1] = (gr_u32x4){0, 0, 0, 0};   // taken out of the product
+          }
+        }
+        gr_st16(vt + kb * (16 * D * 2) + vdst[i], w[0]);
+        gr_st16(vt + kb * (16 * D * 2) + (vdst[i] ^ 16), w[1]);
+      }
+    if constexpr (!PLAIN) ask_v();
+    else load_v(asked++, gr_ic<1>{}, 0u);
     vec8 pt[RB][KB / 2];
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
@@ -248,7 +257,7 @@ __device__ __forceinline__ void gr_paged_rows(const gr_paged_args& a, char* lds_
         bool sees = false;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
-          const int d = (bad >> kb) & 1 ? -1 : delta - 16 * kb;
+          const int d = (mine >> kb) & 1 ? -1 : delta - 16 * kb;
           sees |= d >= 0;
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[rb][kb][e] = e <= d ? s[rb][kb][e] : -GR_INF;
@@ -356,17 +365,22 @@ __device__ __forceinline__ void gr_paged_rows(const gr_paged_args& a, char* lds_
 #pragma unroll
     for (int ds = 0; ds < DS; ++ds) qf[rb][ds] = gr_as<vec8>(gr_ld16(qp + 64 * (ds >> 1) + 16 * g + 8 * (ds & 1)));
   }
-  // Leading tiles of the wave that end before key `end`.
+  // leading tiles of the wave that end before key `end`.
   auto tiles_before = [&](int end) { return end - key0 < (kg + 1) * BN ? 0 : ((end - key0) / BN - kg + KG - 1) / KG; };
   nwhole = gr_imin(ntile, tiles_before(key1));
   if (ntile > 0) refill(0, first_id);
-  ask();
+  ask_k();
+  ask_v();
   const int nclean = gr_imin(nwhole, tiles_before(lim_lo + 1));
   int j = 0;
 #pragma unroll 1
-  for (; j < nclean && !uneven; ++j) tile(j, gr_ic<0>{});
+  while (j < nclean && bad == 0) {
 #pragma unroll 1
-  for (; j < ntile; ++j) tile(j, gr_ic<1>{});
+    for (; j < nclean && asked < plain && bad == 0; ++j) tile(j, gr_ic<0>{}, gr_ic<1>{});
+    if (j < nclean && bad == 0) tile(j++, gr_ic<0>{}, gr_ic<0>{});
+  }
+#pragma unroll 1
+  for (; j < ntile; ++j) tile(j, gr_ic<1>{}, gr_ic<0>{});
 
   if constexpr (KG > 1) {
     // the waves' partials through LDS: O as RB DB quads of floats per lane, then

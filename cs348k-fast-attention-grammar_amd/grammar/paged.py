@@ -78,7 +78,8 @@ class QuantizedPagedCache:
     """Key and value pages of 8-bit rows: k and v torch.float8_e4m3fn [pages, heads,
     page_size, D], as PagedCache's but with strides that are multiples of 16;
     scales torch.float8_e8m0fnu [pages, heads, 2, page_size], a power of two for each
-    key's (index 0) and value's (1) row, unit stride along the slots. dtype: fp16 or
+    key's (index 0) and value's (1) row, unit stride along the slots, other strides
+    multiples of 16. dtype: fp16 or
     bf16, the tokens'.
 
     A row x is held as round(x / scale), scale the least power of two (2^-127 at

@@ -342,8 +342,8 @@ int gr_paged_append(const gr_paged_cache* cache, const gr_paged_batch* batch, co
 /* The scales of a quantised cache. Its k and v hold bytes (e4m3: four significant
  * bits, at most 448) by strides that are multiples of 16, and its dtype is that of the
  * tokens, GR_F16 or GR_BF16. scales: bytes [pages][heads][2: key, value][page_size] by
- * strides {page, head, key to value}, unit stride along the slots, each b standing for 2^(b - 127),
- * or NaN for 255 (E8M0). A row stands for its numbers times its scale, which
+ * strides {page, head, key to value} that are non-negative multiples of 16, unit stride
+ * along the slots, 16-byte aligned, each b standing for 2^(b - 127), or NaN for 255 (E8M0). A row stands for its numbers times its scale, which
  * are numbers of the tokens' type. */
 typedef struct gr_paged_scales {
   void* scales;

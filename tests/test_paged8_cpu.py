@@ -44,9 +44,14 @@ def test_bad_scales_are_refused():
         assert call() == rt.GR_E_ARG and "null" in rt.last_error()
     for i in range(3):
         scales = _scales(d, rt)
-        scales.strides[i] = -1
-        for call in _calls(rt, d, cache, scales, batch, spec):
-            assert call() == rt.GR_E_ARG and "strides" in rt.last_error()
+        for bad in (-16, 8):
+            scales.strides[i] = bad
+            for call in _calls(rt, d, cache, scales, batch, spec):
+                assert call() == rt.GR_E_ARG and "strides" in rt.last_error()
+    scales = _scales(d, rt)
+    scales.scales += 8
+    for call in _calls(rt, d, cache, scales, batch, spec):
+        assert call() == rt.GR_E_ARG and "aligned" in rt.last_error()
     scales = _scales(d, rt)
     for i, (s, keep) in enumerate(((4104, 4096), (1032, 1024), (72, 64))):      # multiples of 8, not of 16
         for strides in (cache.k_strides, cache.v_strides):
