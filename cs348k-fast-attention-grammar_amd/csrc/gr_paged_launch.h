@@ -50,7 +50,7 @@ __global__ __launch_bounds__(256) void gr_paged_merge_kernel(gr_paged_args a) {
 struct Plan {
   int nw;                        // waves of 32 rows
   long long tiles;               // row tiles of a key head
-  int groups;                    // key groups of a tile of 128 rows
+  int groups;                    // key groups of a tile of 128 rows, or (quantised) of 16
   int shares;                    // 0: a workgroup a tile
 };
 
@@ -61,7 +61,7 @@ inline Plan plan_of(const gr_paged_cache& c, const gr_paged_batch& b, int Hq, bo
   const int cus = gr::cu_count() > 0 ? gr::cu_count() : 256;
   const long long cap = (long long)b.width * c.page_size;
   const long long len = b.max_len > 0 && b.max_len < cap ? b.max_len : cap;
-  p.nw = q8 && most * G <= 16 ? 0 : most * G <= 32 ? 1 : most * G <= 64 ? 2 : 4;
+  p.nw = most * G <= 32 ? 1 : most * G <= 64 ? 2 : 4;
   // Chunks whose tiles of 128 rows would leave most CUs idle take tiles of 64
   // with four key groups: 16 or 64 tiles (one chunk of 512, 4 key heads, G 1 or 4)
   // at 512 keys 13.0 us to 9.4 and 13.0 to 9.8 (D 64), 18.1 to 13.4 and 18.5 to
@@ -69,6 +69,16 @@ inline Plan plan_of(const gr_paged_cache& c, const gr_paged_batch& b, int Hq, bo
   // 128 (16 tiles, 2,048 keys 30 to 22 us, 64 tiles, 8,192 keys 62 to 71).
   const long long rows128 = (b.starts ? (long long)b.rows : (long long)b.B * b.rows) * G / 128 * c.heads;
   if (p.nw == 4 && (len <= 1000 ? 4 * rows128 <= cus : D == 128 && 4 * rows128 < cus)) p.nw = 2;
+  if (q8) {
+    // One wave's 16 rows where a sequence has no more (one token of 4 heads to a key head,
+    // 64 contexts of 200-11,000 keys: 132 us, in tiles of 32 rows 167); else 32 up to
+    // 64 rows (4 key heads' worth of 50 rows, 900-9,000 keys 64 us to 45), and for chunks
+    // whose tiles of 32 are at most three a CU, over long contexts at D 128 only: one chunk of
+    // 512 tokens (512 tiles), 800 keys 25 us to 18, 3,000 58 to 41, 8,000 106 to 101 (D 64: 17
+    // to 13, 38 to 28, 63 to 69); 768 tokens, 2,000 keys 50 to 45; 1,000 tokens level.
+    const long long wgs32 = (b.starts ? (long long)b.rows * G / 32 + b.B : (long long)b.B * (((long long)b.rows * G + 31) / 32)) * c.heads;
+    p.nw = most * G <= 16 ? 0 : most * G <= 64 || (wgs32 <= 3LL * cus && (D == 128 || len <= 6000)) ? 1 : 4;
+  }
   const int BM = gr_paged_rows_of(p.nw);
   // packed rows: every sequence may have a part-filled tile
   p.tiles = b.starts ? (long long)b.rows * G / BM + b.B : (long long)b.B * (((long long)b.rows * G + BM - 1) / BM);
@@ -81,6 +91,10 @@ inline Plan plan_of(const gr_paged_cache& c, const gr_paged_batch& b, int Hq, bo
   // to 27.0).
   const long long wgs = p.tiles * c.heads;
   p.groups = p.nw == 4 && rows128 <= cus && 4 * wgs <= 7LL * cus ? 2 : 1;
+  // Tiles of 16 rows, at most one a CU: eight waves share out the keys where they have
+  // two steps each (16 sequences, 16 heads of 64, 300-1,000 keys 8.7 us to 7.8, 60-130
+  // level; 320 tiles, 300-1,000 keys of 128, 17.4 to 19.5).
+  if (p.nw == 0) p.groups = wgs <= cus && len > 256 ? 8 : 4;
   // Work is shared out from a length on that grows with the workgroups that one a
   // tile would make: in brackets shared / a workgroup a tile, lengths spread by a
   // half around the mean. One token, D 128: 64 tiles, mean 600 keys 13.8 / 15.5 us,
@@ -98,7 +112,14 @@ inline Plan plan_of(const gr_paged_cache& c, const gr_paged_batch& b, int Hq, bo
     slope = p.groups == 1 ? 6500 : D == 64 ? 12500 : 8000;
     can = p.groups == 1 ? wgs < resident : 4 * wgs < 3LL * cus;
   }
-  const double from = slope * fill > least ? slope * fill : least;
+  double from = slope * fill > least ? slope * fill : least;
+  // Tiles of 16 and 32 rows over a quantised cache (a workgroup a tile / shared): 16, D 128,
+  // 32 tiles, lengths up to 1,500 keys 12.0 / 14.6 us, 3,000 18.4 / 15.0; 128 tiles, 3,000
+  // 20.0 / 20.4, 6,000 43 / 32; 256 tiles, 3,000 30.0 / 32.6; D 64, 64 tiles, 3,000 12.0 / 12.7, 6,000
+  // 17.3 / 16.0; 256 tiles, 6,000 28.9 / 30.4. 32, D 128, 64 tiles, 1,500 17.6 / 17.8, 3,000 27 / 19;
+  // 192 tiles, 1,500 19.2 / 23.5, 3,000 35 / 31; D 64, 128 tiles, 3,000 17.7 / 18.8, 6,000 30 / 23.
+  if (q8 && p.nw == 0) from = D == 64 ? 3700 + 6500 * fill : 2000 + 4300 * fill;
+  if (q8 && p.nw == 1) from = D == 64 ? 2300 + 4000 * fill : 1450 + 2000 * fill;
   const bool shared = can && (double)len > from && wgs * (cap / 64 + 1 + GR_PAGED_COST) <= 0x7fffffffLL;
   p.shares = !shared ? 0 : resident < GR_PAGED_MAX_SHARES ? resident : GR_PAGED_MAX_SHARES;
   return p;
@@ -133,12 +154,17 @@ int launch_shared(const gr_paged_args& a, hipStream_t st) {
 
 template <class T, int D, bool Q8>
 int launch(const gr_paged_args& a, const Plan& p, hipStream_t st) {
-  constexpr int KGS = Q8 || D == 64 ? 4 : 2;
   if constexpr (Q8) {
-    if (p.nw == 0) return a.shares ? launch_shared<T, D, 32, 0, 4, 1, 0, Q8>(a, st) : launch_alone<T, D, 32, 0, 4, 1, 0, Q8>(a, st);
+    if (p.nw == 0) {
+      if (a.shares) return launch_shared<T, D, 32, 0, 4, 1, 0, true>(a, st);
+      return p.groups == 8 ? launch_alone<T, D, 32, 0, 8, 1, 0, true>(a, st) : launch_alone<T, D, 32, 0, 4, 1, 0, true>(a, st);
+    }
+    if (p.nw == 1) return a.shares ? launch_shared<T, D, 32, 1, 4, 1, 0, true>(a, st) : launch_alone<T, D, 32, 1, 4, 1, 0, true>(a, st);
+  } else {
+    if (p.nw == 1) return a.shares ? launch_shared<T, D, 32, 1, 4, 2, 0, false>(a, st) : launch_alone<T, D, 32, 1, 4, 2, 0, false>(a, st);
+    if (p.nw == 2) return a.shares ? launch_shared<T, D, 32, 2, 4, 2, 0, false>(a, st) : launch_alone<T, D, 32, 2, 4, 2, 0, false>(a, st);
   }
-  if (p.nw == 1) return a.shares ? launch_shared<T, D, 32, 1, 4, 2, 0, Q8>(a, st) : launch_alone<T, D, 32, 1, 4, 2, 0, Q8>(a, st);
-  if (p.nw == 2) return a.shares ? launch_shared<T, D, 32, 2, 4, 2, 0, Q8>(a, st) : launch_alone<T, D, 32, 2, 4, 2, 0, Q8>(a, st);
+  constexpr int KGS = Q8 || D == 64 ? 4 : 2;
   // (keys 32 a step in two groups at D 128: two rings of 64 would take a CU's LDS)
   if (a.shares) return launch_shared<T, D, 64, 4, 1, 2, KGS, Q8>(a, st);
   if (p.groups == 2) return launch_alone<T, D, D == 64 ? 64 : 32, 4, 2, 2, 4, Q8>(a, st);
