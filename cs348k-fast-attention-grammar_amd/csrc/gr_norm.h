@@ -4,12 +4,14 @@
 // y = R(t) n, n = w x r, r = 1 / sqrt(mean x^2 + eps). With g = R(-t) dy:
 //   dw = sum over rows of g x r,   dx = r (g w - x r^2 mean(g w x)).
 //
-// Layout: as gr_rope_body, a wave takes ITER passes over a token's head rows; lane l
-// has the same unit of 8 + 8 elements in every pass and token, so that it sums the
-// weights' gradients of its elements over all its rows in registers. r is computed
-// again from x, which the gradient reads in any case. At its end a
-// workgroup adds its waves' sums and writes them beside the others'; a second launch adds
-// those up, in the order of the workgroups.
+// Layout: as gr_rope_body, a wave takes a token's head rows in passes (all of them, or
+// `per` where tokens are few), and then those of other tokens; lane l has the same unit of 8 + 8
+// elements in every pass and token, so that it sums the weights' gradients of
+// its elements over all its rows in registers. r is computed again from x, which the
+// gradient reads in any case. The rows of the next pass are on their way while
+// one is worked on, and passes of one kind of rows make no choice of weights or sums. At its
+// end a workgroup adds its waves' sums and writes them beside the others'; a second launch
+// adds those up, in the order of the workgroups.
 #pragma once
 #include "gr_rotary.h"
 
@@ -25,18 +27,20 @@ struct gr_norm_bwd_args {
   const void *wq, *wk;
   int w32;
   float eps;
+  int per;                       // passes of a token that a wave takes
   float* part;                   // [workgroup][2][D], or nullptr: no weights' gradients
 };
 
 constexpr int GR_NORM_WAVES = 4;
+template <int V> struct gr_const { static constexpr int value = V; };
 
-template <class T, bool INTER, int ITER>
+template <class T, bool INTER>
 __device__ __forceinline__ void gr_norm_bwd_body(const gr_norm_bwd_args& a, float* lds) {
   const int lane = threadIdx.x & 63;
   const int wave_in = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int units = a.D >> 4, lanes = gr_row_lanes(units), rpp = 64 / lanes;
   const int h0 = a.q.heads, rows = h0 + a.k.heads;
-  const int passes = (rows + rpp - 1) / rpp, groups = (passes + ITER - 1) / ITER;
+  const int passes = (rows + rpp - 1) / rpp, groups = (passes + a.per - 1) / a.per;
   const int u = lane & (lanes - 1), ru = a.pairs >> 3;
   const bool unit = u < units;
   const int u0 = unit ? u : 0;
@@ -47,71 +51,118 @@ __device__ __forceinline__ void gr_norm_bwd_body(const gr_norm_bwd_args& a, floa
   gr_unit_weights<T>(a.wk, a.w32, lo, hi, wk);
   const float inv_d = 1.0f / (float)a.D;
 
-  const long long tasks = (long long)a.tokens * groups;
-#pragma unroll 1
-  for (long long task = (long long)blockIdx.x * GR_NORM_WAVES + wave_in; task < tasks; task += (long long)gridDim.x * GR_NORM_WAVES) {
-    const int tok = (int)(task / groups), grp = (int)(task - (long long)tok * groups);
-    const int row0 = grp * ITER * rpp + lane / lanes;
-    const int b = tok / a.per_seq, i = tok - b * a.per_seq;
-    auto source = [&](const gr_rope_rows& k) { return static_cast<const T*>(k.src) + b * k.sb + i * k.st; };
-    const T *xq = source(a.q), *xk = source(a.k), *yq = source(a.gq), *yk = source(a.gk);
-    gr_rope8<T> x[ITER], y[ITER], gx[ITER], gy[ITER];
-#pragma unroll
-    for (int p = 0; p < ITER; ++p) {
-      const int r = row0 + p * rpp;
-      x[p] = y[p] = gx[p] = gy[p] = {};
-      if (unit && r < rows) {
-        const T* s = r < h0 ? xq + r * a.q.sh : xk + (r - h0) * a.k.sh;
-        const T* d = r < h0 ? yq + r * a.gq.sh : yk + (r - h0) * a.gk.sh;
-        x[p].load(s + lo);
-        y[p].load(s + hi);
-        gx[p].load(d + lo);
-        gy[p].load(d + hi);
-      }
+  // A task is `per` passes of a token.
+  const long long tasks = (long long)a.tokens * groups, step = (long long)gridDim.x * GR_NORM_WAVES;
+  const int sub = lane / lanes;
+  const bool all_units = units == lanes;
+  struct pass_rows {
+    long long task;
+    int pass, b, i;                // of the token's; batch and token
+    gr_rope8<T> x, y, gx, gy;
+  };
+  auto load = [&](pass_rows& d, long long task, int pass) {
+    const int tok = (int)(task / groups), r = pass * rpp + sub;
+    d.task = task;
+    d.pass = pass;
+    d.b = tok / a.per_seq;
+    d.i = tok - d.b * a.per_seq;
+    d.x = d.y = d.gx = d.gy = {};
+    if (unit && r < rows) {
+      auto source = [&](const gr_rope_rows& k, int h) { return static_cast<const T*>(k.src) + d.b * k.sb + d.i * k.st + h * k.sh; };
+      const T* const s = r < h0 ? source(a.q, r) : source(a.k, r - h0);
+      const T* const g = r < h0 ? source(a.gq, r) : source(a.gk, r - h0);
+      d.x.load(s + lo);
+      d.y.load(s + hi);
+      d.gx.load(g + lo);
+      d.gy.load(g + hi);
     }
-    float sn[8] = {}, cs[8] = {};
-    gr_unit_angles(a, a.pos + b * a.ps[1] + i * a.ps[2], 0, u0 < ru ? u0 : 0, lane, true, sn, cs);
-    T *dq = static_cast<T*>(a.q.dst) + b * a.q.db + i * a.q.dt, *dk = static_cast<T*>(a.k.dst) + b * a.k.db + i * a.k.dt;
+  };
+  auto first_pass = [&](long long task) { return (int)(task % groups) * a.per; };
+  // The pass behind d's: of its task, or the first of the wave's next one; false behind the last.
+  auto next = [&](const pass_rows& d, long long& task, int& pass) {
+    task = d.task;
+    pass = d.pass + 1;
+    if (pass < passes && pass - first_pass(task) < a.per) return true;
+    task += step;
+    if (task >= tasks) return false;
+    pass = first_pass(task);
+    return true;
+  };
+  float sn[8] = {}, cs[8] = {};
+  // KIND 0: rows of queries, 1: of keys, all live; 2: any.
+  auto work = [&](const pass_rows& in, auto kind_tag) {
+    constexpr int KIND = decltype(kind_tag)::value;
+    const int r = in.pass * rpp + sub;
+    const bool query = KIND == 2 ? r < h0 : KIND == 0, live = KIND < 2 || (unit && r < rows);
+    auto weight = [&](int e) { return query ? wq[e] : wk[e]; };
+    float f[16], g[16], ss = 0.f, dot = 0.f;
 #pragma unroll
-    for (int p = 0; p < ITER; ++p) {
-      const int r = row0 + p * rpp;
-      const bool query = r < h0, live = unit && r < rows;
-      float f[16], g[16], ss = 0.f, dot = 0.f;
+    for (int e = 0; e < 8; ++e) {
+      f[e] = in.x.get(e);
+      f[8 + e] = in.y.get(e);
+      g[e] = in.gx.get(e);
+      g[8 + e] = in.gy.get(e);
+    }
+    if (u < ru) gr_turn_unit<INTER>(g, sn, cs);
+    float h[16];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        f[e] = x[p].get(e);
-        f[8 + e] = y[p].get(e);
-        g[e] = gx[p].get(e);
-        g[8 + e] = gy[p].get(e);
-      }
-      if (u < ru) gr_turn_unit<INTER>(g, sn, cs);
+    for (int e = 0; e < 16; ++e) {
+      h[e] = g[e] * weight(e);
+      ss = fmaf(f[e], f[e], ss);
+      dot = fmaf(h[e], f[e], dot);
+    }
+    ss = gr_group_sum(ss, lanes);
+    dot = gr_group_sum(dot, lanes);
+    const float rms = rsqrtf(fmaf(ss, inv_d, a.eps));
+    const float c = dot * inv_d * rms * rms;
+    gr_rope8<T> s, t;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        ss = fmaf(f[e], f[e], ss);
-        dot = fmaf(g[e] * (query ? wq[e] : wk[e]), f[e], dot);
-      }
-      ss = gr_group_sum(ss, lanes);
-      dot = gr_group_sum(dot, lanes);
-      const float rms = rsqrtf(fmaf(ss, inv_d, a.eps));
-      const float c = dot * inv_d * rms * rms;
-      gr_rope8<T> s, t;
-      float d[16];
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float v = live ? g[e] * f[e] * rms : 0.f, vq = query ? v : 0.f;
+    for (int e = 0; e < 16; ++e) {
+      if constexpr (KIND == 0) {
+        sq[e] = fmaf(g[e] * rms, f[e], sq[e]);
+      } else if constexpr (KIND == 1) {
+        sk[e] = fmaf(g[e] * rms, f[e], sk[e]);
+      } else {
+        const float v = live ? g[e] * rms * f[e] : 0.f, vq = query ? v : 0.f;
         sq[e] += vq;
         sk[e] += v - vq;
-        d[e] = rms * fmaf(-c, f[e], g[e] * (query ? wq[e] : wk[e]));
       }
-      if (!live) continue;
+      h[e] = rms * fmaf(-c, f[e], h[e]);
+    }
+    if (!live) return;
 #pragma unroll
-      for (int e = 0; e < 8; e += 2) {
-        s.put2(e, d[e], d[e + 1]);
-        t.put2(e, d[8 + e], d[9 + e]);
-      }
-      T* to = query ? dq + r * a.q.dh : dk + (r - h0) * a.k.dh;
-      s.template store<false>(to + lo);
-      t.template store<false>(to + hi);
+    for (int e = 0; e < 8; e += 2) {
+      s.put2(e, h[e], h[e + 1]);
+      t.put2(e, h[8 + e], h[9 + e]);
+    }
+    const gr_rope_rows& to = query ? a.q : a.k;
+    T* const d = static_cast<T*>(to.dst) + in.b * to.db + in.i * to.dt + (query ? r : r - h0) * to.dh;
+    s.template store<false>(d + lo);
+    t.template store<false>(d + hi);
+  };
+  auto pass = [&](const pass_rows& in) {
+    if (in.pass == first_pass(in.task))
+      gr_unit_angles(a, gr_position(a, a.pos + in.b * a.ps[1] + in.i * a.ps[2], 0, lane), a.naxes > 1, u0 < ru ? u0 : 0, true, sn, cs);
+    const int r0 = in.pass * rpp;
+    if (all_units && r0 + rpp <= h0) work(in, gr_const<0>{});
+    else if (all_units && r0 >= h0 && r0 + rpp <= rows) work(in, gr_const<1>{});
+    else work(in, gr_const<2>{});
+  };
+  pass_rows one, two;
+  long long task = (long long)blockIdx.x * GR_NORM_WAVES + wave_in;
+  int at = 0;
+  if (task < tasks) {
+    load(one, task, first_pass(task));
+#pragma unroll 1
+    while (true) {
+      const bool more = next(one, task, at);
+      if (more) load(two, task, at);
+      pass(one);
+      if (!more) break;
+      const bool again = next(two, task, at);
+      if (again) load(one, task, at);
+      pass(two);
+      if (!again) break;
     }
   }
   if (a.part == nullptr) return;

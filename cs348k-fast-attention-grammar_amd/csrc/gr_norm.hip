@@ -7,10 +7,10 @@
 
 namespace {
 
-template <class T, bool INTER, int ITER>
+template <class T, bool INTER>
 __global__ __launch_bounds__(64 * GR_NORM_WAVES) void gr_norm_bwd_kernel(gr_norm_bwd_args a) {
   extern __shared__ float gr_norm_lds[];
-  gr_norm_bwd_body<T, INTER, ITER>(a, gr_norm_lds);
+  gr_norm_bwd_body<T, INTER>(a, gr_norm_lds);
 }
 
 template <class W>
@@ -19,15 +19,17 @@ __global__ __launch_bounds__(1024) void gr_norm_dw_kernel(const float* part, int
 }
 
 struct BwdPlan {
-  int iter, blocks;
+  int per, blocks;                // passes of a token that a wave takes, workgroups
 };
 
 BwdPlan bwd_plan(int rows, int D, int dtype, long long tokens) {
   const int rpp = 64 / row_lanes(D), passes = (rows + rpp - 1) / rpp;
   const int cus = gr::cu_count() > 0 ? gr::cu_count() : 256;
   BwdPlan p;
-  p.iter = passes >= 2 && dtype != GR_F32 && tokens * passes >= 16LL * cus ? 2 : 1;
-  const long long tasks = tokens * ((passes + p.iter - 1) / p.iter), all = (tasks + GR_NORM_WAVES - 1) / GR_NORM_WAVES;
+  // all of a token's where that leaves every wave of the GPU two tokens, else fewer
+  const long long waves = 2LL * cus * GR_NORM_WAVES, full = tokens * passes / (2 * waves);
+  p.per = full < 1 ? 1 : full < passes ? (int)full : passes;
+  const long long tasks = tokens * ((passes + p.per - 1) / p.per), all = (tasks + GR_NORM_WAVES - 1) / GR_NORM_WAVES;
   p.blocks = (int)(all < 2LL * cus ? all : 2LL * cus);
   return p;
 }
@@ -35,8 +37,7 @@ BwdPlan bwd_plan(int rows, int D, int dtype, long long tokens) {
 template <class T, bool INTER>
 int launch_bwd(const gr_norm_bwd_args& a, const BwdPlan& p, hipStream_t st) {
   const size_t lds = (size_t)GR_NORM_WAVES * 2 * a.D * sizeof(float);
-  if (p.iter == 2) hipLaunchKernelGGL((gr_norm_bwd_kernel<T, INTER, 2>), dim3(p.blocks), dim3(64 * GR_NORM_WAVES), lds, st, a);
-  else hipLaunchKernelGGL((gr_norm_bwd_kernel<T, INTER, 1>), dim3(p.blocks), dim3(64 * GR_NORM_WAVES), lds, st, a);
+  hipLaunchKernelGGL((gr_norm_bwd_kernel<T, INTER>), dim3(p.blocks), dim3(64 * GR_NORM_WAVES), lds, st, a);
   return gr::hip_check(hipGetLastError(), GR_E_LAUNCH, "gr_norm_rotary_bwd launch");
 }
 
@@ -120,6 +121,7 @@ extern "C" int gr_norm_rotary_bwd(const gr_rotary_spec* rotary, const gr_head_no
   a.wk = r.wk;
   a.w32 = r.w32;
   a.eps = r.eps;
+  a.per = p.per;
   const bool weights = dq_weight || dk_weight;
   if (weights) {
     if (!workspace || !gr::aligned16(workspace) || workspace_bytes < (size_t)p.blocks * 2 * D * sizeof(float))

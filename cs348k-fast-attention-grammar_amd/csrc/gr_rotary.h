@@ -119,22 +119,26 @@ struct gr_rope8 {
   }
 };
 
-// Sines and cosines of the 8 pairs of unit `u0` of a token: its position on each axis
-// from `pos`, or `at` on every axis. (a: gr_rope_args, or what has its members.)
+// A token's position, from `pos` (several axes: lane i has axis i's), or `at` on every
+// axis. (a: gr_rope_args, or what has its members.)
 template <class A>
-__device__ __forceinline__ void gr_unit_angles(const A& a, const int* pos, int at, int u0, int lane, bool inverse, float (&sn)[8],
+__device__ __forceinline__ int gr_position(const A& a, const int* pos, int at, int lane) {
+  if (!pos) return at;
+  if (a.naxes == 1) return pos[0];
+  return lane < a.naxes ? pos[lane * a.ps[0]] : 0;
+}
+
+// Sines and cosines of the 8 pairs of unit `u0` of a token at `position`; axes: it
+// differs by axis.
+template <class A>
+__device__ __forceinline__ void gr_unit_angles(const A& a, int position, bool axes, int u0, bool inverse, float (&sn)[8],
                                                float (&cs)[8]) {
-  int p1 = at, plane = 0;
-  if (pos) {
-    if (a.naxes == 1) p1 = pos[0];
-    else if (lane < a.naxes) plane = pos[lane * a.ps[0]];
-  }
   unsigned long long ax = 0;
-  if (a.naxes > 1) ax = *reinterpret_cast<const unsigned long long*>(a.axes + 8 * u0);
+  if (axes) ax = *reinterpret_cast<const unsigned long long*>(a.axes + 8 * u0);
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    int pe = p1;
-    if (a.naxes > 1 && pos) pe = __shfl(plane, (int)(ax >> (8 * e)) & 63, 64);
+    int pe = position;
+    if (axes) pe = __shfl(position, (int)(ax >> (8 * e)) & 63, 64);
     const unsigned long long t = (unsigned long long)(long long)pe * a.turns[8 * u0 + e];
     gr_turn_sincos((unsigned)(t >> 32), sn[e], cs[e]);
     if (inverse) sn[e] = -sn[e];
@@ -314,8 +318,10 @@ __device__ __forceinline__ void gr_rope_body(const gr_rope_args& a, bool inverse
   }
 
   float sn[8] = {}, cs[8] = {};
-  if (a.pairs > 0)
-    gr_unit_angles(a, a.pos ? a.pos + brow * a.ps[1] + trow * a.ps[2] : nullptr, at, u < ru ? u : 0, lane, inverse, sn, cs);
+  if (a.pairs > 0) {
+    const int* const pos = a.pos ? a.pos + brow * a.ps[1] + trow * a.ps[2] : nullptr;
+    gr_unit_angles(a, gr_position(a, pos, at, lane), pos && a.naxes > 1, u < ru ? u : 0, inverse, sn, cs);
+  }
 
   auto target = [&](const gr_rope_rows& k, bool cached) {
     return static_cast<T*>(k.dst) + (cached ? page * k.db + slot * k.dt : brow * k.db + trow * k.dt);
@@ -342,8 +348,18 @@ __device__ __forceinline__ void gr_rope_body(const gr_rope_args& a, bool inverse
 #pragma unroll
         for (int e = 0; e < 16; ++e) ss = fmaf(f[e], f[e], ss);
         const float rms = rsqrtf(gr_group_sum(ss, lanes) / (float)a.D + a.eps);
+        // rows of one kind in most passes: a scalar branch instead of a choice of each element
+        const int first = (wave - tok * groups) * ITER * rpp + p * rpp;
+        if (first + rpp <= h0) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) f[e] = APPEND && r >= h1 ? f[e] : f[e] * rms * (r < h0 ? wq[e] : wk[e]);
+          for (int e = 0; e < 16; ++e) f[e] = f[e] * rms * wq[e];
+        } else if (first >= h0 && first + rpp <= h1) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) f[e] = f[e] * rms * wk[e];
+        } else if (!APPEND || first < h1) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) f[e] = APPEND && r >= h1 ? f[e] : f[e] * rms * (r < h0 ? wq[e] : wk[e]);
+        }
       }
       if ((!APPEND || r < h1) && u < ru) gr_turn_unit<INTER>(f, sn, cs);
       if (Q8 && r >= h0) {

@@ -26,6 +26,16 @@ __global__ __launch_bounds__(256) void gr_rope_kernel(gr_rope_args a, int invers
   gr_rope_body<T, APPEND, INTER, ITER, PAST, NORM, Q8>(a, inverse != 0);
 }
 
+// ITER passes to a wave.
+template <class T, bool APPEND, bool INTER, bool PAST, bool NORM, bool Q8, int ITER>
+int launch_iter(const gr_rope_args& a, int passes, int inverse, const char* who, hipStream_t st) {
+  const long long waves = (long long)a.tokens * ((passes + ITER - 1) / ITER);
+  if (waves > 0x7fffffffLL / 64)
+    return gr::fail(GR_E_ARG, "%s: %d tokens of %d head rows are too many for one call", who, a.tokens, a.q.heads + a.k.heads + a.v.heads);
+  hipLaunchKernelGGL((gr_rope_kernel<T, APPEND, INTER, ITER, PAST, NORM, Q8>), dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, st, a, inverse);
+  return gr::hip_check(hipGetLastError(), GR_E_LAUNCH, who);
+}
+
 template <class T, bool APPEND, bool INTER, bool PAST, bool NORM, bool Q8>
 int launch(const gr_rope_args& a, int inverse, const char* who, hipStream_t st) {
   const int rows = a.q.heads + a.k.heads + a.v.heads;
@@ -37,19 +47,18 @@ int launch(const gr_rope_args& a, int inverse, const char* who, hipStream_t st) 
   // 43.3 / 49.0, 48 of 128 33.2 / 32.7).
   const long long full = (long long)a.tokens * passes;
   const int cus = gr::cu_count() > 0 ? gr::cu_count() : 256;
-  const int iter = passes < 2 || full < 8LL * cus ? 1 : passes == 2 || (sizeof(T) == 2 && a.D >= 128) ? 2 : 4;
-  const long long waves = (long long)a.tokens * ((passes + iter - 1) / iter);
-  if (waves > 0x7fffffffLL / 64) return gr::fail(GR_E_ARG, "%s: %d tokens of %d head rows are too many for one call", who, a.tokens, rows);
-  const dim3 grid((unsigned)((waves + 3) / 4));
-  if constexpr (!PAST) {
-    if (iter == 4) {
-      hipLaunchKernelGGL((gr_rope_kernel<T, APPEND, INTER, 4, false, NORM, Q8>), grid, dim3(256), 0, st, a, inverse);
-      return gr::hip_check(hipGetLastError(), GR_E_LAUNCH, who);
-    }
+  int iter = passes < 2 || full < 8LL * cus ? 1 : passes == 2 || (sizeof(T) == 2 && a.D >= 128) ? 2 : 4;
+  if constexpr (NORM || Q8) {
+    const int groups = (passes + 4) / 5;
+    iter = full < 8LL * cus ? 1 : (passes + groups - 1) / groups;
+    if (iter == 5) return launch_iter<T, APPEND, INTER, PAST, NORM, Q8, 5>(a, passes, inverse, who, st);
+    if (iter == 4) return launch_iter<T, APPEND, INTER, PAST, NORM, Q8, 4>(a, passes, inverse, who, st);
+    if (iter == 3) return launch_iter<T, APPEND, INTER, PAST, NORM, Q8, 3>(a, passes, inverse, who, st);
+  } else if constexpr (!PAST) {
+    if (iter == 4) return launch_iter<T, APPEND, INTER, false, false, false, 4>(a, passes, inverse, who, st);
   }
-  if (iter == 2) hipLaunchKernelGGL((gr_rope_kernel<T, APPEND, INTER, 2, PAST, NORM, Q8>), grid, dim3(256), 0, st, a, inverse);
-  else hipLaunchKernelGGL((gr_rope_kernel<T, APPEND, INTER, 1, PAST, NORM, Q8>), grid, dim3(256), 0, st, a, inverse);
-  return gr::hip_check(hipGetLastError(), GR_E_LAUNCH, who);
+  if (iter == 2) return launch_iter<T, APPEND, INTER, PAST, NORM, Q8, 2>(a, passes, inverse, who, st);
+  return launch_iter<T, APPEND, INTER, PAST, NORM, Q8, 1>(a, passes, inverse, who, st);
 }
 
 // Whether every row of a destination begins on a 128-byte line (16-bit elements).
@@ -60,11 +69,12 @@ inline bool on_lines(const gr_rope_rows& k) {
 template <class T, bool APPEND, bool NORM = false, bool Q8 = false>
 int launch_inter(const gr_rope_args& a, bool inter, int inverse, const char* who, hipStream_t st) {
   if (inter) return launch<T, APPEND, true, false, NORM, Q8>(a, inverse, who, st);
-  if constexpr (sizeof(T) == 2 && !Q8) {
+  if constexpr (sizeof(T) == 2) {
     // whole lines: 8 lanes of 16 bytes side by side, in the rotated part and behind it,
     // of rows that begin on a line (2 x 4,096 tokens of 32 + 32 heads of 128: 43.7 us, rows
     // 16 bytes off a line 50.5 and past the caches 93.5, 64 off 45.5 and 47.8)
-    if (2 * a.pairs % 128 == 0 && a.D % 128 == 0 && on_lines(a.q) && on_lines(a.k) && on_lines(a.v))
+    if (2 * a.pairs % 128 == 0 && a.D % 128 == 0 && on_lines(a.q) &&
+        (Q8 || (on_lines(a.k) && on_lines(a.v))))
       return launch<T, APPEND, false, true, NORM, Q8>(a, inverse, who, st);
   }
   return launch<T, APPEND, false, false, NORM, Q8>(a, inverse, who, st);

@@ -12,6 +12,7 @@ There is no CPU path: CPU tensors or a missing library raise.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 from . import runtime as rt
 from .rotary import (Rotary, _dense, _has_tangent, _tokens, check_out, check_positions, head_strides)
@@ -27,21 +28,30 @@ class HeadNorm:
             raise ValueError(f"HeadNorm: eps {eps} must not be negative")
         self.q_weight, self.k_weight, self.eps = q_weight, k_weight, float(eps)
 
-    def spec(self, head_dim: int, dtype, device, who: str):
-        """The gr_head_norm of the weights as they are now, for heads of `dtype`."""
-        import torch
-        code = None
-        for name, w in (("q_weight", self.q_weight), ("k_weight", self.k_weight)):
-            if w is None:
-                continue
-            if w.shape != (head_dim,) or w.device != device or (head_dim > 1 and w.stride(0) != 1):
-                raise ValueError(f"{who}: {name} must be a contiguous [{head_dim}] tensor on {device}, not {tuple(w.shape)} on {w.device}")
-            if w.dtype not in (torch.float32, dtype) or code not in (None, w.dtype):
-                raise ValueError(f"{who}: the norm's weights must both be float32 or {dtype}")
-            code = w.dtype
-        q, k = self.q_weight, self.k_weight
-        return rt.HeadNormSpec(None if q is None else q.data_ptr(), None if k is None else k.data_ptr(),
-                               rt.GR_F32 if code is None else rt.dtype_code(code), self.eps)
+    def spec(self, head_dim: int, dtype, index: int, who: str):
+        """The gr_head_norm of the weights as they are now, for heads of `dtype` on GPU `index`."""
+        return _spec(self.q_weight, self.k_weight, self.eps, head_dim, dtype, index, who)
+
+
+def _spec(q, k, eps, head_dim, dtype, index, who):
+    """The gr_head_norm of weights q and k (or None), checked."""
+    of = dtype
+    for w in (q, k):
+        if w is None:
+            continue
+        if w.dim() != 1 or w.numel() != head_dim or w.get_device() != index or not w.is_contiguous():
+            raise ValueError(f"{who}: the norm's weights must be contiguous [{head_dim}] tensors on GPU {index}, not "
+                             f"{tuple(w.shape)} on {w.device}")
+        of = w.dtype
+    code = rt.dtype_code(of)
+    if (code != rt.GR_F32 and of != dtype) or (q is not None and q.dtype != of):
+        raise ValueError(f"{who}: the norm's weights must both be float32 or {dtype}")
+    return rt.HeadNormSpec(None if q is None else q.data_ptr(), None if k is None else k.data_ptr(), code, eps)
+
+
+@functools.lru_cache(maxsize=4096)
+def _bwd_workspace(*sizes):
+    return int(rt.lib().gr_norm_rotary_bwd_workspace(*sizes))
 
 
 def _sizes(q, k, rot, who):
@@ -70,7 +80,7 @@ def norm_rotary_fwd(q, k, positions, rot: Rotary, norm: HeadNorm, *, out=None, k
     who = "norm_rotary"
     B, N, Hq, qs, Hk, ks = _sizes(q, k, rot, who)
     ps = check_positions(positions, rot, (B, N), who)
-    spec = norm.spec(rot.head_dim, q.dtype, rot.device, who)
+    spec = norm.spec(rot.head_dim, q.dtype, rot.index, who)
     out = check_out(out, q, "out", who, stream)
     head = (rot.ref, ctypes.addressof(spec), q.data_ptr(), out.data_ptr(), Hq, qs, head_strides(out, "out", who))
     if k is None:
@@ -94,22 +104,27 @@ def norm_rotary_bwd(q, k, positions, rot: Rotary, norm: HeadNorm, dq_out, dk_out
     dq_out, dk_out and the weights; None for what there is none of, and the weights' with
     weights=False. The weights' gradients are summed in fp32, in an order that the sizes alone
     decide."""
-    import torch
+    return _bwd(q, k, positions, rot, norm.q_weight, norm.k_weight, norm.eps, dq_out, dk_out, weights, weights, stream)
+
+
+def _bwd(q, k, positions, rot, q_weight, k_weight, eps, dq_out, dk_out, want_q, want_k, stream=None):
+    """norm_rotary_bwd; want_q, want_k: the weights whose gradients are wanted."""
     who = "norm_rotary_bwd"
     B, N, Hq, qs, Hk, ks = _sizes(q, k, rot, who)
     ps = check_positions(positions, rot, (B, N), who)
-    spec = norm.spec(rot.head_dim, q.dtype, rot.device, who)
+    spec = _spec(q_weight, k_weight, eps, rot.head_dim, q.dtype, rot.index, who)
     for name, g, x in (("dq_out", dq_out, q), ("dk_out", dk_out, k)):
         if (g is None) != (x is None) or (g is not None and (g.shape != x.shape or g.dtype != x.dtype or g.device != x.device)):
             raise ValueError(f"{who}: {name} must be as its heads, {None if x is None else tuple(x.shape)}")
     outs = [rt.empty_like(g, stream) if g is not None else None for g in (dq_out, dk_out)]
-    dws = [rt.result((rot.head_dim,), w.dtype, q.device, stream) if weights and w is not None and x is not None else None
-           for w, x in ((norm.q_weight, q), (norm.k_weight, k))]
+    dws = [rt.empty_like(w, stream) if want and w is not None and x is not None else None
+           for w, x, want in ((q_weight, q, want_q), (k_weight, k, want_k))]
     if B == 0 or N == 0:
+        import torch
         with torch.cuda.stream(torch.cuda.current_stream(q.device) if stream is None else rt.torch_stream(stream, q.device)):
             return (*outs, *(None if w is None else w.zero_() for w in dws))
     code = rt.dtype_code(q.dtype)
-    need = int(rt.lib().gr_norm_rotary_bwd_workspace(Hq, Hk, rot.head_dim, code, B, N)) if any(w is not None for w in dws) else 0
+    need = 0 if dws[0] is None and dws[1] is None else _bwd_workspace(Hq, Hk, rot.head_dim, code, B, N)
     ws = rt.workspace(need, q.device, stream) if need else None
 
     def side(x, g, d, H, st):
@@ -129,30 +144,32 @@ def _autograd_function():
         @staticmethod
         def forward(ctx, q, k, q_weight, k_weight, positions, rot, eps):
             ctx.set_materialize_grads(False)
-            norm = HeadNorm(q_weight, k_weight, eps)
             q, k = _dense(q), None if k is None else _dense(k)
             ctx.save_for_backward(q, k, q_weight, k_weight, positions)
             ctx.rot, ctx.eps = rot, eps
-            return norm_rotary_fwd(q, k, positions, rot, norm)
+            return norm_rotary_fwd(q, k, positions, rot, HeadNorm(q_weight, k_weight, eps))
 
         @staticmethod
-        @torch.autograd.function.once_differentiable
         def backward(ctx, dq, dk):
-            # queries and keys in one launch where the gradients of both came
-            q, k, q_weight, k_weight, positions = ctx.saved_tensors
-            weights = ctx.needs_input_grad[2] or ctx.needs_input_grad[3]
-            if dq is None and dk is None:
-                return (None,) * 7
-            if dq is None:                                     # keys alone, as the queries of a call
-                g, _, w, _ = norm_rotary_bwd(k, None, positions, ctx.rot, HeadNorm(k_weight, None, ctx.eps), _dense(dk), None,
-                                             weights=weights)
-                return None, g, None, w, None, None, None
-            if dk is None:
-                g, _, w, _ = norm_rotary_bwd(q, None, positions, ctx.rot, HeadNorm(q_weight, None, ctx.eps), _dense(dq), None,
-                                             weights=weights)
-                return g, None, w, None, None, None, None
-            return (*norm_rotary_bwd(q, k, positions, ctx.rot, HeadNorm(q_weight, k_weight, ctx.eps), _dense(dq), _dense(dk),
-                                     weights=weights), None, None, None)
+            # differentiable once: only where the backward pass is recorded does that
+            # have to be kept track of
+            return recorded(ctx, dq, dk) if torch.is_grad_enabled() else gradients(ctx, dq, dk)
+
+    def gradients(ctx, dq, dk):
+        # queries and keys in one launch where the gradients of both came
+        q, k, q_weight, k_weight, positions = ctx.saved_tensors
+        _, _, want_q, want_k = ctx.needs_input_grad[:4]
+        if dq is None and dk is None:
+            return (None,) * 7
+        if dq is None:                                         # keys alone, as the queries of a call
+            g, _, w, _ = _bwd(k, None, positions, ctx.rot, k_weight, None, ctx.eps, _dense(dk), None, want_k, False)
+            return None, g, None, w, None, None, None
+        if dk is None:
+            g, _, w, _ = _bwd(q, None, positions, ctx.rot, q_weight, None, ctx.eps, _dense(dq), None, want_q, False)
+            return g, None, w, None, None, None, None
+        return (*_bwd(q, k, positions, ctx.rot, q_weight, k_weight, ctx.eps, _dense(dq), _dense(dk), want_q, want_k),
+                None, None, None)
+    recorded = torch.autograd.function.once_differentiable(gradients)
     return NormRotaryFunction
 
 

@@ -29,7 +29,7 @@ import math
 
 from . import runtime as rt
 from .norm import HeadNorm
-from .rotary import Rotary, _head_strides, check_out, check_positions, head_strides
+from .rotary import Rotary, _head_strides, _takes, check_out, check_positions, head_strides
 
 
 class PagedCache:
@@ -217,7 +217,7 @@ def _append_args(k, v, cache, table, lens, starts, q, rotary, norm, positions, m
     keep = (desc, k, v, cache, table, lens, starts, q, rotary, positions, out)
     if norm is None and cache.scales_ref is None:
         return rt.lib().gr_paged_append, (cache.ref, ctypes.addressof(desc), ref) + args, out, keep
-    spec = None if norm is None else norm.spec(cache.head_dim, cache.dtype, cache.k.device, who)
+    spec = None if norm is None else norm.spec(cache.head_dim, cache.dtype, cache.index, who)
     args = (cache.ref, cache.scales_ref, ctypes.addressof(desc), ref, None if spec is None else ctypes.addressof(spec)) + args
     return rt.lib().gr_paged_append_with, args, out, keep + (spec, norm)
 
@@ -347,11 +347,10 @@ def paged_read(cache: PagedCache | QuantizedPagedCache, table, lens, length: int
     elif length is not None and (starts is not None or k_out.dim() != 4 or k_out.shape[2] != length):
         raise ValueError(f"{who}: k_out {tuple(k_out.shape)} is not of length {length}")
     desc, lead = _batch(cache, table, lens, starts, k_out, 0, 0, who)
-    args = ()
-    for name, t in (("k_out", k_out), ("v_out", v_out)):
-        if any(st == 0 and n > 1 for n, st in zip(t.shape, t.stride())):
-            raise ValueError(f"{who}: {name} must not overlap itself (a stride of 0)")
-        args += (_heads(t, name, lead, cache.heads, cache, who),)
+    for t in (k_out, v_out):
+        if not _takes(t.shape, t.stride(), t.shape):
+            raise ValueError(f"{who}: k_out and v_out must not overlap themselves (a stride of 0)")
+    args = (_heads(k_out, "k_out", lead, cache.heads, cache, who), _heads(v_out, "v_out", lead, cache.heads, cache, who))
     if 0 in k_out.shape:
         return k_out, v_out
     rt.launch(rt.lib().gr_paged_read, (cache.ref, cache.scales_ref, ctypes.addressof(desc), k_out.data_ptr(),

@@ -18,10 +18,11 @@ def _calls(rt, d, cache, scales, batch, spec, norm=None):
     L = rt.lib()
     c, sc, b = p(cache), p(scales) if scales else None, p(batch)
     far = d + (1 << 24)
-    return (lambda: L.gr_paged_append_with(c, sc, b, p(spec), p(norm) if norm else None, None, None, 0, None, None, far, far, s, s,
+    keep = (cache, scales, batch, spec, norm)                               # what the addresses are of
+    return (lambda keep=keep: L.gr_paged_append_with(c, sc, b, p(spec), p(norm) if norm else None, None, None, 0, None, None, far, far, s, s,
                                            None, None, None),
-            lambda: L.gr_paged_attn_scaled(c, sc, b, far, far, None, 8, s, s, 1, 0.125, None, 0, None),
-            lambda: L.gr_paged_read(c, sc, b, far, far + (1 << 24), s, s, None))
+            lambda keep=keep: L.gr_paged_attn_scaled(c, sc, b, far, far, None, 8, s, s, 1, 0.125, None, 0, None),
+            lambda keep=keep: L.gr_paged_read(c, sc, b, far, far + (1 << 24), s, s, None))
 
 
 @pytest.mark.parametrize("what,field,value,msg", [("cache", *c) for c in BAD_CACHE] + [("batch", *c) for c in BAD_BATCH])

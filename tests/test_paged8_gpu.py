@@ -101,7 +101,7 @@ def _check(got, want, size, q, s, b, what, scale=None):
     return (u + e[..., 0] + sub * m) * 1.01 + 2.0 ** -22 * (A + 8)
 
 
-def _run(s, news, Hq, causal=True, ragged=False, pad=0, hints=True, strided=False):
+def _run(s, news, Hq, causal=True, ragged=False, pad=0, hints=True, strided=False, workspace=None):
     """paged_attention of `news` new tokens a sequence, checked row by row; returns the result."""
     from grammar.paged import paged_attention
     B, D = len(s.lens_host), s.D
@@ -118,7 +118,8 @@ def _run(s, news, Hq, causal=True, ragged=False, pad=0, hints=True, strided=Fals
         starts, lse = None, torch.full((B, n, Hq), 7.0, device=s.dev)
         out = torch.full(q.shape, 5.0, device=s.dev, dtype=s.dtype)
     more = dict(max_new=max(news), max_len=max(1, max(s.lens_host))) if hints else {}
-    got = paged_attention(q, s.cache, s.table, s.lens, starts=starts, causal=causal, out=out, lse=lse, **more)
+    got = paged_attention(q, s.cache, s.table, s.lens, starts=starts, causal=causal, out=out, lse=lse, workspace=workspace,
+                          **more)
     torch.cuda.synchronize()
     assert got is out
     row = 0
@@ -228,8 +229,9 @@ def test_shared_mixed_batches(dtype, D, G, Hkv):
 
 
 @pytest.mark.parametrize("dtype,D", [("bf16", 128), ("fp16", 64)])
-@pytest.mark.parametrize("G,Hkv", [(8, 16), (4, 8)], ids=["many", "few"])
+@pytest.mark.parametrize("G,Hkv", [(8, 16), (4, 8), (2, 8)], ids=["many", "few", "small"])
 def test_mixed_batches_of_a_workgroup_a_tile(dtype, D, G, Hkv):
+    """Tiles of 128 rows in grids that fill the GPU and that do not, and of 32 rows."""
     news = [1, 130, 0, 33, 300, 1, 16] + [1, 0, 2] * 25 + [34]
     lens = [260, 131, 9, 33, 449, 0, 80] + [5 * i for i in range(75)] + [70]
     s = Setup8(lens, Hkv, 32, D, dtype, seed=G)
@@ -237,6 +239,18 @@ def test_mixed_batches_of_a_workgroup_a_tile(dtype, D, G, Hkv):
     assert _needs_workspace(s, sum(news) + 3, G * Hkv, s.lens.data_ptr()) == 0
     for causal in (True, False):
         _run(s, news, G * Hkv, causal=causal, ragged=True, pad=3, hints=False)
+
+
+@pytest.mark.parametrize("dtype,D", [("bf16", 128), ("fp16", 64)])
+@pytest.mark.parametrize("news,lens,G,Hkv", [([2049] + [1] * 8, [2300, 700, 5, 900, 0, 33, 64, 65, 1500], 4, 8),
+                                             ([513, 0, 700], [513, 9, 1900], 8, 9), ([1100] * 3, [1100, 1500, 1900], 4, 5)])
+def test_long_chunks(dtype, D, news, lens, G, Hkv):
+    """Tiles of 128 rows, in packed and uniform batches, with room in the grid for tiles that the lengths do not make."""
+    print(f"[case] chunks {dtype} D{D} {news} G{G} Hkv{Hkv}", flush=True)
+    s = Setup8(lens, Hkv, 64, D, dtype, seed=D)
+    uniform = len(set(news)) == 1
+    for causal in (True, False):
+        _run(s, news, G * Hkv, causal=causal, ragged=not uniform, pad=0 if uniform else 200, hints=causal)
 
 
 @pytest.mark.parametrize("D", [64, 128])
