@@ -22,7 +22,7 @@ struct BwdPlan {
   int per, blocks;                // passes of a token that a wave takes, workgroups
 };
 
-BwdPlan bwd_plan(int rows, int D, int dtype, long long tokens) {
+BwdPlan bwd_plan(int rows, int D, long long tokens) {
   const int rpp = 64 / row_lanes(D), passes = (rows + rpp - 1) / rpp;
   const int cus = gr::cu_count() > 0 ? gr::cu_count() : 256;
   BwdPlan p;
@@ -47,11 +47,6 @@ int launch_dw(const gr_norm_bwd_args& a, int n, void* dwq, void* dwk, hipStream_
   return gr::hip_check(hipGetLastError(), GR_E_LAUNCH, "gr_norm_rotary_bwd weights launch");
 }
 
-// Whether a weight vector shares memory with some heads.
-bool meets(const void* w, int D, int wsize, const gr::strided& heads, int size) {
-  return w && gr::overlap({w, {1, 1, 1, (long long)D * wsize}, {0, 0, 0, 1}}, gr::bytes_of(heads, size), 1);
-}
-
 }  // namespace
 
 extern "C" int gr_norm_rotary(const gr_rotary_spec* rotary, const gr_head_norm* norm, const void* q, void* q_out, int Hq,
@@ -64,6 +59,9 @@ extern "C" int gr_norm_rotary(const gr_rotary_spec* rotary, const gr_head_norm* 
   int rc = take_heads(a, rotary, q, q_out, Hq, q_strides, q_out_strides, k, k_out, Hk, k_strides, k_out_strides, dtype, B, N,
                       positions, position_strides, who);
   if (rc || (rc = take_norm(a, norm, dtype, who))) return rc;
+  const int D = rotary->head_dim, size = dtype == GR_F32 ? 4 : 2;
+  if ((rc = check_weights(norm, D, gr::heads_of(q_out, B, N, Hq, D, q_out_strides), size, "q_out", who))) return rc;
+  if (k && (rc = check_weights(norm, D, gr::heads_of(k_out, B, N, Hk, D, k_out_strides), size, "k_out", who))) return rc;
   hipStream_t st = (hipStream_t)stream;
   const bool inter = rotary->interleaved != 0;
   if (dtype == GR_F16) return launch_inter<_Float16, false, true>(a, inter, 0, who, st);
@@ -71,9 +69,9 @@ extern "C" int gr_norm_rotary(const gr_rotary_spec* rotary, const gr_head_norm* 
   return launch_inter<float, false, true>(a, inter, 0, who, st);
 }
 
-extern "C" size_t gr_norm_rotary_bwd_workspace(int Hq, int Hk, int head_dim, int dtype, int B, int N) {
+extern "C" size_t gr_norm_rotary_bwd_workspace(int Hq, int Hk, int head_dim, int B, int N) {
   if (Hq <= 0 || Hk < 0 || head_dim < 16 || head_dim > 256 || head_dim % 16 || B <= 0 || N <= 0) return 0;
-  return (size_t)bwd_plan(Hq + Hk, head_dim, dtype, (long long)B * N).blocks * 2 * head_dim * sizeof(float);
+  return (size_t)bwd_plan(Hq + Hk, head_dim, (long long)B * N).blocks * 2 * head_dim * sizeof(float);
 }
 
 extern "C" int gr_norm_rotary_bwd(const gr_rotary_spec* rotary, const gr_head_norm* norm, const void* q, const void* dq_out,
@@ -96,13 +94,15 @@ extern "C" int gr_norm_rotary_bwd(const gr_rotary_spec* rotary, const gr_head_no
   const int D = rotary->head_dim, size = dtype == GR_F32 ? 4 : 2, wsize = norm->dtype == GR_F32 ? 4 : 2;
   if (((uintptr_t)dq_weight & 3) || ((uintptr_t)dk_weight & 3))
     return gr::fail(GR_E_ARG, "gr_norm_rotary_bwd: the weights' gradients must be 4-byte aligned");
-  for (const void* w : {dq_weight, dk_weight}) {
-    if (meets(w, D, wsize, gr::heads_of(dq, B, N, Hq, D, dq_strides), size) ||
-        (k && meets(w, D, wsize, gr::heads_of(dk, B, N, Hk, D, dk_strides), size)) ||
-        (w && dq_weight && dk_weight && (w == dq_weight ? meets(w, D, wsize, {dk_weight, {1, 1, 1, D}, {0, 0, 0, 1}}, wsize) : false)))
+  const gr::strided to[2] = {gr::heads_of(dq, B, N, Hq, D, dq_strides), k ? gr::heads_of(dk, B, N, Hk, D, dk_strides) : gr::strided{}};
+  for (int i = 0; i < (k ? 2 : 1); ++i) {
+    if ((rc = check_weights(norm, D, to[i], size, i ? "dk" : "dq", who))) return rc;
+    if (meets(dq_weight, D, wsize, to[i], size) || meets(dk_weight, D, wsize, to[i], size))
       return gr::fail(GR_E_ARG, "gr_norm_rotary_bwd: a weights' gradient shares memory with another output");
   }
-  const BwdPlan p = bwd_plan(Hq + (k ? Hk : 0), D, dtype, (long long)B * N);
+  if (dk_weight && meets(dq_weight, D, wsize, {dk_weight, {1, 1, 1, D}, {0, 0, 0, 1}}, wsize))
+    return gr::fail(GR_E_ARG, "gr_norm_rotary_bwd: a weights' gradient shares memory with another output");
+  const BwdPlan p = bwd_plan(Hq + (k ? Hk : 0), D, (long long)B * N);
   gr_norm_bwd_args a = {};
   a.q = r.q;
   a.k = r.k;

@@ -49,6 +49,10 @@ int launch(const gr_rope_args& a, int inverse, const char* who, hipStream_t st) 
   const int cus = gr::cu_count() > 0 ? gr::cu_count() : 256;
   int iter = passes < 2 || full < 8LL * cus ? 1 : passes == 2 || (sizeof(T) == 2 && a.D >= 128) ? 2 : 4;
   if constexpr (NORM || Q8) {
+    // Rows that are normed or quantised have more to compute a pass, behind which more loads
+    // hide: up to five, shared out evenly. Norm of 2 x 4,096 tokens of 32 + 8 heads of 128 (10
+    // passes) in twos 40 us, threes 37, fives 31; 9,668 tokens of 48 heads of 128
+    // into a quantised cache in twos 63, threes 53, fours 52; 1,024 tokens 10.8, in fours 8.7.
     const int groups = (passes + 4) / 5;
     iter = full < 8LL * cus ? 1 : (passes + groups - 1) / groups;
     if (iter == 5) return launch_iter<T, APPEND, INTER, PAST, NORM, Q8, 5>(a, passes, inverse, who, st);
@@ -149,6 +153,19 @@ inline int take_heads(gr_rope_args& a, const gr_rotary_spec* rotary, const void*
   return GR_OK;
 }
 
+// Whether a vector of weights shares memory with heads.
+inline bool meets(const void* w, int D, int wsize, const gr::strided& heads, int size) {
+  return w && gr::overlap({w, {1, 1, 1, (long long)D * wsize}, {0, 0, 0, 1}}, gr::bytes_of(heads, size), 1);
+}
+
+// Heads that a call writes are none of its norm's weights.
+inline int check_weights(const gr_head_norm* n, int D, const gr::strided& out, int size, const char* name, const char* who) {
+  const int wsize = n->dtype == GR_F32 ? 4 : 2;
+  return meets(n->q_weight, D, wsize, out, size) || meets(n->k_weight, D, wsize, out, size)
+             ? gr::fail(GR_E_ARG, "%s: %s shares memory with the norm's weights", who, name)
+             : GR_OK;
+}
+
 // A norm's weights, in fp32 or in the rows' type.
 inline int take_norm(gr_rope_args& a, const gr_head_norm* n, int dtype, const char* who) {
   if (!gr::aligned16(n->q_weight) || !gr::aligned16(n->k_weight))
@@ -200,6 +217,7 @@ inline int take_append(gr_rope_args& a, const gr_paged_cache* cache, const gr_pa
       if (gr::overlap(bytes, others[2], 1) || gr::overlap(bytes, others[3], 1) || gr::overlap(bytes, gr::scales_of(cache, scales), 1))
         return gr::fail(GR_E_ARG, "%s: q_out shares memory with the cache", who);
     }
+    if (norm && (rc = check_weights(norm, D, qo, 2, "q_out", who))) return rc;
   }
   a.tokens = batch->starts ? batch->rows : batch->B * batch->rows;
   a.per_seq = batch->starts ? 1 : batch->rows;

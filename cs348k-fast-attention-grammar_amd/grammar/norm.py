@@ -124,7 +124,7 @@ def _bwd(q, k, positions, rot, q_weight, k_weight, eps, dq_out, dk_out, want_q, 
         with torch.cuda.stream(torch.cuda.current_stream(q.device) if stream is None else rt.torch_stream(stream, q.device)):
             return (*outs, *(None if w is None else w.zero_() for w in dws))
     code = rt.dtype_code(q.dtype)
-    need = 0 if dws[0] is None and dws[1] is None else _bwd_workspace(Hq, Hk, rot.head_dim, code, B, N)
+    need = 0 if dws[0] is None and dws[1] is None else _bwd_workspace(Hq, Hk, rot.head_dim, B, N)
     ws = rt.workspace(need, q.device, stream) if need else None
 
     def side(x, g, d, H, st):

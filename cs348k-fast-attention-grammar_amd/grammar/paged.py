@@ -339,20 +339,23 @@ def paged_read(cache: PagedCache | QuantizedPagedCache, table, lens, length: int
     who = "paged_read"
     if (k_out is None) != (v_out is None):
         raise ValueError(f"{who}: k_out and v_out come together")
-    if k_out is None:
+    made = k_out is None
+    if made:
         if starts is not None or length is None or int(length) < 0:
             raise ValueError(f"{who}: needs a length, or k_out and v_out")
         shape = (table.shape[0], cache.heads, int(length), cache.head_dim)
-        k_out, v_out = (rt.result(shape, cache.dtype, cache.k.device, stream) for _ in range(2))
+        k_out, v_out = rt.result(shape, cache.dtype, cache.k.device, stream), rt.result(shape, cache.dtype, cache.k.device, stream)
     elif length is not None and (starts is not None or k_out.dim() != 4 or k_out.shape[2] != length):
         raise ValueError(f"{who}: k_out {tuple(k_out.shape)} is not of length {length}")
     desc, lead = _batch(cache, table, lens, starts, k_out, 0, 0, who)
-    for t in (k_out, v_out):
-        if not _takes(t.shape, t.stride(), t.shape):
-            raise ValueError(f"{who}: k_out and v_out must not overlap themselves (a stride of 0)")
-    args = (_heads(k_out, "k_out", lead, cache.heads, cache, who), _heads(v_out, "v_out", lead, cache.heads, cache, who))
-    if 0 in k_out.shape:
+    ks = vs = _heads(k_out, "k_out", lead, cache.heads, cache, who)
+    if not made:
+        vs = _heads(v_out, "v_out", lead, cache.heads, cache, who)
+        for t in (k_out, v_out):
+            if not _takes(t.shape, t.stride(), t.shape):
+                raise ValueError(f"{who}: k_out and v_out must not overlap themselves (a stride of 0)")
+    if k_out.numel() == 0:
         return k_out, v_out
     rt.launch(rt.lib().gr_paged_read, (cache.ref, cache.scales_ref, ctypes.addressof(desc), k_out.data_ptr(),
-                                       v_out.data_ptr()) + args, k_out, stream, "gr_paged_read")
+                                       v_out.data_ptr(), ks, vs), k_out, stream, "gr_paged_read")
     return k_out, v_out

@@ -133,7 +133,7 @@ def lib() -> ctypes.CDLL:
         L.gr_paged_attn_workspace.restype = sz
         L.gr_paged_attn.argtypes = [vp, vp, vp, vp, vp, i32, pll, pll, i32, ctypes.c_float, vp, sz, vp]
         L.gr_norm_rotary.argtypes = [vp, vp, vp, vp, i32, pll, pll, vp, vp, i32, pll, pll, i32, i32, i32, vp, pll, vp]
-        L.gr_norm_rotary_bwd_workspace.argtypes = [i32] * 6
+        L.gr_norm_rotary_bwd_workspace.argtypes = [i32] * 5
         L.gr_norm_rotary_bwd_workspace.restype = sz
         L.gr_norm_rotary_bwd.argtypes = [vp, vp, vp, vp, vp, i32, pll, pll, pll, vp, vp, vp, i32, pll, pll, pll, i32, i32, i32,
                                          vp, pll, vp, vp, vp, sz, vp]

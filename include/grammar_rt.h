@@ -283,7 +283,7 @@ int gr_norm_rotary(const gr_rotary_spec* rotary, const gr_head_norm* norm, const
  * workspace: device memory of at least gr_norm_rotary_bwd_workspace(...) bytes, 16-byte
  * aligned, not read by calls to come (calls that may overlap in time need one each); not
  * needed without dq_weight and dk_weight. */
-size_t gr_norm_rotary_bwd_workspace(int Hq, int Hk, int head_dim, int dtype, int B, int N);
+size_t gr_norm_rotary_bwd_workspace(int Hq, int Hk, int head_dim, int B, int N);
 int gr_norm_rotary_bwd(const gr_rotary_spec* rotary, const gr_head_norm* norm, const void* q, const void* dq_out, void* dq,
                        int Hq, const long long* q_strides, const long long* dq_out_strides, const long long* dq_strides,
                        const void* k, const void* dk_out, void* dk, int Hk, const long long* k_strides,

@@ -95,13 +95,20 @@ def test_bad_norm_calls_are_refused():
                       ((r, n, d, far[0], 1, s, s, None, None, 0, None, None, 5, 1, 1, d, s, None), "dtype"),
                       ((r, n, d, far[0], 0, s, s, None, None, 0, None, None, bf, 1, 1, d, s, None), "head"),
                       ((r, n, d, far[0], 1, s, s, d, far[0], 1, s, s, bf, 1, 1, d, s, None), "memory"),
+                      ((r, n, far[1], d, 1, s, s, None, None, 0, None, None, bf, 1, 1, far[2], s, None), "weights"),
+                      ((r, n, far[1], far[2], 1, s, s, far[3], d + 64, 1, s, s, bf, 1, 1, far[4], s, None), "weights"),
                       ((r, n, d, far[0], 1, s, s, None, None, 0, None, None, bf, 1 << 16, 1 << 16, d, s, None), "positive")):
         assert L.gr_norm_rotary(*args) == rt.GR_E_ARG and msg in rt.last_error(), rt.last_error()
+
+    at_q = rt.HeadNormSpec(far[3], None, rt.GR_F32, 1e-6)
+    assert L.gr_paged_append_with(p(cache), None, p(batch), r, p(at_q), far[5], far[3], 8, s, s, far[6], far[6], s, s, None, None,
+                                  None) == rt.GR_E_ARG
+    assert "weights" in rt.last_error(), rt.last_error()
 
     def bwd(q=d, g=far[0], dq=far[1], k=far[2], gk=far[3], dk=far[4], wq=far[5], wk=far[6], ws=d + (9 << 24), size=1 << 20, N=1):
         return L.gr_norm_rotary_bwd(r, n, q, g, dq, 1, s, s, s, k, gk, dk, 1, s, s, s, bf, 1, N, d, s, wq, wk, ws, size, None)
     for kw, msg in ((dict(q=None), "null"), (dict(g=None), "null"), (dict(gk=None), "null"), (dict(dk=None), "null"), (dict(dq=far[3]), "memory"),
-                    (dict(dq=far[2]), "memory"), (dict(dq=far[4]), "memory"), (dict(wq=far[1]), "memory"), (dict(wk=far[4] + 64), "memory"),
+                    (dict(dq=far[2]), "memory"), (dict(dq=far[4]), "memory"), (dict(q=far[6], wk=None, dq=d + 96), "weights"), (dict(q=far[6], wk=None, dk=d), "weights"), (dict(wq=far[1]), "memory"), (dict(wk=far[4] + 64), "memory"),
                     (dict(wq=far[6]), "memory"), (dict(wq=far[5] + 2), "aligned"), (dict(ws=None), "workspace"), (dict(size=100), "workspace"),
                     (dict(ws=d + 4), "workspace"), (dict(N=0), "positive"), (dict(dq=d + 16, N=9), "memory")):
         assert bwd(**kw) == rt.GR_E_ARG and msg in rt.last_error(), (kw, rt.last_error())
@@ -110,12 +117,12 @@ def test_bad_norm_calls_are_refused():
 def test_norm_workspace_sizes():
     rt, *_ = _parts()
     size = rt.lib().gr_norm_rotary_bwd_workspace
-    assert size(8, 2, 64, rt.GR_BF16, 1, 1) == 2 * 64 * 4                   # one workgroup
-    many = size(32, 8, 128, rt.GR_BF16, 2, 4096)
+    assert size(8, 2, 64, 1, 1) == 2 * 64 * 4                   # one workgroup
+    many = size(32, 8, 128, 2, 4096)
     assert many % (2 * 128 * 4) == 0 and 1 << 18 <= many <= 1 << 23
     for bad in ((0, 2, 64), (8, -1, 64), (8, 2, 72), (8, 2, 512), (8, 2, 0)):
-        assert size(*bad, rt.GR_BF16, 1, 1) == 0
-    assert size(8, 2, 64, rt.GR_BF16, 0, 1) == 0
+        assert size(*bad, 1, 1) == 0
+    assert size(8, 2, 64, 0, 1) == 0
 
 
 def test_no_rows_are_no_work():
