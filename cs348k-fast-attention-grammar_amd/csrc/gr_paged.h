@@ -936,9 +936,22 @@ __device__ __forceinline__ void gr_paged_body(const gr_paged_args& a, char* lds)
       gr_paged_rows<T, D, BN, BM / 16, KG, WAVES, BM>(a, lds, t, hk, key0, key1, place);
     } else {
       if constexpr (KGS > 0) {
-        if (t.nrows <= 32) {
-          if constexpr (Q8) return gr_paged_rows<T, D, 32, 2, KGS, WAVES, BM>(a, lds, t, hk, key0, key1, place);
-          else return gr_paged_segment<T, D, 32, 1, KGS, 2, WAVES, BM, Q8>(a, lds, t, hk, key0, key1, place);
+        // Quantised, so are the part-filled tiles that chunks end in, and in two passes those of up
+        // to 64 rows (a workgroup a tile; in brackets as tiles of 128): 2,049 tokens of 4 heads
+        // to each of 8 among 8 single ones, 4,000-9,000 keys, 238 us (264), 2,064 tokens
+        // 235 (255); 1,025 alone 164 (219), 1,040 214 (220). Whole tiles follow sooner.
+        if (t.nrows - (Q8 ? t.row0 : 0) <= (Q8 && !SHARED ? 64 : 32)) {
+          if constexpr (Q8) {
+#pragma unroll 1
+            while (true) {
+              gr_paged_rows<T, D, 32, 2, KGS, WAVES, BM>(a, lds, t, hk, key0, key1, place);
+              t.row0 += 32;
+              if (t.row0 >= t.nrows) return;
+              __syncthreads();                                    // the merge's memory is free again
+            }
+          } else {
+            return gr_paged_segment<T, D, 32, 1, KGS, 2, WAVES, BM, Q8>(a, lds, t, hk, key0, key1, place);
+          }
         }
       }
       gr_paged_segment<T, D, BN, NW, KG, NS, WAVES, BM, Q8>(a, lds, t, hk, key0, key1, place);

@@ -305,6 +305,35 @@ def test_hidden_entries_may_hold_anything(dtype, D, n, G, Hkv, width):
     assert out[:2, :2 * G, -1].isnan().all() and out[:2, 2 * G:].isfinite().all()
 
 
+@pytest.mark.parametrize("dtype,D", [("bf16", 128), ("fp16", 64), ("fp16", 128)])
+@pytest.mark.parametrize("Hkv,width", [(24, None), (28, 2048), (40, None)], ids=["two groups", "shared", "tile"])
+@pytest.mark.parametrize("causal", [True, False])
+def test_part_filled_tiles_of_chunks(dtype, D, Hkv, width, causal):
+    """Chunks that end in a tile of 1, 4, 32, 33, 63, 64 and 65 of 128 rows, among sequences of as few; stale slots are
+    NaN, a page does not exist, and the last token of two sequences is NaN, which only rows that see it show."""
+    news = [129, 388, 160, 289, 191, 64, 40, 5, 193]
+    lens = [140, 388, 500, 300, 150, 64, 700, 5, 260]
+    print(f"[case] part-filled {dtype} D{D} Hkv{Hkv} causal={causal}", flush=True)
+    s = Setup8(lens, Hkv, 16, D, dtype, seed=Hkv, width=width)
+    live = torch.zeros(s.k.shape[0], s.S, dtype=torch.bool)
+    for b, m in enumerate(lens):
+        for j in range(m):
+            live[int(s.table[b, j // s.S]), j % s.S] = True
+    dead = (~live).to(s.dev)[:, None, :, None]
+    s.k.masked_fill_(dead, float("nan"))
+    s.v.masked_fill_(dead, float("nan"))
+    if causal:
+        for b in (0, 3):
+            page, slot = int(s.table[b, (lens[b] - 1) // s.S]), (lens[b] - 1) % s.S
+            s.k[page, 0, slot, 3] = s.v[page, 1, slot, 5] = float("nan")
+    s.put()
+    s.table[6, 7], s.table[2, 0] = -1, s.k.shape[0]
+    out = _run(s, news, Hkv, causal=causal, ragged=True, pad=3)
+    bad = out.isnan().any(-1).any(-1).nonzero().flatten().tolist()
+    last = [sum(news[:b + 1]) - 1 for b in (0, 3)]
+    assert bad == (last if causal else [])
+
+
 @pytest.mark.parametrize("width", [None, 2048], ids=["tile", "shared"])
 def test_pages_that_do_not_exist(width):
     from grammar.paged import paged_attention
