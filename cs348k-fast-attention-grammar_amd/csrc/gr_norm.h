@@ -8,10 +8,16 @@
 // `per` where tokens are few), and then those of other tokens; lane l has the same unit of 8 + 8
 // elements in every pass and token, so that it sums the weights' gradients of
 // its elements over all its rows in registers. r is computed again from x, which the
-// gradient reads in any case. The rows of the next pass are on their way while
-// one is worked on, and passes of one kind of rows make no choice of weights or sums. At its
-// end a workgroup adds its waves' sums and writes them beside the others'; a second launch
-// adds those up, in the order of the workgroups.
+// gradient reads in any case. The rows and position of the next pass are on their way while
+// one is worked on, the turns of a lane's pairs are kept, and passes of one kind of rows make
+// no choice of weights or sums. At its end a workgroup adds its waves' sums and writes them
+// beside the others'; a second launch adds those up, in the order of the workgroups.
+//
+// Bound by memory where tokens are many: 2 x 4,096 tokens of 32 + 8 heads of 128 (bf16, 252
+// MB) 56 us, 4.5 TB/s, by two waves a SIMD (209 registers: sums, weights and two passes'
+// rows) with 64 KB a CU on the way, and 4 for the second launch, a chain of trips to
+// memory. 300 tokens of 8 + 4 heads of 64 take 12.3 with it. Before every pass had as many
+// loads, whose number is then known, the first took 66.
 #pragma once
 #include "gr_rotary.h"
 
@@ -47,46 +53,66 @@ __device__ __forceinline__ void gr_norm_bwd_body(const gr_norm_bwd_args& a, floa
   const int lo = u0 < ru ? (INTER ? 16 * u0 : 8 * u0) : 2 * a.pairs + 8 * (u0 - ru);
   const int hi = u0 < ru ? (INTER ? 16 * u0 + 8 : a.pairs + 8 * u0) : lo + 8 * (units - ru);
   float wq[16], wk[16], sq[16] = {}, sk[16] = {};
-  gr_unit_weights<T>(a.wq, a.w32, lo, hi, wq);
-  gr_unit_weights<T>(a.wk, a.w32, lo, hi, wk);
+  gr_unit_weights<T> uq, uk;
+  uq.load(a.wq, a.w32, lo, hi, a.q.src);
+  uk.load(a.wk, a.w32, lo, hi, a.q.src);
+  uq.floats(a.wq, a.w32, wq);
+  uk.floats(a.wk, a.w32, wk);
   const float inv_d = 1.0f / (float)a.D;
 
-  // A task is `per` passes of a token.
-  const long long tasks = (long long)a.tokens * groups, step = (long long)gridDim.x * GR_NORM_WAVES;
+  // A task is `per` passes of a token, the part-th of it; a wave's next one is `step` tasks on.
+  const unsigned step = gridDim.x * GR_NORM_WAVES, step_tok = step / (unsigned)groups, step_part = step % (unsigned)groups;
   const int sub = lane / lanes;
   const bool all_units = units == lanes;
   struct pass_rows {
-    long long task;
-    int pass, b, i;                // of the token's; batch and token
+    unsigned tok;
+    int part, pass, b, i;          // part and pass of the token's; batch and token
+    int position;
     gr_rope8<T> x, y, gx, gy;
   };
-  auto load = [&](pass_rows& d, long long task, int pass) {
-    const int tok = (int)(task / groups), r = pass * rpp + sub;
-    d.task = task;
+  gr_unit_turns turns;
+  turns.load(a, u0 < ru ? u0 : 0);
+  // (in registers: a choice among arguments would become a load from a chosen address)
+  long long qsh = a.q.sh, ksh = a.k.sh, gqsh = a.gq.sh, gksh = a.gk.sh;
+  asm("" : "+s"(qsh), "+s"(ksh), "+s"(gqsh), "+s"(gksh));
+  const long long paxis = (a.naxes > 1 ? gr_imin(lane, a.naxes - 1) : 0) * a.ps[0];
+  // Rows past the token's last and lanes without elements read others': that every pass
+  // has as many loads lets the next one's stay in flight while one is worked on.
+  auto load = [&](pass_rows& d, unsigned tok, int part, int pass) {
+    const int r = gr_imin(pass * rpp + sub, rows - 1);
+    d.tok = tok;
+    d.part = part;
     d.pass = pass;
-    d.b = tok / a.per_seq;
-    d.i = tok - d.b * a.per_seq;
-    d.x = d.y = d.gx = d.gy = {};
-    if (unit && r < rows) {
-      auto source = [&](const gr_rope_rows& k, int h) { return static_cast<const T*>(k.src) + d.b * k.sb + d.i * k.st + h * k.sh; };
-      const T* const s = r < h0 ? source(a.q, r) : source(a.k, r - h0);
-      const T* const g = r < h0 ? source(a.gq, r) : source(a.gk, r - h0);
-      d.x.load(s + lo);
-      d.y.load(s + hi);
-      d.gx.load(g + lo);
-      d.gy.load(g + hi);
-    }
+    d.b = (int)tok / a.per_seq;
+    d.i = (int)tok - d.b * a.per_seq;
+    d.position = a.pos[d.b * a.ps[1] + d.i * a.ps[2] + paxis];
+    auto source = [&](const gr_rope_rows& k) { return static_cast<const T*>(k.src) + d.b * k.sb + d.i * k.st; };
+    const bool query = r < h0;
+    const int h = r - (query ? 0 : h0);
+    const T* const s = (query ? source(a.q) : source(a.k)) + h * (query ? qsh : ksh);
+    const T* const g = (query ? source(a.gq) : source(a.gk)) + h * (query ? gqsh : gksh);
+    d.x.load(s + lo);
+    d.y.load(s + hi);
+    d.gx.load(g + lo);
+    d.gy.load(g + hi);
   };
-  auto first_pass = [&](long long task) { return (int)(task % groups) * a.per; };
-  // The pass behind d's: of its task, or the first of the wave's next one; false behind the last.
-  auto next = [&](const pass_rows& d, long long& task, int& pass) {
-    task = d.task;
-    pass = d.pass + 1;
-    if (pass < passes && pass - first_pass(task) < a.per) return true;
-    task += step;
-    if (task >= tasks) return false;
-    pass = first_pass(task);
-    return true;
+  // Asks for the pass behind d's: of its task, or the first of the wave's next one; d's again
+  // and false behind the last.
+  auto load_next = [&](pass_rows& to, const pass_rows& d) {
+    unsigned tok = d.tok;
+    int part = d.part, pass = d.pass + 1;
+    if (pass >= passes || pass >= (part + 1) * a.per) {
+      tok += step_tok;
+      part += (int)step_part;
+      if (part >= groups) {
+        part -= groups;
+        ++tok;
+      }
+      pass = part * a.per;
+    }
+    const bool more = tok < (unsigned)a.tokens;
+    load(to, more ? tok : d.tok, more ? part : d.part, more ? pass : d.pass);
+    return more;
   };
   float sn[8] = {}, cs[8] = {};
   // KIND 0: rows of queries, 1: of keys, all live; 2: any.
@@ -102,6 +128,13 @@ __device__ __forceinline__ void gr_norm_bwd_body(const gr_norm_bwd_args& a, floa
       f[8 + e] = in.y.get(e);
       g[e] = in.gx.get(e);
       g[8 + e] = in.gy.get(e);
+    }
+    if (KIND == 2 && !all_units) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        f[e] = unit ? f[e] : 0.f;
+        g[e] = unit ? g[e] : 0.f;
+      }
     }
     if (u < ru) gr_turn_unit<INTER>(g, sn, cs);
     float h[16];
@@ -141,28 +174,25 @@ __device__ __forceinline__ void gr_norm_bwd_body(const gr_norm_bwd_args& a, floa
     t.template store<false>(d + hi);
   };
   auto pass = [&](const pass_rows& in) {
-    if (in.pass == first_pass(in.task))
-      gr_unit_angles(a, gr_position(a, a.pos + in.b * a.ps[1] + in.i * a.ps[2], 0, lane), a.naxes > 1, u0 < ru ? u0 : 0, true, sn, cs);
+    if (in.pass == in.part * a.per)
+      turns.angles(in.position, a.naxes > 1, true, sn, cs);
     const int r0 = in.pass * rpp;
     if (all_units && r0 + rpp <= h0) work(in, gr_const<0>{});
     else if (all_units && r0 >= h0 && r0 + rpp <= rows) work(in, gr_const<1>{});
     else work(in, gr_const<2>{});
   };
   pass_rows one, two;
-  long long task = (long long)blockIdx.x * GR_NORM_WAVES + wave_in;
-  int at = 0;
-  if (task < tasks) {
-    load(one, task, first_pass(task));
+  const unsigned task = blockIdx.x * GR_NORM_WAVES + (unsigned)wave_in;
+  if (task / (unsigned)groups < (unsigned)a.tokens) {
+    load(one, task / (unsigned)groups, (int)(task % (unsigned)groups), (int)(task % (unsigned)groups) * a.per);
 #pragma unroll 1
     while (true) {
-      const bool more = next(one, task, at);
-      if (more) load(two, task, at);
+      bool more = load_next(two, one);
       pass(one);
       if (!more) break;
-      const bool again = next(two, task, at);
-      if (again) load(one, task, at);
+      more = load_next(one, two);
       pass(two);
-      if (!again) break;
+      if (!more) break;
     }
   }
   if (a.part == nullptr) return;

@@ -334,7 +334,10 @@ struct gr_paged_lds {
 // through registers, are turned into T exactly (gr_from_e4m3) and written to LDS where
 // the 16-bit tile's loads would have put them, once for all waves that read them:
 // from there on the two are alike. Loads are a tile ahead of the one being written, which
-// is a tile ahead of the products. (Few rows: gr_paged_rows.)
+// is a tile ahead of the products. (Few rows: gr_paged_rows.) Tiles that every row sees in
+// full, with a next one of existing pages, convert behind the scores' products: 4,096 tokens
+// onto 4,096, 32 / 8 heads of 128 427-440 us, level with 16-bit rows; in one loop for all
+// tiles, between the barriers, 498.
 template <class T, int D, int BN, int NW, int KG, int NS, int WAVES, int BM, bool Q8>
 __device__ __forceinline__ void gr_paged_segment(const gr_paged_args& a, char* lds_all, const gr_paged_tile& t, int hk,
                                                  int key0, int key1, int place) {

@@ -19,10 +19,21 @@
 // all of its rows. The rows of all passes are requested before the angles are
 // computed.
 //
+// Rows that are normed (divided by their root mean square) or quantised are reduced, over
+// lanes of a power of two and without LDS. What a token's angles and weights are made of is
+// asked for before its rows, and every lane asks for as much, whatever it is for: the
+// compiler then knows how many loads are behind the ones it waits for, and angles are
+// computed while rows are on their way. (Rows asked for by the lanes that have one, angles'
+// turns behind them: 9,668 tokens of 32 + 8 + 8 heads of 128, normed into a quantised
+// cache, 53.7 us, now 47.5; without the norm 45.4 and 42.)
+//
 // Bound by memory once there are tokens enough: 2 x 4,096 tokens of 32 + 32 heads
 // of 128 (268 MB, bf16) take 43-52 us, 5.2-6.2 TB/s, where a large copy reaches
 // 5.15; 320 tokens of 4 + 4 heads of 64 take 4.0 us, a launch and two trips to
-// memory.
+// memory. Normed: 2 x 4,096 tokens of 32 + 8 heads of 128 (168 MB) 30.7 us, 5.5 TB/s; 288
+// tokens of 8 + 4 heads of 64 4.0; normed into a quantised cache, the 9,668 tokens above
+// (218 MB) 4.6 TB/s: four waves a SIMD (115 registers) with vector work of their own between
+// loads and stores, which without the norm is less (6 waves, 199 MB at 4.7).
 //
 // Stores that write whole lines go past the caches, where the attention that
 // reads the rows runs on other XCDs: 8,193 tokens of 32 + 8 + 8 heads of 128 into
@@ -128,22 +139,34 @@ __device__ __forceinline__ int gr_position(const A& a, const int* pos, int at, i
   return lane < a.naxes ? pos[lane * a.ps[0]] : 0;
 }
 
-// Sines and cosines of the 8 pairs of unit `u0` of a token at `position`; axes: it
-// differs by axis.
-template <class A>
-__device__ __forceinline__ void gr_unit_angles(const A& a, int position, bool axes, int u0, bool inverse, float (&sn)[8],
-                                               float (&cs)[8]) {
-  unsigned long long ax = 0;
-  if (axes) ax = *reinterpret_cast<const unsigned long long*>(a.axes + 8 * u0);
+// What the angles of the 8 pairs of a unit are made of, asked for before a token's rows are,
+// so that they are computed while the rows are on their way (loads return in order).
+struct gr_unit_turns {
+  unsigned long long turns[8], axes;
+  template <class A>
+  __device__ __forceinline__ void load(const A& a, int u0) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    int pe = position;
-    if (axes) pe = __shfl(position, (int)(ax >> (8 * e)) & 63, 64);
-    const unsigned long long t = (unsigned long long)(long long)pe * a.turns[8 * u0 + e];
-    gr_turn_sincos((unsigned)(t >> 32), sn[e], cs[e]);
-    if (inverse) sn[e] = -sn[e];
+    for (int e = 0; e < 8; ++e) turns[e] = a.turns[8 * u0 + e];
+    axes = 0;
+    if (a.naxes > 1) axes = *reinterpret_cast<const unsigned long long*>(a.axes + 8 * u0);
   }
-}
+  // Sines and cosines at `position`; by_axis: lane i has axis i's.
+  __device__ __forceinline__ void angles(int position, bool by_axis, bool inverse, float (&sn)[8], float (&cs)[8]) const {
+    int pe[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) pe[e] = position;
+    if (by_axis) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) pe[e] = __shfl(position, (int)(axes >> (8 * e)) & 63, 64);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const unsigned long long t = (unsigned long long)(long long)pe[e] * turns[e];
+      gr_turn_sincos((unsigned)(t >> 32), sn[e], cs[e]);
+      if (inverse) sn[e] = -sn[e];
+    }
+  }
+};
 
 // Sum, and largest as whole numbers, over the 1, 2, 4, 8 or 16 lanes of a group (a power of
 // two, aligned), for all of them: within four lanes, then by mirrors of 8 and 16, whose
@@ -171,32 +194,41 @@ __device__ __forceinline__ unsigned gr_group_umax(unsigned v, int lanes) {
 // Lanes of a head row that is reduced: its units, up to a power of two.
 __device__ __forceinline__ int gr_row_lanes(int units) { return units > 1 ? 1 << (32 - __builtin_clz(units - 1)) : 1; }
 
-// 16 weights of a lane's unit, from elements lo and hi on.
+// 16 weights of a lane's unit, from elements lo and hi on: asked for, and as floats. (Loads
+// whatever the weights are, from `any` where there are none: loads of one of two ways are
+// waited for where the ways join.)
 template <class T>
-__device__ __forceinline__ void gr_unit_weights(const void* w, int w32, int lo, int hi, float (&f)[16]) {
-  if (w == nullptr) {
+struct gr_unit_weights {
+  gr_u32x4 r[4];
+  __device__ __forceinline__ void load(const void* w, int w32, int lo, int hi, const void* any) {
+    const bool wide = sizeof(T) == 4 || w32;
+    const char* const p = static_cast<const char*>(w ? w : any);
+    const int size = w ? (wide ? 4 : 2) : 0, next = w && wide ? 16 : 0;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) f[e] = 1.f;
-  } else if (sizeof(T) == 4 || w32) {
-    gr_rope8<float> a, b;
-    a.load(static_cast<const float*>(w) + lo);
-    b.load(static_cast<const float*>(w) + hi);
+    for (int i = 0; i < 4; ++i) r[i] = gr_ld16(p + (i < 2 ? lo : hi) * size + (i & 1) * next);
+  }
+  __device__ __forceinline__ void floats(const void* w, int w32, float (&f)[16]) const {
+    if (w == nullptr) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      f[e] = a.get(e);
-      f[8 + e] = b.get(e);
-    }
-  } else {
-    gr_rope8<T> a, b;
-    a.load(static_cast<const T*>(w) + lo);
-    b.load(static_cast<const T*>(w) + hi);
+      for (int e = 0; e < 16; ++e) f[e] = 1.f;
+    } else if (sizeof(T) == 4 || w32) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      f[e] = a.get(e);
-      f[8 + e] = b.get(e);
+      for (int e = 0; e < 16; ++e) {
+        const unsigned u = r[e >> 2][e & 3];   // (a bit cast of the element itself reads element 0)
+        f[e] = __builtin_bit_cast(float, u);
+      }
+    } else {
+      gr_rope8<T> a, b;
+      a.w[0] = r[0];
+      b.w[0] = r[2];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        f[e] = a.get(e);
+        f[8 + e] = b.get(e);
+      }
     }
   }
-}
+};
 
 // Rotates a unit's 8 pairs by its sines and cosines: elements e and 8 + e, or 2e and 2e + 1.
 template <bool INTER>
@@ -267,8 +299,9 @@ __device__ __forceinline__ void gr_rope_body(const gr_rope_args& a, bool inverse
   const int row0 = (wave - tok * groups) * ITER * rpp + lane / lanes, u = lane % lanes;
   const int ru = a.pairs >> 3;                   // rotated units
   const bool lane_live = lane < rpp * lanes && u < units;
-  const int lo = u < ru ? (INTER ? 16 * u : 8 * u) : 2 * a.pairs + 8 * (u - ru);
-  const int hi = u < ru ? (INTER ? 16 * u + 8 : a.pairs + 8 * u) : lo + 8 * (units - ru);
+  const int u0 = !(NORM || Q8) || u < units ? u : 0;   // (a lane without elements reads the first unit's)
+  const int lo = u0 < ru ? (INTER ? 16 * u0 : 8 * u0) : 2 * a.pairs + 8 * (u0 - ru);
+  const int hi = u0 < ru ? (INTER ? 16 * u0 + 8 : a.pairs + 8 * u0) : lo + 8 * (units - ru);
 
   // the token's sequence and index in it
   int b, i, at = 0;
@@ -293,15 +326,41 @@ __device__ __forceinline__ void gr_rope_body(const gr_rope_args& a, bool inverse
   // first element of this token's head 0, per kind (wave-uniform)
   auto source = [&](const gr_rope_rows& k) { return static_cast<const T*>(k.src) + brow * k.sb + trow * k.st; };
   const T *sq = source(a.q), *sk = source(a.k), *sv = APPEND ? source(a.v) : nullptr;
+  const int* const pos = a.pos ? a.pos + brow * a.ps[1] + trow * a.ps[2] : nullptr;
+  gr_unit_turns unit_turns = {};
+  int position = 0;
+  if ((NORM || Q8) && a.pairs > 0) {
+    unit_turns.load(a, u0 < ru ? u0 : 0);
+    // (a load either way: one of two ways to a register would wait where they join)
+    position = *(pos ? pos + (a.naxes > 1 ? gr_imin(lane, a.naxes - 1) * a.ps[0] : 0) : a.lens);
+  }
+  gr_unit_weights<T> uq = {}, uk = {};
+  if constexpr (NORM) {
+    uq.load(a.wq, a.w32, lo, hi, h0 > 0 ? sq : sk);
+    uk.load(a.wk, a.w32, lo, hi, h0 > 0 ? sq : sk);
+  }
   gr_rope8<T> x[ITER], y[ITER];
+  if constexpr (NORM || Q8) {
+    // (in registers: a choice among arguments would become a load from a chosen address)
+    long long qsh = a.q.sh, ksh = a.k.sh, vsh = APPEND ? a.v.sh : 0;
+    asm("" : "+s"(qsh), "+s"(ksh), "+s"(vsh));
 #pragma unroll
-  for (int p = 0; p < ITER; ++p) {
-    const int r = row0 + p * rpp;
-    if (NORM || Q8) x[p] = y[p] = {};            // (lanes without elements add nothing to their row's sum)
-    if (lane_live && r < rows) {
-      const T* s = r < h0 ? sq + r * a.q.sh : !APPEND || r < h1 ? sk + (r - h0) * a.k.sh : sv + (r - h1) * a.v.sh;
+    for (int p = 0; p < ITER; ++p) {
+      const int r = gr_imin(row0 + p * rpp, rows - 1);             // (rows past the end: the last again)
+      const bool is_q = r < h0, is_k = !APPEND || r < h1;
+      const T* s = (is_q ? sq : is_k ? sk : sv) + (r - (is_q ? 0 : is_k ? h0 : h1)) * (is_q ? qsh : is_k ? ksh : vsh);
       x[p].load(s + lo);
       y[p].load(s + hi);
+    }
+  } else {
+#pragma unroll
+    for (int p = 0; p < ITER; ++p) {
+      const int r = row0 + p * rpp;
+      if (lane_live && r < rows) {
+        const T* s = r < h0 ? sq + r * a.q.sh : !APPEND || r < h1 ? sk + (r - h0) * a.k.sh : sv + (r - h1) * a.v.sh;
+        x[p].load(s + lo);
+        y[p].load(s + hi);
+      }
     }
   }
 
@@ -318,9 +377,11 @@ __device__ __forceinline__ void gr_rope_body(const gr_rope_args& a, bool inverse
   }
 
   float sn[8] = {}, cs[8] = {};
-  if (a.pairs > 0) {
-    const int* const pos = a.pos ? a.pos + brow * a.ps[1] + trow * a.ps[2] : nullptr;
-    gr_unit_angles(a, gr_position(a, pos, at, lane), pos && a.naxes > 1, u < ru ? u : 0, inverse, sn, cs);
+  if ((NORM || Q8) && a.pairs > 0) {
+    unit_turns.angles(pos ? position : at, pos && a.naxes > 1, inverse, sn, cs);
+  } else if (a.pairs > 0) {
+    unit_turns.load(a, u < ru ? u : 0);
+    unit_turns.angles(gr_position(a, pos, at, lane), pos && a.naxes > 1, inverse, sn, cs);
   }
 
   auto target = [&](const gr_rope_rows& k, bool cached) {
@@ -329,10 +390,11 @@ __device__ __forceinline__ void gr_rope_body(const gr_rope_args& a, bool inverse
   T* dq = target(a.q, false);
   if constexpr (NORM || Q8) {
     const bool unit = u < units;
+    const float inv_d = 1.0f / (float)a.D;
     float wq[16], wk[16];
     if constexpr (NORM) {
-      gr_unit_weights<T>(a.wq, a.w32, unit ? lo : 0, unit ? hi : 0, wq);
-      gr_unit_weights<T>(a.wk, a.w32, unit ? lo : 0, unit ? hi : 0, wk);
+      uq.floats(a.wq, a.w32, wq);
+      uk.floats(a.wk, a.w32, wk);
     }
 #pragma unroll
     for (int p = 0; p < ITER; ++p) {
@@ -343,11 +405,15 @@ __device__ __forceinline__ void gr_rope_body(const gr_rope_args& a, bool inverse
         f[e] = x[p].get(e);
         f[8 + e] = y[p].get(e);
       }
+      if (units != lanes) {                      // (lanes without elements add nothing to their row's sum)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) f[e] = unit ? f[e] : 0.f;
+      }
       if constexpr (NORM) {
         float ss = 0.f;
 #pragma unroll
         for (int e = 0; e < 16; ++e) ss = fmaf(f[e], f[e], ss);
-        const float rms = rsqrtf(gr_group_sum(ss, lanes) / (float)a.D + a.eps);
+        const float rms = rsqrtf(gr_group_sum(ss, lanes) * inv_d + a.eps);
         // rows of one kind in most passes: a scalar branch instead of a choice of each element
         const int first = (wave - tok * groups) * ITER * rpp + p * rpp;
         if (first + rpp <= h0) {

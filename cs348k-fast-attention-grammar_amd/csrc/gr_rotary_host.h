@@ -49,10 +49,10 @@ int launch(const gr_rope_args& a, int inverse, const char* who, hipStream_t st) 
   const int cus = gr::cu_count() > 0 ? gr::cu_count() : 256;
   int iter = passes < 2 || full < 8LL * cus ? 1 : passes == 2 || (sizeof(T) == 2 && a.D >= 128) ? 2 : 4;
   if constexpr (NORM || Q8) {
-    // Rows that are normed or quantised have more to compute a pass, behind which more loads
-    // hide: up to five, shared out evenly. Norm of 2 x 4,096 tokens of 32 + 8 heads of 128 (10
-    // passes) in twos 40 us, threes 37, fives 31; 9,668 tokens of 48 heads of 128
-    // into a quantised cache in twos 63, threes 53, fours 52; 1,024 tokens 10.8, in fours 8.7.
+    // Rows that are normed or quantised have more to compute for a token and a pass: up to
+    // five, shared out evenly. Norm of 2 x 4,096 tokens of 32 + 8 heads of 128 (10 passes) in
+    // twos 37.5 us, up to three 34.3, fives 30.8; 9,668 tokens of 48 heads of 128 (6) into a
+    // quantised cache in twos 56.6, threes 47.7.
     const int groups = (passes + 4) / 5;
     iter = full < 8LL * cus ? 1 : (passes + groups - 1) / groups;
     if (iter == 5) return launch_iter<T, APPEND, INTER, PAST, NORM, Q8, 5>(a, passes, inverse, who, st);
