@@ -14,10 +14,10 @@
 // beside the others'; a second launch adds those up, in the order of the workgroups.
 //
 // Bound by memory where tokens are many: 2 x 4,096 tokens of 32 + 8 heads of 128 (bf16, 252
-// MB) 56 us, 4.5 TB/s, by two waves a SIMD (209 registers: sums, weights and two passes'
+// MB) 49 us, 5.1 TB/s, by two waves a SIMD (209 registers: sums, weights and two passes'
 // rows) with 64 KB a CU on the way, and 4 for the second launch, a chain of trips to
 // memory. 300 tokens of 8 + 4 heads of 64 take 12.3 with it. Before every pass had as many
-// loads, whose number is then known, the first took 66.
+// loads, whose number is then known, the first took 62.
 #pragma once
 #include "gr_rotary.h"
 

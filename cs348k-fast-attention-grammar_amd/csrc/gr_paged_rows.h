@@ -20,7 +20,7 @@
 // Measured (bf16, 32 / 8 heads of 128). A token each of 64 sequences of 200 to 11,000 keys
 // (672 MB) takes 122 us in tiles of 16 rows, 5.5 TB/s, and 4.7 for the merge: bound by memory
 // (matrix cores 8 % busy, vector units 26 %). With keys through LDS like values, in tiles of
-// 32 rows, 155. Four tokens of 40 / 8 heads each of 12 sequences of 900 to 9,000 keys (111 MB,
+// 32 rows, 167 in all. Four tokens of 40 / 8 heads each of 12 sequences of 900 to 9,000 keys (111 MB,
 // tiles of 32 rows) 28 and 4.2: eight key steps a wave, the first tile's way and the merge
 // inside the workgroup. 613 keys of one token (16 heads of 64) 6.1, a launch and a chain of
 // trips: length, page id, rows, two or three key steps of eight waves and their merge.

@@ -21,7 +21,7 @@ from .rotary import (Rotary, _dense, _has_tangent, _tokens, check_out, check_pos
 class HeadNorm:
     """The norm of heads: q_weight and k_weight are contiguous [head_dim] tensors on
     the GPU, both in float32 or both in the heads' dtype, or None for no weights;
-    eps is added to the mean square."""
+    eps is added to the mean square (with 0, a row of zeros is NaN)."""
 
     def __init__(self, q_weight=None, k_weight=None, eps: float = 1e-6):
         if not 0.0 <= eps < 1e30:

@@ -258,8 +258,8 @@ int gr_rotary(const gr_rotary_spec* rotary, const void* q, void* q_out, int Hq, 
 
 /* A norm of query and key heads: a row x of D elements becomes w x / sqrt(mean
  * x^2 + eps), w its D weights. q_weight, k_weight: device arrays, 16-byte aligned, of
- * dtype GR_F32 or the rows' type; NULL: ones. eps: not negative. No counterpart in
- * the reference. */
+ * dtype GR_F32 or the rows' type; NULL: ones. eps: not negative (with 0 a row of zeros
+ * is NaN). No counterpart in the reference. */
 typedef struct gr_head_norm {
   const void* q_weight;
   const void* k_weight;
