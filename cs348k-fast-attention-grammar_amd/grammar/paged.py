@@ -219,7 +219,7 @@ def _append_args(k, v, cache, table, lens, starts, q, rotary, norm, positions, m
         return rt.lib().gr_paged_append, (cache.ref, ctypes.addressof(desc), ref) + args, out, keep
     spec = None if norm is None else norm.spec(cache.head_dim, cache.dtype, cache.index, who)
     args = (cache.ref, cache.scales_ref, ctypes.addressof(desc), ref, None if spec is None else ctypes.addressof(spec)) + args
-    return rt.lib().gr_paged_append_with, args, out, keep + (spec, norm)
+    return rt.lib().gr_paged_append_with, args, out, keep + (spec,) + (() if norm is None else (norm.q_weight, norm.k_weight))
 
 
 def paged_append(k, v, cache: PagedCache | QuantizedPagedCache, table, lens, *, starts=None, q=None,
@@ -343,7 +343,7 @@ def paged_read(cache: PagedCache | QuantizedPagedCache, table, lens, length: int
     if made:
         if starts is not None or length is None or int(length) < 0:
             raise ValueError(f"{who}: needs a length, or k_out and v_out")
-        shape = (table.shape[0], cache.heads, int(length), cache.head_dim)
+        shape = (table.shape[0] if table.dim() == 2 else 0, cache.heads, int(length), cache.head_dim)
         k_out, v_out = rt.result(shape, cache.dtype, cache.k.device, stream), rt.result(shape, cache.dtype, cache.k.device, stream)
     elif length is not None and (starts is not None or k_out.dim() != 4 or k_out.shape[2] != length):
         raise ValueError(f"{who}: k_out {tuple(k_out.shape)} is not of length {length}")

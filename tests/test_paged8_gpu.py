@@ -783,6 +783,26 @@ def test_bound_steps_on_streams_and_in_graphs():
         assert torch.equal(got, eager) and all(torch.equal(a, b) for a, b in zip(back, back2))
 
 
+def test_a_binding_keeps_its_weights():
+    """Weights that a norm gets after a call was bound are not the binding's, and those it was bound with stay."""
+    import gc
+    import weakref
+    from grammar.norm import HeadNorm
+    from grammar.paged import bind_paged_append, paged_append
+    s = Setup8([20, 33], 2, 16, 64, "bf16", seed=3)
+    q, k = s.randn(2, 4, 3, 64), s.randn(2, 2, 3, 64)
+    norm = HeadNorm(*(1 + 0.2 * torch.randn(64, device=s.dev) for _ in range(2)))
+    want = paged_append(k, k, s.cache, s.table, s.lens, q=q, norm=norm)
+    add, out = bind_paged_append(k, k, s.cache, s.table, s.lens, q=q, norm=norm)
+    held = [weakref.ref(w) for w in (norm.q_weight, norm.k_weight)]
+    norm.q_weight = norm.k_weight = None
+    gc.collect()
+    assert all(w() is not None for w in held)
+    add()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+
+
 def test_calls_of_two_threads_at_once():
     import threading
     from grammar.paged import paged_append, paged_attention
@@ -898,7 +918,8 @@ def test_refusals():
                 lambda: append(k=k.bfloat16(), v=k.bfloat16()), lambda: append(q=q), lambda: append(out=q),
                 lambda: append(q=q, norm=HeadNorm(w.bfloat16())), lambda: append(q=q, norm=HeadNorm(w[:32])),
                 lambda: append(q=q, norm=HeadNorm(w), positions=s.lens), lambda: paged_attention(q.bfloat16(), s.cache, s.table, s.lens),
-                lambda: read(), lambda: read(-1), lambda: read(starts=starts), lambda: read(10, starts=starts),
+                lambda: paged_read(s.cache, s.table[0], s.lens, 5), lambda: paged_read(s.cache, s.table[0, 0], s.lens, 5),
+                lambda: paged_read(s.cache, s.table, s.lens[:1], 5), lambda: read(), lambda: read(-1), lambda: read(starts=starts), lambda: read(10, starts=starts),
                 lambda: read(k_out=s.randn(2, 2, 20, 64)), lambda: read(20, k_out=s.randn(2, 2, 21, 64), v_out=s.randn(2, 2, 21, 64)),
                 lambda: read(k_out=s.randn(2, 3, 20, 64), v_out=s.randn(2, 3, 20, 64)),
                 lambda: read(k_out=s.randn(2, 2, 20, 64).bfloat16(), v_out=s.randn(2, 2, 20, 64).bfloat16()),
