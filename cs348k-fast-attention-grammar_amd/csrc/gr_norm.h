@@ -156,9 +156,9 @@ __device__ __forceinline__ void gr_norm_bwd_body(const gr_norm_bwd_args& a, floa
       } else if constexpr (KIND == 1) {
         sk[e] = fmaf(g[e] * rms, f[e], sk[e]);
       } else {
-        const float v = live ? g[e] * rms * f[e] : 0.f, vq = query ? v : 0.f;
-        sq[e] += vq;
-        sk[e] += v - vq;
+        const float v = live ? g[e] * rms * f[e] : 0.f;   // (no differences: a NaN stays in its own sum)
+        sq[e] += query ? v : 0.f;
+        sk[e] += query ? 0.f : v;
       }
       h[e] = rms * fmaf(-c, f[e], h[e]);
     }

@@ -1,0 +1,38 @@
+"""Gradients of normed and rotated heads: what queries' and keys' weights share, and calls whose waves
+walk over several tokens."""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+from test_norm_gpu import _inputs  # noqa: E402
+from test_rotary_gpu import _cuda  # noqa: E402
+
+
+@pytest.mark.parametrize("B,N,Hq,Hk,D,rd,dtype,weights", [
+    (1, 20, 3, 2, 64, 64, "fp32", "same"),          # all heads in one pass
+    (2, 33, 9, 3, 128, 64, "bf16", "fp32"),         # the last query head beside the keys'
+    (1, 40, 5, 4, 80, 48, "fp16", "same"),          # lanes without elements
+    (1, 700, 17, 2, 64, 32, "fp16", "fp32"),
+])
+@pytest.mark.parametrize("what", ["x", "gradient"])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_values_that_are_not_finite_reach_their_own_weights_only(B, N, Hq, Hk, D, rd, dtype, weights, what, value):
+    """Queries and keys that one pass works on: a query's NaN or infinity is in no sum of the keys' weights, nor a key's
+    in the queries'."""
+    dev = _cuda()
+    from grammar.norm import norm_rotary_bwd
+    print(f"[case] weights B{B} N{N} H{Hq}/{Hk} D{D}/{rd} {dtype} {weights} {what} {value}", flush=True)
+    g, rot, norm, q, k, pos = _inputs(B, N, Hq, Hk, D, rd, None, False, dtype, weights, dev)
+    dq, dk = (torch.randn(t.shape, generator=g).to(t.dtype).to(dev) for t in (q, k))
+    want = norm_rotary_bwd(q, k, pos, rot, norm, dq, dk)
+    assert all(t.isfinite().all() for t in want[2:])
+    for i, (x, dy) in enumerate(((q, dq), (k, dk))):
+        to = x if what == "x" else dy
+        keep = to.clone()
+        to[B - 1, -1 if i == 0 else 0, N // 2, 5] = value
+        got = norm_rotary_bwd(q, k, pos, rot, norm, dq, dk)
+        to.copy_(keep)
+        assert torch.equal(got[3 - i], want[3 - i]) and torch.equal(got[1 - i], want[1 - i])
+        assert not got[2 + i].isfinite().all()
