@@ -156,9 +156,13 @@ def _autograd_function():
             return recorded(ctx, dq, dk) if torch.is_grad_enabled() else gradients(ctx, dq, dk)
 
     def gradients(ctx, dq, dk):
-        # queries and keys in one launch where the gradients of both came
+        # queries and keys in one launch where the gradients of both came and are of use
         q, k, q_weight, k_weight, positions = ctx.saved_tensors
-        _, _, want_q, want_k = ctx.needs_input_grad[:4]
+        need_q, need_k, want_q, want_k = ctx.needs_input_grad[:4]
+        if not (need_q or want_q):
+            dq = None
+        if not (need_k or want_k):
+            dk = None
         if dq is None and dk is None:
             return (None,) * 7
         if dq is None:                                         # keys alone, as the queries of a call

@@ -36,3 +36,28 @@ def test_values_that_are_not_finite_reach_their_own_weights_only(B, N, Hq, Hk, D
         to.copy_(keep)
         assert torch.equal(got[3 - i], want[3 - i]) and torch.equal(got[1 - i], want[1 - i])
         assert not got[2 + i].isfinite().all()
+
+
+@pytest.mark.parametrize("frozen", ["q", "k"])
+@pytest.mark.parametrize("weights", [None, "frozen", "trained"])
+def test_a_side_without_gradients_is_left_out(frozen, weights, monkeypatch):
+    """Queries or keys that need no gradient, nor do their weights: the backward pass does not read or write them."""
+    dev = _cuda()
+    from grammar import norm as gn
+    from grammar.rotary import Rotary
+    rot, pos = Rotary(64, device=dev), torch.arange(40, dtype=torch.int32, device=dev)
+    q, k = torch.randn((2, 6, 40, 64), device=dev).bfloat16(), torch.randn((2, 2, 40, 64), device=dev).bfloat16()
+    leaf = (k if frozen == "q" else q).requires_grad_()
+    w = [None, None] if weights is None else [1 + 0.2 * torch.randn(64, device=dev) for _ in range(2)]
+    if weights == "trained":                                        # the other side's
+        w[frozen == "q"].requires_grad_()
+    dq, dk = torch.randn_like(q), torch.randn_like(k)
+    calls, bwd = [], gn._bwd
+    monkeypatch.setattr(gn, "_bwd", lambda *a, **kw: (calls.append(a[:2]), bwd(*a, **kw))[1])
+    wanted = [leaf] + [t for t in w if t is not None and t.requires_grad]
+    got = torch.autograd.grad(gn.norm_rotary(q, k, pos, rot, gn.HeadNorm(*w)), wanted, (dq, dk))
+    assert [tuple(None if t is None else t.data_ptr() for t in c) for c in calls] == [(leaf.data_ptr(), None)]
+    mine, g = (w[1], dk) if frozen == "q" else (w[0], dq)
+    want = bwd(leaf.detach(), None, pos, rot, None if mine is None else mine.detach(), None, 1e-6, g, None, weights == "trained", False)
+    assert torch.equal(got[0], want[0])
+    assert len(got) == 1 or torch.equal(got[1], want[2])
