@@ -50,8 +50,11 @@ def _spec(q, k, eps, head_dim, dtype, index, who):
 
 
 @functools.lru_cache(maxsize=4096)
-def _bwd_workspace(*sizes):
-    return int(rt.lib().gr_norm_rotary_bwd_workspace(*sizes))
+def _bwd_workspace(index, *sizes):
+    """Bytes of a call on GPU `index`, whose compute units share it out."""
+    import torch
+    with torch.cuda.device(index):
+        return int(rt.lib().gr_norm_rotary_bwd_workspace(*sizes))
 
 
 def _sizes(q, k, rot, who):
@@ -124,7 +127,7 @@ def _bwd(q, k, positions, rot, q_weight, k_weight, eps, dq_out, dk_out, want_q, 
         with torch.cuda.stream(torch.cuda.current_stream(q.device) if stream is None else rt.torch_stream(stream, q.device)):
             return (*outs, *(None if w is None else w.zero_() for w in dws))
     code = rt.dtype_code(q.dtype)
-    need = 0 if dws[0] is None and dws[1] is None else _bwd_workspace(Hq, Hk, rot.head_dim, B, N)
+    need = 0 if dws[0] is None and dws[1] is None else _bwd_workspace(rot.index, Hq, Hk, rot.head_dim, B, N)
     ws = rt.workspace(need, q.device, stream) if need else None
 
     def side(x, g, d, H, st):
