@@ -20,8 +20,9 @@ from .rotary import (Rotary, _dense, _has_tangent, _tokens, check_out, check_pos
 
 class HeadNorm:
     """The norm of heads: q_weight and k_weight are contiguous [head_dim] tensors on
-    the GPU, both in float32 or both in the heads' dtype, or None for no weights;
-    eps is added to the mean square (with 0, a row of zeros is NaN)."""
+    the GPU, at 16-byte aligned addresses, both in float32 or both in the heads' dtype,
+    or None for no weights; eps is added to the mean square (with 0, a row of zeros is
+    NaN, and rows are normed from magnitudes of 2^-60 on: squares of less are lost)."""
 
     def __init__(self, q_weight=None, k_weight=None, eps: float = 1e-6):
         if not 0.0 <= eps < 1e30:
@@ -77,8 +78,8 @@ def _sizes(q, k, rot, who):
 
 def norm_rotary_fwd(q, k, positions, rot: Rotary, norm: HeadNorm, *, out=None, k_out=None, stream=None):
     """rotary_fwd of normed heads: q [B, Hq, N, D] and k [B, Hk, N, D] (or None),
-    fp16, bf16 or fp32, each row normed by `norm` in fp32 (magnitudes up to 2^60)
-    and turned to its position; other arguments, and what is returned, as
+    fp16, bf16 or fp32, each row normed by `norm` in fp32 (magnitudes up to 2^59,
+    beyond which the squares' sum is no fp32 number) and turned to its position; other arguments, and what is returned, as
     rotary_fwd's."""
     who = "norm_rotary"
     B, N, Hq, qs, Hk, ks = _sizes(q, k, rot, who)

@@ -259,7 +259,8 @@ int gr_rotary(const gr_rotary_spec* rotary, const void* q, void* q_out, int Hq, 
 /* A norm of query and key heads: a row x of D elements becomes w x / sqrt(mean
  * x^2 + eps), w its D weights. q_weight, k_weight: device arrays, 16-byte aligned, of
  * dtype GR_F32 or the rows' type; NULL: ones. eps: not negative (with 0 a row of zeros
- * is NaN). No counterpart in the reference. */
+ * is NaN, and rows are normed from magnitudes of 2^-60 on). No counterpart in the
+ * reference. */
 typedef struct gr_head_norm {
   const void* q_weight;
   const void* k_weight;
@@ -268,7 +269,8 @@ typedef struct gr_head_norm {
 } gr_head_norm;
 
 /* gr_rotary of normed heads, in one pass over them; arguments as there. Squares,
- * norm, weights and rotation in fp32 (magnitudes up to 2^60), rounded once. */
+ * norm, weights and rotation in fp32 (magnitudes up to 2^59: 256 squares of 2^60 are no
+ * fp32 number), rounded once. */
 int gr_norm_rotary(const gr_rotary_spec* rotary, const gr_head_norm* norm, const void* q, void* q_out, int Hq,
                    const long long* q_strides, const long long* q_out_strides, const void* k, void* k_out, int Hk,
                    const long long* k_strides, const long long* k_out_strides, int dtype, int B, int N,

@@ -1,13 +1,13 @@
-"""Gradients of normed and rotated heads: what queries' and keys' weights share, and calls whose waves
-walk over several tokens."""
+"""Gradients of normed and rotated heads: what queries' and keys' weights share, what is not needed, magnitudes at the
+ends of the range."""
 import pytest
 
 pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
 
-from test_norm_gpu import _inputs  # noqa: E402
-from test_rotary_gpu import _cuda  # noqa: E402
+from test_norm_gpu import BWD, FWD, _check, _gradients, _inputs, _normed, _size, _turned  # noqa: E402
+from test_rotary_gpu import DT, _cuda  # noqa: E402
 
 
 @pytest.mark.parametrize("B,N,Hq,Hk,D,rd,dtype,weights", [
@@ -61,3 +61,29 @@ def test_a_side_without_gradients_is_left_out(frozen, weights, monkeypatch):
     want = bwd(leaf.detach(), None, pos, rot, None if mine is None else mine.detach(), None, 1e-6, g, None, weights == "trained", False)
     assert torch.equal(got[0], want[0])
     assert len(got) == 1 or torch.equal(got[1], want[2])
+
+
+@pytest.mark.parametrize("D,dtype,weights", [(256, "fp32", "same"), (256, "bf16", "fp32"), (128, "bf16", "same"), (64, "fp32", None)])
+@pytest.mark.parametrize("power,eps", [(59, 1e-6), (59, 0.0), (-60, 0.0), (-60, 1e-6)])
+def test_magnitudes_at_the_ends_of_the_range(D, dtype, weights, power, eps):
+    """Rows of magnitudes up to 2^59, one of them that number throughout (256 squares of 2^60 are no fp32 number), and,
+    without eps, from 2^-60 on: forward and gradient."""
+    dev = _cuda()
+    from grammar.norm import HeadNorm, norm_rotary_bwd, norm_rotary_fwd
+    print(f"[case] ends D{D} {dtype} {weights} 2^{power} eps {eps}", flush=True)
+    g, rot, norm, q, k, pos = _inputs(2, 19, 5, 2, D, D, None, False, dtype, weights, dev)
+    q, k = ((torch.rand(t.shape, generator=g) + 1) * 2.0 ** (power - 1) * (torch.randint(0, 2, t.shape, generator=g) * 2 - 1) for t in (q, k))
+    q[1, 2, 3], k[0, 1, 4] = 2.0 ** power, -2.0 ** power
+    q, k = q.to(DT[dtype]).to(dev), k.to(DT[dtype]).to(dev)
+    assert q.abs().max() == 2.0 ** power and k.abs().max() == 2.0 ** power
+    norm = HeadNorm(norm.q_weight, norm.k_weight, eps)
+    got = norm_rotary_fwd(q, k, pos, rot, norm)
+    dq, dk = (torch.randn(t.shape, generator=g).to(t.dtype).to(dev) for t in (q, k))
+    back = norm_rotary_bwd(q, k, pos, rot, norm, dq, dk)
+    for i, (x, dy, w) in enumerate(((q, dq, norm.q_weight), (k, dk, norm.k_weight))):
+        y, size = _turned(_normed(x, w, eps)[0], pos, rot)
+        _check(got[i], y, _size(y, size), "rows", FWD)
+        dx, dw, xs, ws = _gradients(x, dy, w, pos, rot, eps)
+        _check(back[i], dx, xs, "gradient", BWD)
+        if w is not None:
+            _check(back[2 + i], dw, ws, "weights' gradient", 100 * 2.0 ** -24)
