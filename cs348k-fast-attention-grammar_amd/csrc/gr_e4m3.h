@@ -7,9 +7,9 @@
 template <bool Q8> struct gr_bytes { typedef unsigned short type; };
 template <> struct gr_bytes<true> { typedef unsigned char type; };
 
-// Two numbers of a word times a scale, as T: exact where T can hold them
-// (v_cvt_scalef32_pk_{bf16,f16}_fp8, which takes the exponent of `scale`: checked for every
-// byte and scale).
+// Two numbers of a word times a scale, as T: exact where T can hold them, the nearest
+// number (to even) below its normal range (v_cvt_scalef32_pk_{bf16,f16}_fp8, which takes the
+// exponent of `scale`: checked for every byte and scale).
 template <class T, bool HIGH>
 __device__ __forceinline__ unsigned gr_from_e4m3(unsigned w, float scale) {
   if constexpr (__is_same(T, _Float16))

@@ -331,7 +331,7 @@ struct gr_paged_lds {
 // where its partial result of BM rows goes, or -1 for a tile that is done here.
 //
 // Q8: the cache holds e4m3 bytes and power-of-two scales. A tile's bytes come
-// through registers, are turned into T exactly (gr_from_e4m3) and written to LDS where
+// through registers, are turned into T (gr_from_e4m3) and written to LDS where
 // the 16-bit tile's loads would have put them, once for all waves that read them:
 // from there on the two are alike. Loads are a tile ahead of the one being written, which
 // is a tile ahead of the products. (Few rows: gr_paged_rows.) Tiles that every row sees in

@@ -1,7 +1,8 @@
 // gr_paged_read.h -- a paged cache's sequences as dense keys and values.
 //
 // Row j of a sequence comes from slot j % S of page table[j / S], a quantised one as
-// its e4m3 numbers times its power of two, which v_cvt_scalef32_pk gives exactly.
+// its e4m3 numbers times its power of two, which v_cvt_scalef32_pk gives exactly where T holds
+// them and rounded to nearest below T's normal range.
 //
 // Layout: D / 8 lanes have a row, 8 elements each, so that a store instruction writes
 // whole lines. A wave takes the 512 / D rows of one place for a run of heads, keys and

@@ -283,8 +283,9 @@ __device__ __forceinline__ void gr_store_e4m3(const gr_rope_args& a, float (&f)[
 // e4m3 numbers z 2^-k, k the least power (-127 at least) by which the row's
 // largest magnitude is at most 448, and k + 127 beside them. z 2^-k is exact, so the only rounding is
 // the one to e4m3's four bits, and an attention gets the value back in bf16 or
-// fp16 as it is: rows are clamped to the largest such number of the type first, 61,440
-// in fp16 and 15 2^124 in bf16. A row with a value that is not finite is NaN all over.
+// fp16 as it is (but for normed or turned keys below the type's normal range, which it
+// rounds to the type's smallest steps): rows are clamped to the largest number of four bits
+// in the type first, 61,440 in fp16 and 15 2^124 in bf16. A row with a value that is not finite is NaN all over.
 template <class T, bool APPEND, bool INTER, int ITER, bool PAST, bool NORM = false, bool Q8 = false>
 __device__ __forceinline__ void gr_rope_body(const gr_rope_args& a, bool inverse) {
   const int lane = threadIdx.x & 63;

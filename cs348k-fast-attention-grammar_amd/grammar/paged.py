@@ -85,8 +85,14 @@ class QuantizedPagedCache:
     A row x is held as round(x / scale), scale the least power of two (2^-127 at
     least) by which its largest magnitude is at most 448: four significant
     bits, 2^-4 of each element, and where an element is below 2^-14 of the largest half of
-    2^-17 of that. Rows are clamped to 61440 (fp16) or 15 2^124 (bf16) first, so that each
-    stands for numbers of the tokens' type. A row with a value that is not finite becomes NaN."""
+    2^-17 of that. Rows are clamped to 61440 (fp16) or 15 2^124 (bf16) first, so that none
+    stands for more than the tokens' type holds. A row with a value that is not finite becomes NaN.
+
+    Attention and paged_read take a row's numbers times its scale in the tokens' type. Where
+    that has no such number, the nearest one is taken, a whole number of 2^-24 (fp16) or 2^-133
+    (bf16): under scales below 2^-15 or 2^-124, which tokens of the type stored as they are do
+    not need, but keys that a norm or a rotation made small have (in fp16, rows of at most 448
+    2^-16)."""
 
     def __init__(self, k, v, scales, dtype):
         import torch

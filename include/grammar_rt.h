@@ -345,8 +345,10 @@ int gr_paged_append(const gr_paged_cache* cache, const gr_paged_batch* batch, co
  * bits, at most 448) by strides that are multiples of 16, and its dtype is that of the
  * tokens, GR_F16 or GR_BF16. scales: bytes [pages][heads][2: key, value][page_size] by
  * strides {page, head, key to value} that are non-negative multiples of 16, unit stride
- * along the slots, 16-byte aligned, each b standing for 2^(b - 127), or NaN for 255 (E8M0). A row stands for its numbers times its scale, which
- * are numbers of the tokens' type. */
+ * along the slots, 16-byte aligned, each b standing for 2^(b - 127), or NaN for 255 (E8M0). A row
+ * stands for its numbers times its scale, in the tokens' type: where that has no such number
+ * (below its normal range, under scales below 2^-15 in fp16 and 2^-124 in bf16, as keys that a
+ * norm or a rotation made small can have) the nearest one, a whole number of its smallest steps. */
 typedef struct gr_paged_scales {
   void* scales;
   long long strides[3];
@@ -354,7 +356,7 @@ typedef struct gr_paged_scales {
 
 /* gr_paged_append of normed queries and keys (norm NULL: none) into a cache that
  * is quantised (scales NULL: it is not). A row is quantised after norm and rotation,
- * in fp32: its scale is the least power of two, 2^-127 at least, by which its
+ * from fp32: its scale is the least power of two, 2^-127 at least, by which its
  * largest magnitude is at most 448, its numbers are rounded to nearest even. Rows
  * are clamped to 61440 (fp16) or 15 2^124 (bf16) first; a row with a value that is not finite becomes
  * NaN. Other arguments as gr_paged_append's, of which this is the general form. */
@@ -392,7 +394,7 @@ int gr_paged_attn(const gr_paged_cache* cache, const gr_paged_batch* batch, cons
                   size_t workspace_bytes, void* stream);
 
 /* The same over a quantised cache: keys and values are taken as the numbers of
- * the tokens' type that they stand for. The workspace has a size of its own. */
+ * the tokens' type that they stand for (gr_paged_scales). The workspace has a size of its own. */
 size_t gr_paged_attn_scaled_workspace(const gr_paged_cache* cache, const gr_paged_scales* scales, const gr_paged_batch* batch,
                                       int Hq);
 int gr_paged_attn_scaled(const gr_paged_cache* cache, const gr_paged_scales* scales, const gr_paged_batch* batch,
