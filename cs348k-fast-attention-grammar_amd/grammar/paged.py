@@ -84,8 +84,9 @@ class QuantizedPagedCache:
 
     A row x is held as round(x / scale), scale the least power of two (2^-127 at
     least) by which its largest magnitude is at most 448: four significant
-    bits, 2^-4 of each element, and where an element is below 2^-14 of the largest half of
-    2^-17 of that. Rows are clamped to 61440 (fp16) or 15 2^124 (bf16) first, so that none
+    bits, off by at most 2^-4 of each element or, where that is more, 2^-10 of the scale (of
+    an element below 2^-6 of it; 2^-17.8 of the row's largest magnitude, if that is 2^-119
+    or more). Rows are clamped to 61440 (fp16) or 15 2^124 (bf16) first, so that none
     stands for more than the tokens' type holds. A row with a value that is not finite becomes NaN.
 
     Attention and paged_read take a row's numbers times its scale in the tokens' type. Where

@@ -1,5 +1,5 @@
-"""What the numbers of a quantised cache stand for: numbers below the tokens' type's normal range, and
-keys that a norm made small."""
+"""What the numbers of a quantised cache stand for: numbers below the tokens' type's normal range, the bounds of what
+quantising loses, and keys that a norm made small."""
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -8,7 +8,7 @@ torch = pytest.importorskip("torch")
 
 from test_norm_gpu import FWD, _normed  # noqa: E402
 from test_paged_gpu import _cuda, _rotated  # noqa: E402
-from test_paged8_gpu import E4M3, E8M0, _check_rows, _dequantised  # noqa: E402
+from test_paged8_gpu import E4M3, E8M0, _check_rows, _dequantised, _scale_of  # noqa: E402
 
 DT = {"fp16": torch.float16, "bf16": torch.bfloat16}
 # scale exponents about the least under which the type holds every number, and that least: fp16's and bf16's smallest
@@ -54,6 +54,32 @@ def test_numbers_below_the_normal_range_round_once_more(dtype):
         for h in range(5):
             x = got[:, :, h].reshape(16, 256)
             assert torch.equal(x.isnan(), stand.isnan()) and torch.equal(x[held].double(), want[held])
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_what_quantising_loses(dtype, D):
+    """2^-4 of an element at most, or 2^-10 of the scale, which is 2^-17.8 of the row's largest magnitude; the latter in
+    full by a row of 225 and nearly 1.5 steps."""
+    from grammar.paged import QuantizedPagedCache, paged_append, paged_read
+    dev, dt = _cuda(), DT[dtype]
+    g = torch.Generator("cpu").manual_seed(D)
+    x = torch.randn((1, 4, 300, D), generator=g) * torch.exp2(4 * torch.randn((1, 4, 300, D), generator=g))
+    x *= torch.exp2(torch.randint(-4, 5, (1, 4, 300, 1), generator=g).float())
+    x = x.clamp(-60000, 60000)
+    x[0, 0, 0] = 0
+    x[0, 0, 0, 0], x[0, 0, 0, 1] = 225, 3 * 2.0 ** -10 * (1 - 2.0 ** -8)
+    x = x.to(dt).to(dev)
+    cache = QuantizedPagedCache.empty(20, 4, 16, D, dt)
+    table, lens = torch.arange(20, dtype=torch.int32, device=dev).view(1, 20), torch.tensor([300], dtype=torch.int32, device=dev)
+    paged_append(x, x, cache, table, lens)
+    top = x.double().abs().amax(-1, keepdim=True)
+    scale = torch.exp2(_scale_of(top).double() - 127)
+    for got in paged_read(cache, table, lens, 300):
+        off = (got.double() - x.double()).abs()
+        assert (off <= torch.maximum(2.0 ** -4 * x.double().abs(), 2.0 ** -10 * scale)).all()
+        assert (off <= torch.maximum(2.0 ** -4 * x.double().abs(), 2.0 ** -17.8 * top)).all()
+        assert off[0, 0, 0, 1] > 2.0 ** -18 * top[0, 0, 0, 0]         # not within half of 2^-17 of the largest
 
 
 @pytest.mark.parametrize("dtype,power", [("fp16", -9), ("fp16", -14), ("bf16", -9)])
