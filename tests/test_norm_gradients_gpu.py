@@ -1,12 +1,13 @@
 """Gradients of normed and rotated heads: what queries' and keys' weights share, what is not needed, magnitudes at the
-ends of the range."""
+ends of the range, and calls whose waves walk over several tokens."""
 import pytest
 
 pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
 
-from test_norm_gpu import BWD, FWD, _check, _gradients, _inputs, _normed, _size, _turned  # noqa: E402
+from test_norm_gpu import (BWD, FWD, _check, _gradients, _inputs, _normed, _size, _turned,  # noqa: E402
+                           test_forward as _forward_of, test_gradients as _gradients_of)
 from test_rotary_gpu import DT, _cuda  # noqa: E402
 
 
@@ -87,3 +88,21 @@ def test_magnitudes_at_the_ends_of_the_range(D, dtype, weights, power, eps):
         _check(back[i], dx, xs, "gradient", BWD)
         if w is not None:
             _check(back[2 + i], dw, ws, "weights' gradient", 100 * 2.0 ** -24)
+
+
+@pytest.mark.parametrize("B,N,Hq,Hk,D,rd,sections,inter,dtype,weights", [
+    (3, 1571, 16, 16, 64, 64, [10, 11, 11], True, "fp16", "fp32"),
+    (2, 4096, 32, 8, 128, 128, None, False, "bf16", "same"),
+    (1, 4111, 9, 3, 128, 64, [12, 20], False, "fp32", "same"),
+    (2, 2081, 20, 6, 96, 96, [16, 16, 16], False, "bf16", "fp32"),     # lanes without elements, in every pass
+    (1, 4300, 33, 1, 80, 48, None, True, "fp32", "same"),
+    (4, 1100, 7, 7, 240, 128, [32, 0, 32], False, "fp16", "fp32"),
+    (1, 9001, 6, 2, 64, 32, [8, 8], True, "bf16", "same"),             # one pass a token, five tokens a wave
+    (1, 13_007, 12, 4, 64, 64, [16, 16], False, "fp32", None),
+])
+def test_waves_that_walk_over_tokens(B, N, Hq, Hk, D, rd, sections, inter, dtype, weights):
+    """From 4,096 tokens on, 2 for each wave of 256 compute units, a wave takes all passes of a token and then another's:
+    rows and positions of the next one are asked for ahead, over the end of a token and of a sequence. (Sums of the
+    weights' gradients: at most 20 rows a lane, 4 additions over lanes, 4 over waves and 14 over workgroups.)"""
+    _gradients_of(B, N, Hq, Hk, D, rd, sections, inter, dtype, weights)
+    _forward_of(B, N, Hq, Hk, D, rd, sections, inter, dtype, weights)

@@ -1,5 +1,5 @@
 """What the numbers of a quantised cache stand for: numbers below the tokens' type's normal range, the bounds of what
-quantising loses, and keys that a norm made small."""
+quantising loses, keys that a norm made small, and norm weights in fp32."""
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -7,8 +7,8 @@ pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
 from test_norm_gpu import FWD, _normed  # noqa: E402
-from test_paged_gpu import _cuda, _rotated  # noqa: E402
-from test_paged8_gpu import E4M3, E8M0, _check_rows, _dequantised, _scale_of  # noqa: E402
+from test_paged_gpu import APPENDS, _cuda, _rotated  # noqa: E402
+from test_paged8_gpu import E4M3, E8M0, _check_rows, _dequantised, _scale_of, test_append as _append  # noqa: E402
 
 DT = {"fp16": torch.float16, "bf16": torch.bfloat16}
 # scale exponents about the least under which the type holds every number, and that least: fp16's and bf16's smallest
@@ -110,3 +110,8 @@ def test_keys_that_a_norm_makes_small(dtype, power, rotated):
     stand = _dequantised(q.contiguous().view(E4M3), sb.contiguous().view(E8M0))
     assert (dtype == "fp16") == bool((stand.to(dt).double() != stand).any())
     assert torch.equal(paged_read(cache, table, lens, N)[0][0], stand.float().to(dt))
+
+
+@pytest.mark.parametrize("news,lens,Hq,Hkv,D,S,rd,sections,inter,dtype,ragged", APPENDS)
+def test_append_with_fp32_weights(news, lens, Hq, Hkv, D, S, rd, sections, inter, dtype, ragged):
+    _append(news, lens, Hq, Hkv, D, S, rd, sections, inter, dtype, ragged, "fp32", True)
