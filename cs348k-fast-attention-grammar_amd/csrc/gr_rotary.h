@@ -30,10 +30,12 @@
 // Bound by memory once there are tokens enough: 2 x 4,096 tokens of 32 + 32 heads
 // of 128 (268 MB, bf16) take 43-52 us, 5.2-6.2 TB/s, where a large copy reaches
 // 5.15; 320 tokens of 4 + 4 heads of 64 take 4.0 us, a launch and two trips to
-// memory. Normed: 2 x 4,096 tokens of 32 + 8 heads of 128 (168 MB) 30.7 us, 5.5 TB/s; 288
+// memory. Normed: 2 x 4,096 tokens of 32 + 8 heads of 128 (168 MB) 28-31 us a launch in a row
+// of them, 5.4-6.0 TB/s (34-36 alone, from its first wave to its last), in fp32 61-68; 288
 // tokens of 8 + 4 heads of 64 4.0; normed into a quantised cache, the 9,668 tokens above
-// (218 MB) 43-47.5, 4.6-5.1 TB/s: four waves a SIMD (115 registers) with vector work of their
-// own between loads and stores; without the norm, six waves, 5.2.
+// (218 MB) 43-47.5, 4.6-5.1 TB/s, and into 16-bit pages (238 MB) 43-47: four waves a SIMD
+// (115 registers) with vector work of their own between loads and stores; without the norm,
+// six waves, 5.2.
 //
 // Stores that write whole lines go past the caches, where the attention that
 // reads the rows runs on other XCDs: 8,193 tokens of 32 + 8 + 8 heads of 128 into
